@@ -50,6 +50,7 @@ extern "C" {
 #define SLC_IR_VERSION 2u
 #define SLC_MAX_RANK 8u          /* device.rs:29 */
 #define SLC_MAX_INPUTS 4u        /* device.rs:26 */
+#define SLC_MAX_EXT_INPUTS 6u    /* EXTENSION operators */
 #define SLC_MAX_OUTPUTS 1u       /* device.rs:27 */
 #define SLC_MIN_BUFFER_ALIGN 64u /* docs/ARCH-0004:147-151, runtime.rs:55 */
 
@@ -146,7 +147,49 @@ typedef enum {
      * the benchmark's elementwise sweep): inputs a, b of one shape
      * [..., cols] and bias [cols]; output of a's shape,
      * out = (a + b) + bias[col], each sum rounded as f32 (bit-exact). */
-    SLC_OP_EXT_ADD_BIAS = 0x8002
+    SLC_OP_EXT_ADD_BIAS = 0x8002,
+    /* EXTENSION: paged KV cache (no sl-ir counterpart; KvAppend and
+     * CausalAttention hold one dense cache per batch).
+     *
+     * State: [pages, layers, 2, page, kv_heads, head_dim], the dense cache's
+     * layout with a page of `page` positions in the place of a sequence; dtype
+     * F32, F16 or BF16. It lives in an F32 buffer; a 16-bit state's BufferRef
+     * counts 32-bit words (two elements each). Its offset is a multiple of 4
+     * words (16 bytes). head_dim is a multiple of 8, at most 256.
+     *
+     * Batch: three U32 inputs describe any number of sequences of any lengths.
+     * table [sequences, n]: the pages of each sequence, in order (entry j holds
+     * positions j * page ..); past [sequences]: positions cached before these
+     * tokens; starts [sequences + 1], from 0, nondecreasing: rows starts[b] ..
+     * starts[b + 1] of the token-major inputs are the new tokens of sequence
+     * b, at positions past[b], past[b] + 1, ... (none is allowed). Rows from
+     * starts[sequences] on are padding: not read, and left as they were in
+     * the output. Only table entries of positions that are read or written
+     * are looked at: pages behind a window may have been given away. All are
+     * checked by dispatch, before anything runs. With capture on, a replay
+     * reads what the buffers then hold.
+     *
+     * PAGED_APPEND: inputs k, v [tokens, kv_heads * head_dim] (any leading
+     * dimensions), table, past, starts, state; no output, no scalars. Writes
+     * the new tokens' values, and their keys turned as Rope turns them
+     * (theta, rope_variant) by their positions; theta 0 writes keys as they
+     * come. A page written by two sequences, or twice by one, is refused.
+     *
+     * PAGED_ATTENTION: inputs q [tokens, heads * head_dim], table, past,
+     * starts, state; scalars max_new (at least the most new tokens of one
+     * sequence: it selects kernels), window, sinks. The token at position t
+     * attends, through each head, to the positions p <= t, where window is not
+     * 0 only to those with p > t - window or p < sinks. Its own key must have
+     * been appended. Output of q's shape.
+     *
+     * PREFIX_ATTENTION: PAGED_ATTENTION without a window, for sequences whose
+     * first `prefix` positions are the same pages of the cache; these are read
+     * once for all of them. Scalars max_new, prefix; prefix at most every
+     * past, and the table's rows begin with the same ceil(prefix / page)
+     * entries. */
+    SLC_OP_EXT_PAGED_APPEND = 0x8003,
+    SLC_OP_EXT_PAGED_ATTENTION = 0x8004,
+    SLC_OP_EXT_PREFIX_ATTENTION = 0x8005
 } slc_opcode;
 
 typedef enum { SLC_ROPE_NEOX = 0, SLC_ROPE_GPTJ = 1 } slc_rope_variant;
@@ -155,14 +198,14 @@ typedef enum { SLC_ROPE_NEOX = 0, SLC_ROPE_GPTJ = 1 } slc_rope_variant;
  * (docs/ARCH-0004:237-258). Unused attributes are ignored. */
 typedef struct {
     uint16_t code;         /* slc_opcode */
-    uint16_t rope_variant; /* Rope */
-    uint32_t layer;        /* KvAppend, CausalAttention */
-    uint32_t heads;        /* SplitHeads, MergeHeads, CausalAttention */
-    uint32_t kv_heads;     /* CausalAttention */
-    uint32_t head_dim;     /* SplitHeads, MergeHeads, CausalAttention */
+    uint16_t rope_variant; /* Rope, paged append */
+    uint32_t layer;        /* KvAppend, CausalAttention, paged operators */
+    uint32_t heads;        /* SplitHeads, MergeHeads, CausalAttention, paged attention */
+    uint32_t kv_heads;     /* CausalAttention, paged operators */
+    uint32_t head_dim;     /* SplitHeads, MergeHeads, CausalAttention, paged operators */
     float eps;             /* RmsNorm, RmsNormMatMul */
-    float theta;           /* Rope */
-    float scale;           /* CausalAttention */
+    float theta;           /* Rope, paged append */
+    float scale;           /* CausalAttention, paged attention */
     float factor;          /* Scale */
 } slc_op;
 

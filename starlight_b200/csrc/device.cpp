@@ -160,6 +160,9 @@ bool signature(uint32_t code, Sig *s) {
     case SLC_OP_EXT_ALL_REDUCE: *s = {1, 0, 0, false}; return true;
     case SLC_OP_EXT_ALL_GATHER: *s = {1, 0, 1, false}; return true;
     case SLC_OP_EXT_ADD_BIAS: *s = {3, 0, 1, false}; return true;
+    case SLC_OP_EXT_PAGED_APPEND: *s = {5, 0, 0, true}; return true;
+    case SLC_OP_EXT_PAGED_ATTENTION: *s = {7, 3, 1, true}; return true;
+    case SLC_OP_EXT_PREFIX_ATTENTION: *s = {6, 2, 1, true}; return true;
     default: return false;
     }
 }
@@ -601,7 +604,7 @@ struct Port {
 // validate_call, device.rs:224-286.
 int validate_call(slc_device *d, const slc_op *op, const slc_value *in_vals, uint64_t n_in,
                   uint64_t n_out, uint64_t n_scalars, Sig *sig_out) {
-    if (n_in > SLC_MAX_INPUTS || n_out > SLC_MAX_OUTPUTS)
+    if (n_in > (is_paged(op->code) ? SLC_MAX_EXT_INPUTS : SLC_MAX_INPUTS) || n_out > SLC_MAX_OUTPUTS)
         return exec_err(d, "too many command ports");
     Sig sig;
     if (!signature(op->code, &sig)) {
@@ -634,8 +637,10 @@ int check_range(slc_device *d, const slc_buffer_ref &r, uint64_t capacity) {
     return SLC_OK;
 }
 
-// validate_port, device.rs:288-324 (plus the quantized-Param storage rule).
-int validate_port(slc_device *d, const slc_buffer_ref &r, const slc_value &v, bool output) {
+// validate_port, device.rs:288-324 (plus the quantized-Param storage rule,
+// and the 16-bit State of the paged operators).
+int validate_port(slc_device *d, const slc_buffer_ref &r, const slc_value &v, bool output,
+                  bool paged) {
     if (v.role == SLC_ROLE_SCALAR)
         return exec_err(d, "scalar operands must be passed through the scalars argument");
     Dims dm;
@@ -659,6 +664,13 @@ int validate_port(slc_device *d, const slc_buffer_ref &r, const slc_value &v, bo
         if (words != r.len)
             return exec_err(d, "BufferRef length does not match the quantized payload size");
         DeviceBuffer *b = slot(d, r.buffer, true);
+        if (!b) return invalid_buffer(d, r.buffer);
+        return check_range(d, r, b->elements);
+    }
+    if (paged && v.role == SLC_ROLE_STATE && (v.dtype == SLC_F16 || v.dtype == SLC_BF16)) {
+        if (elements / 2 + elements % 2 != r.len)
+            return exec_err(d, "BufferRef length does not match the 16-bit state size");
+        DeviceBuffer *b = slot(d, r.buffer, false);
         if (!b) return invalid_buffer(d, r.buffer);
         return check_range(d, r, b->elements);
     }
@@ -723,9 +735,10 @@ extern "C" int slc_dispatch(slc_device *d, const slc_op *op, const slc_buffer_re
     int rc = validate_call(d, op, input_values, n_inputs, n_outputs, n_scalars, &sig);
     if (rc != SLC_OK) return rc;
     for (uint64_t i = 0; i < n_inputs; i++)
-        if ((rc = validate_port(d, inputs[i], input_values[i], false)) != SLC_OK) return rc;
+        if ((rc = validate_port(d, inputs[i], input_values[i], false, is_paged(op->code))) != SLC_OK)
+            return rc;
     for (uint64_t i = 0; i < n_outputs; i++)
-        if ((rc = validate_port(d, outputs[i], output_values[i], true)) != SLC_OK) return rc;
+        if ((rc = validate_port(d, outputs[i], output_values[i], true, false)) != SLC_OK) return rc;
     if ((rc = check_disjoint(d, inputs, n_inputs, outputs, n_outputs)) != SLC_OK) return rc;
     return slc_resolve_and_run(d, op, inputs, input_values, n_inputs, outputs, output_values,
                                n_outputs, scalars, n_scalars);

@@ -42,6 +42,9 @@ struct slc_device {
     CaptureState *capture = nullptr;
     CommState *comm = nullptr;
     DecodeRunState *decode = nullptr;
+    // Paged append: page -> number of the check that last saw it written.
+    std::vector<uint32_t> page_seen;
+    uint32_t page_check = 0;
 };
 
 // Device workspace layout (reserved once at creation; dispatch never
@@ -61,6 +64,12 @@ inline uint64_t ws_scratch_bytes(slc_device *d) {
 }
 inline unsigned *ws_attn_tickets(slc_device *d) {
     return reinterpret_cast<unsigned *>(d->workspace + d->workspace_bytes / 2 - kAttnTicketBytes);
+}
+
+// Operators on a paged KV cache (16-bit states, more input ports).
+inline bool is_paged(uint32_t code) {
+    return code == SLC_OP_EXT_PAGED_APPEND || code == SLC_OP_EXT_PAGED_ATTENTION ||
+           code == SLC_OP_EXT_PREFIX_ATTENTION;
 }
 
 // Error helpers shared by the operator layer.

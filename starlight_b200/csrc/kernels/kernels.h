@@ -101,6 +101,50 @@ cudaError_t decode_attention_block(cudaStream_t s, const DecodeBlockIo &io, floa
                                    float theta, int gptj, const AttnScratch &scr,
                                    const uint32_t *d_past, bool early_cache);
 
+// ---- paged_append.cu, paged_attention.cu -------------------------------------------
+// A paged KV cache, the state [pages, layers, 2, page, kv_heads, head_dim]
+// seen from one layer: a page holds `page` positions of every layer, laid out
+// as the dense cache lays out max_seq. Strides in bytes; base 16-byte aligned.
+enum PagedType { kPagedF32 = 0, kPagedF16 = 1, kPagedBf16 = 2 };
+constexpr int kPagedMaxHeadDim = 256;  // and a multiple of 8
+struct PagedCache {
+    char *base;               // the layer's slice of page 0
+    long long page_stride;    // page to page
+    long long parity_stride;  // keys to values
+    long long row_stride;     // position to position
+    int type, page, pages;
+};
+// A ragged batch: sequence b owns rows starts[b] .. starts[b + 1] of the
+// token-major inputs, at positions past[b] onward; table[b] names its pages.
+struct PagedBatch {
+    const uint32_t *table, *past, *starts;  // [seqs, per_seq], [seqs], [seqs + 1]
+    int seqs, per_seq;
+};
+inline bool paged_aligned(const void *base) { return ((uintptr_t)base & 15u) == 0; }
+// theta 0: keys are stored as they come.
+cudaError_t paged_append(cudaStream_t s, const float *k, const float *v, const PagedCache &cache,
+                         const PagedBatch &batch, size_t kv_heads, size_t head_dim, size_t tokens,
+                         float theta, int gptj, uint32_t *err);
+struct PagedAttention {
+    const float *q;  // [tokens, heads, head_dim]
+    float *out;      // the same
+    PagedCache cache;
+    PagedBatch batch;
+    int heads, kv_heads, head_dim, tokens;
+    int max_new;  // most rows of one sequence
+    int window;   // keys a row sees up to its own (0: all), and
+    int sinks;    // first positions seen beside them
+    int prefix;   // leading positions whose pages all sequences share (0: none)
+    float scale;
+    void *workspace;
+    size_t workspace_bytes;
+    unsigned *tickets;  // zeroed, reset by the kernels
+    uint32_t *err;
+};
+size_t paged_attention_workspace_bytes(const PagedAttention &a);
+constexpr size_t kPagedTickets = 1024;  // tickets used at most
+cudaError_t paged_attention(cudaStream_t s, const PagedAttention &a);
+
 // ---- matmul_f32.cu --------------------------------------------------------------
 // out[b] = a[b or 0] . w[b or 0]^T (NT) or a . w (NN), batch broadcast when a
 // batch count is 1 (device.rs:1301-1407).

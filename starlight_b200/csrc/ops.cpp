@@ -3,10 +3,12 @@
 // device.rs:773-1227, and of the reference kernels it calls) followed by the
 // kernel launches. Every check of a command runs before its first launch.
 #include <cuda_runtime.h>
+#include <float.h>
 #include <math.h>
 #include <string.h>
 
 #include <algorithm>
+#include <new>
 
 #include "device_internal.h"
 #include "kernels/kernels.h"
@@ -253,6 +255,146 @@ cudaError_t matmul_rows(slc_device *d, const float *x, uint64_t rows, uint64_t k
 int finish(Checker &ck, cudaError_t e) {
     if (e != cudaSuccess) return ck.exec("CUDA kernel launch failed");
     return SLC_OK;
+}
+
+// ---- paged KV cache ---------------------------------------------------------
+
+// The state and batch of a paged operator, read off its ports: table, past
+// and starts at ports `first` .. first + 2, the state behind them.
+struct Paged {
+    k::PagedCache cache{};
+    k::PagedBatch batch{};
+    uint64_t tokens = 0;       // rows of the token-major inputs
+    uint64_t pages = 0, page = 0;
+    const uint32_t *table = nullptr, *past = nullptr, *starts = nullptr;  // host copies
+};
+
+bool paged_ports(Checker &ck, uint64_t first, uint64_t tokens, Paged *o) {
+    const slc_op &op = *ck.c.op;
+    auto no = [&](const char *msg) {
+        ck.exec(msg);
+        return false;
+    };
+    if (ck.c.state_index != (int64_t)(first + 3)) return no("paged state must be the last input");
+    Dims t, p, s, st;
+    if (!ck.ivalue(first, &t) || !ck.ivalue(first + 1, &p) || !ck.ivalue(first + 2, &s) ||
+        !ck.ivalue(first + 3, &st))
+        return false;
+    if (t.rank != 2 || p.rank != 1 || s.rank != 1 || p[0] != t[0] || s[0] != t[0] + 1)
+        return no("paged batch shapes must be table [sequences, pages], past [sequences], "
+                  "starts [sequences + 1]");
+    if (!ck.u32(first) || !ck.u32(first + 1) || !ck.u32(first + 2)) return false;
+    const uint64_t hkv = op.kv_heads, hd = op.head_dim;
+    if (st.rank != 6 || st[2] != 2 || st[4] != hkv || st[5] != hd)
+        return no("paged state shape must be [pages, layers, 2, page, kv_heads, head_dim]");
+    const slc_value &sv = ck.c.iv[first + 3];
+    const slc_buffer_ref &sr = ck.c.in[first + 3];
+    if (sv.dtype != SLC_F32 && sv.dtype != SLC_F16 && sv.dtype != SLC_BF16)
+        return no("paged state must be F32, F16 or BF16");
+    if (op.layer >= st[1]) return no("attention layer is out of range");
+    if (hkv == 0) return no("kv_heads must be nonzero");
+    if (hd == 0 || hd % 8 != 0 || hd > (uint64_t)k::kPagedMaxHeadDim) {
+        ck.fail(SLC_ERR_UNIMPLEMENTED, "paged operators support head_dim a multiple of 8 up to 256");
+        return false;
+    }
+    if (st[3] == 0) return no("paged state needs a nonzero page size");
+    char *base = ck.d->buffers[sr.buffer].ptr + sr.offset * 4;
+    if (!k::paged_aligned(base)) {
+        ck.fail(SLC_ERR_UNIMPLEMENTED, "paged state must start on a 16-byte boundary");
+        return false;
+    }
+    if (t[1] * st[3] > INT32_MAX || st[0] > INT32_MAX || t[0] > INT32_MAX || tokens > INT32_MAX ||
+        t[1] > INT32_MAX)
+        return no("paged batch exceeds 2^31 - 1 positions, pages, sequences or tokens");
+    const long long size = sv.dtype == SLC_F32 ? 4 : 2;
+    o->cache.type = sv.dtype == SLC_F32 ? k::kPagedF32 : sv.dtype == SLC_F16 ? k::kPagedF16 : k::kPagedBf16;
+    o->cache.row_stride = (long long)(hkv * hd) * size;
+    o->cache.parity_stride = o->cache.row_stride * (long long)st[3];
+    o->cache.page_stride = o->cache.parity_stride * 2 * (long long)st[1];
+    o->cache.base = base + o->cache.parity_stride * 2 * op.layer;
+    o->cache.page = (int)st[3];
+    o->cache.pages = (int)st[0];
+    o->page = st[3];
+    o->pages = st[0];
+    o->tokens = tokens;
+    o->batch.table = ck.u32(first);
+    o->batch.past = ck.u32(first + 1);
+    o->batch.starts = ck.u32(first + 2);
+    o->batch.seqs = (int)t[0];
+    o->batch.per_seq = (int)t[1];
+    o->table = ck.u32_host(first);
+    o->past = ck.u32_host(first + 1);
+    o->starts = ck.u32_host(first + 2);
+    return true;
+}
+
+// Largest of n page ids (0 when there are none).
+uint32_t largest(const uint32_t *ids, uint64_t n) {
+    uint32_t m = 0;
+    for (uint64_t i = 0; i < n; i++) m = ids[i] > m ? ids[i] : m;
+    return m;
+}
+
+// The batch's contents, as uploaded: token ranges, lengths and every page id
+// that the operator will follow (`window` and `sinks` as in the operator).
+bool paged_contents(Checker &ck, const Paged &g, uint64_t window, uint64_t sinks) {
+    auto no = [&](const char *msg) {
+        ck.exec(msg);
+        return false;
+    };
+    if (g.starts[0] != 0) return no("paged batch starts must begin at 0");
+    const uint64_t width = (uint64_t)g.batch.per_seq;
+    for (int b = 0; b < g.batch.seqs; b++) {
+        if (g.starts[b + 1] < g.starts[b]) return no("paged batch starts must not decrease");
+        const uint64_t n = g.starts[b + 1] - g.starts[b], past = g.past[b], end = past + n;
+        if (n == 0) continue;
+        if (g.starts[b + 1] > g.tokens) return no("paged batch starts exceed the token rows");
+        if (end > width * g.page) return no("past + new tokens exceed the table's pages");
+        uint64_t low = 0, sink = 0;
+        if (window) {
+            low = past + 1 > window ? past + 1 - window : 0;
+            sink = std::min(sinks, low);
+        }
+        const uint32_t *row = g.table + (uint64_t)b * width;
+        const uint64_t p0 = low / g.page, p1 = (end + g.page - 1) / g.page;
+        const uint32_t top = std::max(largest(row, (sink + g.page - 1) / g.page),
+                                      largest(row + p0, p1 - p0));
+        if (top >= g.pages) return no("page id out of range");
+    }
+    return true;
+}
+
+// Every page that the append writes is written by one sequence, once.
+bool paged_writes(Checker &ck, const Paged &g) {
+    slc_device *d = ck.d;
+    try {
+        if (d->page_seen.size() < g.pages) d->page_seen.resize(g.pages, 0);
+    } catch (const std::bad_alloc &) {
+        ck.fail(SLC_ERR_OUT_OF_MEMORY, "out of host memory");
+        return false;
+    }
+    if (++d->page_check == 0) {
+        std::fill(d->page_seen.begin(), d->page_seen.end(), 0u);
+        d->page_check = 1;
+    }
+    for (int b = 0; b < g.batch.seqs; b++) {
+        const uint64_t n = g.starts[b + 1] - g.starts[b];
+        if (n == 0) continue;
+        const uint32_t *row = g.table + (uint64_t)b * (uint64_t)g.batch.per_seq;
+        const uint64_t p1 = (g.past[b] + n + g.page - 1) / g.page;
+        for (uint64_t i = g.past[b] / g.page; i < p1; i++) {
+            if (row[i] >= g.pages) {
+                ck.exec("page id out of range");
+                return false;
+            }
+            if (d->page_seen[row[i]] == d->page_check) {
+                ck.exec("paged append writes one page twice");
+                return false;
+            }
+            d->page_seen[row[i]] = d->page_check;
+        }
+    }
+    return true;
 }
 
 #define REQUIRE(expr)             \
@@ -639,6 +781,88 @@ int run_op(slc_device *d, const Cmd &c, bool launch) {
         REQUIRE(ap && bp && zp);
         if (!launch) return SLC_OK;
         return finish(ck, k::add_bias(s, ap, bp, zp, ck.output(), rows, cols));
+    }
+    case SLC_OP_EXT_PAGED_APPEND: {
+        Dims kd, vd;
+        REQUIRE(ck.ivalue(0, &kd) && ck.ivalue(1, &vd));
+        if (!same(kd, vd)) return ck.exec("paged append key and value shapes must match");
+        uint64_t width, tokens, kv;
+        REQUIRE(ck.last(kd, &width) && ck.product(kd, kd.rank - 1, &tokens));
+        if (!checked_mul(c.op->kv_heads, c.op->head_dim, &kv)) return ck.overflow();
+        if (width != kv) return ck.exec("paged append width must equal kv_heads * head_dim");
+        const float *kp = ck.f32(0), *vp = ck.f32(1);
+        REQUIRE(kp && vp);
+        if (!(c.op->theta >= 0.f) || c.op->theta > FLT_MAX)
+            return ck.exec("paged append theta must be finite and not negative");
+        if (c.op->rope_variant > SLC_ROPE_GPTJ)
+            return ck.fail(SLC_ERR_UNIMPLEMENTED, "unknown rope variant");
+        Paged g;
+        // What an append reads is what it writes: a window of one token.
+        REQUIRE(paged_ports(ck, 2, tokens, &g) && paged_contents(ck, g, 1, 0) && paged_writes(ck, g));
+        if (!launch) return SLC_OK;
+        return finish(ck, k::paged_append(s, kp, vp, g.cache, g.batch, c.op->kv_heads,
+                                          c.op->head_dim, tokens, c.op->theta,
+                                          c.op->rope_variant == SLC_ROPE_GPTJ, d->device_flag));
+    }
+    case SLC_OP_EXT_PAGED_ATTENTION:
+    case SLC_OP_EXT_PREFIX_ATTENTION: {
+        const bool shared = c.op->code == SLC_OP_EXT_PREFIX_ATTENTION;
+        Dims qd, od;
+        REQUIRE(ck.ivalue(0, &qd) && ck.ovalue(0, &od));
+        uint64_t width, tokens, hw, max_new, window = 0, sinks = 0, prefix = 0;
+        REQUIRE(ck.last(qd, &width) && ck.product(qd, qd.rank - 1, &tokens) && ck.scalar(0, &max_new));
+        if (shared)
+            REQUIRE(ck.scalar(1, &prefix));
+        else
+            REQUIRE(ck.scalar(1, &window) && ck.scalar(2, &sinks));
+        const uint64_t heads = c.op->heads, kvh = c.op->kv_heads;
+        if (!checked_mul(heads, c.op->head_dim, &hw)) return ck.overflow();
+        if (width != hw) return ck.exec("paged attention width must equal heads * head_dim");
+        if (!same(qd, od)) return ck.exec("paged attention output shape must match the query shape");
+        const float *qp = ck.f32(0);
+        REQUIRE(qp);
+        Paged g;
+        REQUIRE(paged_ports(ck, 1, tokens, &g));
+        if (heads == 0) return ck.exec("heads must be nonzero");
+        if (heads % kvh != 0) return ck.exec("heads must be a multiple of kv_heads");
+        if (heads > (1u << 16)) return ck.fail(SLC_ERR_UNIMPLEMENTED, "paged attention supports 65536 heads");
+        REQUIRE(paged_contents(ck, g, window, sinks));
+        const uint64_t width_pages = (uint64_t)g.batch.per_seq;
+        const uint64_t shared_pages = (prefix + g.page - 1) / g.page;
+        const uint32_t *lead = nullptr;
+        for (int b = 0; b < g.batch.seqs; b++) {
+            const uint64_t n = g.starts[b + 1] - g.starts[b];
+            if (n > max_new) return ck.exec("a sequence brings more tokens than max_new");
+            if (n == 0 || !prefix) continue;
+            if (g.past[b] < prefix) return ck.exec("the shared prefix exceeds a sequence's past");
+            const uint32_t *row = g.table + (uint64_t)b * width_pages;
+            if (!lead) lead = row;  // the kernel reads the prefix through this row too
+            if (memcmp(lead, row, shared_pages * sizeof(uint32_t)) != 0)
+                return ck.exec("the shared prefix's pages differ between sequences");
+        }
+        k::PagedAttention a{};
+        a.q = qp;
+        a.out = ck.output();
+        a.cache = g.cache;
+        a.batch = g.batch;
+        a.heads = (int)heads;
+        a.kv_heads = (int)kvh;
+        a.head_dim = (int)c.op->head_dim;
+        a.tokens = (int)tokens;
+        a.max_new = (int)std::min<uint64_t>(max_new, tokens);
+        a.window = (int)std::min<uint64_t>(window, INT32_MAX);
+        a.sinks = (int)std::min<uint64_t>(sinks, INT32_MAX);
+        a.prefix = (int)std::min<uint64_t>(prefix, INT32_MAX);
+        a.scale = c.op->scale;
+        a.workspace = kernel_scratch(d);
+        a.workspace_bytes = kernel_scratch_bytes(d);
+        a.tickets = ws_attn_tickets(d);
+        a.err = d->device_flag;
+        static_assert(k::kPagedTickets * sizeof(unsigned) <= kAttnTicketBytes, "tickets");
+        if (k::paged_attention_workspace_bytes(a) > a.workspace_bytes)
+            return ck.exec("device workspace is too small for this attention shape");
+        if (!launch) return SLC_OK;
+        return finish(ck, k::paged_attention(s, a));
     }
     case SLC_OP_EXT_ALL_REDUCE: {
         Dims x;

@@ -81,6 +81,9 @@ class OpCode(enum.IntEnum):  # docs/ARCH-0004:226-235, #[repr(u16)] order
     AllReduce = 0x8000  # extension: tensor-parallel sum
     AllGather = 0x8001  # extension: tensor-parallel gather of column blocks
     AddBias = 0x8002  # extension: (a + b) + bias[col], bias broadcast over rows
+    PagedAppend = 0x8003  # extension: rotate and append to a paged KV cache
+    PagedAttention = 0x8004  # extension: causal / windowed attention over a paged cache
+    PrefixAttention = 0x8005  # extension: the same with a prefix shared by the batch
 
 
 class RopeVariant(enum.IntEnum):
@@ -319,6 +322,41 @@ def _ptr(a: np.ndarray):
     return C.c_void_p(a.ctypes.data) if a.size else None
 
 
+class Command:
+    """One dispatch with its ports laid out once (sl-device CommandBuffer
+    entry): calling it dispatches the operator on the same buffer ranges.
+    `scalars` may be given anew with each call."""
+
+    def __init__(self, dev, op, inputs, input_values, outputs, output_values, scalars):
+        if len(inputs) != len(input_values) or len(outputs) != len(output_values):
+            raise DeviceError(Status.Execution, "inputs and input_values have different lengths")
+
+        def refs(rs):
+            return (_BufferRef * max(len(rs), 1))(*[_BufferRef(r.buffer, 0, r.offset, r.len)
+                                                    for r in rs])
+
+        def values(vs):
+            return (_Value * max(len(vs), 1))(*[v._c() for v in vs])
+
+        self._dev = dev
+        self._call = dev._lib.slc_dispatch
+        self._ports = (refs(inputs), values(input_values), len(inputs), refs(outputs),
+                       values(output_values), len(outputs))
+        self._op = op._c()
+        self._op_ref = C.byref(self._op)
+        self._scalars = self._c_scalars(scalars)
+
+    @staticmethod
+    def _c_scalars(scalars):
+        return (C.c_uint32 * max(len(scalars), 1))(*[int(s) for s in scalars]), len(scalars)
+
+    def __call__(self, scalars: Sequence[int] | None = None) -> None:
+        sc = self._scalars if scalars is None else self._c_scalars(scalars)
+        rc = self._call(self._dev._d, self._op_ref, *self._ports, *sc)
+        if rc:
+            self._dev._check(rc)
+
+
 class CudaDevice:
     """backend-cuda device on one GPU (the `impl Device` of the ABI)."""
 
@@ -390,16 +428,13 @@ class CudaDevice:
     def dispatch(self, op: Op, inputs: Sequence[BufferRef], input_values: Sequence[Value],
                  outputs: Sequence[BufferRef], output_values: Sequence[Value],
                  scalars: Sequence[int] = ()) -> None:
-        ni, no, ns = len(inputs), len(outputs), len(scalars)
-        if ni != len(input_values) or no != len(output_values):
-            raise DeviceError(Status.Execution, "inputs and input_values have different lengths")
-        ir = (_BufferRef * max(ni, 1))(*[_BufferRef(r.buffer, 0, r.offset, r.len) for r in inputs])
-        iv = (_Value * max(ni, 1))(*[v._c() for v in input_values])
-        orf = (_BufferRef * max(no, 1))(*[_BufferRef(r.buffer, 0, r.offset, r.len) for r in outputs])
-        ov = (_Value * max(no, 1))(*[v._c() for v in output_values])
-        sc = (C.c_uint32 * max(ns, 1))(*[int(s) for s in scalars])
-        o = op._c()
-        self._check(self._lib.slc_dispatch(self._d, C.byref(o), ir, iv, ni, orf, ov, no, sc, ns))
+        Command(self, op, inputs, input_values, outputs, output_values, scalars)()
+
+    def command(self, op: Op, inputs: Sequence[BufferRef], input_values: Sequence[Value],
+                outputs: Sequence[BufferRef], output_values: Sequence[Value],
+                scalars: Sequence[int] = ()) -> Command:
+        """A dispatch to be repeated: its ports are converted here, once."""
+        return Command(self, op, inputs, input_values, outputs, output_values, scalars)
 
     def synchronize(self) -> None:
         self._check(self._lib.slc_synchronize(self._d))
@@ -509,6 +544,15 @@ def quant_storage_words(rows: int, k: int, fmt: QuantFormat) -> int:
     """u32 words of a packed payload [rows, k] (INT4: ceil(k/2) bytes per row)."""
     row_bytes = (k + 1) // 2 if fmt == QuantFormat.Int4 else k
     return (rows * row_bytes + 3) // 4
+
+
+def state_words(shape: Sequence[int], dtype: DType) -> int:
+    """32-bit words of a dense state (F32, or F16 / BF16 two elements a word):
+    the size of its F32 buffer and its BufferRef's len."""
+    n = 1
+    for d in shape:
+        n *= int(d)
+    return n if dtype == DType.F32 else (n + 1) // 2
 
 
 def quant_groups(k: int, group: int) -> int:

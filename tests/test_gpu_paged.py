@@ -1,0 +1,544 @@
+"""GPU tests of the paged KV-cache operators against their definitions in 64
+bits (tests/paged_util.py), at the lengths, masks, layouts and contents where
+they can go wrong.
+
+Append: an F32 cache holds bit for bit what the Rope operator gives, a 16-bit
+cache those values rounded to nearest; every other slot keeps its bits.
+
+Attention: the bound, elementwise. A tf32 pair keeps x to 2^-20 (its low part
+has 13 bits, of which the MMA reads 11), the product of two low parts is left
+out (2^-20): a product is off by 3 * 2^-20 of its size, and a sum of D of them
+in f32 by at most as much again for D <= 256 and the accumulators used: a
+score's error is below ds = 8 * 2^-20 * scale * sum |q k|. A probability is
+then off by a factor of exp(ds), numerator and denominator both: 2 ds of
+sum p |v|. The products p v add 3 * 2^-20, the exponential 2^-22, the sums
+over the keys (32 or more apart in separate accumulators, 2^-23 a step) at
+most 2^-20 for 64 keys, the merges and the division the rest of 8 * 2^-20.
+The split of rows and keys over CTAs changes which sums are made first, not
+the bound."""
+import math
+
+import numpy as np
+import pytest
+
+from starlight_b200.device import (BufferRef, CudaDevice, DeviceError, DType, Op, OpCode, RopeVariant, Value,
+                                   ValueRole, state_words)
+from tests.gpu_util import get, new_f32, put_f32, put_u32
+from tests.paged_util import HOLE, Batch, from_bits, put_at, to_bits, upload
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = DType.F32, DType.F16, DType.BF16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = CudaDevice(0)
+    yield d
+    d.close()
+
+
+def attend(dev, b, scale=None, window=0, sinks=0, offset=0, refs=None, max_new=None, out=None):
+    """PagedAttention (PrefixAttention where the batch has a prefix) over the
+    batch; the output buffer holds 7.5 before."""
+    scale = 1 / math.sqrt(b.dim) if scale is None else scale
+    tables, cache = refs or upload(dev, b)
+    x = Value.f32((b.tokens, b.heads * b.dim))
+    q = put_at(dev, b.q, offset)
+    out = out or put_at(dev, np.full(b.q.size, 7.5, np.float32), offset)
+    new = b.max_new() if max_new is None else max_new
+    code, scalars = (OpCode.PrefixAttention, [new, b.prefix]) if b.prefix else (OpCode.PagedAttention,
+                                                                                [new, window, sinks])
+    dev.dispatch(b.op(code, scale=scale), [q, *tables, cache], [x, *b.described(), b.state()], [out], [x], scalars)
+    return get(dev, out).reshape(b.tokens, -1)
+
+
+def check(got, b, scale=None, window=0, sinks=0):
+    scale = 1 / math.sqrt(b.dim) if scale is None else scale
+    want, tol = b.attention(scale, window, sinks)
+    live = int(b.starts[-1])
+    err = np.abs(got[:live] - want[:live])
+    assert np.all(np.isfinite(got[:live]))
+    assert np.all(err <= tol[:live]), (err / np.maximum(tol[:live], 1e-30)).max()
+    assert np.all(got[live:] == 7.5)  # rows behind the last sequence
+
+
+# ---------------------------------------------------------------- append ----
+
+APPENDS = [
+    dict(lens=[(0, 1)]),
+    dict(lens=[(5, 1)], page=1, dim=8, kv_heads=1),
+    dict(lens=[(20, 3), (0, 17), (7, 0), (33, 1)], page=5, dim=72, kv_heads=3, layers=3),
+    dict(lens=[(511, 1)] * 9, page=16, dim=128, kv_heads=8, pad=4),
+    dict(lens=[(3, 700), (0, 1), (90, 130)], page=64, dim=64, kv_heads=4, layers=1, layer=0),
+    dict(lens=[(1, 33)], page=100, dim=256, kv_heads=2),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("variant", [RopeVariant.Neox, RopeVariant.GptJ])
+@pytest.mark.parametrize("case", range(len(APPENDS)))
+@pytest.mark.parametrize("offset", [0, 1])
+def test_append(dev, case, dtype, variant, offset):
+    b = Batch(**APPENDS[case], dtype=dtype, seed=case)
+    tables, cache = upload(dev, b)
+    T, kv = b.tokens, b.kv_heads * b.dim
+    k, v = put_at(dev, b.k, offset), put_at(dev, b.v, offset)
+    x = Value.f32((T, kv))
+    for theta in (500000.0, 0.0):
+        turned = b.k
+        pos = np.zeros(T, np.uint32)
+        for i, (p, n) in enumerate(b.lens):
+            pos[b.starts[i]:b.starts[i + 1]] = p + np.arange(n)
+        if theta:
+            out = new_f32(dev, b.k.size)
+            y = Value.f32((T, b.kv_heads, 1, b.dim))
+            dev.dispatch(Op(OpCode.Rope, theta=theta, variant=variant), [k, put_u32(dev, pos)],
+                         [y, Value.u32((T, 1))], [out], [y])
+            turned = get(dev, out)
+        dev.upload_f32(cache.buffer, b.words)
+        dev.dispatch(b.append_op(theta, variant), [k, v, *tables, cache], [x, x, *b.described(), b.state()], [], [])
+        got = from_bits(get(dev, cache), b.shape, dtype)
+        want = b.stored.copy()
+        turned, value = (to_bits(a, dtype)[0].reshape(T, b.kv_heads, b.dim) for a in (turned, b.v))
+        for i, (p, n) in enumerate(b.lens):
+            at = p + np.arange(n)
+            where = b.table[i][at // b.page].astype(np.int64)
+            rows = slice(int(b.starts[i]), int(b.starts[i + 1]))
+            want[where, b.layer, 0, at % b.page] = turned[rows]
+            want[where, b.layer, 1, at % b.page] = value[rows]
+        assert np.array_equal(got, want, equal_nan=True)
+
+
+def test_append_positions_far_out(dev):
+    # Angles of positions near 2^24: the f64 path, as the Rope operator's.
+    b = Batch([(0, 2)], page=1 << 23, layers=1, layer=0, kv_heads=1, heads=1, dim=8, extra_pages=0,
+              width=4)
+    b.past[:] = (1 << 24) - 2
+    b.table[0] = [HOLE, 0, HOLE, HOLE]
+    tables = [put_u32(dev, a) for a in (b.table, b.past, b.starts)]
+    cache = new_f32(dev, state_words(b.shape, F32))
+    k, v = put_f32(dev, b.k), put_f32(dev, b.v)
+    x = Value.f32((2, 8))
+    dev.dispatch(b.append_op(), [k, v, *tables, cache], [x, x, *b.described(), b.state()], [], [])
+    out = new_f32(dev, 16)
+    y = Value.f32((2, 1, 1, 8))
+    pos = put_u32(dev, (1 << 24) - 2 + np.arange(2))
+    dev.dispatch(Op(OpCode.Rope, theta=500000.0), [k, pos], [y, Value.u32((2, 1))], [out], [y])
+    got = get(dev, cache).reshape(b.shape)
+    assert np.array_equal(got[0, 0, 0, -2:, 0].ravel(), get(dev, out))
+    assert np.array_equal(got[0, 0, 1, -2:, 0].ravel(), b.v.ravel())
+
+
+# ------------------------------------------------------------- attention ----
+
+SHAPES = [
+    dict(heads=1, kv_heads=1, dim=8, page=1),
+    dict(heads=4, kv_heads=4, dim=64, page=16),
+    dict(heads=8, kv_heads=2, dim=128, page=16),
+    dict(heads=6, kv_heads=2, dim=72, page=5),
+    dict(heads=16, kv_heads=2, dim=128, page=64, layers=3),
+    dict(heads=16, kv_heads=1, dim=96, page=7),
+    dict(heads=71, kv_heads=1, dim=64, page=32),
+    dict(heads=2, kv_heads=1, dim=256, page=16),
+    dict(heads=3, kv_heads=1, dim=200, page=100, layers=1, layer=0),
+]
+LENGTHS = [
+    [(0, 1)],
+    [(1, 1), (63, 1), (64, 1), (65, 1), (500, 1)],
+    [(0, 1), (130, 0), (17, 2), (15, 1), (0, 5)],
+    [(40, 33), (3, 1), (0, 70)],
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens", range(len(LENGTHS)))
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_attention(dev, shape, lens, dtype):
+    b = Batch(LENGTHS[lens], **SHAPES[shape], dtype=dtype, seed=10 * shape + lens, pad=lens)
+    refs = upload(dev, b)
+    check(attend(dev, b, offset=lens % 2, refs=refs), b)
+    check(attend(dev, b, window=16, sinks=4, refs=refs), b, window=16, sinks=4)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (7, 0), (64, 4), (65, 63), (100, 1000), (1 << 31, 5),
+                                          (400, 0)])
+def test_windows_and_sinks(dev, window, sinks, dtype):
+    b = Batch([(0, 1), (300, 1), (62, 9), (390, 20), (5, 130)], heads=8, kv_heads=2, dim=64, page=16, dtype=dtype)
+    check(attend(dev, b, window=window, sinks=sinks), b, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_pages_behind_the_window_may_be_gone(dev, new):
+    b = Batch([(200, new), (90, new)], heads=4, kv_heads=2, dim=64, page=8)
+    want, tol = b.attention(0.125, 24, 3)
+    for i, (p, _) in enumerate(b.lens):
+        b.table[i, 1:(p + 1 - 24) // 8] = HOLE
+    got = attend(dev, b, scale=0.125, window=24, sinks=3)
+    assert np.all(np.abs(got - want) <= tol)
+
+
+@pytest.mark.parametrize("dtype,lens", [(F32, [(70000, 1)]), (BF16, [(70000, 1), (9, 1), (33333, 3)]),
+                                        (F16, [(20000, 1)] * 3 + [(0, 1)] * 40)])
+def test_long_sequences(dev, dtype, lens):
+    b = Batch(lens, heads=4, kv_heads=1, dim=128, page=16, layers=1, layer=0, dtype=dtype)
+    check(attend(dev, b), b)
+
+
+def test_offsets_past_32_bits(dev):
+    # A cache of more than 2^32 bytes; the sequence lives in its last pages.
+    pages, page, hkv, d = 5000, 64, 8, 128
+    shape = (pages, 2, 2, page, hkv, d)
+    n = int(np.prod(shape))
+    assert n * 4 > 1 << 32
+    b = Batch([(100, 1)], heads=8, kv_heads=8, dim=128, page=page, layers=2, layer=1, extra_pages=0)
+    buf = dev.allocate_f32(n)
+    last = b.stored.astype(np.float32)
+    per_page = n // pages
+    import torch
+
+    class Memory:
+        __cuda_array_interface__ = dict(shape=(2 * per_page,), typestr="<f4", version=3,
+                                        data=(dev.device_ptr(buf) + 4 * (n - 2 * per_page), False))
+
+    dev.synchronize()
+    torch.as_tensor(Memory(), device="cuda").copy_(torch.from_numpy(last.ravel()))
+    torch.cuda.synchronize()
+    b.table = b.table + np.uint32(pages - 2)
+    b.pages, b.shape = pages, shape
+    tables = [put_u32(dev, a) for a in (b.table, b.past, b.starts)]
+    got = attend(dev, b, refs=(tables, BufferRef(buf, 0, n)))
+    b.stored = np.zeros((0,))
+    b.keys = lambda i: tuple(last[(b.table[0] - pages + 2).astype(np.int64)][:, 1, x].reshape(-1, hkv, d)[:101]
+                             .astype(np.float64) for x in (0, 1))
+    check(got, b)
+    # Append there as well.
+    x = Value.f32((1, hkv * d))
+    dev.dispatch(b.append_op(theta=0.0), [put_f32(dev, b.k), put_f32(dev, b.v), *tables, BufferRef(buf, 0, n)],
+                 [x, x, *b.described(), b.state()], [], [])
+    dev.synchronize()
+    tail = torch.as_tensor(Memory(), device="cuda").cpu().numpy().reshape(2, *shape[1:])
+    at = tail[int(b.table[0, 1]) - pages + 2, 1, :, 100 - 64]
+    assert np.array_equal(at[0].ravel(), b.k.ravel()) and np.array_equal(at[1].ravel(), b.v.ravel())
+    dev.release(buf)
+
+
+# ------------------------------------------------- values out of the ordinary
+
+def put_values(b, places):
+    """Sets keys / values of (sequence, position) to given numbers."""
+    for seq, pos, parity, value in places:
+        b.stored[int(b.table[seq, pos // b.page]), b.layer, parity, pos % b.page] = value
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), b.dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("value", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("heads,new", [(2, 6), (16, 40)])
+def test_keys_and_values_that_a_row_does_not_see(dev, value, dtype, heads, new):
+    # Position 100 + 3 is not finite: it belongs to the fourth new token, so
+    # three rows of the same block must come out clean; and position 60 is
+    # behind the window of the rows from 60 + 50 on.
+    b = Batch([(100, new), (10, 1)], heads=heads, kv_heads=2, dim=64, page=16, dtype=dtype)
+    put_values(b, [(0, 103, 0, value), (0, 103, 1, value)])
+    got = attend(dev, b)
+    want, tol = b.attention(0.125)
+    clean = [0, 1, 2, new]  # the last: the other sequence
+    assert np.all(np.abs(got[clean] - want[clean]) <= tol[clean])
+    assert not np.any(np.isfinite(got[3]))
+    b = Batch([(100, new)], heads=heads, kv_heads=2, dim=64, page=16, dtype=dtype)
+    put_values(b, [(0, 60, 0, value), (0, 60, 1, value)])
+    got = attend(dev, b, window=41 + 3)  # rows 0 .. 3 see positions > 56 .. 59, row 4 onward not 60
+    want, tol = b.attention(0.125, 44)
+    assert np.all(np.abs(got[4:] - want[4:]) <= tol[4:])
+    assert not np.any(np.isfinite(got[:4]))
+
+
+@pytest.mark.parametrize("new", [1, 70])
+def test_scores_of_minus_infinity_leave_the_others(dev, new):
+    # A visible key of -inf times a positive query: its probability is 0.
+    b = Batch([(100, new)], heads=2, kv_heads=2, dim=8, page=16)
+    b.q = np.abs(b.q) + 0.1
+    put_values(b, [(0, 50, 0, -np.inf)])
+    got = attend(dev, b)
+    with np.errstate(invalid="ignore"):
+        k, v = b.keys(0)
+    keep = np.arange(100 + new) != 50
+    for t in range(new):
+        for h in range(2):
+            seen = keep & (np.arange(100 + new) <= 100 + t)
+            s = k[seen, h] @ b.q[t, 8 * h:8 * h + 8].astype(np.float64) / math.sqrt(8)
+            w = np.exp(s - s.max())
+            want = (w / w.sum()) @ v[seen, h]
+            # ds for scores of up to 8 terms of size 5; see the module's note.
+            assert np.all(np.abs(got[t, 8 * h:8 * h + 8] - want) <= 1e-3)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -12, 2.0 ** 12, 2.0 ** 60])
+def test_sizes_of_keys_values_and_queries(dev, size, dtype, new):
+    # The same scores from keys and queries of any size, values of any size.
+    if dtype == F16 and not 2.0 ** -13 < size < 2.0 ** 13:
+        pytest.skip("beyond F16")
+    b = Batch([(150, new)], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)
+    b.stored, b.words = to_bits((b.stored * size).astype(np.float32), dtype)
+    check(attend(dev, b, scale=0.125 / size), b, scale=0.125 / size)
+    b.q = (b.q / np.float32(size)).astype(np.float32)
+    check(attend(dev, b, scale=0.125), b, scale=0.125)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_of_very_different_sizes(dev, dtype, new):
+    # One key with a huge value that no row gives weight, among small ones.
+    b = Batch([(150, new)], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)
+    b.q = np.abs(b.q) + 0.5
+    put_values(b, [(0, 30, 0, -200.0), (0, 30, 1, 2.0 ** 40)])
+    got = attend(dev, b)
+    want, tol = b.attention(0.125)
+    assert np.all(np.abs(got - want) <= tol + 1e-30)
+
+
+def test_extreme_scores(dev):
+    # Scores of +-20000: only differences count.
+    b = Batch([(200, 1), (90, 40)], heads=4, kv_heads=2, dim=64, page=16)
+    check(attend(dev, b, scale=300.0), b, scale=300.0)
+    check(attend(dev, b, scale=0.0), b, scale=0.0)
+    check(attend(dev, b, scale=-0.125), b, scale=-0.125)
+
+
+# ---------------------------------------------------------------- prefix ----
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", [
+    dict(lens=[(20, 1)], prefix=1, page=16),
+    dict(lens=[(20, 1), (40, 1), (16, 1)], prefix=16, page=16, heads=8, kv_heads=2, dim=128),
+    dict(lens=[(300, 1), (301, 3), (257, 0), (700, 1)], prefix=257, page=16, heads=4, kv_heads=4, dim=64),
+    dict(lens=[(130, 0), (130, 1), (131, 17)], prefix=130, page=5, heads=6, kv_heads=2, dim=72, pad=3),
+    dict(lens=[(2000 + i, 1) for i in range(40)], prefix=2000, page=64, heads=8, kv_heads=1, dim=128, layers=1,
+         layer=0),
+    dict(lens=[(90, 2), (99, 1)], prefix=64, page=16, heads=2, kv_heads=1, dim=256),
+    dict(lens=[(200, 70), (150, 1)], prefix=150, page=32, heads=16, kv_heads=2, dim=64),
+])
+def test_prefix(dev, case, dtype):
+    b = Batch(**case, dtype=dtype)
+    check(attend(dev, b, offset=1), b)
+    prefix, b.prefix = b.prefix, 0
+    plain = attend(dev, b)  # the operator without a prefix gives the same
+    check(plain, b)
+    b.prefix = prefix
+
+
+def test_prefix_of_zero(dev):
+    b = Batch([(20, 1), (3, 2)], heads=4, kv_heads=2, dim=64)
+    refs = upload(dev, b)
+    x = Value.f32((b.tokens, 256))
+    out = new_f32(dev, b.q.size)
+    dev.dispatch(b.op(OpCode.PrefixAttention, scale=0.125), [put_f32(dev, b.q), *refs[0], refs[1]],
+                 [x, *b.described(), b.state()], [out], [x], [2, 0])
+    check(get(dev, out).reshape(b.tokens, -1), b, scale=0.125)
+
+
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_prefix_with_a_value_that_is_not_finite_in_one_sequence(dev, value):
+    b = Batch([(40, 1), (50, 1), (41, 1)], prefix=40, page=8, heads=4, kv_heads=2, dim=64)
+    put_values(b, [(1, 45, 1, value)])
+    got = attend(dev, b)
+    want, tol = b.attention(0.125)
+    assert np.all(np.abs(got[[0, 2]] - want[[0, 2]]) <= tol[[0, 2]])
+    assert not np.any(np.isfinite(got[1]))
+
+
+# ------------------------------------------------------- the device's manner
+
+@pytest.mark.parametrize("prefix", [0, 64])
+def test_results_do_not_depend_on_the_run(dev, prefix):
+    b = Batch([(5000, 1), (64, 1), (900, 3), (300, 60)], prefix=prefix, heads=8, kv_heads=2, dim=128, layers=1, layer=0)
+    refs = upload(dev, b)
+    first = attend(dev, b, refs=refs)
+    for _ in range(5):
+        assert np.array_equal(first, attend(dev, b, refs=refs))
+
+
+def test_empty_calls(dev):
+    for lens, pad in ([], 0), ([(5, 0)], 0), ([(5, 0), (3, 0)], 2):
+        b = Batch(lens, pad=pad)
+        tables, cache = upload(dev, b)
+        x, y = Value.f32((b.tokens, b.heads * b.dim)), Value.f32((b.tokens, b.kv_heads * b.dim))
+        out = new_f32(dev, b.q.size, 7.5)
+        for code, scalars in (OpCode.PagedAttention, [0, 0, 0]), (OpCode.PrefixAttention, [0, 0]):
+            dev.dispatch(b.op(code, scale=1.0), [put_f32(dev, b.q), *tables, cache],
+                         [x, *b.described(), b.state()], [out], [x], scalars)
+        dev.dispatch(b.append_op(), [put_f32(dev, b.k), put_f32(dev, b.v), *tables, cache],
+                     [y, y, *b.described(), b.state()], [], [])
+        assert np.all(get(dev, out) == 7.5)
+
+
+def test_refusals_leave_the_device_usable(dev):
+    b = Batch([(20, 3), (5, 1)])
+    refs = upload(dev, b)
+    bad = b.table.copy()
+    bad[0, 0] = b.pages
+    with pytest.raises(DeviceError, match="page id out of range"):
+        attend(dev, b, refs=([put_u32(dev, bad), *refs[0][1:]], refs[1]))
+    with pytest.raises(DeviceError, match="max_new"):
+        attend(dev, b, refs=refs, max_new=2)
+    check(attend(dev, b, refs=refs), b)
+
+
+def test_small_workspace_is_refused():
+    d = CudaDevice(0, workspace_bytes=1 << 20)
+    try:
+        b = Batch([(20, 3)])
+        with pytest.raises(DeviceError, match="workspace is too small"):
+            attend(d, b)
+    finally:
+        d.close()
+
+
+def test_two_devices_on_one_gpu(dev):
+    # Separate streams and workspaces: both run the same batch at once.
+    other = CudaDevice(0)
+    try:
+        b = Batch([(4000, 1), (700, 2)], heads=8, kv_heads=2, dim=128, layers=1, layer=0)
+        sides = []
+        for d in (dev, other):
+            tables, cache = upload(d, b)
+            x = Value.f32((b.tokens, b.heads * b.dim))
+            out = new_f32(d, b.q.size)
+            cmd = d.command(b.op(OpCode.PagedAttention, scale=0.088), [put_f32(d, b.q), *tables, cache],
+                            [x, *b.described(), b.state()], [out], [x], [2, 0, 0])
+            sides.append((d, cmd, out))
+        for _ in range(20):
+            for _, cmd, _ in sides:
+                cmd()
+        for d, _, out in sides:
+            check(get(d, out).reshape(b.tokens, -1), b, scale=0.088)
+    finally:
+        other.close()
+
+
+class Server:
+    """A decoding loop over two layers as a serving program writes it: per
+    layer PagedAppend, Rope of the queries, attention; the batch's description
+    uploaded once per step."""
+
+    def __init__(self, dev, heads, kv_heads, dim, page, seqs, width, pages, dtype, prefix=0, shape=None):
+        self.dev, self.n, self.prefix, self.dtype = dev, seqs, prefix, dtype
+        self.heads, self.kv_heads, self.dim = heads, kv_heads, dim
+        self.shape = (pages, 2, 2, page, kv_heads, dim)
+        state = Value(dtype, self.shape, ValueRole.State)
+        self.cache = new_f32(dev, state_words(self.shape, dtype))
+        self.table, self.past, self.starts, self.pos = (
+            put_u32(dev, np.zeros(s)) for s in ((seqs, width), seqs, seqs + 1, seqs))
+        described = [Value.u32((seqs, width)), Value.u32((seqs,)), Value.u32((seqs + 1,))]
+        ports = [self.table, self.past, self.starts]
+        x, y = Value.f32((seqs, heads * dim)), Value.f32((seqs, kv_heads * dim))
+        r = Value.f32((seqs, heads, 1, dim))
+        self.q, self.k, self.v, self.turned, self.out = [], [], [], [], []
+        self.commands = []
+        code = OpCode.PrefixAttention if prefix else OpCode.PagedAttention
+        scalars = [1, prefix] if prefix else [1, 0, 0]
+        for layer in range(2):
+            q, k, v = new_f32(dev, seqs * heads * dim), new_f32(dev, seqs * kv_heads * dim), new_f32(
+                dev, seqs * kv_heads * dim)
+            turned, out = new_f32(dev, seqs * heads * dim), new_f32(dev, seqs * heads * dim)
+            attrs = dict(layer=layer, heads=heads, kv_heads=kv_heads, head_dim=dim)
+            self.commands += [
+                dev.command(Op(OpCode.PagedAppend, theta=500000.0, **attrs), [k, v, *ports, self.cache],
+                            [y, y, *described, state], [], []),
+                dev.command(Op(OpCode.Rope, theta=500000.0), [q, self.pos], [r, Value.u32((seqs, 1))], [turned], [r]),
+                dev.command(Op(code, scale=1 / math.sqrt(dim), **attrs), [turned, *ports, self.cache],
+                            [x, *described, state], [out], [x], scalars)]
+            for name, ref in zip(("q", "k", "v", "turned", "out"), (q, k, v, turned, out)):
+                getattr(self, name).append(ref)
+
+    def step(self, table, past, qkv):
+        d = self.dev
+        d.upload_u32(self.table.buffer, table)
+        d.upload_u32(self.past.buffer, past)
+        d.upload_u32(self.starts.buffer, np.arange(self.n + 1))
+        d.upload_u32(self.pos.buffer, past)
+        for layer, (q, k, v) in enumerate(qkv):
+            d.upload_f32(self.q[layer].buffer, q)
+            d.upload_f32(self.k[layer].buffer, k)
+            d.upload_f32(self.v[layer].buffer, v)
+        for cmd in self.commands:
+            cmd()
+        d.synchronize()
+        return [get(d, o).reshape(self.n, -1) for o in self.out]
+
+
+@pytest.mark.parametrize("prefix", [0, 24])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_decoding_captured_and_replayed(dtype, prefix):
+    # Three sequences of different lengths decode 12 steps; the captured run
+    # replays one graph while lengths and tables change, and gives what the
+    # eager one gives, bit for bit.
+    heads, kv_heads, dim, page, steps = 8, 2, 64, 8, 12
+    rng = np.random.RandomState(3)
+    table = np.full((3, 8), 63, np.uint32)
+    table[:, :3] = [4, 9, 2]
+    free = iter(rng.permutation(np.arange(10, 60)))
+    for b in range(3):
+        table[b, 3:] = [next(free) for _ in range(5)]
+    results, replays = [], []
+    for capture in (False, True):
+        d = CudaDevice(0)
+        try:
+            d.set_capture(capture)
+            s = Server(d, heads, kv_heads, dim, page, 3, 8, 64, dtype, prefix)
+            r = np.random.RandomState(5)
+            past = np.array([24, 31, 26], np.uint32)
+            fill = r.randn(int(np.prod(s.shape))).astype(np.float32)
+            d.upload_f32(s.cache.buffer, to_bits(fill, dtype)[1])
+            outs = []
+            for i in range(steps):
+                qkv = [(r.randn(3, heads * dim), r.randn(3, kv_heads * dim), r.randn(3, kv_heads * dim))
+                       for _ in range(2)]
+                outs.append(s.step(table, past, qkv))
+                past = past + 1
+            results.append((outs, get(d, s.cache)))
+            replays.append(d.capture_stats()["replays"])
+        finally:
+            d.close()
+    assert replays[0] == 0 and replays[1] >= steps - 3
+    for a, b in zip(results[0][0], results[1][0]):
+        assert all(np.array_equal(x, y) for x, y in zip(a, b))
+    assert np.array_equal(results[0][1].view(np.uint32), results[1][1].view(np.uint32))
+
+
+def test_decoding_matches_the_dense_cache(dev):
+    # The same tokens through Rope, CausalAttention and a dense cache, one
+    # sequence at a time.
+    heads, kv_heads, dim, page, steps, width = 4, 2, 64, 4, 9, 4
+    s = Server(dev, heads, kv_heads, dim, page, 2, width, 16, F32)
+    table = np.array([[3, 8, 1, 15], [7, 2, 9, 4]], np.uint32)
+    r = np.random.RandomState(8)
+    max_seq = width * page
+    dense = [new_f32(dev, 2 * 2 * max_seq * kv_heads * dim) for _ in range(2)]
+    state = Value.f32((1, 2, 2, max_seq, kv_heads, dim), ValueRole.State)
+    for i in range(steps):
+        past = np.array([i, i], np.uint32)
+        qkv = [[r.randn(2, n * dim).astype(np.float32) for n in (heads, kv_heads, kv_heads)] for _ in range(2)]
+        got = s.step(table, past, qkv)
+        for b in range(2):
+            pos = put_u32(dev, [i])
+            for layer, (q, k, v) in enumerate(qkv):
+                x, y = Value.f32((1, heads, 1, dim)), Value.f32((1, kv_heads, 1, dim))
+                tq, tk, out = new_f32(dev, heads * dim), new_f32(dev, kv_heads * dim), new_f32(dev, heads * dim)
+                for val, src, dst in (x, q, tq), (y, k, tk):
+                    dev.dispatch(Op(OpCode.Rope, theta=500000.0), [put_f32(dev, src[b]), pos],
+                                 [val, Value.u32((1, 1))], [dst], [val])
+                dev.dispatch(Op(OpCode.CausalAttention, layer=layer, heads=heads, kv_heads=kv_heads, head_dim=dim,
+                                scale=1 / math.sqrt(dim)), [tq, tk, put_f32(dev, v[b]), dense[b]],
+                             [x, y, y, state], [out], [x], [i])
+                # Both are within 2^-14 of the definition (values up to 4).
+                assert np.all(np.abs(get(dev, out) - got[layer][b]) <= 2.0 ** -13)
+    # The caches agree bit for bit.
+    paged = get(dev, s.cache).reshape(s.shape)
+    for b in range(2):
+        rows = paged[table[b].astype(np.int64)].transpose(1, 2, 0, 3, 4, 5).reshape(2, 2, max_seq, kv_heads, dim)
+        assert np.array_equal(rows[:, :, :steps], get(dev, dense[b]).reshape(2, 2, max_seq, kv_heads, dim)[:, :, :steps])
