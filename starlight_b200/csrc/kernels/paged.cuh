@@ -4,6 +4,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "tma.cuh"
@@ -40,6 +42,110 @@ __device__ __forceinline__ int paged_sequence_of(const PagedBatch &batch, uint32
     }
     return lo;
 }
+
+// One pass of the attention: the rows of each sequence against its own keys,
+// or all rows against the shared prefix.
+struct PagedPass {
+    PagedAttention a;
+    int prefix_pass;  // one segment list over all rows, keys [0, prefix), no mask
+    int first;        // keys below it are left out (a prefix pass saw them)
+    float *pre_o;     // [tokens * heads][head_dim] unnormalised, and
+    float *pre_ml;    // [tokens * heads][2]: written by the prefix pass, merged by the other
+    float *part_o;    // pieces of segments: unnormalised outputs, and
+    float *part_ml;   // their (m, l)
+    float scale_log2;
+    // Sequences of more query rows per kv head (tokens * group) than this go
+    // to paged_rows_kernel, the others to paged_attention_kernel.
+    int small_rows;
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// 16 bytes of a cache row as floats, and one element of it.
+template <typename T>
+struct Frag;
+template <>
+struct Frag<float> {
+    __device__ static __forceinline__ void ld(const void *p, float (&x)[4]) {
+        const float4 v = *reinterpret_cast<const float4 *>(p);
+        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+    }
+    __device__ static __forceinline__ float get(const void *p) { return *static_cast<const float *>(p); }
+};
+template <>
+struct Frag<__nv_bfloat16> {
+    __device__ static __forceinline__ void ld(const void *p, float (&x)[8]) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    __device__ static __forceinline__ float get(const void *p) {
+        return __bfloat162float(*static_cast<const __nv_bfloat16 *>(p));
+    }
+};
+template <>
+struct Frag<__half> {
+    __device__ static __forceinline__ void ld(const void *p, float (&x)[8]) {
+        const uint4 v = *reinterpret_cast<const uint4 *>(p);
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        }
+    }
+    __device__ static __forceinline__ float get(const void *p) {
+        return __half2float(*static_cast<const __half *>(p));
+    }
+};
+
+// One query row against the keys i in [k0, k1) for which pos(i) is not
+// negative, in plain f32, by one warp: for rows whose tiles hold values that
+// are not finite. o[y]: dimension lane + 32 y, unnormalised; m in log2 units.
+template <typename T, int DP, typename Pos>
+__device__ __noinline__ void plain_row(const PagedPass &p, const float *q, int b, int kvh, int k0, int k1, Pos pos,
+                                       float &m, float &l, float (&o)[DP / 32]) {
+    const int lane = threadIdx.x & 31, D = p.a.head_dim;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int y = 0; y < DP / 32; y++) o[y] = 0.f;
+    for (int i = k0; i < k1; i++) {
+        const int at = pos(i);
+        if (at < 0) continue;
+        const char *src = p.a.cache.base + paged_row(p.a.cache, p.a.batch, b, at, p.a.err) +
+                          (long long)kvh * D * (int)sizeof(T);
+        float dot = 0.f;
+        for (int d = lane; d < D; d += 32) dot = fmaf(q[d], Frag<T>::get(src + d * sizeof(T)), dot);
+        const float x = warp_sum(dot) * p.scale_log2;
+        const float nm = fmaxf(m, x), f = m == -INFINITY ? 0.f : ex2(m - nm);
+        const float e = x == -INFINITY ? 0.f : ex2(x - nm);
+        l = m == -INFINITY ? l + e : fmaf(l, f, e);
+#pragma unroll
+        for (int y = 0; y < DP / 32; y++) {
+            const int d = lane + 32 * y;
+            const float v = d < D ? Frag<T>::get(src + p.a.cache.parity_stride + d * sizeof(T)) : 0.f;
+            o[y] = fmaf(e, v, m == -INFINITY ? o[y] : o[y] * f);
+        }
+        m = nm;
+    }
+}
+
+// paged_rows.cu: the pass on the tensor cores, 128 query rows at a time.
+bool paged_rows_supported(const PagedAttention &a);
+size_t paged_rows_part_floats(const PagedAttention &a);
+cudaError_t paged_rows(cudaStream_t s, const PagedPass &p);
 
 }  // namespace k
 }  // namespace slc

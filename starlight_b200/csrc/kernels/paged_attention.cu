@@ -37,6 +37,8 @@
 // split of an infinity is NaN).
 #include <math.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.cuh"
@@ -51,18 +53,7 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;
 constexpr int kWarpKeys = 16;
 constexpr int kTileKeys = kWarps * kWarpKeys;
-constexpr float kLog2e = 1.4426950408889634f;
-
-struct AttnArgs {
-    PagedAttention a;
-    int prefix_pass;  // one segment list over all rows, keys [0, prefix), no mask
-    int first;        // keys below it are left out (a prefix pass saw them)
-    float *pre_o;     // [tokens * heads][head_dim] unnormalised, and
-    float *pre_ml;    // [tokens * heads][2]: written by the prefix pass, merged by the other
-    float *part_o;    // [2 * grid][kRows][DP]
-    float *part_ml;   // [2 * grid][kRows][2]
-    float scale_log2;
-};
+constexpr int kSmallRows = 32;  // query rows per kv head taken here; more go to paged_rows.cu
 
 template <typename T, int DP>
 struct Cfg {
@@ -88,7 +79,7 @@ struct Cursor {
     int tiles, kvh, rb, tile;
 };
 
-__device__ __forceinline__ void seq_load(const AttnArgs &p, int b, Cursor &c) {
+__device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor &c) {
     c.b = b;
     if (p.prefix_pass) {
         c.b = paged_sequence_of(p.a.batch, 0);  // the first with tokens: its table row
@@ -101,6 +92,7 @@ __device__ __forceinline__ void seq_load(const AttnArgs &p, int b, Cursor &c) {
     } else {
         c.tok0 = (int)p.a.batch.starts[b];
         c.ntok = (int)p.a.batch.starts[b + 1] - c.tok0;
+        if ((long long)c.ntok * (p.a.heads / p.a.kv_heads) > p.small_rows) c.ntok = 0;
         c.past = (int)p.a.batch.past[b];
         c.sink = 0;
         c.low = p.first;
@@ -112,13 +104,13 @@ __device__ __forceinline__ void seq_load(const AttnArgs &p, int b, Cursor &c) {
     }
     c.tiles = (c.keys + kTileKeys - 1) / kTileKeys;
 }
-__device__ __forceinline__ long long seq_units(const AttnArgs &p, const Cursor &c) {
+__device__ __forceinline__ long long seq_units(const PagedPass &p, const Cursor &c) {
     const long long rb = (c.ntok * (long long)(p.a.heads / p.a.kv_heads) + kRows - 1) / kRows;
     return c.ntok > 0 ? rb * p.a.kv_heads * c.tiles : 0;
 }
 
 // Places the cursor on unit `at` counted from the start of sequence c.b.
-__device__ __forceinline__ void cursor_at(const AttnArgs &p, Cursor &c, long long at) {
+__device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor &c, long long at) {
     const int seqs = p.prefix_pass ? 1 : p.a.batch.seqs;
     long long n = seq_units(p, c);
     while (!p.prefix_pass && at >= n && c.b + 1 < seqs) {
@@ -133,7 +125,7 @@ __device__ __forceinline__ void cursor_at(const AttnArgs &p, Cursor &c, long lon
     c.kvh = (int)(seg - (long long)c.rb * p.a.kv_heads);
 }
 
-__device__ __forceinline__ void cursor_next(const AttnArgs &p, Cursor &c) {
+__device__ __forceinline__ void cursor_next(const PagedPass &p, Cursor &c) {
     if (--c.left == 0) {
         cursor_at(p, c, seq_units(p, c));
         return;
@@ -159,62 +151,12 @@ __device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x)
 __device__ __forceinline__ uint32_t tf32_lo(float x, uint32_t hi) {
     return __float_as_uint(x - __uint_as_float(hi));
 }
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
-
-// One 128-bit shared load as kEpl floats.
-template <typename T>
-struct Frag;
-template <>
-struct Frag<float> {
-    __device__ static __forceinline__ void ld(const void *p, float (&x)[4]) {
-        const float4 v = *reinterpret_cast<const float4 *>(p);
-        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-    }
-    __device__ static __forceinline__ float get(const void *p) { return *static_cast<const float *>(p); }
-};
-template <>
-struct Frag<__nv_bfloat16> {
-    __device__ static __forceinline__ void ld(const void *p, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x[2 * i] = __uint_as_float(w[i] << 16);
-            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-        }
-    }
-    __device__ static __forceinline__ float get(const void *p) {
-        return __bfloat162float(*static_cast<const __nv_bfloat16 *>(p));
-    }
-};
-template <>
-struct Frag<__half> {
-    __device__ static __forceinline__ void ld(const void *p, float (&x)[8]) {
-        const uint4 v = *reinterpret_cast<const uint4 *>(p);
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
-        }
-    }
-    __device__ static __forceinline__ float get(const void *p) {
-        return __half2float(*static_cast<const __half *>(p));
-    }
-};
-
 // Position of compressed key index i.
 __device__ __forceinline__ int key_pos(const Cursor &c, int i) {
     return i < c.sink ? i : i - c.sink + c.low;
 }
 // Whether row position `at` sees key index i.
-__device__ __forceinline__ bool sees(const AttnArgs &p, const Cursor &c, int i, int at) {
+__device__ __forceinline__ bool sees(const PagedPass &p, const Cursor &c, int i, int at) {
     if (i >= c.keys) return false;
     if (p.prefix_pass) return true;
     const int pos = key_pos(c, i);
@@ -222,7 +164,7 @@ __device__ __forceinline__ bool sees(const AttnArgs &p, const Cursor &c, int i, 
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ AttnArgs p) {
+__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ PagedPass p) {
     using C = Cfg<T, DP>;
     constexpr int EPL = C::kEpl, KB = DP / C::kKBlk, VB = DP / C::kVBlk, NT = DP / 16;
     extern __shared__ __align__(128) unsigned char smem[];
@@ -421,20 +363,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         pr[1] = ex2(sc[1] - u_1);
         pr[2] = ex2(sc[2] - u_0);
         pr[3] = ex2(sc[3] - u_1);
-        if (__any_sync(0xffffffffu, n0 != m0 || n1 != m1)) {
-            const float f0 = ex2(m0 - u_0), f1 = ex2(m1 - u_1);
-            l0 *= f0;
-            l1 *= f1;
-#pragma unroll
-            for (int i = 0; i < NT; i++) {
-                acc[i][0] *= f0;
-                acc[i][1] *= f1;
-                acc[i][2] *= f0;
-                acc[i][3] *= f1;
-            }
-            m0 = n0;
-            m1 = n1;
-        }
+        const float f0 = ex2(m0 - u_0), f1 = ex2(m1 - u_1);
+        l0 *= f0;
+        l1 *= f1;
+        m0 = n0;
+        m1 = n1;
         l0 += pr[0] + pr[2];
         l1 += pr[1] + pr[3];
         // P as the B fragments of the two 8-key steps: row g, keys t and t + 4.
@@ -450,30 +383,46 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
                 bh[ks8][x] = tf32_hi(v);
                 bl[ks8][x] = tf32_lo(v, bh[ks8][x]);
             }
+        // The tile's P V starts from zero and is added to the running output
+        // outside the tensor core, whose accumulation truncates: over
+        // thousands of keys that bias would grow past f32 rounding.
 #pragma unroll
-        for (int ks8 = 0; ks8 < 2; ks8++)
+        for (int j = 0; j < VB; j++) {
+            float o[EPL / 2][4];
 #pragma unroll
-            for (int j = 0; j < VB; j++) {
+            for (int x = 0; x < EPL / 2; x++)
+#pragma unroll
+                for (int z = 0; z < 4; z++) o[x][z] = 0.f;
+#pragma unroll
+            for (int ks8 = 0; ks8 < 2; ks8++) {
                 float va[EPL], vb[EPL];
                 Frag<T>::ld(vs + (8 * ks8 + t) * C::kVStride + (j * C::kVBlk + EPL * g) * sizeof(T), va);
                 Frag<T>::ld(vs + (8 * ks8 + t + 4) * C::kVStride + (j * C::kVBlk + EPL * g) * sizeof(T), vb);
 #pragma unroll
                 for (int x = 0; x < EPL / 2; x++) {
                     const float f[4] = {va[2 * x], va[2 * x + 1], vb[2 * x], vb[2 * x + 1]};
-                    float(&o)[4] = acc[j * (EPL / 2) + x];
                     uint32_t hi[4];
 #pragma unroll
                     for (int z = 0; z < 4; z++) hi[z] = sizeof(T) == 4 ? tf32_hi(f[z]) : __float_as_uint(f[z]);
-                    mma_tf32(o, hi, bl[ks8][0], bl[ks8][1]);
+                    mma_tf32(o[x], hi, bl[ks8][0], bl[ks8][1]);
                     if (sizeof(T) == 4) {
                         uint32_t lo[4];
 #pragma unroll
                         for (int z = 0; z < 4; z++) lo[z] = tf32_lo(f[z], hi[z]);
-                        mma_tf32(o, lo, bh[ks8][0], bh[ks8][1]);
+                        mma_tf32(o[x], lo, bh[ks8][0], bh[ks8][1]);
                     }
-                    mma_tf32(o, hi, bh[ks8][0], bh[ks8][1]);
+                    mma_tf32(o[x], hi, bh[ks8][0], bh[ks8][1]);
                 }
             }
+#pragma unroll
+            for (int x = 0; x < EPL / 2; x++) {
+                float(&a)[4] = acc[j * (EPL / 2) + x];
+                a[0] = fmaf(a[0], f0, o[x][0]);
+                a[1] = fmaf(a[1], f1, o[x][1]);
+                a[2] = fmaf(a[2], f0, o[x][2]);
+                a[3] = fmaf(a[3], f1, o[x][3]);
+            }
+        }
         __syncwarp();
         done++;
         if (issued < units && !*abort) {
@@ -545,28 +494,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
                 if (!((*bad_s >> r) & 1)) continue;
                 const int row = cc.rb * kRows + r, tok = row / G, at = cc.past + tok;
                 const float *q = p.a.q + ((size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G)) * D;
-                float mm = -INFINITY, ll = 0.f, o[DP / 32];
-#pragma unroll
-                for (int x = 0; x < DP / 32; x++) o[x] = 0.f;
-                for (int i = k0; i < k1; i++) {
-                    if (!sees(p, cc, i, at)) continue;
-                    const char *src = p.a.cache.base +
-                                      paged_row(p.a.cache, p.a.batch, cc.b, key_pos(cc, i), p.a.err) +
-                                      (long long)cc.kvh * row_bytes;
-                    float dot = 0.f;
-                    for (int d = lane; d < D; d += 32) dot = fmaf(q[d], Frag<T>::get(src + d * sizeof(T)), dot);
-                    const float x = warp_sum(dot) * p.scale_log2;
-                    const float nm = fmaxf(mm, x), f = mm == -INFINITY ? 0.f : ex2(mm - nm);
-                    const float e = x == -INFINITY ? 0.f : ex2(x - nm);
-                    ll = fmaf(ll, f, e);
-#pragma unroll
-                    for (int y = 0; y < DP / 32; y++) {
-                        const int d = lane + 32 * y;
-                        const float v = d < D ? Frag<T>::get(src + p.a.cache.parity_stride + d * sizeof(T)) : 0.f;
-                        o[y] = fmaf(e, v, mm == -INFINITY ? 0.f : o[y] * f);
-                    }
-                    mm = nm;
-                }
+                float mm, ll, o[DP / 32];
+                plain_row<T, DP>(
+                    p, q, cc.b, cc.kvh, k0, k1, [&](int i) { return sees(p, cc, i, at) ? key_pos(cc, i) : -1; }, mm,
+                    ll, o);
 #pragma unroll
                 for (int y = 0; y < DP / 32; y++) mo[r * C::kMergeStride + lane + 32 * y] = o[y];
                 if (lane == 0) {
@@ -684,7 +615,7 @@ size_t prefix_floats(const PagedAttention &a) {
 }
 
 template <typename T, int DP>
-cudaError_t launch_pass(cudaStream_t s, const AttnArgs &p) {
+cudaError_t launch_pass(cudaStream_t s, const PagedPass &p) {
     using C = Cfg<T, DP>;
     static_assert(C::kSmem <= 227 * 1024, "shared layout");
     static std::atomic<uint64_t> smem_set{0};
@@ -695,7 +626,7 @@ cudaError_t launch_pass(cudaStream_t s, const AttnArgs &p) {
 }
 
 template <typename T>
-cudaError_t launch_dim(cudaStream_t s, const AttnArgs &p) {
+cudaError_t launch_dim(cudaStream_t s, const PagedPass &p) {
     switch (padded_dim(p.a.head_dim)) {
     case 64: return launch_pass<T, 64>(s, p);
     case 128: return launch_pass<T, 128>(s, p);
@@ -703,7 +634,7 @@ cudaError_t launch_dim(cudaStream_t s, const AttnArgs &p) {
     }
 }
 
-cudaError_t launch_type(cudaStream_t s, const AttnArgs &p) {
+cudaError_t launch_type(cudaStream_t s, const PagedPass &p) {
     switch (p.a.cache.type) {
     case kPagedF16: return launch_dim<__half>(s, p);
     case kPagedBf16: return launch_dim<__nv_bfloat16>(s, p);
@@ -711,29 +642,48 @@ cudaError_t launch_type(cudaStream_t s, const AttnArgs &p) {
     }
 }
 
+// Whether rows * group query rows of one kv head are too many for
+// paged_attention_kernel, which reads the keys once per kRows of them.
+bool many_rows(const PagedAttention &a, size_t rows) {
+    return paged_rows_supported(a) && rows * (size_t)(a.heads / a.kv_heads) > (size_t)kSmallRows;
+}
+
+size_t part_floats(const PagedAttention &a) {
+    const size_t few = partial_floats(padded_dim(a.head_dim));
+    const bool rows = many_rows(a, a.max_new) || (a.prefix && many_rows(a, a.tokens));
+    return rows ? std::max(few, paged_rows_part_floats(a)) : few;
+}
+
 }  // namespace
 
 size_t paged_attention_workspace_bytes(const PagedAttention &a) {
-    return (partial_floats(padded_dim(a.head_dim)) + prefix_floats(a)) * sizeof(float);
+    return (part_floats(a) + prefix_floats(a)) * sizeof(float);
 }
 
 cudaError_t paged_attention(cudaStream_t s, const PagedAttention &a) {
     if (a.tokens == 0 || a.batch.seqs == 0) return cudaSuccess;
     if (paged_attention_workspace_bytes(a) > a.workspace_bytes) return cudaErrorMemoryAllocation;
-    const int dp = padded_dim(a.head_dim);
-    AttnArgs p{};
+    PagedPass p{};
     p.a = a;
     p.scale_log2 = a.scale * kLog2e;
     p.part_o = static_cast<float *>(a.workspace);
-    p.part_ml = p.part_o + (size_t)2 * kSmCount * kRows * dp;
+    p.part_ml = p.part_o + (size_t)2 * kSmCount * kRows * padded_dim(a.head_dim);
+    p.small_rows = INT32_MAX;
+    cudaError_t e = cudaSuccess;
     if (a.prefix) {
-        p.pre_o = p.part_ml + (size_t)2 * kSmCount * kRows * 2;
+        p.pre_o = p.part_o + part_floats(a);
         p.pre_ml = p.pre_o + (size_t)a.tokens * a.heads * a.head_dim;
         p.prefix_pass = 1;
-        const cudaError_t e = launch_type(s, p);
+        e = many_rows(a, a.tokens) ? paged_rows(s, p) : launch_type(s, p);
         if (e != cudaSuccess) return e;
         p.prefix_pass = 0;
         p.first = a.prefix;
+    }
+    // Sequences with many rows first, those with few after them.
+    if (many_rows(a, a.max_new)) {
+        p.small_rows = kSmallRows;
+        e = paged_rows(s, p);
+        if (e != cudaSuccess) return e;
     }
     return launch_type(s, p);
 }

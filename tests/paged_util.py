@@ -30,6 +30,11 @@ def from_bits(words, shape, dtype):
     return raw.view(torch.float16 if dtype == DType.F16 else torch.bfloat16).double().numpy().reshape(shape)
 
 
+def dim_sum(k, q):
+    """The sizes that the smallest steps of f16 pairs multiply in q . k."""
+    return np.abs(k).max() * np.abs(q).sum() + np.abs(q).max() * np.abs(k).sum(1).max()
+
+
 class Batch:
     """Sequences of (past, new) over a paged cache of random values; every
     slot that no sequence holds is NaN, every table entry past a sequence's
@@ -96,7 +101,9 @@ class Batch:
                     w = np.exp(s - s.max())
                     out[row, h] = (w / w.sum()) @ vv
                     ds = 8 * 2.0 ** -20 * abs(scale) * (np.abs(kk) @ np.abs(q)).max()
+                    ds += 2.0 ** -38 * abs(scale) * dim_sum(kk, q)
                     tol[row, h] = (w / w.sum()) @ np.abs(vv) * (2 * ds + (8 + len(pos) / 64) * 2.0 ** -20)
+                    tol[row, h] += 2.0 ** -38 * np.abs(vv).max()
         return out.reshape(self.tokens, -1), tol.reshape(self.tokens, -1)
 
     # ---- ports -----------------------------------------------------------
