@@ -113,6 +113,14 @@ struct PagedCache {
     long long parity_stride;  // keys to values
     long long row_stride;     // position to position
     int type, page, pages;
+    // pos / page == (umulhi(pos, page_mul) + pos) >> page_shift for pos < 2^31.
+    uint32_t page_mul, page_shift;
+    void set_page(int n) {
+        page = n;
+        page_shift = 0;
+        while ((1ull << page_shift) < (uint64_t)n) page_shift++;
+        page_mul = (uint32_t)(((1ull << 32) * ((1ull << page_shift) - (uint64_t)n)) / (uint64_t)n + 1);
+    }
 };
 // A ragged batch: sequence b owns rows starts[b] .. starts[b + 1] of the
 // token-major inputs, at positions past[b] onward; table[b] names its pages.

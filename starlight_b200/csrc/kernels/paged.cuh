@@ -13,13 +13,18 @@
 namespace slc {
 namespace k {
 
+// pos / page by a multiplication (set_page below).
+__device__ __forceinline__ int page_of(const PagedCache &c, int pos) {
+    return (int)((__umulhi((uint32_t)pos, c.page_mul) + (uint32_t)pos) >> c.page_shift);
+}
+
 // Byte offset (from cache.base) of the key row of position `pos` of sequence
 // `b`, head 0. The host has checked every page id that a position in use
 // names; the guard keeps a wrong one from leaving the cache (page 0 then
 // stands in, and the device error word is set).
 __device__ __forceinline__ long long paged_row(const PagedCache &c, const PagedBatch &batch, int b,
                                                int pos, uint32_t *err) {
-    const int pg = pos / c.page, off = pos - pg * c.page;
+    const int pg = page_of(c, pos), off = pos - pg * c.page;
     uint32_t id = 0;
     if (pg < batch.per_seq) id = batch.table[(long long)b * batch.per_seq + pg];
     if (pg >= batch.per_seq || id >= (uint32_t)c.pages) {
@@ -66,6 +71,13 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) < INFINITY; }
+
+// Powers of two that bring the largest magnitude of a set (its bits) to
+// [2^k, 2^(k + 1)): the scale is pow2(k - scale_exponent(bits)).
+__device__ __forceinline__ int scale_exponent(uint32_t bits) {
+    return bits ? max((int)(bits >> 23) - 127, -100) : 0;
+}
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // 16 bytes of a cache row as floats, and one element of it.
 template <typename T>

@@ -17,20 +17,26 @@
 // on the order of execution.
 //
 // A tile is 16 keys for each of the CTA's warps. A warp fetches its keys and
-// values row by row (one bulk copy per row and lane) into a ring of its own,
-// kStages tiles ahead and across segment borders, and shares nothing with the
-// other warps until the segment's end, where the warps' m, l and o merge in
-// shared memory.
+// values with 16-byte asynchronous copies into a ring of its own, kStages
+// tiles ahead and across segment borders (bulk copies of single rows, 256 or
+// 512 bytes, were bound by the copy unit: about 35 cycles each), and shares
+// nothing with the other warps until the segment's end, where the warps' m, l
+// and o merge in shared memory.
 //
-// Arithmetic. mma.sync m16n8k8 on tf32 pairs: x = hi + lo with hi the top 11
-// significant bits and lo the rest, three products (hi hi, hi lo, lo hi) for
-// an F32 cache: 2^-21 relative, f32 accumulators. F16 and BF16 values are
-// exact as one tf32, two products. The tiles are transposed (S^T = K Q^T,
-// O^T = V^T P^T), so that the 16 of the MMA are keys and dimensions and the 8
-// are query rows: decode has 1 to 8 rows per kv head (GQA), and rows beyond
-// that would be padding. Dimensions and keys inside a tile are permuted so
-// that every fragment is one 128-bit shared load without bank conflicts (row
-// strides of 16 mod 32 words for keys, 8 mod 32 for values).
+// Arithmetic. The tiles are transposed (S^T = K Q^T, O^T = V^T P^T), so that
+// the 16 of the MMA are keys and dimensions and the 8 are query rows: decode
+// has 1 to 8 rows per kv head (GQA), and rows beyond that would be padding.
+//   F32   m16n8k8 on tf32 pairs: x = hi + lo with hi rounded to 11 bits, three
+//         products (lo hi, hi lo, hi hi), 2^-21 relative. Dimensions and keys
+//         inside a tile are permuted so that a fragment is one 128-bit shared
+//         load without bank conflicts.
+//   F16   m16n8k16; keys and values are exact, queries (each row scaled by a
+//         power of two to 2^14) and probabilities (times 2^14) are pairs of
+//         f16, 22 bits, two products.
+//   BF16  m16n8k16; queries and probabilities are three bf16, 24 bits, three
+//         products.
+// The probabilities of a tile turn from S^T's accumulator layout into B
+// fragments by shuffles (F32) or movmatrix (16 bit), without shared memory.
 //
 // Rows that meet a NaN or an infinity are recomputed in plain f32 over the
 // keys that they see alone (the MMA multiplies masked values by zero, and the
@@ -48,29 +54,36 @@ namespace slc {
 namespace k {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 8;
 constexpr int kWarpKeys = 16;
-constexpr int kTileKeys = kWarps * kWarpKeys;
 constexpr int kSmallRows = 32;  // query rows per kv head taken here; more go to paged_rows.cu
 
 template <typename T, int DP>
 struct Cfg {
-    static constexpr int kEpl = 16 / (int)sizeof(T);  // elements of a 128-bit shared load
-    static constexpr int kKBlk = 4 * kEpl;             // dims per K fragment block
-    static constexpr int kVBlk = 8 * kEpl;             // dims per V fragment block
-    static constexpr int kKStride = DP * (int)sizeof(T) + 64;
-    static constexpr int kVStride = DP * (int)sizeof(T) + 32;
+    static constexpr bool kHalf = sizeof(T) == 2;
+    static constexpr int kWarps = !kHalf && DP == 256 ? 4 : 8;
+    static constexpr int kThreads = kWarps * 32;
+    static constexpr int kTileKeys = kWarps * kWarpKeys;
+    static constexpr int kTerms = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;  // of a query or probability
+    static constexpr int kShift = std::is_same<T, __half>::value ? 14 : 0;        // f16: scaled by 2^14
+    static constexpr int kEpl = 16 / (int)sizeof(T);  // elements of 16 bytes
+    static constexpr int kLpr = DP / kEpl;             // 16-byte pieces of a cache row
+    // Row strides: 128-bit fragment loads of keys want 16 mod 32 words, of
+    // values 8 mod 32; ldmatrix wants 16 mod 128 bytes.
+    static constexpr int kKStride = DP * (int)sizeof(T) + (kHalf ? 16 : 64);
+    static constexpr int kVStride = DP * (int)sizeof(T) + (kHalf ? 16 : 32);
     static constexpr int kStageBytes = kWarpKeys * (kKStride + kVStride);
     static constexpr int kMergeStride = DP + 4;  // floats
-    static constexpr int kFixed = 2 * kRows * DP * 4 + kWarps * kRows * (kMergeStride + 2) * 4 + 4096;
-    static constexpr int kFit = (220 * 1024 - kFixed) / (kWarps * kStageBytes);
-    static constexpr int kStages = kFit > 4 ? 4 : (kFit < 1 ? 1 : kFit);
+    static constexpr int kQBytes = kRows * DP * (kHalf ? 2 * kTerms : 8);
+    static constexpr int kFixed = kQBytes + kWarps * kRows * (kMergeStride + 2) * 4 + 512;
+    static constexpr int kFit = (224 * 1024 - kFixed) / (kWarps * kStageBytes);
+    static constexpr int kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kSmem = kFixed + kStages * kWarps * kStageBytes;
 };
 
-// Segment and tile of a unit of the work line, walked forward.
+// Segment and tile of a unit of the work line, walked forward (kTile: keys of
+// a tile).
+template <int kTile>
 struct Cursor {
     long long left;  // units of this sequence from the current one on, itself included
     int b;           // sequence
@@ -79,7 +92,8 @@ struct Cursor {
     int tiles, kvh, rb, tile;
 };
 
-__device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor &c) {
+template <int kTile>
+__device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor<kTile> &c) {
     c.b = b;
     if (p.prefix_pass) {
         c.b = paged_sequence_of(p.a.batch, 0);  // the first with tokens: its table row
@@ -102,15 +116,17 @@ __device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor &c) {
         }
         c.keys = c.sink + c.past + c.ntok - c.low;
     }
-    c.tiles = (c.keys + kTileKeys - 1) / kTileKeys;
+    c.tiles = (c.keys + kTile - 1) / kTile;
 }
-__device__ __forceinline__ long long seq_units(const PagedPass &p, const Cursor &c) {
+template <int kTile>
+__device__ __forceinline__ long long seq_units(const PagedPass &p, const Cursor<kTile> &c) {
     const long long rb = (c.ntok * (long long)(p.a.heads / p.a.kv_heads) + kRows - 1) / kRows;
     return c.ntok > 0 ? rb * p.a.kv_heads * c.tiles : 0;
 }
 
 // Places the cursor on unit `at` counted from the start of sequence c.b.
-__device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor &c, long long at) {
+template <int kTile>
+__device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor<kTile> &c, long long at) {
     const int seqs = p.prefix_pass ? 1 : p.a.batch.seqs;
     long long n = seq_units(p, c);
     while (!p.prefix_pass && at >= n && c.b + 1 < seqs) {
@@ -125,7 +141,8 @@ __device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor &c, long lo
     c.kvh = (int)(seg - (long long)c.rb * p.a.kv_heads);
 }
 
-__device__ __forceinline__ void cursor_next(const PagedPass &p, Cursor &c) {
+template <int kTile>
+__device__ __forceinline__ void cursor_next(const PagedPass &p, Cursor<kTile> &c) {
     if (--c.left == 0) {
         cursor_at(p, c, seq_units(p, c));
         return;
@@ -147,148 +164,257 @@ __device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], 
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t tf32_hi(float x) { return __float_as_uint(x) & 0xffffe000u; }
+__device__ __forceinline__ uint32_t tf32_hi(float x) { return (__float_as_uint(x) + 0x1000u) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_lo(float x, uint32_t hi) {
     return __float_as_uint(x - __uint_as_float(hi));
 }
+template <typename T>
+__device__ __forceinline__ void mma_16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if (std::is_same<T, __half>::value)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <bool kTrans>
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    if (kTrans)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(addr)
+                     : "memory");
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t a) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+    return d;
+}
+// (a, b) rounded to a pair of T, a in the low half; a and b become what is left.
+template <typename T>
+__device__ __forceinline__ uint32_t take_pair(float &a, float &b) {
+    if (std::is_same<T, __half>::value) {
+        const __half2 h = __floats2half2_rn(a, b);
+        const float2 f = __half22float2(h);
+        a -= f.x;
+        b -= f.y;
+        return *reinterpret_cast<const uint32_t *>(&h);
+    }
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const uint32_t w = *reinterpret_cast<const uint32_t *>(&h);
+    a -= __uint_as_float(w << 16);
+    b -= __uint_as_float(w & 0xffff0000u);
+    return w;
+}
+
 // Position of compressed key index i.
-__device__ __forceinline__ int key_pos(const Cursor &c, int i) {
+template <int kTile>
+__device__ __forceinline__ int key_pos(const Cursor<kTile> &c, int i) {
     return i < c.sink ? i : i - c.sink + c.low;
 }
 // Whether row position `at` sees key index i.
-__device__ __forceinline__ bool sees(const PagedPass &p, const Cursor &c, int i, int at) {
+template <int kTile>
+__device__ __forceinline__ bool sees(const PagedPass &p, const Cursor<kTile> &c, int i, int at) {
     if (i >= c.keys) return false;
     if (p.prefix_pass) return true;
     const int pos = key_pos(c, i);
     return pos <= at && (!p.a.window || pos > at - p.a.window || pos < p.a.sinks);
 }
+// Whether every row of the segment sees every key of [i0, i1).
+template <int kTile>
+__device__ __forceinline__ bool all_see(const PagedPass &p, const Cursor<kTile> &c, int i0, int i1) {
+    if (p.prefix_pass) return i1 <= c.keys;
+    if (i1 > c.keys - (c.ntok - 1)) return false;
+    return !p.a.window || i1 <= c.sink || i0 >= c.sink + max(c.past + c.ntok - p.a.window - c.low, 0);
+}
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __grid_constant__ PagedPass p) {
+__global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
+    paged_attention_kernel(const __grid_constant__ PagedPass p) {
     using C = Cfg<T, DP>;
-    constexpr int EPL = C::kEpl, KB = DP / C::kKBlk, VB = DP / C::kVBlk, NT = DP / 16;
+    using Cur = Cursor<C::kTileKeys>;
+    constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kTileKeys = C::kTileKeys, S = C::kStages;
+    constexpr int NT = DP / 16;
     extern __shared__ __align__(128) unsigned char smem[];
     unsigned char *ring = smem;
-    float *q_hi = reinterpret_cast<float *>(ring + C::kStages * kWarps * C::kStageBytes);
-    float *q_lo = q_hi + kRows * DP;
-    float *mo = q_lo + kRows * DP;                          // [kWarps][kRows][kMergeStride]
-    float *mml = mo + kWarps * kRows * C::kMergeStride;     // [kWarps][kRows][2]
-    float *row_ml = mml + kWarps * kRows * 2;               // [kRows][2]
-    long long *sums = reinterpret_cast<long long *>(row_ml + kRows * 2);  // [kThreads + 1]
-    uint64_t *full = reinterpret_cast<uint64_t *>(sums + kThreads + 1);   // [kWarps][kStages]
-    int *flags = reinterpret_cast<int *>(full + kWarps * C::kStages);
-    volatile int *abort = flags;
-    int *last_s = flags + 1, *bad_s = flags + 2;  // bad_s: bit per row
+    unsigned char *q_s = ring + S * kWarps * C::kStageBytes;            // fragments of the queries
+    float *mo = reinterpret_cast<float *>(q_s + C::kQBytes);           // [kWarps][kRows][kMergeStride]
+    float *mml = mo + kWarps * kRows * C::kMergeStride;                 // [kWarps][kRows][2]
+    float *row_ml = mml + kWarps * kRows * 2;                           // [kRows][2]
+    float *q_scale = row_ml + kRows * 2;                                // [kRows]
+    long long *sums = reinterpret_cast<long long *>(q_scale + kRows);   // [kWarps]
+    int *last_s = reinterpret_cast<int *>(sums + kWarps), *bad_s = last_s + 1;  // bad_s: bit per row
+    long long *found = sums + kWarps + 1;                               // [2]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
     const int D = p.a.head_dim, H = p.a.heads, Hkv = p.a.kv_heads, G = H / Hkv;
     const int seqs = p.prefix_pass ? 1 : p.a.batch.seqs;
-    uint64_t *my_full = full + warp * C::kStages;
 
     pdl_trigger();
-    if (threadIdx.x == 0) {
-        for (int i = 0; i < kWarps * C::kStages; i++) mbar_init(&full[i], 1);
-        fence_mbar_init();
-        *abort = 0;
-        *bad_s = 0;
-    }
-    // Dims past head_dim stay zero in the ring (never copied).
-    if (D < DP)
-        for (int i = threadIdx.x; i < C::kStages * kWarps * C::kStageBytes / 16; i += kThreads)
-            reinterpret_cast<uint4 *>(ring)[i] = make_uint4(0, 0, 0, 0);
-    fence_proxy_async_smem();
 
-    // The work line: every thread adds up a run of sequences, thread 0 the runs.
+    // The work line: every thread adds up a run of sequences; a scan over the
+    // threads finds the run in which this CTA's share begins.
     const int per = (seqs + kThreads - 1) / kThreads;
-    {
-        long long n = 0;
-        for (int i = 0; i < per; i++) {
-            const int b = threadIdx.x * per + i;
-            if (b < seqs) {
-                Cursor c;
-                seq_load(p, b, c);
-                n += seq_units(p, c);
-            }
+    long long mine = 0;
+    for (int i = 0; i < per; i++) {
+        const int b = threadIdx.x * per + i;
+        if (b < seqs) {
+            Cur c;
+            seq_load(p, b, c);
+            mine += seq_units(p, c);
         }
-        sums[threadIdx.x + 1] = n;
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        sums[0] = 0;
-        for (int i = 1; i <= kThreads; i++) sums[i] += sums[i - 1];
+    long long upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += x;
     }
+    if (lane == 31) sums[warp] = upto;
     __syncthreads();
-    const long long U = sums[kThreads];
+    long long U = 0;
+    for (int w = 0; w < kWarps; w++) {
+        if (w < warp) upto += sums[w];
+        U += sums[w];
+    }
     const long long grid = min((long long)gridDim.x, U);
     if (blockIdx.x >= grid) {
         pdl_wait();
         return;
     }
     const long long u0 = U * blockIdx.x / grid, u1 = U * (blockIdx.x + 1) / grid;
-    Cursor cc, pc;  // consumer and producer
-    {
-        int lo = 0;
-        for (int i = kThreads; i > 0; i >>= 1)
-            while (lo + i <= kThreads && sums[lo + i] <= u0) lo += i;
-        seq_load(p, min(lo * per, seqs - 1), cc);
-        cursor_at(p, cc, u0 - sums[lo]);
-        pc = cc;
+    if (upto - mine <= u0 && u0 < upto) {
+        found[0] = threadIdx.x;
+        found[1] = upto - mine;
     }
+    if (threadIdx.x == 0) *bad_s = 0;
+    __syncthreads();
+    Cur cc, pc;  // consumer and producer
+    seq_load(p, (int)found[0] * per, cc);
+    cursor_at(p, cc, u0 - found[1]);
+    pc = cc;
     pdl_wait();  // q and the cache come from earlier kernels; workspace use may overlap none
 
-    const uint64_t policy = policy_evict_first();
-    const uint32_t row_bytes = (uint32_t)(D * sizeof(T));
-    // Copies the warp's 16 keys (lanes 0..15) and values (lanes 16..31) of
-    // the producer's unit into a stage. Rows past the segment's keys: values
-    // are zeroed (they meet zero probabilities), scores are masked.
-    auto issue = [&](int stage) {
-        unsigned char *st = ring + (warp * C::kStages + stage) * C::kStageBytes;
-        const int r = lane & 15, parity = lane >> 4;
-        const int i = pc.tile * kTileKeys + warp * kWarpKeys + r;
-        const bool live = i < pc.keys;
-        unsigned char *dst = parity ? st + kWarpKeys * C::kKStride + r * C::kVStride : st + r * C::kKStride;
-        const int rows = __popc(__ballot_sync(0xffffffffu, live));
-        if (!live && parity)
-            for (int j = 0; j < DP * (int)sizeof(T) / 16; j++)
-                reinterpret_cast<uint4 *>(dst)[j] = make_uint4(0, 0, 0, 0);
-        if (rows < 32) fence_proxy_async_smem();
-        if (lane == 0) mbar_arrive_expect_tx(&my_full[stage], rows * row_bytes);
-        __syncwarp();
-        if (live) {
-            const char *src = p.a.cache.base + paged_row(p.a.cache, p.a.batch, pc.b, key_pos(pc, i), p.a.err) +
-                              parity * p.a.cache.parity_stride + (long long)pc.kvh * row_bytes;
-            bulk_g2s(dst, src, row_bytes, &my_full[stage], policy);
+    // The producer's unit: lane r (and r + 16) holds the table entry and the
+    // place in its page of the warp's key r, read a tile before its use.
+    uint32_t next_id = 0;
+    int next_in = -1;  // -1: past the segment's keys
+    auto look_up = [&] {
+        const int i = pc.tile * kTileKeys + warp * kWarpKeys + (lane & 15);
+        next_in = -1;
+        if (i < pc.keys) {
+            const int pos = key_pos(pc, i), pg = page_of(p.a.cache, pos);
+            next_in = pos - pg * p.a.cache.page;
+            next_id = pg < p.a.batch.per_seq ? p.a.batch.table[(long long)pc.b * p.a.batch.per_seq + pg] : ~0u;
+        }
+    };
+    // Copies the warp's 16 keys of the producer's unit into a stage, or its
+    // 16 values: zeros for rows past the segment's keys (values meet zero
+    // probabilities there) and for dims past head_dim.
+    const int head_bytes = D * (int)sizeof(T);
+    long long off = -1;
+    auto place = [&] {
+        off = -1;
+        if (next_in < 0) return;
+        if (next_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
+            report_error(p.a.err, kErrGatherId);
+            next_id = 0;
+        }
+        off = next_id * p.a.cache.page_stride + next_in * p.a.cache.row_stride + (long long)pc.kvh * head_bytes;
+    };
+    auto issue = [&](int stage, int parity) {
+        unsigned char *st = ring + (warp * S + stage) * C::kStageBytes + (parity ? kWarpKeys * C::kKStride : 0);
+        const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0);
+#pragma unroll
+        for (int x = 0; x < kWarpKeys * C::kLpr / 32; x++) {
+            const int r = (x * 32 + lane) / C::kLpr, c = (x * 32 + lane) % C::kLpr * 16;
+            const long long o = __shfl_sync(0xffffffffu, off, r);
+            const bool live = o >= 0 && c < head_bytes;
+            cp_async16_zfill(st + r * (parity ? C::kVStride : C::kKStride) + c, base + (live ? o + c : 0),
+                             live ? 16 : 0);
         }
     };
     const int units = (int)(u1 - u0);
     int issued = 0;
-    for (; issued < C::kStages && issued < units; issued++) {
-        if (issued) cursor_next(p, pc);
-        issue(issued);
+    look_up();
+    for (; issued < S; issued++) {
+        if (issued < units) {
+            place();
+            issue(issued, 0);
+            cp_async_commit();
+            issue(issued, 1);
+            if (issued + 1 < units) {
+                cursor_next(p, pc);
+                look_up();
+            }
+        } else {
+            cp_async_commit();
+        }
+        cp_async_commit();
     }
 
     float acc[NT][4];  // O^T: dims x rows
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-    int at0 = 0, at1 = 0;      // positions of rows 2t, 2t + 1
-    long long seg_u0 = u0;     // this CTA's first unit of the current segment
+    float qf0 = 0.f, qf1 = 0.f;  // S to log2 units, rows 2t and 2t + 1
+    int at0 = 0, at1 = 0;        // their positions
+    long long seg_u0 = u0;       // this CTA's first unit of the current segment
     bool fresh = true;
-    int done = 0;
+    int stage = 0;
     for (long long u = u0; u < u1; u++) {
         if (fresh) {
-            // Queries of the segment as tf32 pairs, in fragment order: block j
-            // of kKBlk dims, lane (g, t) holds row g, dims j kKBlk + EPL t + e.
-            for (int i = threadIdx.x; i < kRows * DP; i += kThreads) {
-                const int e = i % 4, ln = (i / 4) % 32, x = i / 128;  // x = j * (EPL / 4) + e / 4
-                const int j = x / (EPL / 4), ee = (x % (EPL / 4)) * 4 + e;
-                const int r = ln >> 2, d = j * C::kKBlk + EPL * (ln & 3) + ee;
+            // Queries of the segment, a warp per row, into fragment order.
+            for (int r = warp; r < kRows; r += kWarps) {
                 const int row = cc.rb * kRows + r, tok = row / G;
-                float v = 0.f;
-                if (tok < cc.ntok && d < D)
-                    v = p.a.q[((size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G)) * D + d];
-                const uint32_t hi = tf32_hi(v);
-                q_hi[i] = __uint_as_float(hi);
-                q_lo[i] = __uint_as_float(tf32_lo(v, hi));
+                const float *q = p.a.q + ((size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G)) * D;
+                float v[DP / 32];
+                uint32_t top = 0;
+#pragma unroll
+                for (int y = 0; y < DP / 32; y++) {
+                    const int d = lane + 32 * y;
+                    v[y] = tok < cc.ntok && d < D ? q[d] : 0.f;
+                    top = max(top, __float_as_uint(v[y]) & 0x7fffffffu);
+                }
+                float f = p.scale_log2;
+                if (C::kShift) {
+                    const int ex = scale_exponent(__reduce_max_sync(0xffffffffu, top));
+                    f *= pow2(ex - C::kShift);
+#pragma unroll
+                    for (int y = 0; y < DP / 32; y++) v[y] *= pow2(C::kShift - ex);
+                }
+                if (lane == 0) q_scale[r] = f;
+#pragma unroll
+                for (int y = 0; y < DP / 32; y++) {
+                    const int d = lane + 32 * y, j = d / 16, k = d % 16;
+                    if (C::kHalf) {
+                        // k step j, lane (r, t): b0 = dims 2t, 2t + 1, b1 = 8 + 2t, ...
+                        T *dst = reinterpret_cast<T *>(q_s) + (j * C::kTerms * 32 + r * 4 + (k % 8) / 2) * 4 +
+                                 k / 8 * 2 + k % 2;
+#pragma unroll
+                        for (int x = 0; x < C::kTerms; x++) {
+                            float none = 0.f;
+                            const uint32_t w = take_pair<T>(v[y], none);
+                            *reinterpret_cast<uint16_t *>(dst + x * 128) = (uint16_t)w;
+                        }
+                    } else {
+                        // Block j, lane (r, t): dims 4t .. 4t + 3; hi, then lo.
+                        float *dst = reinterpret_cast<float *>(q_s) + (j * 32 + r * 4 + k / 4) * 4 + k % 4;
+                        const uint32_t hi = tf32_hi(v[y]);
+                        dst[0] = __uint_as_float(hi);
+                        dst[kRows * DP] = __uint_as_float(tf32_lo(v[y], hi));
+                    }
+                }
             }
             at0 = cc.past + (cc.rb * kRows + 2 * t) / G;
             at1 = cc.past + (cc.rb * kRows + 2 * t + 1) / G;
@@ -301,54 +427,75 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
             seg_u0 = u;
             fresh = false;
             __syncthreads();
+            qf0 = q_scale[2 * t];
+            qf1 = q_scale[2 * t + 1];
         }
-        const int stage = done % C::kStages;
-        mbar_wait(&my_full[stage], (done / C::kStages) & 1, p.a.err, abort);
-        const unsigned char *ks = ring + (warp * C::kStages + stage) * C::kStageBytes;
+        cp_async_wait<2 * S - 1>();
+        __syncwarp();
+        const unsigned char *ks = ring + (warp * S + stage) * C::kStageBytes;
         const unsigned char *vs = ks + kWarpKeys * C::kKStride;
 
-        // S^T: keys g, g + 8 x rows 2t, 2t + 1.
+        // S^T: keys g, g + 8 x rows 2t, 2t + 1; small products apart.
         float s[4][4];
 #pragma unroll
         for (int i = 0; i < 4; i++)
 #pragma unroll
             for (int j = 0; j < 4; j++) s[i][j] = 0.f;
+        if constexpr (C::kHalf) {
+            const uint32_t ka = smem_addr(ks) + (lane & 15) * C::kKStride + (lane >> 4) * 16;
 #pragma unroll
-        for (int j = 0; j < KB; j++) {
-            float ka[EPL], kb[EPL];
-            Frag<T>::ld(ks + g * C::kKStride + (j * C::kKBlk + EPL * t) * sizeof(T), ka);
-            Frag<T>::ld(ks + (g + 8) * C::kKStride + (j * C::kKBlk + EPL * t) * sizeof(T), kb);
+            for (int j = 0; j < DP / 16; j++) {
+                uint32_t a[4];
+                ldmatrix4<false>(ka + j * 32, a);
 #pragma unroll
-            for (int x = 0; x < EPL / 4; x++) {
-                const float4 qh = reinterpret_cast<const float4 *>(q_hi)[(j * (EPL / 4) + x) * 32 + lane];
-                const float4 ql = reinterpret_cast<const float4 *>(q_lo)[(j * (EPL / 4) + x) * 32 + lane];
+                for (int x = 0; x < C::kTerms; x++) {
+                    const uint2 b = reinterpret_cast<const uint2 *>(q_s)[(j * C::kTerms + x) * 32 + lane];
+                    mma_16<T>(s[x], a, b.x, b.y);
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < DP / 16; j++) {
+                float ka[4], kb[4];
+                Frag<T>::ld(ks + g * C::kKStride + (j * 16 + 4 * t) * sizeof(T), ka);
+                Frag<T>::ld(ks + (g + 8) * C::kKStride + (j * 16 + 4 * t) * sizeof(T), kb);
+                const float4 qh = reinterpret_cast<const float4 *>(q_s)[j * 32 + lane];
+                const float4 ql = reinterpret_cast<const float4 *>(q_s)[kRows * DP / 4 + j * 32 + lane];
                 const float h4[4] = {qh.x, qh.y, qh.z, qh.w}, w4[4] = {ql.x, ql.y, ql.z, ql.w};
 #pragma unroll
                 for (int y = 0; y < 2; y++) {
-                    const int e = 4 * x + 2 * y;
-                    const float f[4] = {ka[e], kb[e], ka[e + 1], kb[e + 1]};
-                    uint32_t hi[4];
+                    const float f[4] = {ka[2 * y], kb[2 * y], ka[2 * y + 1], kb[2 * y + 1]};
+                    uint32_t hi[4], lo[4];
 #pragma unroll
-                    for (int z = 0; z < 4; z++) hi[z] = sizeof(T) == 4 ? tf32_hi(f[z]) : __float_as_uint(f[z]);
+                    for (int z = 0; z < 4; z++) {
+                        hi[z] = tf32_hi(f[z]);
+                        lo[z] = tf32_lo(f[z], hi[z]);
+                    }
                     const uint32_t b0 = __float_as_uint(h4[2 * y]), b1 = __float_as_uint(h4[2 * y + 1]);
                     mma_tf32(s[2 + y], hi, __float_as_uint(w4[2 * y]), __float_as_uint(w4[2 * y + 1]));
                     mma_tf32(s[y], hi, b0, b1);
-                    if (sizeof(T) == 4) {
-                        uint32_t lo[4];
-#pragma unroll
-                        for (int z = 0; z < 4; z++) lo[z] = tf32_lo(f[z], hi[z]);
-                        mma_tf32(s[2 + y], lo, b0, b1);
-                    }
+                    mma_tf32(s[2 + y], lo, b0, b1);
                 }
             }
         }
-        const int i0 = cc.tile * kTileKeys + warp * kWarpKeys + g, i1 = i0 + 8;
+        // The keys are read: their slot takes those of S tiles on.
+        __syncwarp();
+        const bool more = issued < units;
+        if (more) {
+            place();
+            issue(stage, 0);
+        }
+        cp_async_commit();
+
+        const int w0i = cc.tile * kTileKeys + warp * kWarpKeys, i0 = w0i + g, i1 = i0 + 8;
         float sc[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            const float x = ((s[2][j] + s[3][j]) + (s[0][j] + s[1][j])) * p.scale_log2;
-            sc[j] = sees(p, cc, j < 2 ? i0 : i1, (j & 1) ? at1 : at0) ? x : -INFINITY;
-        }
+        for (int j = 0; j < 4; j++)
+            sc[j] = ((s[3][j] + s[2][j]) + (s[1][j] + s[0][j])) * ((j & 1) ? qf1 : qf0);
+        if (!all_see(p, cc, w0i, w0i + kWarpKeys))
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (!sees(p, cc, j < 2 ? i0 : i1, (j & 1) ? at1 : at0)) sc[j] = -INFINITY;
         float n0 = fmaxf(sc[0], sc[2]), n1 = fmaxf(sc[1], sc[3]);
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
@@ -359,10 +506,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         n1 = fmaxf(n1, m1);
         const float u_0 = n0 == -INFINITY ? 0.f : n0, u_1 = n1 == -INFINITY ? 0.f : n1;
         float pr[4];
-        pr[0] = ex2(sc[0] - u_0);
-        pr[1] = ex2(sc[1] - u_1);
-        pr[2] = ex2(sc[2] - u_0);
-        pr[3] = ex2(sc[3] - u_1);
+        pr[0] = ex2(sc[0] - (u_0 - C::kShift));
+        pr[1] = ex2(sc[1] - (u_1 - C::kShift));
+        pr[2] = ex2(sc[2] - (u_0 - C::kShift));
+        pr[3] = ex2(sc[3] - (u_1 - C::kShift));
         const float f0 = ex2(m0 - u_0), f1 = ex2(m1 - u_1);
         l0 *= f0;
         l1 *= f1;
@@ -370,66 +517,90 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         m1 = n1;
         l0 += pr[0] + pr[2];
         l1 += pr[1] + pr[3];
-        // P as the B fragments of the two 8-key steps: row g, keys t and t + 4.
-        uint32_t bh[2][2], bl[2][2];
-#pragma unroll
-        for (int ks8 = 0; ks8 < 2; ks8++)
-#pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const int src = (t + 4 * x) * 4 + (g >> 1);
-                const float a = __shfl_sync(0xffffffffu, pr[2 * ks8], src);
-                const float b = __shfl_sync(0xffffffffu, pr[2 * ks8 + 1], src);
-                const float v = (g & 1) ? b : a;
-                bh[ks8][x] = tf32_hi(v);
-                bl[ks8][x] = tf32_lo(v, bh[ks8][x]);
-            }
-        // The tile's P V starts from zero and is added to the running output
+        cp_async_wait<2 * S - 1>();
+        __syncwarp();
+
+        // A tile's P V starts from zero and is added to the running output
         // outside the tensor core, whose accumulation truncates: over
         // thousands of keys that bias would grow past f32 rounding.
+        if constexpr (C::kHalf) {
+            // B fragments: row g, keys 2t, 2t + 1 and 8 + 2t, 9 + 2t.
+            uint32_t b[3][2];
 #pragma unroll
-        for (int j = 0; j < VB; j++) {
-            float o[EPL / 2][4];
-#pragma unroll
-            for (int x = 0; x < EPL / 2; x++)
-#pragma unroll
-                for (int z = 0; z < 4; z++) o[x][z] = 0.f;
-#pragma unroll
-            for (int ks8 = 0; ks8 < 2; ks8++) {
-                float va[EPL], vb[EPL];
-                Frag<T>::ld(vs + (8 * ks8 + t) * C::kVStride + (j * C::kVBlk + EPL * g) * sizeof(T), va);
-                Frag<T>::ld(vs + (8 * ks8 + t + 4) * C::kVStride + (j * C::kVBlk + EPL * g) * sizeof(T), vb);
-#pragma unroll
-                for (int x = 0; x < EPL / 2; x++) {
-                    const float f[4] = {va[2 * x], va[2 * x + 1], vb[2 * x], vb[2 * x + 1]};
-                    uint32_t hi[4];
-#pragma unroll
-                    for (int z = 0; z < 4; z++) hi[z] = sizeof(T) == 4 ? tf32_hi(f[z]) : __float_as_uint(f[z]);
-                    mma_tf32(o[x], hi, bl[ks8][0], bl[ks8][1]);
-                    if (sizeof(T) == 4) {
-                        uint32_t lo[4];
-#pragma unroll
-                        for (int z = 0; z < 4; z++) lo[z] = tf32_lo(f[z], hi[z]);
-                        mma_tf32(o[x], lo, bh[ks8][0], bh[ks8][1]);
-                    }
-                    mma_tf32(o[x], hi, bh[ks8][0], bh[ks8][1]);
-                }
+            for (int x = 0; x < C::kTerms; x++) {
+                b[x][0] = movmatrix(take_pair<T>(pr[0], pr[1]));
+                b[x][1] = movmatrix(take_pair<T>(pr[2], pr[3]));
             }
+            const uint32_t va = smem_addr(vs) + ((lane & 7) + (lane >> 4) * 8) * C::kVStride + ((lane >> 3) & 1) * 16;
 #pragma unroll
-            for (int x = 0; x < EPL / 2; x++) {
-                float(&a)[4] = acc[j * (EPL / 2) + x];
-                a[0] = fmaf(a[0], f0, o[x][0]);
-                a[1] = fmaf(a[1], f1, o[x][1]);
-                a[2] = fmaf(a[2], f0, o[x][2]);
-                a[3] = fmaf(a[3], f1, o[x][3]);
+            for (int i = 0; i < NT; i++) {
+                uint32_t a[4];
+                ldmatrix4<true>(va + i * 32, a);
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int x = C::kTerms - 1; x >= 0; x--) mma_16<T>(o, a, b[x][0], b[x][1]);
+                acc[i][0] = fmaf(acc[i][0], f0, o[0]);
+                acc[i][1] = fmaf(acc[i][1], f1, o[1]);
+                acc[i][2] = fmaf(acc[i][2], f0, o[2]);
+                acc[i][3] = fmaf(acc[i][3], f1, o[3]);
+            }
+        } else {
+            // B fragments of the two 8-key steps: row g, keys t and t + 4.
+            uint32_t bh[2][2], bl[2][2];
+#pragma unroll
+            for (int k8 = 0; k8 < 2; k8++)
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int src = (t + 4 * x) * 4 + (g >> 1);
+                    const float a = __shfl_sync(0xffffffffu, pr[2 * k8], src);
+                    const float b = __shfl_sync(0xffffffffu, pr[2 * k8 + 1], src);
+                    const float v = (g & 1) ? b : a;
+                    bh[k8][x] = tf32_hi(v);
+                    bl[k8][x] = tf32_lo(v, bh[k8][x]);
+                }
+#pragma unroll
+            for (int j = 0; j < DP / 32; j++) {
+                float o[2][4] = {};
+#pragma unroll
+                for (int k8 = 0; k8 < 2; k8++) {
+                    float va[4], vb[4];
+                    Frag<T>::ld(vs + (8 * k8 + t) * C::kVStride + (j * 32 + 4 * g) * sizeof(T), va);
+                    Frag<T>::ld(vs + (8 * k8 + t + 4) * C::kVStride + (j * 32 + 4 * g) * sizeof(T), vb);
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const float f[4] = {va[2 * x], va[2 * x + 1], vb[2 * x], vb[2 * x + 1]};
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            hi[z] = tf32_hi(f[z]);
+                            lo[z] = tf32_lo(f[z], hi[z]);
+                        }
+                        mma_tf32(o[x], hi, bl[k8][0], bl[k8][1]);
+                        mma_tf32(o[x], lo, bh[k8][0], bh[k8][1]);
+                        mma_tf32(o[x], hi, bh[k8][0], bh[k8][1]);
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    float(&a)[4] = acc[2 * j + x];
+                    a[0] = fmaf(a[0], f0, o[x][0]);
+                    a[1] = fmaf(a[1], f1, o[x][1]);
+                    a[2] = fmaf(a[2], f0, o[x][2]);
+                    a[3] = fmaf(a[3], f1, o[x][3]);
+                }
             }
         }
         __syncwarp();
-        done++;
-        if (issued < units && !*abort) {
-            cursor_next(p, pc);
-            issue(stage);
+        if (more) {
+            issue(stage, 1);
             issued++;
+            if (issued < units) {
+                cursor_next(p, pc);
+                look_up();
+            }
         }
+        cp_async_commit();
+        stage = stage + 1 == S ? 0 : stage + 1;
 
         const bool seg_end = cc.tile == cc.tiles - 1;
         if (!seg_end && u + 1 < u1) {
@@ -447,10 +618,19 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         float *w0 = mo + (warp * kRows + 2 * t) * C::kMergeStride, *w1 = w0 + C::kMergeStride;
 #pragma unroll
         for (int i = 0; i < NT; i++) {
-            const int d = (i / (EPL / 2)) * C::kVBlk + EPL * g + 2 * (i % (EPL / 2));
-            *reinterpret_cast<float2 *>(w0 + d) = make_float2(acc[i][0], acc[i][2]);
-            *reinterpret_cast<float2 *>(w1 + d) = make_float2(acc[i][1], acc[i][3]);
+            if (C::kHalf) {  // tile i: dims 16 i + g and 16 i + 8 + g
+                w0[16 * i + g] = acc[i][0];
+                w1[16 * i + g] = acc[i][1];
+                w0[16 * i + 8 + g] = acc[i][2];
+                w1[16 * i + 8 + g] = acc[i][3];
+            } else {  // dims 32 (i / 2) + 4 g + 2 (i % 2) and the next
+                const int d = i / 2 * 32 + 4 * g + i % 2 * 2;
+                *reinterpret_cast<float2 *>(w0 + d) = make_float2(acc[i][0], acc[i][2]);
+                *reinterpret_cast<float2 *>(w1 + d) = make_float2(acc[i][1], acc[i][3]);
+            }
         }
+        m0 -= C::kShift;  // l and o are 2^kShift times as large
+        m1 -= C::kShift;
         if (g == 0) {
             float *ml = mml + (warp * kRows + 2 * t) * 2;
             ml[0] = m0, ml[1] = l0, ml[2] = m1, ml[3] = l1;
@@ -594,17 +774,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_attention_kernel(const __gr
         fresh = true;
         if (u + 1 < u1) cursor_next(p, cc);
     }
-    // After a wait that gave up, copies may still be in flight: let them land
-    // before the CTA's shared memory is released.
-    if (*abort) {
-        const int from = issued > C::kStages ? issued - C::kStages : 0;
-        for (int i = from; i < issued; i++) {
-            const uint64_t t0 = global_ns();
-            while (!mbar_try_wait(&my_full[i % C::kStages], (i / C::kStages) & 1) &&
-                   global_ns() - t0 < 100000000ull) {
-            }
-        }
-    }
 }
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -617,10 +786,10 @@ size_t prefix_floats(const PagedAttention &a) {
 template <typename T, int DP>
 cudaError_t launch_pass(cudaStream_t s, const PagedPass &p) {
     using C = Cfg<T, DP>;
-    static_assert(C::kSmem <= 227 * 1024, "shared layout");
+    static_assert(C::kStages >= 1 && C::kSmem <= 227 * 1024, "shared layout");
     static std::atomic<uint64_t> smem_set{0};
     set_smem_limit_once(paged_attention_kernel<T, DP>, C::kSmem, &smem_set);
-    launch_k(paged_attention_kernel<T, DP>, kSmCount, kThreads, C::kSmem, s, p);
+    launch_k(paged_attention_kernel<T, DP>, kSmCount, C::kThreads, C::kSmem, s, p);
     count_launch();
     return cudaGetLastError();
 }

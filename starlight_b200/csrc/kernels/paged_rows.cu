@@ -199,12 +199,6 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 __device__ __forceinline__ float2 unpack_h2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
-// Exponent e of the scale 2^(kShift - e) for a largest magnitude (its bits).
-__device__ __forceinline__ int scale_exponent(uint32_t bits) {
-    return bits ? max((int)(bits >> 23) - 127, -100) : kShift;
-}
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-
 // Element (row, dim) of a swizzled operand: block dim / 64 of rows of 128
 // bytes, 16-byte chunks xored with the row.
 __device__ __forceinline__ uint32_t operand_at(int row, int dim, int rows) {

@@ -142,6 +142,18 @@ __device__ __forceinline__ void cp_async4(void *dst, const void *src) {
                  : "memory");
 }
 
+// 16-byte asynchronous copy past L1, of `bytes` (0 or 16) and zeros after them.
+__device__ __forceinline__ void cp_async16_zfill(void *dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Waits until at most N of this thread's groups are in flight.
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // Makes `bar` track this thread's prior cp.async copies: its current phase
 // cannot complete before they land (net-zero change of the pending count).
 __device__ __forceinline__ void cp_async_mbar_arrive(uint64_t *bar) {

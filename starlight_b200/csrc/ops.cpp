@@ -312,7 +312,7 @@ bool paged_ports(Checker &ck, uint64_t first, uint64_t tokens, Paged *o) {
     o->cache.parity_stride = o->cache.row_stride * (long long)st[3];
     o->cache.page_stride = o->cache.parity_stride * 2 * (long long)st[1];
     o->cache.base = base + o->cache.parity_stride * 2 * op.layer;
-    o->cache.page = (int)st[3];
+    o->cache.set_page((int)st[3]);
     o->cache.pages = (int)st[0];
     o->page = st[3];
     o->pages = st[0];
