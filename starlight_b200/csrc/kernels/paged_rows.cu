@@ -16,17 +16,20 @@
 // times).
 //
 // One CTA per SM, 16 warps:
-//   0..3   softmax: one thread per row; S from TMEM, running maximum, P as
-//          f16 pairs back into the TMEM columns that S held
+//   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
+//          S from TMEM, running maximum, P as f16 pairs back into the TMEM
+//          columns that S held
 //   4..7   output: one thread per row; O += P V of each tile in registers,
 //          the merge of a split segment, the result
-//   8..14  producers: K and V tiles from the pages through registers (the
-//          tile's largest value, scale, f16 pair) into 128-byte swizzled
-//          shared memory, and Q at a segment's start
+//   8..14  producers: K and V tiles from the pages by 16-byte asynchronous
+//          copies into a ring of slots, then in place (the tile's largest
+//          value, scale, f16 or f16 pair) the 128-byte swizzled operand
 //   15     issues the MMAs: Q K^T of the next tile before P V of this one
-// K is read K-major and V MN-major from the same layout ([key][64 dims] rows
-// of 128 bytes), P as the A operand from TMEM. TMEM: two S / P buffers and two
-// O buffers of 128 columns.
+// The ring holds operands in the order of their MMAs (K0 K1 V0 K2 V1 ...), so
+// a slot is free as soon as the MMA kSlots back is done; three slots of pairs
+// or six of single f16. Q and P are A operands from TMEM; K is read K-major
+// and V MN-major from the same layout ([key][64 dims] rows of 128 bytes).
+// TMEM: Q, two S / P buffers and O, 128 columns each.
 //
 // Tensor-bound: 4 * pairs * D flops take 4 (16-bit cache) or 6 (F32) passes of
 // half as many MMA flops each.
@@ -61,10 +64,10 @@ struct Cfg {
     static constexpr int kBlockBytes = kKeys * 128;          // 16 KiB
     static constexpr int kHalfBytes = kBlocks * kBlockBytes;  // one of hi, lo
     static constexpr int kTileBytes = kHalfBytes * (kPair ? 2 : 1);
-    static constexpr int kStages = kPair ? (DP == 64 ? 2 : 1) : 2;
-    static constexpr int kQBytes = 2 * kHalfBytes;
-    static constexpr int kRing = kQBytes + 2 * kStages * kTileBytes;
-    static constexpr int kSmall = 4 * (4 * kM + 2 * 4 * kM + 4 * kM + 16 + 16 + 4 * DP + 16) + 8 * (kM + 2 + 4 * kStages + 11 + 16 + 2);
+    static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
+    static constexpr int kAhead = kSlots / 2;                // operands copied ahead of the one converted
+    static constexpr int kRing = kSlots * kTileBytes;
+    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 4 * DP + 16) + 8 * (8 + 2 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
     static constexpr int kLpr = DP / kEpl;               // lanes per cache row
@@ -165,16 +168,6 @@ __device__ __forceinline__ void cursor_next(const PagedPass &p, Cursor &c) {
     cursor_at(p, c, 0);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-        : "memory");
-}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
@@ -201,26 +194,23 @@ __device__ __forceinline__ float2 unpack_h2(uint32_t w) {
 }
 // Element (row, dim) of a swizzled operand: block dim / 64 of rows of 128
 // bytes, 16-byte chunks xored with the row.
-__device__ __forceinline__ uint32_t operand_at(int row, int dim, int rows) {
-    return (uint32_t)((dim >> 6) * rows * 128 + row * 128 + ((((dim & 63) >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2);
+__device__ __forceinline__ uint32_t operand_at(int row, int dim) {
+    return (uint32_t)((dim >> 6) * kKeys * 128 + row * 128 + ((((dim & 63) >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2);
 }
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ PagedPass p) {
     using C = Cfg<T, DP>;
-    constexpr int S = C::kStages;
+    constexpr int S = C::kSlots;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     unsigned char *smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
-    unsigned char *q_s = smem;                          // hi, lo
-    unsigned char *k_s = q_s + C::kQBytes;              // [S] hi[, lo]
-    unsigned char *v_s = k_s + S * C::kTileBytes;       // [S] hi[, lo]
-    float *q_scale = reinterpret_cast<float *>(smem + C::kRing);  // [4 segments][kM]
-    float *row_ml = q_scale + 4 * kM;                   // [4 tiles][kM][2]
+    unsigned char *ring = smem;                         // [S] operands: hi[, lo]
+    float *row_ml = reinterpret_cast<float *>(smem + C::kRing);  // [4 tiles][kM][2]
     float *alpha = row_ml + 4 * kM * 2;                 // [4 tiles][kM]
-    float *k_scale = alpha + 4 * kM;                    // [4 tiles]
-    float *v_scale = k_scale + 4;                       // [4 tiles]
-    uint32_t *k_max = reinterpret_cast<uint32_t *>(v_scale + 4);  // [4 tiles]
+    float *k_scale = alpha + 4 * kM;                    // [8 tiles]
+    float *v_scale = k_scale + 8;                       // [8 tiles]
+    uint32_t *k_max = reinterpret_cast<uint32_t *>(v_scale + 8);  // [4 tiles]
     uint32_t *v_max = k_max + 4;                        // [4 tiles]
     int *poison = reinterpret_cast<int *>(v_max + 4);   // [8 segments]
     float *scratch = reinterpret_cast<float *>(poison + 8);       // [4 warps][DP]
@@ -228,15 +218,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     volatile int *abort = flags;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(flags + 1);
     int *last_s = flags + 2;
-    long long *sums = reinterpret_cast<long long *>(flags + 4);   // [kM + 1]
-    uint64_t *bars = reinterpret_cast<uint64_t *>(sums + kM + 2);
-    uint64_t *k_full = bars, *k_empty = k_full + S, *v_full = k_empty + S, *v_empty = v_full + S;
-    uint64_t *q_full = v_empty + S, *q_empty = q_full + 1;
-    uint64_t *s_full = q_empty + 1, *p_full = s_full + 2, *o_full = p_full + 2, *o_empty = o_full + 2;
-    uint64_t *done = o_empty + 2;
-    // What threads pass each other beside the operands, in rings of four (a
-    // producer can be two tiles ahead of the MMAs, those two of a reader).
-    uint64_t *q_sc = done + 1, *k_sc = q_sc + 4, *v_sc = k_sc + 4, *a_full = v_sc + 4;
+    long long *sums = reinterpret_cast<long long *>(flags + 4);   // [4] a scan's warps, [2] what it found
+    uint64_t *bars = reinterpret_cast<uint64_t *>(sums + 6);
+    uint64_t *full = bars, *empty = full + S;           // [S] the ring's
+    uint64_t *q_full = empty + S, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2,
+             *o_empty = o_full + 1, *done = o_empty + 1;
+    // What threads pass each other beside the operands, in rings long enough
+    // for the lead that the barriers above allow.
+    uint64_t *k_sc = done + 1, *v_sc = k_sc + 8, *a_full = v_sc + 8;  // [8], [8], [4]
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int D = p.a.head_dim, H = p.a.heads, G = group_of(p);
@@ -244,53 +233,54 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     pdl_trigger();
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; i++) {
-            mbar_init(&k_full[i], kProducers);
-            mbar_init(&k_empty[i], 1);
-            mbar_init(&v_full[i], kProducers);
-            mbar_init(&v_empty[i], 1);
+            mbar_init(&full[i], kProducers);
+            mbar_init(&empty[i], 1);
         }
-        mbar_init(q_full, kProducers);
-        mbar_init(q_empty, 1);
+        mbar_init(q_full, 4);
         for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], 4);
-            mbar_init(&o_full[i], 1);
-            mbar_init(&o_empty[i], 4);
         }
+        mbar_init(o_full, 1);
+        mbar_init(o_empty, 4);
         mbar_init(done, 1);
-        for (int i = 0; i < 4; i++) {
-            mbar_init(&q_sc[i], kProducers);
+        for (int i = 0; i < 8; i++) {
             mbar_init(&k_sc[i], 1);
             mbar_init(&v_sc[i], 1);
-            mbar_init(&a_full[i], 4);
         }
+        for (int i = 0; i < 4; i++) mbar_init(&a_full[i], 4);
         fence_mbar_init();
         *abort = 0;
         for (int i = 0; i < 4; i++) k_max[i] = v_max[i] = 0;
         for (int i = 0; i < 8; i++) poison[i] = 0;
     }
-    // The work line, as in paged_attention_kernel.
+    // The work line, as in paged_attention_kernel (the first kM threads).
     const int seqs = seq_count(p);
     const int per = (seqs + kM - 1) / kM;
-    if (threadIdx.x < kM) {
-        long long n = 0;
+    long long mine = 0, upto = 0;
+    if (warp < 4) {
         for (int i = 0; i < per; i++) {
             const int b = threadIdx.x * per + i;
             if (b < seqs) {
                 Cursor c;
                 seq_load(p, b, c);
-                n += seq_units(p, c);
+                mine += seq_units(p, c);
             }
         }
-        sums[threadIdx.x + 1] = n;
+        upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) sums[warp] = upto;
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        sums[0] = 0;
-        for (int i = 1; i <= kM; i++) sums[i] += sums[i - 1];
+    long long U = 0;
+    for (int w = 0; w < 4; w++) {
+        if (w < warp) upto += sums[w];
+        U += sums[w];
     }
-    __syncthreads();
-    const long long U = sums[kM];
     const long long grid = min((long long)gridDim.x, U);
     if (blockIdx.x >= grid) {
         pdl_wait();
@@ -302,21 +292,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    const long long u0 = U * blockIdx.x / grid, u1 = U * (blockIdx.x + 1) / grid;
+    if (warp < 4 && upto - mine <= u0 && u0 < upto) {
+        sums[4] = threadIdx.x;
+        sums[5] = upto - mine;
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t s_tm = tmem, o_tm = tmem + 2 * 128;  // two buffers of 128 columns each
-    const long long u0 = U * blockIdx.x / grid, u1 = U * (blockIdx.x + 1) / grid;
+    const uint32_t s_tm = tmem, o_tm = tmem + 256, q_tm = tmem + 384;  // S: two buffers
     const int N = (int)(u1 - u0);
     Cursor c;
-    {
-        int lo = 0;
-        for (int i = kM; i > 0; i >>= 1)
-            while (lo + i <= kM && sums[lo + i] <= u0) lo += i;
-        seq_load(p, min(lo * per, seqs - 1), c);
-        cursor_at(p, c, u0 - sums[lo]);
-    }
+    seq_load(p, (int)sums[4] * per, c);
+    cursor_at(p, c, u0 - sums[5]);
     pdl_wait();
 
     // No wait below ends a loop: after one that gave up (the abort word is
@@ -333,71 +322,127 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         const int r = threadIdx.x;
         const uint32_t lane_tm = (uint32_t)(warp * 32) << 16;
         float m = -INFINITY, l = 0.f, qs = 1.f;
-        int hi = 0, lo = 0, seg = -1;
+        int hi = 0, lo = 0;
         bool first = true;
         for (int n = 0; n < N; n++) {
-            mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-            tc_fence_after();
             if (first) {
-                seg++;
-                mbar_wait(&q_sc[seg & 3], (seg >> 2) & 1, p.a.err, abort, kLimitNs);
-                qs = q_scale[(seg & 3) * kM + r];
+                // The row to TMEM: hi in columns 0 .. DP / 2, lo behind them.
+                // The segment before is through with Q (its last S is read).
+                const int row = c.r0 + r, tok = row / G;
+                const bool live = r < c.rows;
+                const float *q = p.a.q + (live ? ((size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G)) * D : 0);
+                const bool vec = aligned16(p.a.q);
+                auto load4 = [&](int d, float(&x)[4]) {
+                    if (live && d < D && vec) {
+                        const float4 v = *reinterpret_cast<const float4 *>(q + d);
+                        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) x[e] = live && d < D ? q[d + e] : 0.f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[e] *= p.scale_log2;
+                };
+                uint32_t top = 0;
+#pragma unroll 8
+                for (int d = 0; d < DP; d += 4) {
+                    float x[4];
+                    load4(d, x);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                }
+                const int ex = scale_exponent(top);
+                const float sc = pow2(kShift - ex);
+                qs = pow2(ex - kShift);
+#pragma unroll 1
+                for (int h = 0; h < DP / 32; h++) {
+                    uint32_t qh[16], ql[16];
+#pragma unroll
+                    for (int d = 0; d < 32; d += 4) {
+                        float x[4];
+                        load4(32 * h + d, x);
+#pragma unroll
+                        for (int e = 0; e < 4; e += 2) {
+                            const float u = x[e] * sc, v = x[e + 1] * sc;
+                            qh[(d + e) / 2] = pack_h2(u, v);
+                            const float2 b = unpack_h2(qh[(d + e) / 2]);
+                            ql[(d + e) / 2] = pack_h2(u - b.x, v - b.y);
+                        }
+                    }
+                    tmem_st16(q_tm + lane_tm + 16 * h, qh);
+                    tmem_st16(q_tm + lane_tm + DP / 2 + 16 * h, ql);
+                }
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(q_full);
                 m = -INFINITY;
                 l = 0.f;
                 // Row r sees key indexes i < hi with i >= lo or i < sinks.
                 hi = c.keys;
                 lo = 0;
                 if (!p.prefix_pass) {
-                    const int at = c.past + (c.r0 + r) / G;
+                    const int at = c.past + tok;
                     hi = min(hi, at + 1 - c.low + c.sink);
                     if (p.a.window) lo = max(at - p.a.window + 1 - c.low, 0) + c.sink;
                 }
             }
+            mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
+            mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
+            tc_fence_after();
             const int i0 = c.tile * kKeys;
             // Rows past the tile's last hold zeros; they need no mask.
             const bool whole = i0 + kKeys <= hi && (i0 >= lo || i0 + kKeys <= p.a.sinks);
             const bool masked = __any_sync(0xffffffffu, !whole);
-            mbar_wait(&k_sc[n & 3], (n >> 2) & 1, p.a.err, abort, kLimitNs);
-            const float f = qs * k_scale[n & 3];
+            const float f = qs * k_scale[n & 7];
             const uint32_t st = s_tm + (n & 1) * 128 + lane_tm;
-            float mx = -INFINITY;
+            // Both passes over the row, with the mask only where a row needs it.
+            float nm, a, sum = 0.f;
+            auto row = [&](auto mask) {
+                constexpr bool kMask = decltype(mask)::value;
+                const int h0 = hi - i0, l0 = lo - i0, s0 = p.a.sinks - i0;
+                float mx = -INFINITY;
 #pragma unroll 1
-            for (int h = 0; h < 4; h++) {
-                uint32_t x[32];
-                tmem_ld32_async(st + 32 * h, x);
-                tmem_wait_ld(x);
+                for (int h = 0; h < 4; h++) {
+                    uint32_t x[32];
+                    tmem_ld32_async(st + 32 * h, x);
+                    tmem_wait_ld(x);
 #pragma unroll
-                for (int j = 0; j < 32; j++) {
-                    const int i = i0 + 32 * h + j;
-                    if (!masked || (i < hi && (i >= lo || i < p.a.sinks))) mx = fmaxf(mx, __uint_as_float(x[j]));
-                }
-            }
-            const float nm = fmaxf(m, mx == -INFINITY ? mx : mx * f);
-            const float mu = nm == -INFINITY ? 0.f : nm - (float)kShift;
-            const float a = m == -INFINITY ? 0.f : ex2(m - nm);
-            float sum = 0.f;
-#pragma unroll 1
-            for (int h = 0; h < 4; h++) {
-                uint32_t x[32], ph[16], pl[16];
-                tmem_ld32_async(st + 32 * h, x);
-                tmem_wait_ld(x);
-#pragma unroll
-                for (int j = 0; j < 16; j++) {
-                    float e[2];
-#pragma unroll
-                    for (int y = 0; y < 2; y++) {
-                        const int i = i0 + 32 * h + 2 * j + y;
-                        e[y] = ex2(fmaf(__uint_as_float(x[2 * j + y]), f, -mu));
-                        if (masked && !(i < hi && (i >= lo || i < p.a.sinks))) e[y] = 0.f;
+                    for (int j = 0; j < 32; j++) {
+                        const int i = 32 * h + j;
+                        if (!kMask || (i < h0 && (i >= l0 || i < s0))) mx = fmaxf(mx, __uint_as_float(x[j]));
                     }
-                    sum += e[0] + e[1];
-                    ph[j] = pack_h2(e[0], e[1]);
-                    const float2 b = unpack_h2(ph[j]);
-                    pl[j] = pack_h2(e[0] - b.x, e[1] - b.y);
                 }
-                tmem_st16(st + 32 * h, ph);
-                tmem_st16(st + 32 * h + 16, pl);
-            }
+                nm = fmaxf(m, mx == -INFINITY ? mx : mx * f);
+                const float mu = nm == -INFINITY ? 0.f : nm - (float)kShift;
+                a = m == -INFINITY ? 0.f : ex2(m - nm);
+#pragma unroll 1
+                for (int h = 0; h < 4; h++) {
+                    uint32_t x[32], ph[16], pl[16];
+                    tmem_ld32_async(st + 32 * h, x);
+                    tmem_wait_ld(x);
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        float e[2];
+#pragma unroll
+                        for (int y = 0; y < 2; y++) {
+                            const int i = 32 * h + 2 * j + y;
+                            e[y] = ex2(fmaf(__uint_as_float(x[2 * j + y]), f, -mu));
+                            if (kMask && !(i < h0 && (i >= l0 || i < s0))) e[y] = 0.f;
+                        }
+                        sum += e[0] + e[1];
+                        ph[j] = pack_h2(e[0], e[1]);
+                        const float2 b = unpack_h2(ph[j]);
+                        pl[j] = pack_h2(e[0] - b.x, e[1] - b.y);
+                    }
+                    tmem_st16(st + 32 * h, ph);
+                    tmem_st16(st + 32 * h + 16, pl);
+                }
+            };
+            if (masked)
+                row(std::true_type());
+            else
+                row(std::false_type());
             m = nm;
             l = fmaf(l, a, sum);
             alpha[(n & 3) * kM + r] = a;
@@ -425,12 +470,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         for (int d = 0; d < DP; d++) acc[d] = 0.f;
         for (int n = 0; n < N; n++) {
             mbar_wait(&a_full[n & 3], (n >> 2) & 1, p.a.err, abort, kLimitNs);
-            mbar_wait(&v_sc[n & 3], (n >> 2) & 1, p.a.err, abort, kLimitNs);
-            mbar_wait(&o_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
+            mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
+            mbar_wait(o_full, n & 1, p.a.err, abort, kLimitNs);
             tc_fence_after();
-            const float a = alpha[(n & 3) * kM + r], vs = v_scale[n & 3];
+            const float a = alpha[(n & 3) * kM + r], vs = v_scale[n & 7];
             float m = row_ml[((n & 3) * kM + r) * 2], l = row_ml[((n & 3) * kM + r) * 2 + 1];
-            const uint32_t ot = o_tm + (n & 1) * 128 + lane_tm;
+            const uint32_t ot = o_tm + lane_tm;
 #pragma unroll
             for (int h = 0; h < DP / 16; h++) {
                 float x[16];
@@ -442,7 +487,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             const bool seg_end = c.tile == c.tiles - 1;
             if (!seg_end && n + 1 < N) {
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&o_empty[n & 1]);
+                if (lane == 0) mbar_arrive(o_empty);
                 cursor_next(p, c);
                 continue;
             }
@@ -451,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             bar_sync(2, 128);
             if (r == 0) poison[seg & 7] = 0;
             __syncwarp();
-            if (lane == 0) mbar_arrive(&o_empty[n & 1]);
+            if (lane == 0) mbar_arrive(o_empty);
             const bool live = r < c.rows;
             const int row = c.r0 + r, tok = row / G, at = c.past + tok;
             const size_t qrow = (size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G);
@@ -588,198 +633,192 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         const int pw = warp - 8;
         // Load i of a warp covers rows (i kProducers + pw) kRpi + sub.
         const int sub = lane / C::kLpr, col = (lane % C::kLpr) * C::kEpl;  // row of a load, first dim
+        // Where a row's 16 bytes land: in the operand's own place, or, for
+        // pairs, in the row's bytes of the slot (hi and lo blocks) in order.
+        auto raw_at = [&](int r) {
+            const int ch = lane % C::kLpr;
+            return C::kPair ? (uint32_t)((ch >> 3) * C::kBlockBytes + r * 128 + (ch & 7) * 16) : operand_at(r, col);
+        };
         const long long row_bytes = (long long)D * (int)sizeof(T);
-        bool first = true;
-        int seg = -1;
-        for (int n = 0; n < N; n++) {
-            if (first) {
-                seg++;
-                if (seg) mbar_wait(q_empty, (seg - 1) & 1, p.a.err, abort, kLimitNs);
-                const uint32_t qa = smem_addr(q_s);
-                for (int r = pw; r < kM; r += kProducers) {
-                    const int row = c.r0 + r, tok = row / G;
-                    const bool live = r < c.rows;
-                    const float *q =
-                        p.a.q + (live ? ((size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G)) * D : 0);
-                    constexpr int E = DP / 32;  // dims per lane: 2 or 4
-                    float x[E];
-                    uint32_t top = 0;
-#pragma unroll
-                    for (int e = 0; e < E; e++) {
-                        const int d = lane * E + e;
-                        x[e] = live && d < D ? q[d] * p.scale_log2 : 0.f;
-                        top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
-                    }
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    const int ex = scale_exponent(top);
-                    const float sc = pow2(kShift - ex);
-                    uint32_t h[E / 2], w[E / 2];
-#pragma unroll
-                    for (int e = 0; e < E / 2; e++) {
-                        const float u = x[2 * e] * sc, v = x[2 * e + 1] * sc;
-                        h[e] = pack_h2(u, v);
-                        const float2 b = unpack_h2(h[e]);
-                        w[e] = pack_h2(u - b.x, v - b.y);
-                    }
-                    const uint32_t at = qa + operand_at(r, lane * E, kM);
-                    if (E == 4) {
-                        sts64(at, h[0], h[E / 2 - 1]);
-                        sts64(at + C::kHalfBytes, w[0], w[E / 2 - 1]);
-                    } else {
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(h[0]) : "memory");
-                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + C::kHalfBytes), "r"(w[0]) : "memory");
-                    }
-                    if (lane == 0) q_scale[(seg & 3) * kM + r] = pow2(ex - kShift);
+        // Operand j is K of tile 0, then K of tile (j + 1) / 2 (odd j) or V of
+        // tile j / 2 - 1 (even j), while those tiles last: 2 N of them.
+        const int total = 2 * N;
+        auto is_v = [&](int j) { return j == total - 1 || (j > 0 && j % 2 == 0); };
+        auto tile_of = [&](int j) { return j == total - 1 ? N - 1 : j == 0 ? 0 : j % 2 ? (j + 1) / 2 : j / 2 - 1; };
+        // Rows that the lanes copy: of the tile whose keys come next, and of
+        // the one before it, whose values follow.
+        long long off_k = -1, off_v = -1;
+        // Segments of the operands being converted, for the poison flags.
+        Cursor cv = c;
+        int seg_k = 0, seg_v = 0;
+        auto copy = [&](int j) {
+            const bool v = is_v(j);
+            if (!v) {
+                if (j) {
+                    cursor_next(p, c);
+                    off_v = off_k;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&q_sc[seg & 3]);
-                    mbar_arrive(q_full);
-                }
-            }
-            // Lane i kRpi + sub looks up the row that load i takes there.
-            long long mine = -1;
-            {
+                // Lane i kRpi + sub looks up the row that load i takes there.
                 const int r = (lane / C::kRpi * kProducers + pw) * C::kRpi + lane % C::kRpi;
                 const int i = c.tile * kKeys + r;
+                off_k = -1;
                 if (r < kKeys && i < c.keys)
-                    mine = paged_row(p.a.cache, p.a.batch, c.b, i < c.sink ? i : i - c.sink + c.low, p.a.err) +
-                           c.kvh * row_bytes;
+                    off_k = paged_row(p.a.cache, p.a.batch, c.b, i < c.sink ? i : i - c.sink + c.low, p.a.err) +
+                            c.kvh * row_bytes;
             }
+            const long long mine = v ? (j == total - 1 ? off_k : off_v) : off_k;
+            if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+            unsigned char *slot = ring + (j % S) * C::kTileBytes;
+            const char *base = p.a.cache.base + (v ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
 #pragma unroll
-            for (int parity = 0; parity < 2; parity++) {
+            for (int i = 0; i < C::kLoads; i++) {
+                const int r = (i * kProducers + pw) * C::kRpi + sub;
+                const long long off = __shfl_sync(0xffffffffu, mine, i * C::kRpi + sub);
+                const bool live = off >= 0 && col < D;
+                if (r < kKeys) cp_async16_zfill(slot + raw_at(r), base + (live ? off : 0), live ? 16 : 0);
+            }
+        };
+        auto convert = [&](int j) {
+            const bool v = is_v(j);
+            const int n = tile_of(j);
+            unsigned char *slot = ring + (j % S) * C::kTileBytes;
+            const uint32_t at = smem_addr(slot);
+            int ex = kShift;  // the scale is 2^(kShift - ex)
+            if (!C::kRaw) {
+                // The tile's largest magnitude, over all producer warps.
                 uint4 x[C::kLoads];
+                uint32_t top = 0;
 #pragma unroll
                 for (int i = 0; i < C::kLoads; i++) {
-                    const long long off = __shfl_sync(0xffffffffu, mine, i * C::kRpi + sub);
-                    x[i] = off >= 0 && col < D
-                               ? __ldcg(reinterpret_cast<const uint4 *>(p.a.cache.base + off +
-                                                                        parity * p.a.cache.parity_stride +
-                                                                        col * (int)sizeof(T)))
-                               : make_uint4(0, 0, 0, 0);
-                }
-                int ex = kShift;  // the scale is 2^(kShift - ex)
-                bool inf = false;
-                if (!C::kRaw) {
-                    // The tile's largest magnitude, over all producer warps.
-                    uint32_t top = 0;
+                    const int r = (i * kProducers + pw) * C::kRpi + sub;
+                    x[i] = make_uint4(0, 0, 0, 0);
+                    if (r < kKeys) x[i] = *reinterpret_cast<const uint4 *>(slot + raw_at(r));
+                    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
 #pragma unroll
-                    for (int i = 0; i < C::kLoads; i++) {
-                        const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-#pragma unroll
-                        for (int y = 0; y < 4; y++) {
-                            if (C::kPair) {
-                                top = max(top, w[y] & 0x7fffffffu);
-                            } else {
-                                top = max(top, (w[y] << 16) & 0x7fffffffu);
-                                top = max(top, w[y] & 0x7fff0000u);
-                            }
+                    for (int y = 0; y < 4; y++) {
+                        if (C::kPair) {
+                            top = max(top, w[y] & 0x7fffffffu);
+                        } else {
+                            top = max(top, (w[y] << 16) & 0x7fffffffu);
+                            top = max(top, w[y] & 0x7fff0000u);
                         }
                     }
-                    top = __reduce_max_sync(0xffffffffu, top);
-                    uint32_t *slot = (parity ? v_max : k_max);
-                    if (lane == 0) atomicMax(&slot[n & 3], top);
-                    bar_sync(1, kProducers * 32);
-                    top = *reinterpret_cast<volatile uint32_t *>(&slot[n & 3]);
-                    // Next used in two tiles; last read two tiles ago.
-                    if (threadIdx.x == 8 * 32) slot[(n + 2) & 3] = 0;
-                    ex = scale_exponent(top);
-                    inf = top >= 0x7f800000u;
                 }
+                top = __reduce_max_sync(0xffffffffu, top);
+                uint32_t *most = v ? v_max : k_max;
+                if (lane == 0) atomicMax(&most[n & 3], top);
+                bar_sync(1, kProducers * 32);  // also: every row of the slot has been read
+                top = *reinterpret_cast<volatile uint32_t *>(&most[n & 3]);
+                // Next used in two tiles; last read two tiles ago.
+                if (threadIdx.x == 8 * 32) most[(n + 2) & 3] = 0;
+                ex = scale_exponent(top);
+                if (threadIdx.x == 8 * 32 && top >= 0x7f800000u) poison[(v ? seg_v : seg_k) & 7] = 1;
                 const float sc = pow2(kShift - ex);
-                uint64_t *empty = parity ? v_empty : k_empty, *full = parity ? v_full : k_full;
-                const int st = n % S;
-                if (n >= S) mbar_wait(&empty[st], (n / S - 1) & 1, p.a.err, abort, kLimitNs);
-                // After the wait: the readers of the slots' last tile are through.
-                if (threadIdx.x == 8 * 32) {
-                    (parity ? v_scale : k_scale)[n & 3] = pow2(ex - kShift);
-                    if (inf) poison[seg & 7] = 1;
-                    mbar_arrive(&(parity ? v_sc : k_sc)[n & 3]);
-                }
-                const uint32_t base = smem_addr((parity ? v_s : k_s) + st * C::kTileBytes);
 #pragma unroll
                 for (int i = 0; i < C::kLoads; i++) {
                     const int r = (i * kProducers + pw) * C::kRpi + sub;
                     if (r >= kKeys) continue;
-                    const uint32_t at = base + operand_at(r, col, kKeys);
+                    const uint32_t to = at + operand_at(r, col);
                     const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                    if (C::kRaw) {
-                        sts128(at, x[i]);
-                    } else if (C::kPair) {
+                    if (C::kPair) {
                         const float a = __uint_as_float(w[0]) * sc, b = __uint_as_float(w[1]) * sc,
                                     d = __uint_as_float(w[2]) * sc, e = __uint_as_float(w[3]) * sc;
                         const uint32_t h0 = pack_h2(a, b), h1 = pack_h2(d, e);
                         const float2 f0 = unpack_h2(h0), f1 = unpack_h2(h1);
-                        sts64(at, h0, h1);
-                        sts64(at + C::kHalfBytes, pack_h2(a - f0.x, b - f0.y), pack_h2(d - f1.x, e - f1.y));
+                        sts64(to, h0, h1);
+                        sts64(to + C::kHalfBytes, pack_h2(a - f0.x, b - f0.y), pack_h2(d - f1.x, e - f1.y));
                     } else {
                         uint32_t h[4];
 #pragma unroll
                         for (int y = 0; y < 4; y++)
-                            h[y] = pack_h2(__uint_as_float(w[y] << 16) * sc,
-                                           __uint_as_float(w[y] & 0xffff0000u) * sc);
-                        sts128(at, make_uint4(h[0], h[1], h[2], h[3]));
+                            h[y] = pack_h2(__uint_as_float(w[y] << 16) * sc, __uint_as_float(w[y] & 0xffff0000u) * sc);
+                        sts128(to, make_uint4(h[0], h[1], h[2], h[3]));
                     }
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&full[st]);
             }
-            first = c.tile == c.tiles - 1;
-            if (n + 1 < N) cursor_next(p, c);
+            if (threadIdx.x == 8 * 32) {
+                (v ? v_scale : k_scale)[n & 7] = pow2(ex - kShift);
+                mbar_arrive(&(v ? v_sc : k_sc)[n & 7]);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&full[j % S]);
+        };
+        for (int j = 0; j < total + C::kAhead; j++) {
+            if (j < total) copy(j);
+            cp_async_commit();
+            const int k = j - C::kAhead;
+            if (k < 0) continue;
+            cp_async_wait<C::kAhead>();
+            if (C::kRaw) {
+                convert(k);
+                continue;
+            }
+            if (!is_v(k) && k > 0) {
+                seg_v = seg_k;  // the values that follow are of the tile before
+                seg_k += cv.tile == cv.tiles - 1;
+                cursor_next(p, cv);
+            }
+            if (k == total - 1) seg_v = seg_k;
+            convert(k);
         }
     } else {
         // ---- MMA issue ----------------------------------------------------
         if (lane == 0) {
-        const uint32_t qa = smem_addr(q_s), ka = smem_addr(k_s), va = smem_addr(v_s);
-        int seg = 0;
+        const uint32_t ra = smem_addr(ring);
+        int seg = 0, j = 0;  // j: the next operand
         bool first = true;
+        auto slot_wait = [&] {
+            mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
+            return ra + (j % S) * C::kTileBytes;
+        };
         auto qk = [&](int n) {
-            if (first) mbar_wait(q_full, seg & 1, p.a.err, abort, kLimitNs);
-            const int st = n % S;
-            mbar_wait(&k_full[st], (n / S) & 1, p.a.err, abort, kLimitNs);
-            first = c.tile == c.tiles - 1;
+            if (first) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
+            const uint32_t kb = slot_wait();
             if (!*abort) {
                 tc_fence_after();
-                const uint32_t d = s_tm + (n & 1) * 128, kb = ka + st * C::kTileBytes;
+                const uint32_t d = s_tm + (n & 1) * 128;
 #pragma unroll
                 for (int ks = 0; ks < DP / 16; ks++) {
                     const uint32_t off = (ks / 4) * C::kBlockBytes + (ks % 4) * 32;
+                    const uint32_t qh = q_tm + ks * 8;
                     const uint64_t kh = sw128_desc(kb + off);
-                    mma_ss(d, sw128_desc(qa + C::kHalfBytes + off), kh, C::kIdescS, ks > 0);
-                    if (C::kPair)
-                        mma_ss(d, sw128_desc(qa + off), sw128_desc(kb + C::kHalfBytes + off), C::kIdescS, 1u);
-                    mma_ss(d, sw128_desc(qa + off), kh, C::kIdescS, 1u);
+                    mma_ts(d, qh + DP / 2, kh, C::kIdescS, ks > 0);
+                    if (C::kPair) mma_ts(d, qh, sw128_desc(kb + C::kHalfBytes + off), C::kIdescS, 1u);
+                    mma_ts(d, qh, kh, C::kIdescS, 1u);
                 }
-                mma_commit(&k_empty[st]);
+                mma_commit(&empty[j % S]);
                 mma_commit(&s_full[n & 1]);
-                if (first) mma_commit(q_empty);
             }
-            if (first) seg++;
+            j++;
+            first = c.tile == c.tiles - 1;  // of the next tile
             if (n + 1 < N) cursor_next(p, c);
+        };
+        auto pv = [&](int n) {
+            mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
+            const uint32_t vb = slot_wait();
+            if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
+            if (!*abort) {
+                tc_fence_after();
+                const uint32_t pt = s_tm + (n & 1) * 128;
+#pragma unroll
+                for (int ks = 0; ks < kKeys / 16; ks++) {
+                    const uint32_t ph = pt + (ks / 2) * 32 + (ks % 2) * 8;
+                    const uint64_t vh = sw128_desc_mn(vb + ks * 2048, C::kBlockBytes);
+                    mma_ts(o_tm, ph + 16, vh, C::kIdescO, ks > 0);
+                    if (C::kPair)
+                        mma_ts(o_tm, ph, sw128_desc_mn(vb + C::kHalfBytes + ks * 2048, C::kBlockBytes), C::kIdescO, 1u);
+                    mma_ts(o_tm, ph, vh, C::kIdescO, 1u);
+                }
+                mma_commit(&empty[j % S]);
+                mma_commit(o_full);
+            }
+            j++;
         };
         qk(0);
         for (int n = 0; n < N; n++) {
             if (n + 1 < N) qk(n + 1);
-            const int st = n % S;
-            mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-            mbar_wait(&v_full[st], (n / S) & 1, p.a.err, abort, kLimitNs);
-            if (n >= 2) mbar_wait(&o_empty[n & 1], ((n >> 1) - 1) & 1, p.a.err, abort, kLimitNs);
-            if (*abort) continue;
-            tc_fence_after();
-            const uint32_t d = o_tm + (n & 1) * 128, pt = s_tm + (n & 1) * 128, vb = va + st * C::kTileBytes;
-#pragma unroll
-            for (int ks = 0; ks < kKeys / 16; ks++) {
-                const uint32_t ph = pt + (ks / 2) * 32 + (ks % 2) * 8;
-                const uint64_t vh = sw128_desc_mn(vb + ks * 2048, C::kBlockBytes);
-                mma_ts(d, ph + 16, vh, C::kIdescO, ks > 0);
-                if (C::kPair)
-                    mma_ts(d, ph, sw128_desc_mn(vb + C::kHalfBytes + ks * 2048, C::kBlockBytes), C::kIdescO, 1u);
-                mma_ts(d, ph, vh, C::kIdescO, 1u);
-            }
-            mma_commit(&v_empty[st]);
-            mma_commit(&o_full[n & 1]);
+            pv(n);
         }
         // Every MMA issued must complete before TMEM is freed.
         mma_commit(done);
