@@ -4,16 +4,15 @@
 // query rows, kv head), a tile 128 keys, and the products run on tcgen05.
 //
 // Arithmetic. kind::f16 with f32 accumulators on pairs of f16: x = hi + lo
-// keeps 22 bits, and f16's denormals keep 2^-39 of the largest value below
-// that, given scales (powers of two, exact) that bring the largest value of a
-// query row, of a key tile and of a value tile to [2^14, 2^15). Probabilities
-// are taken 2^14 times as large for the same reason. An F32 cache needs three
-// products (lo hi, hi lo, hi hi) for S = Q K^T and for P V; F16 and BF16
-// values are one f16 each (to the same 2^-39), two products. A value that is
-// more than 2^18 times smaller than its tile's largest keeps fewer than 22
-// bits. Every tile's P V starts from zero and is added in f32 registers
-// (TMEM accumulation over thousands of keys would truncate thousands of
-// times).
+// keeps 22 bits, and f16's denormals keep what is below 2^-25, given scales
+// (powers of two, exact) that bring the largest value of a query row to
+// [2^14, 2^15) and of a key or value tile to [2^9, 2^15): the smallest step is
+// 2^-39 of a row's largest value, 2^-34 of a tile's. Probabilities are taken
+// 2^14 times as large for the same reason. An F32 cache needs three products
+// (lo hi, hi lo, hi hi) for S = Q K^T and for P V; F16 values are taken as
+// they are and BF16 values are one f16 each, two products. Every tile's P V
+// starts from zero and is added in f32 registers (TMEM accumulation over
+// thousands of keys would truncate thousands of times).
 //
 // One CTA per SM, 16 warps:
 //   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
@@ -21,15 +20,21 @@
 //          columns that S held
 //   4..7   output: one thread per row; O += P V of each tile in registers,
 //          the merge of a split segment, the result
-//   8..14  producers: K and V tiles from the pages by 16-byte asynchronous
-//          copies into a ring of slots, then in place (the tile's largest
-//          value, scale, f16 or f16 pair) the 128-byte swizzled operand
-//   15     issues the MMAs: Q K^T of the next tile before P V of this one
-// The ring holds operands in the order of their MMAs (K0 K1 V0 K2 V1 ...), so
-// a slot is free as soon as the MMA kSlots back is done; three slots of pairs
-// or six of single f16. Q and P are A operands from TMEM; K is read K-major
-// and V MN-major from the same layout ([key][64 dims] rows of 128 bytes).
-// TMEM: Q, two S / P buffers and O, 128 columns each.
+//   8..11  conversion in place: scale, f16 or f16 pair, zeros in rows that no
+//          query sees (they may hold anything). The scale is that of the
+//          operand before; a tile whose largest value does not suit it is
+//          read from the cache once more (a pass over each tile for its
+//          maximum would cost a quarter of the shared memory's bandwidth,
+//          which is what bounds an F32 cache).
+//   12     issues the MMAs: Q K^T of the next tile before P V of this one
+//   13     copies: one TMA box per page and 128-byte block into a ring of
+//          slots (pages that do not tile 128 rows in multiples of 8: 16-byte
+//          asynchronous copies, by warps 13..15)
+// The ring holds operands in the order K0 K1 V0 K2 V1 ..., so a slot is free
+// as soon as the MMAs kSlots back are done; three slots of pairs or six of
+// single f16. Q and P are A operands from TMEM; K is read K-major and V
+// MN-major from the same layout ([key][64 dims] rows of 128 bytes, 128-byte
+// swizzle). TMEM: Q, two S / P buffers and O, 128 columns each.
 //
 // Tensor-bound: 4 * pairs * D flops take 4 (16-bit cache) or 6 (F32) passes of
 // half as many MMA flops each.
@@ -39,6 +44,7 @@
 #include "kernels.h"
 #include "paged.cuh"
 #include "tcgen05.cuh"
+#include "tensormap.h"
 #include "tma.cuh"
 
 namespace slc {
@@ -47,13 +53,14 @@ namespace {
 
 constexpr int kM = 128;     // query rows per segment
 constexpr int kKeys = 128;  // keys per tile
-constexpr int kProducers = 7;
+constexpr int kConv = 4;    // conversion warps
+constexpr int kCopy = 3;    // copying warps where TMA boxes do not fit the pages
 constexpr int kThreads = 16 * 32;
-constexpr int kShift = 14;  // largest scaled value in [2^14, 2^15)
-// Registers a thread: 128 at launch; softmax, output, and the two warpgroups of
-// producers (the MMA warp is the last of them).
-constexpr int kLaunchRegs = 128, kSoftRegs = 104, kOutRegs = 200, kProdRegs = 104;
-static_assert(kSoftRegs + kOutRegs + 2 * kProdRegs <= 4 * kLaunchRegs, "register split");
+constexpr int kShift = 14;  // a query row's largest value in [2^14, 2^15), probabilities up to 2^14
+constexpr int kTop = 11;    // a tile's largest value around 2^11: from 2^9 to 2^15
+// Registers a thread, by warpgroup: 128 at launch.
+constexpr int kLaunchRegs = 128, kSoftRegs = 120, kOutRegs = 184, kConvRegs = 104, kRestRegs = 104;
+static_assert(kSoftRegs + kOutRegs + kConvRegs + kRestRegs <= 4 * kLaunchRegs, "register split");
 constexpr uint64_t kLimitNs = 4000000000ull;  // rows of values that are not finite take long
 
 template <typename T, int DP>
@@ -65,26 +72,34 @@ struct Cfg {
     static constexpr int kHalfBytes = kBlocks * kBlockBytes;  // one of hi, lo
     static constexpr int kTileBytes = kHalfBytes * (kPair ? 2 : 1);
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
-    static constexpr int kAhead = kSlots / 2;                // operands copied ahead of the one converted
+    static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 4 * DP + 16) + 8 * (8 + 2 * kSlots + 8 + 20);
+    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 4 * DP + 16) + 8 * (8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
     static constexpr int kLpr = DP / kEpl;               // lanes per cache row
     static constexpr int kRpi = 32 / kLpr;               // rows per warp load
-    static constexpr int kLoads = (kKeys / kRpi + kProducers - 1) / kProducers;
+    static constexpr int kRows = kKeys / kConv / kRpi;   // 16-byte pieces per conversion lane
     // f32 accumulators, f16 operands, K-major A; B K-major (S) or MN-major (O).
     static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
     static constexpr uint32_t kIdescO =
         (1u << 4) | (1u << 16) | ((uint32_t)(DP >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
 };
 
-// A segment of the work line and a place in it.
+struct RowsArgs {
+    PagedPass pass;
+    CUtensorMap map;  // [pages][2][page][kv_heads][head_dim], box [128 bytes][1][unit][1][1]
+    int unit;         // keys per box; 1: no boxes
+};
+
+// A segment of the work line and a place in it. Key indexes run over
+// positions [0, sink) and from `low` on, both widened to whole boxes; the
+// positions that some row sees are those below `sinks` and from `from` on.
 struct Cursor {
     int b, rt, kvh, tile;  // sequence, row tile, kv head, key tile
     int tok0, ntok, past;  // of the sequence
     int r0, rows;          // of the row tile
-    int sink, low, keys, tiles;
+    int sink, low, from, keys, tiles;
 };
 
 __device__ __forceinline__ int group_of(const PagedPass &p) { return p.a.heads / p.a.kv_heads; }
@@ -108,39 +123,43 @@ __device__ __forceinline__ int row_tiles(const PagedPass &p, const Cursor &c) {
     return (int)(((long long)c.ntok * group_of(p) + kM - 1) / kM);
 }
 // The keys of row tile c.rt: those that any of its rows sees.
-__device__ __forceinline__ void row_tile_load(const PagedPass &p, Cursor &c) {
+__device__ __forceinline__ void row_tile_load(const PagedPass &p, int unit, Cursor &c) {
     const int G = group_of(p);
     c.r0 = c.rt * kM;
     c.rows = min(kM, c.ntok * G - c.r0);
     c.sink = 0;
-    c.low = p.first;
+    c.from = p.first;
+    c.low = p.first - p.first % unit;
     if (p.prefix_pass) {
         c.keys = p.a.prefix;
     } else {
         const int first = c.past + c.r0 / G, last = c.past + (c.r0 + c.rows - 1) / G;
         if (p.a.window) {
-            c.low = max(first + 1 - p.a.window, 0);
-            c.sink = min(p.a.sinks, c.low);
+            c.from = max(first + 1 - p.a.window, 0);
+            c.low = c.from - c.from % unit;
+            const int sinks = min(p.a.sinks, c.from);
+            c.sink = (sinks + unit - 1) / unit * unit;
+            if (c.sink >= c.low) c.sink = c.low = 0;
         }
         c.keys = c.sink + last + 1 - c.low;
     }
     c.tiles = (c.keys + kKeys - 1) / kKeys;
 }
-__device__ __forceinline__ long long seq_units(const PagedPass &p, Cursor &c) {
+__device__ __forceinline__ long long seq_units(const PagedPass &p, int unit, Cursor &c) {
     long long n = 0;
     const int rts = row_tiles(p, c);
     for (c.rt = 0; c.rt < rts; c.rt++) {
-        row_tile_load(p, c);
+        row_tile_load(p, unit, c);
         n += c.tiles;
     }
     return n * p.a.kv_heads;
 }
 // Places the cursor on unit `at` of the line from sequence c.b on (c.rt 0).
-__device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor &c, long long at) {
+__device__ __forceinline__ void cursor_at(const PagedPass &p, int unit, Cursor &c, long long at) {
     for (;;) {
         const int rts = row_tiles(p, c);
         for (c.rt = 0; c.rt < rts; c.rt++) {
-            row_tile_load(p, c);
+            row_tile_load(p, unit, c);
             const long long n = (long long)c.tiles * p.a.kv_heads;
             if (at < n) {
                 c.kvh = (int)(at / c.tiles);
@@ -154,20 +173,36 @@ __device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor &c, long lo
     }
 }
 // The next unit; the line's end is the caller's to know.
-__device__ __forceinline__ void cursor_next(const PagedPass &p, Cursor &c) {
+__device__ __forceinline__ void cursor_next(const PagedPass &p, int unit, Cursor &c) {
     if (++c.tile < c.tiles) return;
     c.tile = 0;
     if (++c.kvh < p.a.kv_heads) return;
     c.kvh = 0;
     if (++c.rt < row_tiles(p, c)) {
-        row_tile_load(p, c);
+        row_tile_load(p, unit, c);
         return;
     }
     if (p.prefix_pass || c.b + 1 >= p.a.batch.seqs) return;
     seq_load(p, c.b + 1, c);
-    cursor_at(p, c, 0);
+    cursor_at(p, unit, c, 0);
 }
 
+// Position of key index i.
+__device__ __forceinline__ int key_pos(const Cursor &c, int i) { return i < c.sink ? i : i - c.sink + c.low; }
+// Whether some row of the segment may see key index i.
+__device__ __forceinline__ bool live_key(const PagedPass &p, const Cursor &c, int i) {
+    const int pos = key_pos(c, i);
+    return i < c.keys && (pos >= c.from || ((i < c.sink || c.sink == c.low) && pos < p.a.sinks));
+}
+
+__device__ __forceinline__ void tma_load_5d(void *dst, const void *map, int x, int y, int z, int u, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(w), "r"(smem_addr(bar))
+        : "memory");
+}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
@@ -192,6 +227,43 @@ __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
 __device__ __forceinline__ float2 unpack_h2(uint32_t w) {
     return __half22float2(*reinterpret_cast<const __half2 *>(&w));
 }
+// Two f32 operations at a time.
+struct F2 {
+    uint64_t v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float a, float b) {
+        asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b));
+    }
+    __device__ __forceinline__ float2 get() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+// An f16 pair of x, and of what it leaves.
+__device__ __forceinline__ void split2(F2 x, uint32_t &hi, uint32_t &lo) {
+    const float2 f = x.get();
+    hi = pack_h2(f.x, f.y);
+    const float2 b = unpack_h2(hi);
+    const float2 r = fma2(F2(b.x, b.y), F2(-1.f, -1.f), x).get();
+    lo = pack_h2(r.x, r.y);
+}
+
 // Element (row, dim) of a swizzled operand: block dim / 64 of rows of 128
 // bytes, 16-byte chunks xored with the row.
 __device__ __forceinline__ uint32_t operand_at(int row, int dim) {
@@ -199,20 +271,20 @@ __device__ __forceinline__ uint32_t operand_at(int row, int dim) {
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ PagedPass p) {
+__global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ RowsArgs args) {
+    const PagedPass &p = args.pass;
+    const int unit = args.unit;
     using C = Cfg<T, DP>;
     constexpr int S = C::kSlots;
     extern __shared__ __align__(1024) unsigned char smem_raw[];
-    const uint32_t raw = smem_addr(smem_raw);
-    unsigned char *smem = smem_raw + ((1024 - (raw & 1023)) & 1023);
+    unsigned char *smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     unsigned char *ring = smem;                         // [S] operands: hi[, lo]
     float *row_ml = reinterpret_cast<float *>(smem + C::kRing);  // [4 tiles][kM][2]
     float *alpha = row_ml + 4 * kM * 2;                 // [4 tiles][kM]
     float *k_scale = alpha + 4 * kM;                    // [8 tiles]
     float *v_scale = k_scale + 8;                       // [8 tiles]
-    uint32_t *k_max = reinterpret_cast<uint32_t *>(v_scale + 8);  // [4 tiles]
-    uint32_t *v_max = k_max + 4;                        // [4 tiles]
-    int *poison = reinterpret_cast<int *>(v_max + 4);   // [8 segments]
+    uint32_t *most = reinterpret_cast<uint32_t *>(v_scale + 8);   // [4 operands, 4 unused]
+    int *poison = reinterpret_cast<int *>(most + 8);    // [8 segments]
     float *scratch = reinterpret_cast<float *>(poison + 8);       // [4 warps][DP]
     int *flags = reinterpret_cast<int *>(scratch + 4 * DP);
     volatile int *abort = flags;
@@ -220,7 +292,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     int *last_s = flags + 2;
     long long *sums = reinterpret_cast<long long *>(flags + 4);   // [4] a scan's warps, [2] what it found
     uint64_t *bars = reinterpret_cast<uint64_t *>(sums + 6);
-    uint64_t *full = bars, *empty = full + S;           // [S] the ring's
+    uint64_t *raw = bars, *full = raw + S, *empty = full + S;  // [S] the ring's: copied, converted, used
     uint64_t *q_full = empty + S, *s_full = q_full + 1, *p_full = s_full + 2, *o_full = p_full + 2,
              *o_empty = o_full + 1, *done = o_empty + 1;
     // What threads pass each other beside the operands, in rings long enough
@@ -233,7 +305,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     pdl_trigger();
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; i++) {
-            mbar_init(&full[i], kProducers);
+            mbar_init(&raw[i], unit > 1 ? 1 : kCopy);
+            mbar_init(&full[i], kConv);
             mbar_init(&empty[i], 1);
         }
         mbar_init(q_full, 4);
@@ -251,7 +324,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         for (int i = 0; i < 4; i++) mbar_init(&a_full[i], 4);
         fence_mbar_init();
         *abort = 0;
-        for (int i = 0; i < 4; i++) k_max[i] = v_max[i] = 0;
+        for (int i = 0; i < 4; i++) most[i] = 0;
         for (int i = 0; i < 8; i++) poison[i] = 0;
     }
     // The work line, as in paged_attention_kernel (the first kM threads).
@@ -264,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             if (b < seqs) {
                 Cursor c;
                 seq_load(p, b, c);
-                mine += seq_units(p, c);
+                mine += seq_units(p, unit, c);
             }
         }
         upto = mine;
@@ -286,7 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         pdl_wait();
         return;
     }
-    if (warp == 15) {
+    if (warp == 12) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                          smem_addr(tmem_slot))
                      : "memory");
@@ -305,8 +378,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     const int N = (int)(u1 - u0);
     Cursor c;
     seq_load(p, (int)sums[4] * per, c);
-    cursor_at(p, c, u0 - sums[5]);
+    cursor_at(p, unit, c, u0 - sums[5]);
     pdl_wait();
+
+    // Operand j of the ring: K of tile 0, then K of tile (j + 1) / 2 (odd j)
+    // or V of tile j / 2 - 1 (even j) while those last, 2 N in all.
+    const int total = 2 * N;
+    auto is_v = [&](int j) { return j == total - 1 || (j > 0 && j % 2 == 0); };
+    auto tile_of = [&](int j) { return j == total - 1 ? N - 1 : j == 0 ? 0 : j % 2 ? (j + 1) / 2 : j / 2 - 1; };
 
     // No wait below ends a loop: after one that gave up (the abort word is
     // set) every role runs through its remaining steps without waiting, so
@@ -315,8 +394,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     else if (warp < 8)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kOutRegs));
+    else if (warp < 12)
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
     else
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kProdRegs));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
     if (warp < 4) {
         // ---- softmax ------------------------------------------------------
         const int r = threadIdx.x;
@@ -326,51 +407,58 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         bool first = true;
         for (int n = 0; n < N; n++) {
             if (first) {
-                // The row to TMEM: hi in columns 0 .. DP / 2, lo behind them.
-                // The segment before is through with Q (its last S is read).
+                // The row to TMEM: first as it is, 128 columns, while its largest
+                // value is found, then every 32 columns in place as 16 of hi
+                // and 16 of lo. The segment before is through with Q (its
+                // last S is read).
                 const int row = c.r0 + r, tok = row / G;
                 const bool live = r < c.rows;
                 const float *q = p.a.q + (live ? ((size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G)) * D : 0);
                 const bool vec = aligned16(p.a.q);
-                auto load4 = [&](int d, float(&x)[4]) {
-                    if (live && d < D && vec) {
-                        const float4 v = *reinterpret_cast<const float4 *>(q + d);
-                        x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
-                    } else {
+                float top = 0.f;
+#pragma unroll 1
+                for (int h = 0; h < DP; h += 64) {
+                    uint32_t x[4][16];
 #pragma unroll
-                        for (int e = 0; e < 4; e++) x[e] = live && d < D ? q[d + e] : 0.f;
+                    for (int d = 0; d < 64; d += 4) {
+                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (live && h + d < D) {
+                            if (vec)
+                                v = *reinterpret_cast<const float4 *>(q + h + d);
+                            else
+                                v = make_float4(q[h + d], q[h + d + 1], q[h + d + 2], q[h + d + 3]);
+                        }
+                        x[d / 16][d % 16] = __float_as_uint(v.x);
+                        x[d / 16][d % 16 + 1] = __float_as_uint(v.y);
+                        x[d / 16][d % 16 + 2] = __float_as_uint(v.z);
+                        x[d / 16][d % 16 + 3] = __float_as_uint(v.w);
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[e] *= p.scale_log2;
-                };
-                uint32_t top = 0;
-#pragma unroll 8
-                for (int d = 0; d < DP; d += 4) {
-                    float x[4];
-                    load4(d, x);
+                    for (int y = 0; y < 4; y++) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) top = max(top, __float_as_uint(x[e]) & 0x7fffffffu);
+                        for (int d = 0; d < 16; d++) {
+                            const float f = __uint_as_float(x[y][d]) * p.scale_log2;
+                            x[y][d] = __float_as_uint(f);
+                            top = fmaxf(top, fabsf(f));
+                        }
+                        tmem_st16(q_tm + lane_tm + h + 16 * y, x[y]);
+                    }
                 }
-                const int ex = scale_exponent(top);
+                tmem_wait_st();
+                const int ex = scale_exponent(__float_as_uint(top));
                 const float sc = pow2(kShift - ex);
                 qs = pow2(ex - kShift);
 #pragma unroll 1
-                for (int h = 0; h < DP / 32; h++) {
-                    uint32_t qh[16], ql[16];
+                for (int h = 0; h < DP; h += 32) {
+                    uint32_t x[32], qh[16], ql[16];
+                    tmem_ld32_async(q_tm + lane_tm + h, x);
+                    tmem_wait_ld(x);
 #pragma unroll
-                    for (int d = 0; d < 32; d += 4) {
-                        float x[4];
-                        load4(32 * h + d, x);
-#pragma unroll
-                        for (int e = 0; e < 4; e += 2) {
-                            const float u = x[e] * sc, v = x[e + 1] * sc;
-                            qh[(d + e) / 2] = pack_h2(u, v);
-                            const float2 b = unpack_h2(qh[(d + e) / 2]);
-                            ql[(d + e) / 2] = pack_h2(u - b.x, v - b.y);
-                        }
-                    }
-                    tmem_st16(q_tm + lane_tm + 16 * h, qh);
-                    tmem_st16(q_tm + lane_tm + DP / 2 + 16 * h, ql);
+                    for (int d = 0; d < 16; d++)
+                        split2(mul2(F2(__uint_as_float(x[2 * d]), __uint_as_float(x[2 * d + 1])), F2(sc, sc)), qh[d],
+                               ql[d]);
+                    tmem_st16(q_tm + lane_tm + h, qh);
+                    tmem_st16(q_tm + lane_tm + h + 16, ql);
                 }
                 tmem_wait_st();
                 tc_fence_before();
@@ -380,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 l = 0.f;
                 // Row r sees key indexes i < hi with i >= lo or i < sinks.
                 hi = c.keys;
-                lo = 0;
+                lo = c.from - c.low + c.sink;
                 if (!p.prefix_pass) {
                     const int at = c.past + tok;
                     hi = min(hi, at + 1 - c.low + c.sink);
@@ -397,7 +485,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             const float f = qs * k_scale[n & 7];
             const uint32_t st = s_tm + (n & 1) * 128 + lane_tm;
             // Both passes over the row, with the mask only where a row needs it.
-            float nm, a, sum = 0.f;
+            float nm, a;
+            F2 sum2(0.f, 0.f);
             auto row = [&](auto mask) {
                 constexpr bool kMask = decltype(mask)::value;
                 const int h0 = hi - i0, l0 = lo - i0, s0 = p.a.sinks - i0;
@@ -423,17 +512,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     tmem_wait_ld(x);
 #pragma unroll
                     for (int j = 0; j < 16; j++) {
-                        float e[2];
-#pragma unroll
-                        for (int y = 0; y < 2; y++) {
-                            const int i = 32 * h + 2 * j + y;
-                            e[y] = ex2(fmaf(__uint_as_float(x[2 * j + y]), f, -mu));
-                            if (kMask && !(i < h0 && (i >= l0 || i < s0))) e[y] = 0.f;
+                        const float2 z =
+                            fma2(F2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), F2(f, f), F2(-mu, -mu))
+                                .get();
+                        float e0 = ex2(z.x), e1 = ex2(z.y);
+                        if (kMask) {
+                            const int i = 32 * h + 2 * j;
+                            if (!(i < h0 && (i >= l0 || i < s0))) e0 = 0.f;
+                            if (!(i + 1 < h0 && (i + 1 >= l0 || i + 1 < s0))) e1 = 0.f;
                         }
-                        sum += e[0] + e[1];
-                        ph[j] = pack_h2(e[0], e[1]);
-                        const float2 b = unpack_h2(ph[j]);
-                        pl[j] = pack_h2(e[0] - b.x, e[1] - b.y);
+                        const F2 e(e0, e1);
+                        sum2 = add2(sum2, e);
+                        split2(e, ph[j], pl[j]);
                     }
                     tmem_st16(st + 32 * h, ph);
                     tmem_st16(st + 32 * h + 16, pl);
@@ -444,7 +534,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             else
                 row(std::false_type());
             m = nm;
-            l = fmaf(l, a, sum);
+            l = fmaf(l, a, sum2.get().x + sum2.get().y);
             alpha[(n & 3) * kM + r] = a;
             first = c.tile == c.tiles - 1;
             if (first || n == N - 1) {
@@ -458,16 +548,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 mbar_arrive(&a_full[n & 3]);
                 mbar_arrive(&p_full[n & 1]);
             }
-            if (n + 1 < N) cursor_next(p, c);
+            if (n + 1 < N) cursor_next(p, unit, c);
         }
     } else if (warp < 8) {
         // ---- output -------------------------------------------------------
         const int r = threadIdx.x - 128, ow = warp - 4;
         const uint32_t lane_tm = (uint32_t)(ow * 32) << 16;
-        float acc[DP];
+        F2 acc[DP / 2];
         int seg = 0, seg_n = 0;
 #pragma unroll
-        for (int d = 0; d < DP; d++) acc[d] = 0.f;
+        for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
         for (int n = 0; n < N; n++) {
             mbar_wait(&a_full[n & 3], (n >> 2) & 1, p.a.err, abort, kLimitNs);
             mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
@@ -481,17 +571,24 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 float x[16];
                 tmem_ld16(ot + 16 * h, x);
 #pragma unroll
-                for (int j = 0; j < 16; j++) acc[16 * h + j] = fmaf(acc[16 * h + j], a, x[j] * vs);
+                for (int j = 0; j < 8; j++) {
+                    F2 &d = acc[8 * h + j];
+                    d = fma2(d, F2(a, a), mul2(F2(x[2 * j], x[2 * j + 1]), F2(vs, vs)));
+                }
             }
             tc_fence_before();
             const bool seg_end = c.tile == c.tiles - 1;
             if (!seg_end && n + 1 < N) {
                 __syncwarp();
                 if (lane == 0) mbar_arrive(o_empty);
-                cursor_next(p, c);
+                cursor_next(p, unit, c);
                 continue;
             }
             // ---- end of this CTA's piece of the segment.
+            auto four = [&](int d) {
+                const float2 x = acc[2 * d].get(), y = acc[2 * d + 1].get();
+                return make_float4(x.x, x.y, y.x, y.y);
+            };
             const bool bad_tiles = poison[seg & 7] != 0;
             bar_sync(2, 128);
             if (r == 0) poison[seg & 7] = 0;
@@ -502,7 +599,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             const size_t qrow = (size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G);
             bool bad = bad_tiles || !finite(l) || !(m < INFINITY);
 #pragma unroll
-            for (int d = 0; d < DP; d++) bad |= !finite(acc[d]);
+            for (int d = 0; d < DP / 2; d++) bad |= !finite(acc[d].get().x) || !finite(acc[d].get().y);
             unsigned todo = __ballot_sync(0xffffffffu, bad && live);
             while (todo) {
                 const int src = __ffs(todo) - 1;
@@ -517,7 +614,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                         const int pos = i < c.sink ? i : i - c.sink + c.low;
                         if (p.prefix_pass) return pos;
                         const bool sees =
-                            pos <= rat && (!p.a.window || pos > rat - p.a.window || pos < p.a.sinks);
+                            pos <= rat && pos >= p.first && (!p.a.window || pos > rat - p.a.window || pos < p.a.sinks);
                         return sees ? pos : -1;
                     },
                     rm, rl, ro);
@@ -528,7 +625,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     m = rm;
                     l = rl;
 #pragma unroll
-                    for (int d = 0; d < DP; d++) acc[d] = scratch[ow * DP + d];
+                    for (int d = 0; d < DP / 2; d++)
+                        acc[d] = F2(scratch[ow * DP + 2 * d], scratch[ow * DP + 2 * d + 1]);
                 }
                 __syncwarp();
             }
@@ -539,8 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 const size_t slot = 2 * blockIdx.x + (a0 >= u0 ? 1 : 0);
                 float4 *po = reinterpret_cast<float4 *>(p.part_o) + slot * (DP / 4) * kM + r;
 #pragma unroll
-                for (int d = 0; d < DP / 4; d++)
-                    po[d * kM] = make_float4(acc[4 * d], acc[4 * d + 1], acc[4 * d + 2], acc[4 * d + 3]);
+                for (int d = 0; d < DP / 4; d++) po[d * kM] = four(d);
                 reinterpret_cast<float2 *>(p.part_ml)[slot * kM + r] = make_float2(m, l);
                 bar_sync(2, 128);
                 if (r == 0) {
@@ -566,10 +663,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                         for (int d = 0; d < DP / 4; d++) {
                             const float4 v = __ldcg(pp + d * kM);
-                            acc[4 * d] = fmaf(v.x, e, x == 0 ? 0.f : acc[4 * d] * f);
-                            acc[4 * d + 1] = fmaf(v.y, e, x == 0 ? 0.f : acc[4 * d + 1] * f);
-                            acc[4 * d + 2] = fmaf(v.z, e, x == 0 ? 0.f : acc[4 * d + 2] * f);
-                            acc[4 * d + 3] = fmaf(v.w, e, x == 0 ? 0.f : acc[4 * d + 3] * f);
+                            const F2 z(0.f, 0.f);
+                            acc[2 * d] = fma2(F2(v.x, v.y), F2(e, e), x == 0 ? z : mul2(acc[2 * d], F2(f, f)));
+                            acc[2 * d + 1] =
+                                fma2(F2(v.z, v.w), F2(e, e), x == 0 ? z : mul2(acc[2 * d + 1], F2(f, f)));
                         }
                         m = nm;
                     }
@@ -581,8 +678,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                     for (int d = 0; d < DP; d += 4)
                         if (d < D)
-                            *reinterpret_cast<float4 *>(dst + d) =
-                                make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+                            *reinterpret_cast<float4 *>(dst + d) = four(d / 4);
                     *reinterpret_cast<float2 *>(p.pre_ml + qrow * 2) = make_float2(m, l);
                 } else {
                     float f = 1.f, e = 0.f;
@@ -599,7 +695,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                     for (int d = 0; d < DP; d += 4) {
                         if (d >= D) continue;
-                        float4 o = make_float4(acc[d], acc[d + 1], acc[d + 2], acc[d + 3]);
+                        float4 o = four(d / 4);
                         if (pre) {
                             const float4 v = __ldcg(reinterpret_cast<const float4 *>(pre + d));
                             o.x = fmaf(v.x, e, o.x * f);
@@ -623,202 +719,300 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 }
             }
 #pragma unroll
-            for (int d = 0; d < DP; d++) acc[d] = 0.f;
+            for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
             seg++;
             seg_n = n + 1;
-            if (n + 1 < N) cursor_next(p, c);
+            if (n + 1 < N) cursor_next(p, unit, c);
         }
-    } else if (warp < 15) {
-        // ---- producers ----------------------------------------------------
+    } else if (warp < 12) {
+        // ---- conversion ---------------------------------------------------
         const int pw = warp - 8;
-        // Load i of a warp covers rows (i kProducers + pw) kRpi + sub.
-        const int sub = lane / C::kLpr, col = (lane % C::kLpr) * C::kEpl;  // row of a load, first dim
-        // Where a row's 16 bytes land: in the operand's own place, or, for
-        // pairs, in the row's bytes of the slot (hi and lo blocks) in order.
-        auto raw_at = [&](int r) {
-            const int ch = lane % C::kLpr;
-            return C::kPair ? (uint32_t)((ch >> 3) * C::kBlockBytes + r * 128 + (ch & 7) * 16) : operand_at(r, col);
-        };
-        const long long row_bytes = (long long)D * (int)sizeof(T);
-        // Operand j is K of tile 0, then K of tile (j + 1) / 2 (odd j) or V of
-        // tile j / 2 - 1 (even j), while those tiles last: 2 N of them.
-        const int total = 2 * N;
-        auto is_v = [&](int j) { return j == total - 1 || (j > 0 && j % 2 == 0); };
-        auto tile_of = [&](int j) { return j == total - 1 ? N - 1 : j == 0 ? 0 : j % 2 ? (j + 1) / 2 : j / 2 - 1; };
-        // Rows that the lanes copy: of the tile whose keys come next, and of
-        // the one before it, whose values follow.
-        long long off_k = -1, off_v = -1;
-        // Segments of the operands being converted, for the poison flags.
-        Cursor cv = c;
-        int seg_k = 0, seg_v = 0;
-        auto copy = [&](int j) {
-            const bool v = is_v(j);
-            if (!v) {
-                if (j) {
-                    cursor_next(p, c);
-                    off_v = off_k;
-                }
-                // Lane i kRpi + sub looks up the row that load i takes there.
-                const int r = (lane / C::kRpi * kProducers + pw) * C::kRpi + lane % C::kRpi;
-                const int i = c.tile * kKeys + r;
-                off_k = -1;
-                if (r < kKeys && i < c.keys)
-                    off_k = paged_row(p.a.cache, p.a.batch, c.b, i < c.sink ? i : i - c.sink + c.low, p.a.err) +
-                            c.kvh * row_bytes;
-            }
-            const long long mine = v ? (j == total - 1 ? off_k : off_v) : off_k;
-            if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
-            unsigned char *slot = ring + (j % S) * C::kTileBytes;
-            const char *base = p.a.cache.base + (v ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
-#pragma unroll
-            for (int i = 0; i < C::kLoads; i++) {
-                const int r = (i * kProducers + pw) * C::kRpi + sub;
-                const long long off = __shfl_sync(0xffffffffu, mine, i * C::kRpi + sub);
-                const bool live = off >= 0 && col < D;
-                if (r < kKeys) cp_async16_zfill(slot + raw_at(r), base + (live ? off : 0), live ? 16 : 0);
-            }
-        };
-        auto convert = [&](int j) {
+        // Piece i of a lane: row (i kConv + pw) kRpi + sub, 16 raw bytes from
+        // dim `col` on.
+        const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+        constexpr int kBatch = C::kRows < 8 ? C::kRows : 8;
+        auto row_of = [&](int i) { return (i * kConv + pw) * C::kRpi + sub; };
+        // Raw place of a row's piece, and the operand places of even and odd
+        // pieces: two pieces on is a multiple of 8 rows on.
+        const uint32_t raw0 = C::kPair ? (ch >> 3) * C::kBlockBytes + row_of(0) * 128 + (ch & 7) * 16
+                                       : operand_at(row_of(0), col);
+        const uint32_t raw1 = C::kPair ? raw0 + kConv * C::kRpi * 128 : operand_at(row_of(1), col);
+        const uint32_t op0 = operand_at(row_of(0), col), op1 = operand_at(row_of(1), col);
+        constexpr int kTwo = 2 * kConv * C::kRpi * 128;
+        auto raw_at = [&](int i) { return (i & 1 ? raw1 : raw0) + i / 2 * kTwo; };
+        Cursor cv = c;              // of the values that come next; c: of the keys
+        int seg_k = 0, seg_v = 0;  // their segments, for the poison flags
+        int e_k = 2, e_v = 2;      // exponents of the scales of the operands before
+        for (int j = 0; j < total; j++) {
             const bool v = is_v(j);
             const int n = tile_of(j);
+            if (!v && j > 0) {
+                cv = c;
+                seg_v = seg_k;
+                seg_k += c.tile == c.tiles - 1;
+                cursor_next(p, unit, c);
+            }
+            if (j == total - 1) {
+                cv = c;
+                seg_v = seg_k;
+            }
+            mbar_wait(&raw[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
             unsigned char *slot = ring + (j % S) * C::kTileBytes;
-            const uint32_t at = smem_addr(slot);
-            int ex = kShift;  // the scale is 2^(kShift - ex)
+            const Cursor &cu = v ? cv : c;
+            const int i0 = cu.tile * kKeys;
+            const bool whole = i0 + kKeys <= cu.keys &&
+                               (key_pos(cu, i0) >= cu.from || key_pos(cu, i0 + kKeys - 1) < p.a.sinks);
+            // Rows that no query sees may hold anything, or be of a tile before.
+            if (!whole && (v || !C::kRaw))
+#pragma unroll 1
+                for (int i = 0; i < C::kRows; i++)
+                    if (!live_key(p, cu, i0 + row_of(i)))
+                        *reinterpret_cast<uint4 *>(slot + raw_at(i)) = make_uint4(0, 0, 0, 0);
+            int ex = kTop;  // the scale is 2^(kTop - ex)
             if (!C::kRaw) {
-                // The tile's largest magnitude, over all producer warps.
-                uint4 x[C::kLoads];
-                uint32_t top = 0;
+                const uint32_t at = smem_addr(slot);
+                ex = v ? e_v : e_k;
+                for (int again = 0; again < 2; again++) {
+                    const F2 sc(pow2(kTop - ex), pow2(kTop - ex));
+                    float top = 0.f;
+#pragma unroll 1
+                    for (int ib = 0; ib < C::kRows; ib += kBatch) {
+                        const unsigned char *from = slot + ib / 2 * kTwo;
+                        const uint32_t to = at + ib / 2 * kTwo;
+                        uint4 x[kBatch];
 #pragma unroll
-                for (int i = 0; i < C::kLoads; i++) {
-                    const int r = (i * kProducers + pw) * C::kRpi + sub;
-                    x[i] = make_uint4(0, 0, 0, 0);
-                    if (r < kKeys) x[i] = *reinterpret_cast<const uint4 *>(slot + raw_at(r));
-                    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
+                        for (int y = 0; y < kBatch; y++) x[y] = *reinterpret_cast<const uint4 *>(from + raw_at(y));
+                        __syncwarp();  // a row of pairs is read whole before it is written
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
-                        if (C::kPair) {
-                            top = max(top, w[y] & 0x7fffffffu);
-                        } else {
-                            top = max(top, (w[y] << 16) & 0x7fffffffu);
-                            top = max(top, w[y] & 0x7fff0000u);
+                        for (int y = 0; y < kBatch; y++) {
+                            const uint32_t dst = to + (y & 1 ? op1 : op0) + y / 2 * kTwo;
+                            const uint32_t w[4] = {x[y].x, x[y].y, x[y].z, x[y].w};
+                            if (C::kPair) {
+#pragma unroll
+                                for (int z = 0; z < 4; z++) top = fmaxf(top, fabsf(__uint_as_float(w[z])));
+                                uint32_t h0, h1, l0, l1;
+                                split2(mul2(F2(__uint_as_float(w[0]), __uint_as_float(w[1])), sc), h0, l0);
+                                split2(mul2(F2(__uint_as_float(w[2]), __uint_as_float(w[3])), sc), h1, l1);
+                                sts64(dst, h0, h1);
+                                sts64(dst + C::kHalfBytes, l0, l1);
+                            } else {
+                                uint32_t h[4];
+#pragma unroll
+                                for (int z = 0; z < 4; z++) {
+                                    const float a = __uint_as_float(w[z] << 16),
+                                                b = __uint_as_float(w[z] & 0xffff0000u);
+                                    top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
+                                    const float2 f = mul2(F2(a, b), sc).get();
+                                    h[z] = pack_h2(f.x, f.y);
+                                }
+                                sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
+                            }
                         }
                     }
-                }
-                top = __reduce_max_sync(0xffffffffu, top);
-                uint32_t *most = v ? v_max : k_max;
-                if (lane == 0) atomicMax(&most[n & 3], top);
-                bar_sync(1, kProducers * 32);  // also: every row of the slot has been read
-                top = *reinterpret_cast<volatile uint32_t *>(&most[n & 3]);
-                // Next used in two tiles; last read two tiles ago.
-                if (threadIdx.x == 8 * 32) most[(n + 2) & 3] = 0;
-                ex = scale_exponent(top);
-                if (threadIdx.x == 8 * 32 && top >= 0x7f800000u) poison[(v ? seg_v : seg_k) & 7] = 1;
-                const float sc = pow2(kShift - ex);
-#pragma unroll
-                for (int i = 0; i < C::kLoads; i++) {
-                    const int r = (i * kProducers + pw) * C::kRpi + sub;
-                    if (r >= kKeys) continue;
-                    const uint32_t to = at + operand_at(r, col);
-                    const uint32_t w[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-                    if (C::kPair) {
-                        const float a = __uint_as_float(w[0]) * sc, b = __uint_as_float(w[1]) * sc,
-                                    d = __uint_as_float(w[2]) * sc, e = __uint_as_float(w[3]) * sc;
-                        const uint32_t h0 = pack_h2(a, b), h1 = pack_h2(d, e);
-                        const float2 f0 = unpack_h2(h0), f1 = unpack_h2(h1);
-                        sts64(to, h0, h1);
-                        sts64(to + C::kHalfBytes, pack_h2(a - f0.x, b - f0.y), pack_h2(d - f1.x, e - f1.y));
-                    } else {
-                        uint32_t h[4];
-#pragma unroll
-                        for (int y = 0; y < 4; y++)
-                            h[y] = pack_h2(__uint_as_float(w[y] << 16) * sc, __uint_as_float(w[y] & 0xffff0000u) * sc);
-                        sts128(to, make_uint4(h[0], h[1], h[2], h[3]));
+                    // The tile's largest magnitude, over the conversion warps
+                    // (a NaN is not counted: it shows in the results).
+                    const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
+                    const int place = (2 * j + again) & 3;
+                    if (lane == 0) atomicMax(&most[place], mine);
+                    bar_sync(1, kConv * 32);
+                    const uint32_t all = *reinterpret_cast<volatile uint32_t *>(&most[place]);
+                    bar_sync(1, kConv * 32);
+                    if (threadIdx.x == 8 * 32) most[place] = 0;
+                    if (all == 0) break;
+                    const int found = scale_exponent(all);
+                    if (threadIdx.x == 8 * 32 && all >= 0x7f800000u) poison[(v ? seg_v : seg_k) & 7] = 1;
+                    (v ? e_v : e_k) = found;
+                    if (again || (found <= ex + 3 && found >= ex - 2)) break;
+                    // Once more, from the cache.
+                    ex = found;
+#pragma unroll 1
+                    for (int i = 0; i < C::kRows; i++) {
+                        const int key = i0 + row_of(i);
+                        uint4 x = make_uint4(0, 0, 0, 0);
+                        if (live_key(p, cu, key) && col < D)
+                            x = __ldcg(reinterpret_cast<const uint4 *>(
+                                p.a.cache.base + paged_row(p.a.cache, p.a.batch, cu.b, key_pos(cu, key), p.a.err) +
+                                (v ? p.a.cache.parity_stride : 0) + (cu.kvh * D + col) * (long long)sizeof(T)));
+                        *reinterpret_cast<uint4 *>(slot + raw_at(i)) = x;
                     }
+                    __syncwarp();
                 }
             }
             if (threadIdx.x == 8 * 32) {
-                (v ? v_scale : k_scale)[n & 7] = pow2(ex - kShift);
+                (v ? v_scale : k_scale)[n & 7] = C::kRaw ? 1.f : pow2(ex - kTop);
                 mbar_arrive(&(v ? v_sc : k_sc)[n & 7]);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[j % S]);
-        };
-        for (int j = 0; j < total + C::kAhead; j++) {
-            if (j < total) copy(j);
-            cp_async_commit();
-            const int k = j - C::kAhead;
-            if (k < 0) continue;
-            cp_async_wait<C::kAhead>();
-            if (C::kRaw) {
-                convert(k);
-                continue;
+        }
+    } else if (warp > 12) {
+        // ---- copies -------------------------------------------------------
+        if (unit > 1) {
+            if (warp == 13) {
+                // Lane i copies box row i of the tile: `unit` keys of a page.
+                const int boxes = kKeys / unit;
+                constexpr int kBlk = DP * (int)sizeof(T) / 128;
+                uint32_t id = 0, id_v = 0;
+                int z = -1, z_v = -1, kvh_v = 0;  // key within the page; -1: no keys there
+                auto look_up = [&] {
+                    const int i = c.tile * kKeys + lane * unit;
+                    z = -1;
+                    if (lane < boxes && i < c.keys) {
+                        const int pos = key_pos(c, i), pg = page_of(p.a.cache, pos);
+                        z = pos - pg * p.a.cache.page;
+                        id = pg < p.a.batch.per_seq ? p.a.batch.table[(long long)c.b * p.a.batch.per_seq + pg] : ~0u;
+                    }
+                };
+                auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity) {
+                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+                    if (__any_sync(0xffffffffu, *abort)) return;
+                    if (at >= 0 && page_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
+                        report_error(p.a.err, kErrGatherId);
+                        page_id = 0;
+                    }
+                    const int count = __popc(__ballot_sync(0xffffffffu, at >= 0));
+                    if (lane == 0) mbar_arrive_expect_tx(&raw[j % S], count * unit * 128 * kBlk);
+                    __syncwarp();
+                    unsigned char *slot = ring + (j % S) * C::kTileBytes + lane * unit * 128;
+                    if (at >= 0)
+#pragma unroll
+                        for (int y = 0; y < kBlk; y++)
+                            tma_load_5d(slot + y * C::kBlockBytes, &args.map, y * (128 / (int)sizeof(T)), kvh, at, parity,
+                                        (int)page_id, &raw[j % S]);
+                };
+                if (lane == 0) prefetch_tensormap(&args.map);
+                look_up();
+                for (int n = 0; n < N; n++) {
+                    copy(n ? 2 * n - 1 : 0, id, z, c.kvh, 0);
+                    if (n) copy(2 * n, id_v, z_v, kvh_v, 1);
+                    id_v = id;
+                    z_v = z;
+                    kvh_v = c.kvh;
+                    if (n + 1 < N) {
+                        cursor_next(p, unit, c);
+                        look_up();
+                    }
+                }
+                copy(total - 1, id_v, z_v, kvh_v, 1);
+                // Copies still in flight must land before the CTA's shared
+                // memory is released (after a wait that gave up; else the
+                // MMAs have used them all).
+                if (*abort)
+                    for (int j = max(total - S, 0); j < total; j++) drain_wait(&raw[j % S], (j / S) & 1);
             }
-            if (!is_v(k) && k > 0) {
-                seg_v = seg_k;  // the values that follow are of the tile before
-                seg_k += cv.tile == cv.tiles - 1;
-                cursor_next(p, cv);
+        } else {
+            // Row (i kCopy + w) kRpi + sub by 16-byte pieces.
+            const int w = warp - 13, sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+            Cursor cv = c;
+            auto copy = [&](int j, const Cursor &cu, int parity) {
+                if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+                unsigned char *slot = ring + (j % S) * C::kTileBytes;
+#pragma unroll 2
+                for (int r = w * C::kRpi + sub; r < kKeys; r += kCopy * C::kRpi) {
+                    const int i = cu.tile * kKeys + r;
+                    const bool live = i < cu.keys && col < D;
+                    const char *src = p.a.cache.base;
+                    if (live)
+                        src += paged_row(p.a.cache, p.a.batch, cu.b, key_pos(cu, i), p.a.err) +
+                               (parity ? p.a.cache.parity_stride : 0) + (cu.kvh * D + col) * (long long)sizeof(T);
+                    cp_async16_zfill(slot + (C::kPair ? (ch >> 3) * C::kBlockBytes + r * 128 + (ch & 7) * 16
+                                                      : operand_at(r, col)),
+                                     src, live ? 16 : 0);
+                }
+            };
+            int done_j = 0;
+            auto landed = [&](int j) {
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&raw[j % S]);
+            };
+            for (int j = 0; j < total; j++) {
+                const bool v = is_v(j);
+                if (!v && j > 0) {
+                    cv = c;
+                    cursor_next(p, unit, c);
+                }
+                if (j == total - 1) cv = c;
+                copy(j, v ? cv : c, v);
+                cp_async_commit();
+                if (j >= C::kAhead) {
+                    cp_async_wait<C::kAhead>();
+                    landed(done_j++);
+                }
             }
-            if (k == total - 1) seg_v = seg_k;
-            convert(k);
+            cp_async_wait<0>();
+            while (done_j < total) landed(done_j++);
         }
     } else {
         // ---- MMA issue ----------------------------------------------------
         if (lane == 0) {
         const uint32_t ra = smem_addr(ring);
-        int seg = 0, j = 0;  // j: the next operand
-        bool first = true;
-        auto slot_wait = [&] {
+        int seg = 0;
+        bool first = true;  // the next tile begins a segment
+        auto slot_wait = [&](int j) {
             mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
             return ra + (j % S) * C::kTileBytes;
         };
         auto qk = [&](int n) {
             if (first) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
-            const uint32_t kb = slot_wait();
+            const int j = n ? 2 * n - 1 : 0;
+            const uint32_t kb = slot_wait(j);
             if (!*abort) {
                 tc_fence_after();
                 const uint32_t d = s_tm + (n & 1) * 128;
+                const uint64_t desc = sw128_desc(kb);
+#pragma unroll 1
+                for (int b = 0; b < C::kBlocks; b++) {
+                    // 64 dims: descriptors hold addresses in 16-byte units.
+                    const uint64_t kh = desc + b * (C::kBlockBytes / 16);
+                    const uint32_t qh = q_tm + b * 64;
 #pragma unroll
-                for (int ks = 0; ks < DP / 16; ks++) {
-                    const uint32_t off = (ks / 4) * C::kBlockBytes + (ks % 4) * 32;
-                    const uint32_t qh = q_tm + ks * 8;
-                    const uint64_t kh = sw128_desc(kb + off);
-                    mma_ts(d, qh + DP / 2, kh, C::kIdescS, ks > 0);
-                    if (C::kPair) mma_ts(d, qh, sw128_desc(kb + C::kHalfBytes + off), C::kIdescS, 1u);
-                    mma_ts(d, qh, kh, C::kIdescS, 1u);
+                    for (int ks = 0; ks < 4; ks++) {
+                        const uint32_t at = qh + ks / 2 * 32 + ks % 2 * 8;
+                        mma_ts(d, at + 16, kh + ks * 2, C::kIdescS, b + ks);
+                        if (C::kPair) mma_ts(d, at, kh + ks * 2 + C::kHalfBytes / 16, C::kIdescS, 1u);
+                        mma_ts(d, at, kh + ks * 2, C::kIdescS, 1u);
+                    }
                 }
                 mma_commit(&empty[j % S]);
                 mma_commit(&s_full[n & 1]);
             }
-            j++;
-            first = c.tile == c.tiles - 1;  // of the next tile
-            if (n + 1 < N) cursor_next(p, c);
+            first = c.tile == c.tiles - 1;
+            if (n + 1 < N) cursor_next(p, unit, c);
         };
         auto pv = [&](int n) {
             mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-            const uint32_t vb = slot_wait();
+            const int j = n == N - 1 ? total - 1 : 2 * n + 2;
+            const uint32_t vb = slot_wait(j);
             if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
             if (!*abort) {
                 tc_fence_after();
                 const uint32_t pt = s_tm + (n & 1) * 128;
+                const uint64_t desc = sw128_desc_mn(vb, C::kBlockBytes);
+#pragma unroll 1
+                for (int b = 0; b < kKeys / 32; b++) {
+                    const uint64_t vh = desc + b * (2 * 2048 / 16);
+                    const uint32_t ph = pt + b * 32;
 #pragma unroll
-                for (int ks = 0; ks < kKeys / 16; ks++) {
-                    const uint32_t ph = pt + (ks / 2) * 32 + (ks % 2) * 8;
-                    const uint64_t vh = sw128_desc_mn(vb + ks * 2048, C::kBlockBytes);
-                    mma_ts(o_tm, ph + 16, vh, C::kIdescO, ks > 0);
-                    if (C::kPair)
-                        mma_ts(o_tm, ph, sw128_desc_mn(vb + C::kHalfBytes + ks * 2048, C::kBlockBytes), C::kIdescO, 1u);
-                    mma_ts(o_tm, ph, vh, C::kIdescO, 1u);
+                    for (int ks = 0; ks < 2; ks++) {
+                        mma_ts(o_tm, ph + ks * 8 + 16, vh + ks * 128, C::kIdescO, b + ks);
+                        if (C::kPair)
+                            mma_ts(o_tm, ph + ks * 8, vh + ks * 128 + C::kHalfBytes / 16, C::kIdescO, 1u);
+                        mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
+                    }
                 }
                 mma_commit(&empty[j % S]);
                 mma_commit(o_full);
             }
-            j++;
         };
-        qk(0);
-        for (int n = 0; n < N; n++) {
-            if (n + 1 < N) qk(n + 1);
-            pv(n);
+        // Q K^T one tile ahead, but a segment's first waits for its Q, which
+        // the softmax warps write after the tile before: P V goes first there.
+        for (int nq = 0, np = 0; np < N;) {
+            if (nq < N && nq <= np + 1 && !(first && np < nq))
+                qk(nq++);
+            else
+                pv(np++);
         }
         // Every MMA issued must complete before TMEM is freed.
         mma_commit(done);
@@ -827,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 15) {
+    if (warp == 12) {
         __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
@@ -840,6 +1034,24 @@ template <typename T, int DP>
 cudaError_t launch(cudaStream_t s, const PagedPass &p) {
     using C = Cfg<T, DP>;
     static_assert(C::kSmem <= 227 * 1024, "shared layout");
+    // Boxes of whole pages, or of 128 keys of a larger one, where they fill a
+    // tile without overlap and start on the swizzle's 8 rows.
+    RowsArgs args{};
+    args.pass = p;
+    args.unit = 1;
+    const PagedCache &c = p.a.cache;
+    if (c.page % 8 == 0 && (c.page % kKeys == 0 || kKeys % c.page == 0)) {
+        const int unit = c.page < kKeys ? c.page : kKeys;
+        const uint64_t dims[5] = {(uint64_t)p.a.head_dim, (uint64_t)p.a.kv_heads, (uint64_t)c.page, 2,
+                                  (uint64_t)c.pages};
+        const uint64_t strides[4] = {(uint64_t)p.a.head_dim * sizeof(T), (uint64_t)c.row_stride,
+                                     (uint64_t)c.parity_stride, (uint64_t)c.page_stride};
+        const uint32_t box[5] = {128 / (uint32_t)sizeof(T), 1, (uint32_t)unit, 1, 1};
+        const CUtensorMapDataType type = C::kPair  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                         : C::kRaw ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+        if (encode_tensor_map_5d(&args.map, type, c.base, dims, strides, box, !C::kPair)) args.unit = unit;
+    }
     static std::atomic<uint64_t> smem_set{0};
     cudaError_t e = set_smem_limit_once(paged_rows_kernel<T, DP>, C::kSmem, &smem_set);
     if (e != cudaSuccess) return e;
@@ -849,7 +1061,7 @@ cudaError_t launch(cudaStream_t s, const PagedPass &p) {
         return cudaFuncGetAttributes(&at, paged_rows_kernel<T, DP>) == cudaSuccess ? at.numRegs : 0;
     }();
     if (regs < kLaunchRegs) return cudaErrorInvalidConfiguration;
-    launch_k(paged_rows_kernel<T, DP>, kSmCount, kThreads, C::kSmem, s, p);
+    launch_k(paged_rows_kernel<T, DP>, kSmCount, kThreads, C::kSmem, s, args);
     count_launch();
     return cudaGetLastError();
 }

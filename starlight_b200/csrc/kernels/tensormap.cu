@@ -69,5 +69,23 @@ bool encode_tensor_map_3d(CUtensorMap *map, CUtensorMapDataType dtype, const voi
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool encode_tensor_map_5d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                          const uint64_t dims[5], const uint64_t strides_bytes[4],
+                          const uint32_t box[5], bool swizzle128) {
+    PFN_cuTensorMapEncodeTiled_v12000 fn = encode_fn();
+    if (!fn) return false;
+    cuuint64_t d[5], st[4];
+    cuuint32_t bx[5], elem[5];
+    for (int i = 0; i < 5; i++) {
+        d[i] = dims[i];
+        bx[i] = box[i];
+        elem[i] = 1;
+        if (i < 4) st[i] = strides_bytes[i];
+    }
+    return fn(map, dtype, 5, const_cast<void *>(base), d, st, bx, elem, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              swizzle128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace k
 }  // namespace slc

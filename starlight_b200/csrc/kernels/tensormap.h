@@ -28,5 +28,10 @@ bool encode_tensor_map_3d(CUtensorMap *map, CUtensorMapDataType dtype, const voi
                           const uint64_t dims[3], const uint64_t strides_bytes[2],
                           const uint32_t box[3]);
 
+// A 5-D tensor, boxes likewise, with an optional 128-byte swizzle.
+bool encode_tensor_map_5d(CUtensorMap *map, CUtensorMapDataType dtype, const void *base,
+                          const uint64_t dims[5], const uint64_t strides_bytes[4],
+                          const uint32_t box[5], bool swizzle128);
+
 }  // namespace k
 }  // namespace slc

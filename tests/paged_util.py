@@ -101,9 +101,9 @@ class Batch:
                     w = np.exp(s - s.max())
                     out[row, h] = (w / w.sum()) @ vv
                     ds = 8 * 2.0 ** -20 * abs(scale) * (np.abs(kk) @ np.abs(q)).max()
-                    ds += 2.0 ** -38 * abs(scale) * dim_sum(kk, q)
+                    ds += 2.0 ** -33 * abs(scale) * dim_sum(kk, q)
                     tol[row, h] = (w / w.sum()) @ np.abs(vv) * (2 * ds + (8 + len(pos) / 64) * 2.0 ** -20)
-                    tol[row, h] += 2.0 ** -38 * np.abs(vv).max()
+                    tol[row, h] += 2.0 ** -33 * np.abs(vv).max()
         return out.reshape(self.tokens, -1), tol.reshape(self.tokens, -1)
 
     # ---- ports -----------------------------------------------------------

@@ -16,8 +16,8 @@ over the keys (32 or more apart in separate accumulators, 2^-23 a step) at
 most 2^-20 for 64 keys, the merges and the division the rest of 8 * 2^-20.
 The split of rows and keys over CTAs changes which sums are made first, not
 the bound. Rows on the tcgen05 path use f16 pairs (22 bits, inside the above)
-whose smallest step is 2^-39 of a tile's largest key or value and of the
-query's largest element: as much again, rounded up to 2^-38, times the largest
+whose smallest step is 2^-34 of a tile's largest key or value and 2^-39 of the
+query's largest element: as much again, rounded up to 2^-33, times the largest
 value, and times what multiplies it in a score."""
 import math
 
