@@ -14,22 +14,22 @@
 // starts from zero and is added in f32 registers (TMEM accumulation over
 // thousands of keys would truncate thousands of times).
 //
-// One CTA per SM, 16 warps:
+// One CTA per SM, 20 warps:
 //   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
 //          S from TMEM, running maximum, P as f16 pairs back into the TMEM
 //          columns that S held
 //   4..7   output: one thread per row; O += P V of each tile in registers,
 //          the merge of a split segment, the result
-//   8..11  conversion in place: scale, f16 or f16 pair, zeros in rows that no
+//   8..15  conversion in place: scale, f16 or f16 pair, zeros in rows that no
 //          query sees (they may hold anything). The scale is that of the
 //          operand before; a tile whose largest value does not suit it is
 //          read from the cache once more (a pass over each tile for its
 //          maximum would cost a quarter of the shared memory's bandwidth,
 //          which is what bounds an F32 cache).
-//   12     issues the MMAs: Q K^T of the next tile before P V of this one
-//   13     copies: one TMA box per page and 128-byte block into a ring of
+//   16     issues the MMAs: Q K^T of the next tile before P V of this one
+//   17     copies: one TMA box per page and 128-byte block into a ring of
 //          slots (pages that do not tile 128 rows in multiples of 8: 16-byte
-//          asynchronous copies, by warps 13..15)
+//          asynchronous copies, by warps 17..19)
 // The ring holds operands in the order K0 K1 V0 K2 V1 ..., so a slot is free
 // as soon as the MMAs kSlots back are done; three slots of pairs or six of
 // single f16. Q and P are A operands from TMEM; K is read K-major and V
@@ -53,14 +53,15 @@ namespace {
 
 constexpr int kM = 128;     // query rows per segment
 constexpr int kKeys = 128;  // keys per tile
-constexpr int kConv = 4;    // conversion warps
+constexpr int kConv = 8;    // conversion warps
 constexpr int kCopy = 3;    // copying warps where TMA boxes do not fit the pages
-constexpr int kThreads = 16 * 32;
+constexpr int kThreads = 20 * 32;
 constexpr int kShift = 14;  // a query row's largest value in [2^14, 2^15), probabilities up to 2^14
 constexpr int kTop = 11;    // a tile's largest value around 2^11: from 2^9 to 2^15
-// Registers a thread, by warpgroup: 128 at launch.
-constexpr int kLaunchRegs = 128, kSoftRegs = 120, kOutRegs = 184, kConvRegs = 104, kRestRegs = 104;
-static_assert(kSoftRegs + kOutRegs + kConvRegs + kRestRegs <= 4 * kLaunchRegs, "register split");
+// Registers a thread, by warpgroup: softmax keeps the 96 of the launch,
+// conversion has two warpgroups.
+constexpr int kLaunchRegs = 96, kOutRegs = 184, kConvRegs = 64, kRestRegs = 72;
+static_assert(kLaunchRegs + kOutRegs + 2 * kConvRegs + kRestRegs <= 5 * kLaunchRegs, "register split");
 constexpr uint64_t kLimitNs = 4000000000ull;  // rows of values that are not finite take long
 
 template <typename T, int DP>
@@ -74,7 +75,7 @@ struct Cfg {
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
     static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 4 * DP + 16) + 8 * (8 + 3 * kSlots + 8 + 20);
+    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 8 * 12 + 4 * DP + 16) + 8 * (8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
     static constexpr int kLpr = DP / kEpl;               // lanes per cache row
@@ -189,9 +190,17 @@ __device__ __forceinline__ void cursor_next(const PagedPass &p, int unit, Cursor
 
 // Position of key index i.
 __device__ __forceinline__ int key_pos(const Cursor &c, int i) { return i < c.sink ? i : i - c.sink + c.low; }
+// What the copying warp tells the others of a tile.
+struct Tile {
+    int begins, whole;  // first of a segment; every key index is seen by some row
+    int seg;            // its segment, counted from this CTA's first
+    int b, kvh, i0;
+    int sink, low, from, keys;
+};
 // Whether some row of the segment may see key index i.
-__device__ __forceinline__ bool live_key(const PagedPass &p, const Cursor &c, int i) {
-    const int pos = key_pos(c, i);
+template <typename C>
+__device__ __forceinline__ bool live_key(const PagedPass &p, const C &c, int i) {
+    const int pos = i < c.sink ? i : i - c.sink + c.low;
     return i < c.keys && (pos >= c.from || ((i < c.sink || c.sink == c.low) && pos < p.a.sinks));
 }
 
@@ -285,7 +294,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     float *v_scale = k_scale + 8;                       // [8 tiles]
     uint32_t *most = reinterpret_cast<uint32_t *>(v_scale + 8);   // [4 operands, 4 unused]
     int *poison = reinterpret_cast<int *>(most + 8);    // [8 segments]
-    float *scratch = reinterpret_cast<float *>(poison + 8);       // [4 warps][DP]
+    Tile *tiles = reinterpret_cast<Tile *>(poison + 8);           // [8 tiles]
+    float *scratch = reinterpret_cast<float *>(tiles + 8);        // [4 warps][DP]
     int *flags = reinterpret_cast<int *>(scratch + 4 * DP);
     volatile int *abort = flags;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(flags + 1);
@@ -359,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         pdl_wait();
         return;
     }
-    if (warp == 12) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                          smem_addr(tmem_slot))
                      : "memory");
@@ -390,13 +400,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     // No wait below ends a loop: after one that gave up (the abort word is
     // set) every role runs through its remaining steps without waiting, so
     // that the barriers between its own threads stay matched.
-    if (warp < 4)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
-    else if (warp < 8)
+    if (warp >= 4 && warp < 8)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kOutRegs));
-    else if (warp < 12)
+    else if (warp >= 8 && warp < 16)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
-    else
+    else if (warp >= 16)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
     if (warp < 4) {
         // ---- softmax ------------------------------------------------------
@@ -724,50 +732,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             seg_n = n + 1;
             if (n + 1 < N) cursor_next(p, unit, c);
         }
-    } else if (warp < 12) {
+    } else if (warp < 16) {
         // ---- conversion ---------------------------------------------------
         const int pw = warp - 8;
         // Piece i of a lane: row (i kConv + pw) kRpi + sub, 16 raw bytes from
-        // dim `col` on.
+        // dim `col` on. A piece on is a multiple of 8 rows on.
         const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
-        constexpr int kBatch = C::kRows < 8 ? C::kRows : 8;
+        constexpr int kBatch = 4, kStep = kConv * C::kRpi * 128;
+        static_assert(C::kRows % kBatch == 0 && kConv % 8 == 0, "batches of pieces 8 rows apart");
         auto row_of = [&](int i) { return (i * kConv + pw) * C::kRpi + sub; };
-        // Raw place of a row's piece, and the operand places of even and odd
-        // pieces: two pieces on is a multiple of 8 rows on.
-        const uint32_t raw0 = C::kPair ? (ch >> 3) * C::kBlockBytes + row_of(0) * 128 + (ch & 7) * 16
-                                       : operand_at(row_of(0), col);
-        const uint32_t raw1 = C::kPair ? raw0 + kConv * C::kRpi * 128 : operand_at(row_of(1), col);
-        const uint32_t op0 = operand_at(row_of(0), col), op1 = operand_at(row_of(1), col);
-        constexpr int kTwo = 2 * kConv * C::kRpi * 128;
-        auto raw_at = [&](int i) { return (i & 1 ? raw1 : raw0) + i / 2 * kTwo; };
-        Cursor cv = c;              // of the values that come next; c: of the keys
-        int seg_k = 0, seg_v = 0;  // their segments, for the poison flags
-        int e_k = 2, e_v = 2;      // exponents of the scales of the operands before
+        const uint32_t op0 = operand_at(row_of(0), col);
+        const uint32_t raw0 = C::kPair ? (ch >> 3) * C::kBlockBytes + row_of(0) * 128 + (ch & 7) * 16 : op0;
+        int e_k = 2, e_v = 2;  // exponents of the scales of the operands before
         for (int j = 0; j < total; j++) {
             const bool v = is_v(j);
             const int n = tile_of(j);
-            if (!v && j > 0) {
-                cv = c;
-                seg_v = seg_k;
-                seg_k += c.tile == c.tiles - 1;
-                cursor_next(p, unit, c);
-            }
-            if (j == total - 1) {
-                cv = c;
-                seg_v = seg_k;
-            }
             mbar_wait(&raw[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
             unsigned char *slot = ring + (j % S) * C::kTileBytes;
-            const Cursor &cu = v ? cv : c;
-            const int i0 = cu.tile * kKeys;
-            const bool whole = i0 + kKeys <= cu.keys &&
-                               (key_pos(cu, i0) >= cu.from || key_pos(cu, i0 + kKeys - 1) < p.a.sinks);
+            const Tile &cu = tiles[n & 7];
+            const bool whole = cu.whole;
             // Rows that no query sees may hold anything, or be of a tile before.
             if (!whole && (v || !C::kRaw))
 #pragma unroll 1
                 for (int i = 0; i < C::kRows; i++)
-                    if (!live_key(p, cu, i0 + row_of(i)))
-                        *reinterpret_cast<uint4 *>(slot + raw_at(i)) = make_uint4(0, 0, 0, 0);
+                    if (!live_key(p, cu, cu.i0 + row_of(i)))
+                        *reinterpret_cast<uint4 *>(slot + raw0 + i * kStep) = make_uint4(0, 0, 0, 0);
             int ex = kTop;  // the scale is 2^(kTop - ex)
             if (!C::kRaw) {
                 const uint32_t at = smem_addr(slot);
@@ -777,15 +766,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     float top = 0.f;
 #pragma unroll 1
                     for (int ib = 0; ib < C::kRows; ib += kBatch) {
-                        const unsigned char *from = slot + ib / 2 * kTwo;
-                        const uint32_t to = at + ib / 2 * kTwo;
+                        const unsigned char *from = slot + raw0 + ib * kStep;
+                        const uint32_t to = at + op0 + ib * kStep;
                         uint4 x[kBatch];
 #pragma unroll
-                        for (int y = 0; y < kBatch; y++) x[y] = *reinterpret_cast<const uint4 *>(from + raw_at(y));
+                        for (int y = 0; y < kBatch; y++) x[y] = *reinterpret_cast<const uint4 *>(from + y * kStep);
                         __syncwarp();  // a row of pairs is read whole before it is written
 #pragma unroll
                         for (int y = 0; y < kBatch; y++) {
-                            const uint32_t dst = to + (y & 1 ? op1 : op0) + y / 2 * kTwo;
+                            const uint32_t dst = to + y * kStep;
                             const uint32_t w[4] = {x[y].x, x[y].y, x[y].z, x[y].w};
                             if (C::kPair) {
 #pragma unroll
@@ -820,20 +809,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     if (threadIdx.x == 8 * 32) most[place] = 0;
                     if (all == 0) break;
                     const int found = scale_exponent(all);
-                    if (threadIdx.x == 8 * 32 && all >= 0x7f800000u) poison[(v ? seg_v : seg_k) & 7] = 1;
+                    if (threadIdx.x == 8 * 32 && all >= 0x7f800000u) poison[cu.seg & 7] = 1;
                     (v ? e_v : e_k) = found;
                     if (again || (found <= ex + 3 && found >= ex - 2)) break;
                     // Once more, from the cache.
                     ex = found;
 #pragma unroll 1
                     for (int i = 0; i < C::kRows; i++) {
-                        const int key = i0 + row_of(i);
+                        const int key = cu.i0 + row_of(i), pos = key < cu.sink ? key : key - cu.sink + cu.low;
                         uint4 x = make_uint4(0, 0, 0, 0);
                         if (live_key(p, cu, key) && col < D)
                             x = __ldcg(reinterpret_cast<const uint4 *>(
-                                p.a.cache.base + paged_row(p.a.cache, p.a.batch, cu.b, key_pos(cu, key), p.a.err) +
+                                p.a.cache.base + paged_row(p.a.cache, p.a.batch, cu.b, pos, p.a.err) +
                                 (v ? p.a.cache.parity_stride : 0) + (cu.kvh * D + col) * (long long)sizeof(T)));
-                        *reinterpret_cast<uint4 *>(slot + raw_at(i)) = x;
+                        *reinterpret_cast<uint4 *>(slot + raw0 + i * kStep) = x;
                     }
                     __syncwarp();
                 }
@@ -846,10 +835,23 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[j % S]);
         }
-    } else if (warp > 12) {
+    } else if (warp > 16) {
         // ---- copies -------------------------------------------------------
+        int seg = 0;
+        // Before the copy of a tile's keys: the ring of eight is far behind.
+        auto tell = [&](int n, bool begins) {
+            Tile t;
+            t.begins = begins;
+            t.i0 = c.tile * kKeys;
+            t.whole = t.i0 + kKeys <= c.keys &&
+                      (key_pos(c, t.i0) >= c.from || key_pos(c, t.i0 + kKeys - 1) < p.a.sinks);
+            t.seg = seg;
+            t.b = c.b, t.kvh = c.kvh;
+            t.sink = c.sink, t.low = c.low, t.from = c.from, t.keys = c.keys;
+            tiles[n & 7] = t;
+        };
         if (unit > 1) {
-            if (warp == 13) {
+            if (warp == 17) {
                 // Lane i copies box row i of the tile: `unit` keys of a page.
                 const int boxes = kKeys / unit;
                 constexpr int kBlk = DP * (int)sizeof(T) / 128;
@@ -864,7 +866,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                         id = pg < p.a.batch.per_seq ? p.a.batch.table[(long long)c.b * p.a.batch.per_seq + pg] : ~0u;
                     }
                 };
-                auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity) {
+                auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity, int n, bool begins) {
                     if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
                     if (__any_sync(0xffffffffu, *abort)) return;
                     if (at >= 0 && page_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
@@ -872,7 +874,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                         page_id = 0;
                     }
                     const int count = __popc(__ballot_sync(0xffffffffu, at >= 0));
-                    if (lane == 0) mbar_arrive_expect_tx(&raw[j % S], count * unit * 128 * kBlk);
+                    if (lane == 0) {
+                        if (!parity) tell(n, begins);
+                        mbar_arrive_expect_tx(&raw[j % S], count * unit * 128 * kBlk);
+                    }
                     __syncwarp();
                     unsigned char *slot = ring + (j % S) * C::kTileBytes + lane * unit * 128;
                     if (at >= 0)
@@ -883,18 +888,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 };
                 if (lane == 0) prefetch_tensormap(&args.map);
                 look_up();
+                bool begins = true;
                 for (int n = 0; n < N; n++) {
-                    copy(n ? 2 * n - 1 : 0, id, z, c.kvh, 0);
-                    if (n) copy(2 * n, id_v, z_v, kvh_v, 1);
+                    copy(n ? 2 * n - 1 : 0, id, z, c.kvh, 0, n, begins);
+                    if (n) copy(2 * n, id_v, z_v, kvh_v, 1, n, false);
                     id_v = id;
                     z_v = z;
                     kvh_v = c.kvh;
+                    begins = c.tile == c.tiles - 1;
+                    seg += begins;
                     if (n + 1 < N) {
                         cursor_next(p, unit, c);
                         look_up();
                     }
                 }
-                copy(total - 1, id_v, z_v, kvh_v, 1);
+                copy(total - 1, id_v, z_v, kvh_v, 1, N, false);
                 // Copies still in flight must land before the CTA's shared
                 // memory is released (after a wait that gave up; else the
                 // MMAs have used them all).
@@ -903,7 +911,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             }
         } else {
             // Row (i kCopy + w) kRpi + sub by 16-byte pieces.
-            const int w = warp - 13, sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+            const int w = warp - 17, sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
             Cursor cv = c;
             auto copy = [&](int j, const Cursor &cu, int parity) {
                 if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
@@ -929,12 +937,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             };
             for (int j = 0; j < total; j++) {
                 const bool v = is_v(j);
+                bool begins = j == 0;
                 if (!v && j > 0) {
                     cv = c;
+                    begins = c.tile == c.tiles - 1;
+                    seg += begins;
                     cursor_next(p, unit, c);
                 }
                 if (j == total - 1) cv = c;
                 copy(j, v ? cv : c, v);
+                if (!v && w == 0 && lane == 0) tell(tile_of(j), begins);
                 cp_async_commit();
                 if (j >= C::kAhead) {
                     cp_async_wait<C::kAhead>();
@@ -949,15 +961,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         if (lane == 0) {
         const uint32_t ra = smem_addr(ring);
         int seg = 0;
-        bool first = true;  // the next tile begins a segment
         auto slot_wait = [&](int j) {
             mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
             return ra + (j % S) * C::kTileBytes;
         };
-        auto qk = [&](int n) {
-            if (first) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
+        auto qk = [&](int n, bool begins, uint32_t kb) {
             const int j = n ? 2 * n - 1 : 0;
-            const uint32_t kb = slot_wait(j);
+            if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
             if (!*abort) {
                 tc_fence_after();
                 const uint32_t d = s_tm + (n & 1) * 128;
@@ -978,8 +988,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 mma_commit(&empty[j % S]);
                 mma_commit(&s_full[n & 1]);
             }
-            first = c.tile == c.tiles - 1;
-            if (n + 1 < N) cursor_next(p, unit, c);
         };
         auto pv = [&](int n) {
             mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
@@ -1008,11 +1016,20 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         };
         // Q K^T one tile ahead, but a segment's first waits for its Q, which
         // the softmax warps write after the tile before: P V goes first there.
-        for (int nq = 0, np = 0; np < N;) {
-            if (nq < N && nq <= np + 1 && !(first && np < nq))
-                qk(nq++);
-            else
+        bool begins = true;
+        uint32_t kb = 0;
+        for (int nq = 0, np = 0, known = 0; np < N;) {
+            if (nq < N && nq <= np + 1 && known <= nq) {
+                kb = slot_wait(nq ? 2 * nq - 1 : 0);
+                begins = tiles[nq & 7].begins;
+                known = nq + 1;
+            }
+            if (nq < N && nq <= np + 1 && !(begins && np < nq)) {
+                qk(nq, begins, kb);
+                nq++;
+            } else {
                 pv(np++);
+            }
         }
         // Every MMA issued must complete before TMEM is freed.
         mma_commit(done);
@@ -1021,7 +1038,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == 16) {
         __syncwarp();
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
