@@ -75,7 +75,7 @@ struct Cfg {
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
     static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 8 * 12 + 4 * DP + 16) + 8 * (8 + 3 * kSlots + 8 + 20);
+    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 8 * 12 + 4 * DP + 16) + 8 * (3 * kKeys + 8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
     static constexpr int kLpr = DP / kEpl;               // lanes per cache row
@@ -295,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     uint32_t *most = reinterpret_cast<uint32_t *>(v_scale + 8);   // [4 operands, 4 unused]
     int *poison = reinterpret_cast<int *>(most + 8);    // [8 segments]
     Tile *tiles = reinterpret_cast<Tile *>(poison + 8);           // [8 tiles]
-    float *scratch = reinterpret_cast<float *>(tiles + 8);        // [4 warps][DP]
+    long long *row_off = reinterpret_cast<long long *>(tiles + 8);  // [3 tiles][kKeys]
+    float *scratch = reinterpret_cast<float *>(row_off + 3 * kKeys);  // [4 warps][DP]
     int *flags = reinterpret_cast<int *>(scratch + 4 * DP);
     volatile int *abort = flags;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(flags + 1);
@@ -425,31 +426,30 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 const bool vec = aligned16(p.a.q);
                 float top = 0.f;
 #pragma unroll 1
-                for (int h = 0; h < DP; h += 64) {
-                    uint32_t x[4][16];
+                for (int h = 0; h < DP; h += 32) {
+                    float4 v[8];
 #pragma unroll
-                    for (int d = 0; d < 64; d += 4) {
-                        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (live && h + d < D) {
-                            if (vec)
-                                v = *reinterpret_cast<const float4 *>(q + h + d);
-                            else
-                                v = make_float4(q[h + d], q[h + d + 1], q[h + d + 2], q[h + d + 3]);
-                        }
-                        x[d / 16][d % 16] = __float_as_uint(v.x);
-                        x[d / 16][d % 16 + 1] = __float_as_uint(v.y);
-                        x[d / 16][d % 16 + 2] = __float_as_uint(v.z);
-                        x[d / 16][d % 16 + 3] = __float_as_uint(v.w);
+                    for (int y = 0; y < 8; y++) {
+                        const float *at = q + h + 4 * y;
+                        v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (live && h + 4 * y < D)
+                            v[y] = vec ? *reinterpret_cast<const float4 *>(at)
+                                       : make_float4(at[0], at[1], at[2], at[3]);
                     }
 #pragma unroll
-                    for (int y = 0; y < 4; y++) {
+                    for (int y = 0; y < 2; y++) {
+                        uint32_t x[16];
 #pragma unroll
-                        for (int d = 0; d < 16; d++) {
-                            const float f = __uint_as_float(x[y][d]) * p.scale_log2;
-                            x[y][d] = __float_as_uint(f);
-                            top = fmaxf(top, fabsf(f));
+                        for (int z = 0; z < 4; z++) {
+                            const float4 f = v[4 * y + z];
+                            x[4 * z] = __float_as_uint(f.x * p.scale_log2);
+                            x[4 * z + 1] = __float_as_uint(f.y * p.scale_log2);
+                            x[4 * z + 2] = __float_as_uint(f.z * p.scale_log2);
+                            x[4 * z + 3] = __float_as_uint(f.w * p.scale_log2);
                         }
-                        tmem_st16(q_tm + lane_tm + h + 16 * y, x[y]);
+#pragma unroll
+                        for (int z = 0; z < 16; z++) top = fmaxf(top, fabsf(__uint_as_float(x[z])));
+                        tmem_st16(q_tm + lane_tm + h + 16 * y, x);
                     }
                 }
                 tmem_wait_st();
@@ -910,23 +910,31 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     for (int j = max(total - S, 0); j < total; j++) drain_wait(&raw[j % S], (j / S) & 1);
             }
         } else {
-            // Row (i kCopy + w) kRpi + sub by 16-byte pieces.
+            // Rows kRpi at a time, every kCopy-th of them a warp's, by 16-byte
+            // pieces; their places in the cache through a ring of three tiles.
             const int w = warp - 17, sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
-            Cursor cv = c;
-            auto copy = [&](int j, const Cursor &cu, int parity) {
+            auto look_up = [&](int n) {
+                for (int r = threadIdx.x - 17 * 32; r < kKeys; r += kCopy * 32) {
+                    const int i = c.tile * kKeys + r;
+                    long long off = -1;
+                    if (i < c.keys)
+                        off = paged_row(p.a.cache, p.a.batch, c.b, key_pos(c, i), p.a.err) +
+                              c.kvh * D * (long long)sizeof(T);
+                    row_off[n % 3 * kKeys + r] = off;
+                }
+                bar_sync(3, kCopy * 32);
+            };
+            auto copy = [&](int j, int n, int parity) {
                 if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
                 unsigned char *slot = ring + (j % S) * C::kTileBytes;
-#pragma unroll 2
+                const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
+#pragma unroll 4
                 for (int r = w * C::kRpi + sub; r < kKeys; r += kCopy * C::kRpi) {
-                    const int i = cu.tile * kKeys + r;
-                    const bool live = i < cu.keys && col < D;
-                    const char *src = p.a.cache.base;
-                    if (live)
-                        src += paged_row(p.a.cache, p.a.batch, cu.b, key_pos(cu, i), p.a.err) +
-                               (parity ? p.a.cache.parity_stride : 0) + (cu.kvh * D + col) * (long long)sizeof(T);
+                    const long long off = row_off[n % 3 * kKeys + r];
+                    const bool live = off >= 0 && col < D;
                     cp_async16_zfill(slot + (C::kPair ? (ch >> 3) * C::kBlockBytes + r * 128 + (ch & 7) * 16
                                                       : operand_at(r, col)),
-                                     src, live ? 16 : 0);
+                                     live ? base + off : p.a.cache.base, live ? 16 : 0);
                 }
             };
             int done_j = 0;
@@ -937,16 +945,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             };
             for (int j = 0; j < total; j++) {
                 const bool v = is_v(j);
-                bool begins = j == 0;
-                if (!v && j > 0) {
-                    cv = c;
-                    begins = c.tile == c.tiles - 1;
-                    seg += begins;
-                    cursor_next(p, unit, c);
+                const int n = tile_of(j);
+                if (!v) {
+                    bool begins = n == 0;
+                    if (n) {
+                        begins = c.tile == c.tiles - 1;
+                        seg += begins;
+                        cursor_next(p, unit, c);
+                    }
+                    look_up(n);
+                    if (w == 0 && lane == 0) tell(n, begins);
                 }
-                if (j == total - 1) cv = c;
-                copy(j, v ? cv : c, v);
-                if (!v && w == 0 && lane == 0) tell(tile_of(j), begins);
+                copy(j, n, v);
                 cp_async_commit();
                 if (j >= C::kAhead) {
                     cp_async_wait<C::kAhead>();
