@@ -365,6 +365,65 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         cp_async_commit();
     }
 
+    // Queries of a segment, a warp per row: read a tile before they are used,
+    // then put into fragment order.
+    constexpr int kOwn = kRows / kWarps, kItems = (kRows * DP / 4 + kThreads - 1) / kThreads;
+    float qv[kOwn][DP / 32];
+    auto load_q = [&](const Cur &c) {
+#pragma unroll
+        for (int x = 0; x < kOwn; x++) {
+            const int row = c.rb * kRows + warp + x * kWarps, tok = row / G;
+            const float *q = p.a.q + ((size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G)) * D;
+#pragma unroll
+            for (int y = 0; y < DP / 32; y++) {
+                const int d = lane + 32 * y;
+                qv[x][y] = tok < c.ntok && d < D ? q[d] : 0.f;
+            }
+        }
+    };
+    auto stage_q = [&] {
+#pragma unroll
+        for (int o = 0; o < kOwn; o++) {
+            const int r = warp + o * kWarps;
+            float(&v)[DP / 32] = qv[o];
+            float f = p.scale_log2;
+            if (C::kShift) {
+                float top = 0.f;
+#pragma unroll
+                for (int y = 0; y < DP / 32; y++) top = fmaxf(top, fabsf(v[y]));
+                const int ex = scale_exponent(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+                f *= pow2(ex - C::kShift);
+#pragma unroll
+                for (int y = 0; y < DP / 32; y++) v[y] *= pow2(C::kShift - ex);
+            }
+            if (lane == 0) q_scale[r] = f;
+#pragma unroll
+            for (int y = 0; y < DP / 32; y++) {
+                const int d = lane + 32 * y, j = d / 16, k = d % 16;
+                if (C::kHalf) {
+                    // k step j, lane (r, t): b0 = dims 2t, 2t + 1, b1 = 8 + 2t, ...
+                    T *dst = reinterpret_cast<T *>(q_s) + (j * C::kTerms * 32 + r * 4 + (k % 8) / 2) * 4 + k / 8 * 2 +
+                             k % 2;
+#pragma unroll
+                    for (int x = 0; x < C::kTerms; x++) {
+                        float none = 0.f;
+                        const uint32_t w = take_pair<T>(v[y], none);
+                        *reinterpret_cast<uint16_t *>(dst + x * 128) = (uint16_t)w;
+                    }
+                } else {
+                    // Block j, lane (r, t): dims 4t .. 4t + 3; hi, then lo.
+                    float *dst = reinterpret_cast<float *>(q_s) + (j * 32 + r * 4 + k / 4) * 4 + k % 4;
+                    const uint32_t hi = tf32_hi(v[y]);
+                    dst[0] = __uint_as_float(hi);
+                    dst[kRows * DP] = __uint_as_float(tf32_lo(v[y], hi));
+                }
+            }
+        }
+    };
+    load_q(cc);
+    stage_q();
+    __syncthreads();
+
     float acc[NT][4];  // O^T: dims x rows
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float qf0 = 0.f, qf1 = 0.f;  // S to log2 units, rows 2t and 2t + 1
@@ -372,50 +431,40 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
     long long seg_u0 = u0;       // this CTA's first unit of the current segment
     bool fresh = true;
     int stage = 0;
+    Cur nc = cc;                 // first unit of the segment after this one
+    // The outputs of a segment that this thread merges and writes: item i is
+    // row r, dims d .. d + 3; what a prefix pass left for them.
+    float4 pre_v[kItems];
+    float2 pre_ml[kItems];
+    auto item = [&](int i, int &r, int &d) {
+        const int x = threadIdx.x + i * kThreads;
+        r = x / (DP / 4);
+        d = 4 * (x % (DP / 4));
+    };
+    auto out_row = [&](int r) {
+        const int row = cc.rb * kRows + r, tok = row / G;
+        return (size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G);
+    };
     for (long long u = u0; u < u1; u++) {
-        if (fresh) {
-            // Queries of the segment, a warp per row, into fragment order.
-            for (int r = warp; r < kRows; r += kWarps) {
-                const int row = cc.rb * kRows + r, tok = row / G;
-                const float *q = p.a.q + ((size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G)) * D;
-                float v[DP / 32];
-                uint32_t top = 0;
+        const bool seg_end = cc.tile == cc.tiles - 1, ends = seg_end || u + 1 == u1;
+        if (ends) {
+            if (u + 1 < u1) {
+                nc = cc;
+                cursor_next(p, nc);
+                load_q(nc);
+            }
+            if (p.pre_o && !p.prefix_pass)
 #pragma unroll
-                for (int y = 0; y < DP / 32; y++) {
-                    const int d = lane + 32 * y;
-                    v[y] = tok < cc.ntok && d < D ? q[d] : 0.f;
-                    top = max(top, __float_as_uint(v[y]) & 0x7fffffffu);
-                }
-                float f = p.scale_log2;
-                if (C::kShift) {
-                    const int ex = scale_exponent(__reduce_max_sync(0xffffffffu, top));
-                    f *= pow2(ex - C::kShift);
-#pragma unroll
-                    for (int y = 0; y < DP / 32; y++) v[y] *= pow2(C::kShift - ex);
-                }
-                if (lane == 0) q_scale[r] = f;
-#pragma unroll
-                for (int y = 0; y < DP / 32; y++) {
-                    const int d = lane + 32 * y, j = d / 16, k = d % 16;
-                    if (C::kHalf) {
-                        // k step j, lane (r, t): b0 = dims 2t, 2t + 1, b1 = 8 + 2t, ...
-                        T *dst = reinterpret_cast<T *>(q_s) + (j * C::kTerms * 32 + r * 4 + (k % 8) / 2) * 4 +
-                                 k / 8 * 2 + k % 2;
-#pragma unroll
-                        for (int x = 0; x < C::kTerms; x++) {
-                            float none = 0.f;
-                            const uint32_t w = take_pair<T>(v[y], none);
-                            *reinterpret_cast<uint16_t *>(dst + x * 128) = (uint16_t)w;
-                        }
-                    } else {
-                        // Block j, lane (r, t): dims 4t .. 4t + 3; hi, then lo.
-                        float *dst = reinterpret_cast<float *>(q_s) + (j * 32 + r * 4 + k / 4) * 4 + k % 4;
-                        const uint32_t hi = tf32_hi(v[y]);
-                        dst[0] = __uint_as_float(hi);
-                        dst[kRows * DP] = __uint_as_float(tf32_lo(v[y], hi));
+                for (int i = 0; i < kItems; i++) {
+                    int r, d;
+                    item(i, r, d);
+                    if (r < min(kRows, cc.ntok * G - cc.rb * kRows) && d < D) {
+                        pre_ml[i] = __ldcg(reinterpret_cast<const float2 *>(p.pre_ml) + out_row(r));
+                        pre_v[i] = __ldcg(reinterpret_cast<const float4 *>(p.pre_o + out_row(r) * D + d));
                     }
                 }
-            }
+        }
+        if (fresh) {
             at0 = cc.past + (cc.rb * kRows + 2 * t) / G;
             at1 = cc.past + (cc.rb * kRows + 2 * t + 1) / G;
 #pragma unroll
@@ -426,7 +475,6 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             l0 = l1 = 0.f;
             seg_u0 = u;
             fresh = false;
-            __syncthreads();
             qf0 = q_scale[2 * t];
             qf1 = q_scale[2 * t + 1];
         }
@@ -602,8 +650,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         cp_async_commit();
         stage = stage + 1 == S ? 0 : stage + 1;
 
-        const bool seg_end = cc.tile == cc.tiles - 1;
-        if (!seg_end && u + 1 < u1) {
+        if (!ends) {
             cc.tile++;
             cc.left--;
             continue;
@@ -635,58 +682,77 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             float *ml = mml + (warp * kRows + 2 * t) * 2;
             ml[0] = m0, ml[1] = l0, ml[2] = m1, ml[3] = l1;
         }
-        __syncthreads();
+        __syncthreads();  // q_s is free from here on
         const int rows = min(kRows, cc.ntok * G - cc.rb * kRows);
-        // Row r, dims d .. d + 3 of the merge, d = 4 (i % (DP / 4)).
-        for (int i = threadIdx.x; i < kRows * DP / 4; i += kThreads) {
-            const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
-            float mm = -INFINITY;
-            for (int w = 0; w < kWarps; w++) mm = fmaxf(mm, mml[(w * kRows + r) * 2]);
-            const float mu = mm == -INFINITY ? 0.f : mm;
-            float ll = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 o[kItems];
+        float mm[kItems], ll[kItems];
+        auto add = [&](int i, float m, float l, float4 v) {  // to an item's running sums
+            const float nm = fmaxf(mm[i], m), mu = nm == -INFINITY ? 0.f : nm;
+            const float f = ex2(mm[i] - mu), e = ex2(m - mu);
+            ll[i] = fmaf(l, e, ll[i] * f);
+            o[i].x = fmaf(v.x, e, o[i].x * f);
+            o[i].y = fmaf(v.y, e, o[i].y * f);
+            o[i].z = fmaf(v.z, e, o[i].z * f);
+            o[i].w = fmaf(v.w, e, o[i].w * f);
+            mm[i] = nm;
+        };
+#pragma unroll
+        for (int i = 0; i < kItems; i++) {
+            int r, d;
+            item(i, r, d);
+            o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            mm[i] = -INFINITY;
+            ll[i] = 0.f;
+            if (r >= rows || d >= D) continue;
+            for (int w = 0; w < kWarps; w++) mm[i] = fmaxf(mm[i], mml[(w * kRows + r) * 2]);
+            const float mu = mm[i] == -INFINITY ? 0.f : mm[i];
             bool odd = false;
+#pragma unroll
             for (int w = 0; w < kWarps; w++) {
-                const float mw = mml[(w * kRows + r) * 2], lw = mml[(w * kRows + r) * 2 + 1];
-                const float f = ex2(mw - mu);
+                const float mw = mml[(w * kRows + r) * 2], lw = mml[(w * kRows + r) * 2 + 1], f = ex2(mw - mu);
                 const float4 x = *reinterpret_cast<const float4 *>(mo + (w * kRows + r) * C::kMergeStride + d);
-                ll = fmaf(lw, f, ll);
-                o.x = fmaf(x.x, f, o.x);
-                o.y = fmaf(x.y, f, o.y);
-                o.z = fmaf(x.z, f, o.z);
-                o.w = fmaf(x.w, f, o.w);
+                ll[i] = fmaf(lw, f, ll[i]);
+                o[i].x = fmaf(x.x, f, o[i].x);
+                o[i].y = fmaf(x.y, f, o[i].y);
+                o[i].z = fmaf(x.z, f, o[i].z);
+                o[i].w = fmaf(x.w, f, o[i].w);
                 odd |= !(mw < INFINITY);
             }
-            odd |= !finite(ll) || !finite(o.x) || !finite(o.y) || !finite(o.z) || !finite(o.w);
-            if (odd && r < rows && d < D) atomicOr(bad_s, 1 << r);
-            *reinterpret_cast<float4 *>(mo + r * C::kMergeStride + d) = o;  // warp 0's rows, read above by this thread alone
-            if (d == 0) {
-                row_ml[2 * r] = mm;
-                row_ml[2 * r + 1] = ll;
-            }
+            odd |= !finite(ll[i]) || !finite(o[i].x) || !finite(o[i].y) || !finite(o[i].z) || !finite(o[i].w);
+            if (odd) atomicOr(bad_s, 1 << r);
         }
+        if (u + 1 < u1) stage_q();
         __syncthreads();
-        if (*bad_s) {
+        if (const int bad = *bad_s) {
             // Plain f32 over the visible keys of the piece, a warp per row.
             const int k0 = (cc.tile - (int)(u - seg_u0)) * kTileKeys;
             const int k1 = min(cc.keys, (cc.tile + 1) * kTileKeys);
             for (int r = warp; r < rows; r += kWarps) {
-                if (!((*bad_s >> r) & 1)) continue;
-                const int row = cc.rb * kRows + r, tok = row / G, at = cc.past + tok;
-                const float *q = p.a.q + ((size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G)) * D;
-                float mm, ll, o[DP / 32];
+                if (!((bad >> r) & 1)) continue;
+                const int at = cc.past + (cc.rb * kRows + r) / G;
+                float m, l, v[DP / 32];
                 plain_row<T, DP>(
-                    p, q, cc.b, cc.kvh, k0, k1, [&](int i) { return sees(p, cc, i, at) ? key_pos(cc, i) : -1; }, mm,
-                    ll, o);
+                    p, p.a.q + out_row(r) * D, cc.b, cc.kvh, k0, k1,
+                    [&](int i) { return sees(p, cc, i, at) ? key_pos(cc, i) : -1; }, m, l, v);
 #pragma unroll
-                for (int y = 0; y < DP / 32; y++) mo[r * C::kMergeStride + lane + 32 * y] = o[y];
+                for (int y = 0; y < DP / 32; y++) mo[r * C::kMergeStride + lane + 32 * y] = v[y];
                 if (lane == 0) {
-                    row_ml[2 * r] = mm;
-                    row_ml[2 * r + 1] = ll;
+                    row_ml[2 * r] = m;
+                    row_ml[2 * r + 1] = l;
                 }
             }
             __syncthreads();
             if (threadIdx.x == 0) *bad_s = 0;
+#pragma unroll
+            for (int i = 0; i < kItems; i++) {
+                int r, d;
+                item(i, r, d);
+                if (r >= rows || !((bad >> r) & 1)) continue;
+                o[i] = *reinterpret_cast<const float4 *>(mo + r * C::kMergeStride + d);
+                mm[i] = row_ml[2 * r];
+                ll[i] = row_ml[2 * r + 1];
+            }
+            __syncthreads();
         }
 
         // ---- the segment's result, or a piece of it for the merge.
@@ -695,13 +761,15 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         if (a0 < u0 || a1 > u1) {
             const int c_first = (int)(((a0 + 1) * grid - 1) / U), c_last = (int)((a1 * grid - 1) / U);
             const int slot = 2 * blockIdx.x + (a0 >= u0 ? 1 : 0);
-            float *po = p.part_o + (size_t)slot * kRows * DP, *pml = p.part_ml + (size_t)slot * kRows * 2;
-            for (int i = threadIdx.x; i < rows * DP / 4; i += kThreads) {
-                const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
-                *reinterpret_cast<float4 *>(po + r * DP + d) =
-                    *reinterpret_cast<const float4 *>(mo + r * C::kMergeStride + d);
+#pragma unroll
+            for (int i = 0; i < kItems; i++) {
+                int r, d;
+                item(i, r, d);
+                if (r >= rows || d >= D) continue;
+                *reinterpret_cast<float4 *>(p.part_o + ((size_t)slot * kRows + r) * DP + d) = o[i];
+                if (d == 0)
+                    reinterpret_cast<float2 *>(p.part_ml)[(size_t)slot * kRows + r] = make_float2(mm[i], ll[i]);
             }
-            if (threadIdx.x < 2 * rows) pml[threadIdx.x] = row_ml[threadIdx.x];
             __syncthreads();
             if (threadIdx.x == 0) {
                 __threadfence();
@@ -713,66 +781,54 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             __syncthreads();
             write = *last_s;
             if (write) {
-                const int pieces = c_last - c_first + 1;
-                for (int i = threadIdx.x; i < rows * DP / 4; i += kThreads) {
-                    const int r = i / (DP / 4), d = 4 * (i % (DP / 4));
-                    float mm = -INFINITY, ll = 0.f;
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int x = 0; x < pieces; x++) {
-                        const size_t sl = x == 0 ? 2 * (size_t)c_first + 1 : 2 * (size_t)(c_first + x);
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.part_ml) + sl * kRows + r);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (sl * kRows + r) * DP + d));
-                        const float nm = fmaxf(mm, ml.x), mu = nm == -INFINITY ? 0.f : nm;
-                        const float f = ex2(mm - mu), e = ex2(ml.x - mu);
-                        ll = fmaf(ml.y, e, ll * f);
-                        o.x = fmaf(v.x, e, o.x * f);
-                        o.y = fmaf(v.y, e, o.y * f);
-                        o.z = fmaf(v.z, e, o.z * f);
-                        o.w = fmaf(v.w, e, o.w * f);
-                        mm = nm;
-                    }
-                    *reinterpret_cast<float4 *>(mo + r * C::kMergeStride + d) = o;
-                    if (d == 0) {
-                        row_ml[2 * r] = mm;
-                        row_ml[2 * r + 1] = ll;
+#pragma unroll
+                for (int i = 0; i < kItems; i++) {
+                    int r, d;
+                    item(i, r, d);
+                    if (r >= rows || d >= D) continue;
+                    mm[i] = -INFINITY;
+                    ll[i] = 0.f;
+                    o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    // Eight pieces in flight, added in ascending order.
+                    for (int x = c_first; x <= c_last; x += 8) {
+                        float2 ml[8];
+                        float4 v[8];
+#pragma unroll
+                        for (int y = 0; y < 8; y++) {
+                            const size_t sl = 2 * (size_t)min(x + y, c_last) + (x + y == c_first ? 1 : 0);
+                            ml[y] = __ldcg(reinterpret_cast<const float2 *>(p.part_ml) + sl * kRows + r);
+                            v[y] = __ldcg(reinterpret_cast<const float4 *>(p.part_o + (sl * kRows + r) * DP + d));
+                        }
+#pragma unroll
+                        for (int y = 0; y < 8; y++)
+                            if (x + y <= c_last) add(i, ml[y].x, ml[y].y, v[y]);
                     }
                 }
-                __syncthreads();
             }
+            __syncthreads();  // last_s is read
         }
         if (write) {
-            for (int i = threadIdx.x; i < rows * D / 4; i += kThreads) {
-                const int r = i / (D / 4), d = 4 * (i % (D / 4));
-                const int row = cc.rb * kRows + r, tok = row / G;
-                const size_t at = (size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G);
-                float4 o = *reinterpret_cast<const float4 *>(mo + r * C::kMergeStride + d);
-                float mm = row_ml[2 * r], ll = row_ml[2 * r + 1];
+#pragma unroll
+            for (int i = 0; i < kItems; i++) {
+                int r, d;
+                item(i, r, d);
+                if (r >= rows || d >= D) continue;
+                const size_t at = out_row(r);
                 if (p.prefix_pass) {
-                    *reinterpret_cast<float4 *>(p.pre_o + at * D + d) = o;
-                    if (d == 0) *reinterpret_cast<float2 *>(p.pre_ml + at * 2) = make_float2(mm, ll);
+                    *reinterpret_cast<float4 *>(p.pre_o + at * D + d) = o[i];
+                    if (d == 0) *reinterpret_cast<float2 *>(p.pre_ml + at * 2) = make_float2(mm[i], ll[i]);
                     continue;
                 }
-                if (p.pre_o) {
-                    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.pre_ml) + at);
-                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(p.pre_o + at * D + d));
-                    const float nm = fmaxf(mm, ml.x), mu = nm == -INFINITY ? 0.f : nm;
-                    const float f = ex2(mm - mu), e = ex2(ml.x - mu);
-                    ll = fmaf(ml.y, e, ll * f);
-                    o.x = fmaf(v.x, e, o.x * f);
-                    o.y = fmaf(v.y, e, o.y * f);
-                    o.z = fmaf(v.z, e, o.z * f);
-                    o.w = fmaf(v.w, e, o.w * f);
-                }
+                if (p.pre_o) add(i, pre_ml[i].x, pre_ml[i].y, pre_v[i]);
                 float *dst = p.a.out + at * D + d;  // 4-byte aligned
-                dst[0] = __fdiv_rn(o.x, ll);
-                dst[1] = __fdiv_rn(o.y, ll);
-                dst[2] = __fdiv_rn(o.z, ll);
-                dst[3] = __fdiv_rn(o.w, ll);
+                dst[0] = __fdiv_rn(o[i].x, ll[i]);
+                dst[1] = __fdiv_rn(o[i].y, ll[i]);
+                dst[2] = __fdiv_rn(o[i].z, ll[i]);
+                dst[3] = __fdiv_rn(o[i].w, ll[i]);
             }
         }
-        __syncthreads();
         fresh = true;
-        if (u + 1 < u1) cursor_next(p, cc);
+        cc = nc;
     }
 }
 
