@@ -8,6 +8,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tensormap.h"
 #include "tma.cuh"
 
 namespace slc {
@@ -48,6 +49,33 @@ __device__ __forceinline__ int paged_sequence_of(const PagedBatch &batch, uint32
     return lo;
 }
 
+// The cache's layer as a tensor map [pages][2][page][kv_heads][head_dim] with
+// boxes of 128 bytes by `unit` keys: the largest power of two, at least 8 (the
+// rows of a swizzle) and at most `most`, that divides the page, so that boxes
+// stack to any tile. Returns unit, or 1 where there is none.
+inline int paged_boxes(const PagedAttention &a, int most, size_t size, bool f16, bool swizzle, CUtensorMap *map) {
+    const PagedCache &c = a.cache;
+    int unit = most;
+    while (unit >= 8 && c.page % unit) unit /= 2;
+    if (unit < 8) return 1;
+    const uint64_t dims[5] = {(uint64_t)a.head_dim, (uint64_t)a.kv_heads, (uint64_t)c.page, 2, (uint64_t)c.pages};
+    const uint64_t strides[4] = {(uint64_t)a.head_dim * size, (uint64_t)c.row_stride, (uint64_t)c.parity_stride,
+                                 (uint64_t)c.page_stride};
+    const uint32_t box[5] = {128 / (uint32_t)size, 1, (uint32_t)unit, 1, 1};
+    const CUtensorMapDataType type = size == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : f16     ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                               : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    return encode_tensor_map_5d(map, type, c.base, dims, strides, box, swizzle) ? unit : 1;
+}
+
+__device__ __forceinline__ void tma_load_5d(void *dst, const void *map, int x, int y, int z, int u, int w,
+                                            uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(w), "r"(smem_addr(bar))
+        : "memory");
+}
 // One pass of the attention: the rows of each sequence against its own keys,
 // or all rows against the shared prefix.
 struct PagedPass {
@@ -63,6 +91,13 @@ struct PagedPass {
     // to paged_rows_kernel, the others to paged_attention_kernel.
     int small_rows;
 };
+
+// Whether some row of the segment may see key index i.
+template <typename C>
+__device__ __forceinline__ bool live_key(const PagedPass &p, const C &c, int i) {
+    const int pos = i < c.sink ? i : i - c.sink + c.low;
+    return i < c.keys && (pos >= c.from || ((i < c.sink || c.sink == c.low) && pos < p.a.sinks));
+}
 
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) {

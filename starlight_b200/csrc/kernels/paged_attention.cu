@@ -16,25 +16,28 @@
 // (ticket, no waiting), its pieces in ascending order: results do not depend
 // on the order of execution.
 //
-// A tile is 16 keys for each of the CTA's warps. A warp fetches its keys and
-// values with 16-byte asynchronous copies into a ring of its own, kStages
-// tiles ahead and across segment borders (bulk copies of single rows, 256 or
-// 512 bytes, were bound by the copy unit: about 35 cycles each), and shares
-// nothing with the other warps until the segment's end, where the warps' m, l
-// and o merge in shared memory.
+// A tile is 16 or 32 keys for each of the CTA's warps. A warp fetches its keys and
+// values into a ring of its own, kStages tiles ahead and across segment
+// borders, and shares nothing with the other warps until the segment's end,
+// where the warps' m, l and o merge in shared memory. It fetches them as TMA
+// boxes of 8 to 32 keys by 128 bytes, swizzled. (Pages that are not a
+// multiple of 8 keys go by 16-byte asynchronous copies: twice the
+// instructions in all, which is what bounds two warps per scheduler. Bulk
+// copies of single rows, 256 or 512 bytes, were bound by the copy unit, about
+// 35 cycles each.)
 //
 // Arithmetic. The tiles are transposed (S^T = K Q^T, O^T = V^T P^T), so that
 // the 16 of the MMA are keys and dimensions and the 8 are query rows: decode
 // has 1 to 8 rows per kv head (GQA), and rows beyond that would be padding.
 //   F32   m16n8k8 on tf32 pairs: x = hi + lo with hi rounded to 11 bits, three
-//         products (lo hi, hi lo, hi hi), 2^-21 relative. Dimensions and keys
-//         inside a tile are permuted so that a fragment is one 128-bit shared
-//         load without bank conflicts.
+//         products (lo hi, hi lo, hi hi), 2^-21 relative.
 //   F16   m16n8k16; keys and values are exact, queries (each row scaled by a
 //         power of two to 2^14) and probabilities (times 2^14) are pairs of
 //         f16, 22 bits, two products.
 //   BF16  m16n8k16; queries and probabilities are three bf16, 24 bits, three
 //         products.
+// Keys are fragments by ldmatrix, values by its transposed form (16 bit) or
+// by 128-bit loads with keys and dims permuted (F32), without bank conflicts.
 // The probabilities of a tile turn from S^T's accumulator layout into B
 // fragments by shuffles (F32) or movmatrix (16 bit), without shared memory.
 //
@@ -55,7 +58,6 @@ namespace k {
 namespace {
 
 constexpr int kRows = 8;
-constexpr int kWarpKeys = 16;
 constexpr int kSmallRows = 32;  // query rows per kv head taken here; more go to paged_rows.cu
 
 template <typename T, int DP>
@@ -63,19 +65,21 @@ struct Cfg {
     static constexpr bool kHalf = sizeof(T) == 2;
     static constexpr int kWarps = !kHalf && DP == 256 ? 4 : 8;
     static constexpr int kThreads = kWarps * 32;
+    // 16 keys an MMA; two of them a tile give a warp independent work to
+    // overlap and halve the rest (16-bit rows fit twice).
+    static constexpr int kSub = kHalf && DP <= 128 ? 2 : 1;
+    static constexpr int kWarpKeys = 16 * kSub;
     static constexpr int kTileKeys = kWarps * kWarpKeys;
     static constexpr int kTerms = std::is_same<T, __nv_bfloat16>::value ? 3 : 2;  // of a query or probability
     static constexpr int kShift = std::is_same<T, __half>::value ? 14 : 0;        // f16: scaled by 2^14
     static constexpr int kEpl = 16 / (int)sizeof(T);  // elements of 16 bytes
     static constexpr int kLpr = DP / kEpl;             // 16-byte pieces of a cache row
-    // Row strides: 128-bit fragment loads of keys want 16 mod 32 words, of
-    // values 8 mod 32; ldmatrix wants 16 mod 128 bytes.
-    static constexpr int kKStride = DP * (int)sizeof(T) + (kHalf ? 16 : 64);
-    static constexpr int kVStride = DP * (int)sizeof(T) + (kHalf ? 16 : 32);
-    static constexpr int kStageBytes = kWarpKeys * (kKStride + kVStride);
+    static constexpr int kBlk = DP * (int)sizeof(T) / 128;      // 128-byte blocks of one
+    static constexpr int kHalfStage = kBlk * kWarpKeys * 128;  // keys, or values: [block][key][128 bytes]
+    static constexpr int kStageBytes = 2 * kHalfStage;
     static constexpr int kMergeStride = DP + 4;  // floats
     static constexpr int kQBytes = kRows * DP * (kHalf ? 2 * kTerms : 8);
-    static constexpr int kFixed = kQBytes + kWarps * kRows * (kMergeStride + 2) * 4 + 512;
+    static constexpr int kFixed = kQBytes + kWarps * kRows * (kMergeStride + 2) * 4 + 1024 + 1024;
     static constexpr int kFit = (224 * 1024 - kFixed) / (kWarps * kStageBytes);
     static constexpr int kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kSmem = kFixed + kStages * kWarps * kStageBytes;
@@ -88,20 +92,21 @@ struct Cursor {
     long long left;  // units of this sequence from the current one on, itself included
     int b;           // sequence
     int tok0, ntok, past;
-    int sink, low, keys;  // visible keys: [0, sink) and [low, low + keys - sink)
+    // Key indexes run over positions [0, sink) and from `low` on, both widened
+    // to whole boxes; visible are those below `sinks` and from `from` on.
+    int sink, low, from, keys;
     int tiles, kvh, rb, tile;
 };
 
 template <int kTile>
-__device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor<kTile> &c) {
+__device__ __forceinline__ void seq_load(const PagedPass &p, int unit, int b, Cursor<kTile> &c) {
     c.b = b;
     if (p.prefix_pass) {
         c.b = paged_sequence_of(p.a.batch, 0);  // the first with tokens: its table row
         c.tok0 = 0;
         c.ntok = (int)p.a.batch.starts[p.a.batch.seqs];
         c.past = p.a.prefix;
-        c.sink = 0;
-        c.low = 0;
+        c.sink = c.low = c.from = 0;
         c.keys = p.a.prefix;
     } else {
         c.tok0 = (int)p.a.batch.starts[b];
@@ -109,10 +114,12 @@ __device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor<kTile
         if ((long long)c.ntok * (p.a.heads / p.a.kv_heads) > p.small_rows) c.ntok = 0;
         c.past = (int)p.a.batch.past[b];
         c.sink = 0;
-        c.low = p.first;
+        c.from = p.first;
+        if (p.a.window) c.from = max(c.past + 1 - p.a.window, 0);
+        c.low = c.from - c.from % unit;
         if (p.a.window) {
-            c.low = max(c.past + 1 - p.a.window, 0);
-            c.sink = min(p.a.sinks, c.low);
+            c.sink = (min(p.a.sinks, c.from) + unit - 1) / unit * unit;
+            if (c.sink >= c.low) c.sink = c.low = 0;
         }
         c.keys = c.sink + c.past + c.ntok - c.low;
     }
@@ -126,12 +133,12 @@ __device__ __forceinline__ long long seq_units(const PagedPass &p, const Cursor<
 
 // Places the cursor on unit `at` counted from the start of sequence c.b.
 template <int kTile>
-__device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor<kTile> &c, long long at) {
+__device__ __forceinline__ void cursor_at(const PagedPass &p, int unit, Cursor<kTile> &c, long long at) {
     const int seqs = p.prefix_pass ? 1 : p.a.batch.seqs;
     long long n = seq_units(p, c);
     while (!p.prefix_pass && at >= n && c.b + 1 < seqs) {
         at -= n;
-        seq_load(p, c.b + 1, c);
+        seq_load(p, unit, c.b + 1, c);
         n = seq_units(p, c);
     }
     c.left = n - at;
@@ -142,9 +149,9 @@ __device__ __forceinline__ void cursor_at(const PagedPass &p, Cursor<kTile> &c, 
 }
 
 template <int kTile>
-__device__ __forceinline__ void cursor_next(const PagedPass &p, Cursor<kTile> &c) {
+__device__ __forceinline__ void cursor_next(const PagedPass &p, int unit, Cursor<kTile> &c) {
     if (--c.left == 0) {
-        cursor_at(p, c, seq_units(p, c));
+        cursor_at(p, unit, c, seq_units(p, c));
         return;
     }
     if (++c.tile == c.tiles) {
@@ -229,25 +236,35 @@ __device__ __forceinline__ bool sees(const PagedPass &p, const Cursor<kTile> &c,
     if (i >= c.keys) return false;
     if (p.prefix_pass) return true;
     const int pos = key_pos(c, i);
-    return pos <= at && (!p.a.window || pos > at - p.a.window || pos < p.a.sinks);
+    return pos <= at && pos >= p.first && (!p.a.window || pos > at - p.a.window || pos < p.a.sinks);
 }
 // Whether every row of the segment sees every key of [i0, i1).
 template <int kTile>
 __device__ __forceinline__ bool all_see(const PagedPass &p, const Cursor<kTile> &c, int i0, int i1) {
     if (p.prefix_pass) return i1 <= c.keys;
     if (i1 > c.keys - (c.ntok - 1)) return false;
-    return !p.a.window || i1 <= c.sink || i0 >= c.sink + max(c.past + c.ntok - p.a.window - c.low, 0);
+    const int from = p.a.window ? max(c.past + c.ntok - p.a.window, c.from) : c.from;
+    return i0 >= c.sink + from - c.low || (i1 <= max(c.sink, c.from) && i1 <= p.a.sinks);
 }
+
+struct PassArgs {
+    PagedPass pass;
+    CUtensorMap map;
+    int unit;  // keys per box (paged_boxes); 1: no boxes
+};
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
-    paged_attention_kernel(const __grid_constant__ PagedPass p) {
+    paged_attention_kernel(const __grid_constant__ PassArgs args) {
+    const PagedPass &p = args.pass;
+    const int unit = args.unit;
     using C = Cfg<T, DP>;
     using Cur = Cursor<C::kTileKeys>;
     constexpr int kWarps = C::kWarps, kThreads = C::kThreads, kTileKeys = C::kTileKeys, S = C::kStages;
+    constexpr int kWarpKeys = C::kWarpKeys, kSub = C::kSub;
     constexpr int NT = DP / 16;
-    extern __shared__ __align__(128) unsigned char smem[];
-    unsigned char *ring = smem;
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    unsigned char *ring = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     unsigned char *q_s = ring + S * kWarps * C::kStageBytes;            // fragments of the queries
     float *mo = reinterpret_cast<float *>(q_s + C::kQBytes);           // [kWarps][kRows][kMergeStride]
     float *mml = mo + kWarps * kRows * C::kMergeStride;                 // [kWarps][kRows][2]
@@ -256,6 +273,8 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
     long long *sums = reinterpret_cast<long long *>(q_scale + kRows);   // [kWarps]
     int *last_s = reinterpret_cast<int *>(sums + kWarps), *bad_s = last_s + 1;  // bad_s: bit per row
     long long *found = sums + kWarps + 1;                               // [2]
+    uint64_t *bars = reinterpret_cast<uint64_t *>(found + 2);           // [kWarps][S][2] keys, values landed
+    volatile int *abort = reinterpret_cast<int *>(bars + kWarps * S * 2);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
@@ -272,7 +291,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         const int b = threadIdx.x * per + i;
         if (b < seqs) {
             Cur c;
-            seq_load(p, b, c);
+            seq_load(p, unit, b, c);
             mine += seq_units(p, c);
         }
     }
@@ -299,70 +318,94 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         found[0] = threadIdx.x;
         found[1] = upto - mine;
     }
-    if (threadIdx.x == 0) *bad_s = 0;
+    if (threadIdx.x == 0) {
+        *bad_s = 0;
+        *abort = 0;
+        for (int i = 0; i < kWarps * S * 2; i++) mbar_init(&bars[i], 1);
+        fence_mbar_init();
+    }
     __syncthreads();
     Cur cc, pc;  // consumer and producer
-    seq_load(p, (int)found[0] * per, cc);
-    cursor_at(p, cc, u0 - found[1]);
+    seq_load(p, unit, (int)found[0] * per, cc);
+    cursor_at(p, unit, cc, u0 - found[1]);
     pc = cc;
     pdl_wait();  // q and the cache come from earlier kernels; workspace use may overlap none
 
-    // The producer's unit: lane r (and r + 16) holds the table entry and the
-    // place in its page of the warp's key r, read a tile before its use.
+    // The producer's unit: lane b holds the table entry and the place in its
+    // page of box b of the warp's keys, or, without boxes, lane r those of key
+    // r (modulo the keys); read a tile before their use.
+    uint64_t *bar = bars + warp * S * 2;
     uint32_t next_id = 0;
     int next_in = -1;  // -1: past the segment's keys
     auto look_up = [&] {
-        const int i = pc.tile * kTileKeys + warp * kWarpKeys + (lane & 15);
+        const int k = unit > 1 ? lane * unit : lane % kWarpKeys, i = pc.tile * kTileKeys + warp * kWarpKeys + k;
         next_in = -1;
-        if (i < pc.keys) {
+        if (k < kWarpKeys && i < pc.keys) {
             const int pos = key_pos(pc, i), pg = page_of(p.a.cache, pos);
             next_in = pos - pg * p.a.cache.page;
             next_id = pg < p.a.batch.per_seq ? p.a.batch.table[(long long)pc.b * p.a.batch.per_seq + pg] : ~0u;
         }
     };
-    // Copies the warp's 16 keys of the producer's unit into a stage, or its
-    // 16 values: zeros for rows past the segment's keys (values meet zero
-    // probabilities there) and for dims past head_dim.
     const int head_bytes = D * (int)sizeof(T);
-    long long off = -1;
-    auto place = [&] {
-        off = -1;
-        if (next_in < 0) return;
-        if (next_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
+    // Copies the warp's keys of the producer's unit into a stage, or its
+    // values. (checked on the host: page ids; see paged_row)
+    auto issue = [&](int stage, int parity) {
+        unsigned char *st = ring + (warp * S + stage) * C::kStageBytes + parity * C::kHalfStage;
+        if (next_in >= 0 && next_id >= (uint32_t)p.a.cache.pages) {
             report_error(p.a.err, kErrGatherId);
             next_id = 0;
         }
-        off = next_id * p.a.cache.page_stride + next_in * p.a.cache.row_stride + (long long)pc.kvh * head_bytes;
-    };
-    auto issue = [&](int stage, int parity) {
-        unsigned char *st = ring + (warp * S + stage) * C::kStageBytes + (parity ? kWarpKeys * C::kKStride : 0);
-        const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0);
+        if (unit > 1) {
+            if (__any_sync(0xffffffffu, *abort)) return;
+            uint64_t *full = bar + 2 * stage + parity;
+            const int count = __popc(__ballot_sync(0xffffffffu, next_in >= 0));
+            if (lane == 0) mbar_arrive_expect_tx(full, count * unit * 128 * C::kBlk);
+            __syncwarp();
+            if (next_in >= 0)
 #pragma unroll
-        for (int x = 0; x < kWarpKeys * C::kLpr / 32; x++) {
-            const int r = (x * 32 + lane) / C::kLpr, c = (x * 32 + lane) % C::kLpr * 16;
-            const long long o = __shfl_sync(0xffffffffu, off, r);
-            const bool live = o >= 0 && c < head_bytes;
-            cp_async16_zfill(st + r * (parity ? C::kVStride : C::kKStride) + c, base + (live ? o + c : 0),
-                             live ? 16 : 0);
+                for (int y = 0; y < C::kBlk; y++)
+                    tma_load_5d(st + (y * kWarpKeys + lane * unit) * 128, &args.map, y * (128 / (int)sizeof(T)), pc.kvh,
+                                next_in, parity, (int)next_id, full);
+            return;
         }
+        // Zeros for rows past the segment's keys and for dims past head_dim.
+        long long off = -1;
+        if (next_in >= 0)
+            off = next_id * p.a.cache.page_stride + next_in * p.a.cache.row_stride + (long long)pc.kvh * head_bytes;
+        const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0);
+#pragma unroll 2
+        for (int x = 0; x < kWarpKeys * C::kLpr / 32; x++) {
+            const int r = (x * 32 + lane) / C::kLpr, c = (x * 32 + lane) % C::kLpr;
+            const long long o = __shfl_sync(0xffffffffu, off, r);
+            const bool live = o >= 0 && c * 16 < head_bytes;
+            cp_async16_zfill(st + (c / 8 * kWarpKeys + r) * 128 + ((c % 8) ^ (r & 7)) * 16,
+                             base + (live ? o + c * 16 : 0), live ? 16 : 0);
+        }
+        cp_async_commit();
+    };
+    auto landed = [&](int stage, int parity, int phase) {
+        if (unit > 1)
+            mbar_wait(bar + 2 * stage + parity, phase, p.a.err, abort);
+        else
+            cp_async_wait<2 * S - 1>();
+        __syncwarp();
     };
     const int units = (int)(u1 - u0);
     int issued = 0;
+    if (unit > 1 && threadIdx.x == 0) prefetch_tensormap(&args.map);
     look_up();
     for (; issued < S; issued++) {
         if (issued < units) {
-            place();
             issue(issued, 0);
-            cp_async_commit();
             issue(issued, 1);
             if (issued + 1 < units) {
-                cursor_next(p, pc);
+                cursor_next(p, unit, pc);
                 look_up();
             }
-        } else {
+        } else if (unit == 1) {  // one group a half, empty ones at the end
+            cp_async_commit();
             cp_async_commit();
         }
-        cp_async_commit();
     }
 
     // Queries of a segment, a warp per row: read a tile before they are used,
@@ -411,11 +454,11 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
                         *reinterpret_cast<uint16_t *>(dst + x * 128) = (uint16_t)w;
                     }
                 } else {
-                    // Block j, lane (r, t): dims 4t .. 4t + 3; hi, then lo.
-                    float *dst = reinterpret_cast<float *>(q_s) + (j * 32 + r * 4 + k / 4) * 4 + k % 4;
+                    // k step d / 8, lane (r, t): dims t and 4 + t, hi and lo.
+                    float *dst = reinterpret_cast<float *>(q_s) + (d / 8 * 32 + r * 4 + d % 4) * 4 + d / 4 % 2;
                     const uint32_t hi = tf32_hi(v[y]);
                     dst[0] = __uint_as_float(hi);
-                    dst[kRows * DP] = __uint_as_float(tf32_lo(v[y], hi));
+                    dst[2] = __uint_as_float(tf32_lo(v[y], hi));
                 }
             }
         }
@@ -430,7 +473,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
     int at0 = 0, at1 = 0;        // their positions
     long long seg_u0 = u0;       // this CTA's first unit of the current segment
     bool fresh = true;
-    int stage = 0;
+    int stage = 0, phase = 0;
     Cur nc = cc;                 // first unit of the segment after this one
     // The outputs of a segment that this thread merges and writes: item i is
     // row r, dims d .. d + 3; what a prefix pass left for them.
@@ -450,7 +493,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         if (ends) {
             if (u + 1 < u1) {
                 nc = cc;
-                cursor_next(p, nc);
+                cursor_next(p, unit, nc);
                 load_q(nc);
             }
             if (p.pre_o && !p.prefix_pass)
@@ -478,73 +521,81 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             qf0 = q_scale[2 * t];
             qf1 = q_scale[2 * t + 1];
         }
-        cp_async_wait<2 * S - 1>();
-        __syncwarp();
-        const unsigned char *ks = ring + (warp * S + stage) * C::kStageBytes;
-        const unsigned char *vs = ks + kWarpKeys * C::kKStride;
+        landed(stage, 0, phase);
+        unsigned char *ks = ring + (warp * S + stage) * C::kStageBytes, *vs = ks + C::kHalfStage;
 
         // S^T: keys g, g + 8 x rows 2t, 2t + 1; small products apart.
-        float s[4][4];
+        float s[kSub][4][4];
 #pragma unroll
-        for (int i = 0; i < 4; i++)
+        for (int h = 0; h < kSub; h++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[i][j] = 0.f;
-        if constexpr (C::kHalf) {
-            const uint32_t ka = smem_addr(ks) + (lane & 15) * C::kKStride + (lane >> 4) * 16;
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-            for (int j = 0; j < DP / 16; j++) {
-                uint32_t a[4];
-                ldmatrix4<false>(ka + j * 32, a);
+                for (int j = 0; j < 4; j++) s[h][i][j] = 0.f;
+        {
+            // 32 bytes of 16 keys a step: row lane % 16, 16-byte piece 2 (j % 4)
+            // + lane / 16 of its 128-byte block, xored with the row.
+            const uint32_t ka = smem_addr(ks) + (lane & 15) * 128, x0 = (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
-                for (int x = 0; x < C::kTerms; x++) {
-                    const uint2 b = reinterpret_cast<const uint2 *>(q_s)[(j * C::kTerms + x) * 32 + lane];
-                    mma_16<T>(s[x], a, b.x, b.y);
-                }
-            }
-        } else {
+            for (int j = 0; j < 4 * C::kBlk; j++) {
+                uint32_t a[kSub][4];
 #pragma unroll
-            for (int j = 0; j < DP / 16; j++) {
-                float ka[4], kb[4];
-                Frag<T>::ld(ks + g * C::kKStride + (j * 16 + 4 * t) * sizeof(T), ka);
-                Frag<T>::ld(ks + (g + 8) * C::kKStride + (j * 16 + 4 * t) * sizeof(T), kb);
-                const float4 qh = reinterpret_cast<const float4 *>(q_s)[j * 32 + lane];
-                const float4 ql = reinterpret_cast<const float4 *>(q_s)[kRows * DP / 4 + j * 32 + lane];
-                const float h4[4] = {qh.x, qh.y, qh.z, qh.w}, w4[4] = {ql.x, ql.y, ql.z, ql.w};
+                for (int h = 0; h < kSub; h++)
+                    ldmatrix4<false>(ka + (j / 4 * kWarpKeys + h * 16) * 128 + (x0 ^ (j % 4 * 32)), a[h]);
+                if constexpr (C::kHalf) {
 #pragma unroll
-                for (int y = 0; y < 2; y++) {
-                    const float f[4] = {ka[2 * y], kb[2 * y], ka[2 * y + 1], kb[2 * y + 1]};
-                    uint32_t hi[4], lo[4];
+                    for (int x = 0; x < C::kTerms; x++) {
+                        const uint2 b = reinterpret_cast<const uint2 *>(q_s)[(j * C::kTerms + x) * 32 + lane];
 #pragma unroll
-                    for (int z = 0; z < 4; z++) {
-                        hi[z] = tf32_hi(f[z]);
-                        lo[z] = tf32_lo(f[z], hi[z]);
+                        for (int h = 0; h < kSub; h++) mma_16<T>(s[h][x], a[h], b.x, b.y);
                     }
-                    const uint32_t b0 = __float_as_uint(h4[2 * y]), b1 = __float_as_uint(h4[2 * y + 1]);
-                    mma_tf32(s[2 + y], hi, __float_as_uint(w4[2 * y]), __float_as_uint(w4[2 * y + 1]));
-                    mma_tf32(s[y], hi, b0, b1);
-                    mma_tf32(s[2 + y], lo, b0, b1);
+                } else {
+                    const float4 b = reinterpret_cast<const float4 *>(q_s)[j * 32 + lane];
+                    const uint32_t h0 = __float_as_uint(b.x), h1 = __float_as_uint(b.y);
+#pragma unroll
+                    for (int h = 0; h < kSub; h++) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int z = 0; z < 4; z++) {
+                            const float f = __uint_as_float(a[h][z]);
+                            hi[z] = tf32_hi(f);
+                            lo[z] = tf32_lo(f, hi[z]);
+                        }
+                        mma_tf32(s[h][2 + (j & 1)], hi, __float_as_uint(b.z), __float_as_uint(b.w));
+                        mma_tf32(s[h][j & 1], hi, h0, h1);
+                        mma_tf32(s[h][2 + (j & 1)], lo, h0, h1);
+                    }
                 }
             }
         }
         // The keys are read: their slot takes those of S tiles on.
         __syncwarp();
         const bool more = issued < units;
-        if (more) {
-            place();
+        if (more)
             issue(stage, 0);
-        }
-        cp_async_commit();
+        else if (unit == 1)
+            cp_async_commit();
 
-        const int w0i = cc.tile * kTileKeys + warp * kWarpKeys, i0 = w0i + g, i1 = i0 + 8;
-        float sc[4];
+        const int w0i = cc.tile * kTileKeys + warp * kWarpKeys;
+        float pr[kSub][4];
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            sc[j] = ((s[3][j] + s[2][j]) + (s[1][j] + s[0][j])) * ((j & 1) ? qf1 : qf0);
-        if (!all_see(p, cc, w0i, w0i + kWarpKeys))
+        for (int h = 0; h < kSub; h++)
 #pragma unroll
             for (int j = 0; j < 4; j++)
-                if (!sees(p, cc, j < 2 ? i0 : i1, (j & 1) ? at1 : at0)) sc[j] = -INFINITY;
-        float n0 = fmaxf(sc[0], sc[2]), n1 = fmaxf(sc[1], sc[3]);
+                pr[h][j] =
+                    ((s[h][3][j] + s[h][2][j]) + (s[h][1][j] + s[h][0][j])) * ((j & 1) ? qf1 : qf0);
+        const bool clear = all_see(p, cc, w0i, w0i + kWarpKeys);
+        if (!clear)
+#pragma unroll
+            for (int h = 0; h < kSub; h++)
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (!sees(p, cc, w0i + h * 16 + g + j / 2 * 8, (j & 1) ? at1 : at0)) pr[h][j] = -INFINITY;
+        float n0 = fmaxf(pr[0][0], pr[0][2]), n1 = fmaxf(pr[0][1], pr[0][3]);
+        if (kSub == 2) {
+            n0 = fmaxf(n0, fmaxf(pr[kSub - 1][0], pr[kSub - 1][2]));
+            n1 = fmaxf(n1, fmaxf(pr[kSub - 1][1], pr[kSub - 1][3]));
+        }
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) {
             n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
@@ -553,55 +604,72 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         n0 = fmaxf(n0, m0);
         n1 = fmaxf(n1, m1);
         const float u_0 = n0 == -INFINITY ? 0.f : n0, u_1 = n1 == -INFINITY ? 0.f : n1;
-        float pr[4];
-        pr[0] = ex2(sc[0] - (u_0 - C::kShift));
-        pr[1] = ex2(sc[1] - (u_1 - C::kShift));
-        pr[2] = ex2(sc[2] - (u_0 - C::kShift));
-        pr[3] = ex2(sc[3] - (u_1 - C::kShift));
         const float f0 = ex2(m0 - u_0), f1 = ex2(m1 - u_1);
         l0 *= f0;
         l1 *= f1;
         m0 = n0;
         m1 = n1;
-        l0 += pr[0] + pr[2];
-        l1 += pr[1] + pr[3];
-        cp_async_wait<2 * S - 1>();
-        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < kSub; h++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) pr[h][j] = ex2(pr[h][j] - (((j & 1) ? u_1 : u_0) - C::kShift));
+            l0 += pr[h][0] + pr[h][2];
+            l1 += pr[h][1] + pr[h][3];
+        }
+        landed(stage, 1, phase);
+        if (!clear && unit > 1) {
+            // Values of keys that no row sees may be anything, and meet zero
+            // probabilities: they become zero.
+            for (int r = 0; r < kWarpKeys; r++)
+                if (!live_key(p, cc, w0i + r))
+                    for (int c = lane; c < C::kBlk * 8; c += 32)
+                        *reinterpret_cast<uint4 *>(vs + (c / 8 * kWarpKeys + r) * 128 + c % 8 * 16) =
+                            make_uint4(0, 0, 0, 0);
+            fence_proxy_async_smem();
+            __syncwarp();
+        }
 
         // A tile's P V starts from zero and is added to the running output
         // outside the tensor core, whose accumulation truncates: over
         // thousands of keys that bias would grow past f32 rounding.
         if constexpr (C::kHalf) {
             // B fragments: row g, keys 2t, 2t + 1 and 8 + 2t, 9 + 2t.
-            uint32_t b[3][2];
+            uint32_t b[kSub][C::kTerms][2];
 #pragma unroll
-            for (int x = 0; x < C::kTerms; x++) {
-                b[x][0] = movmatrix(take_pair<T>(pr[0], pr[1]));
-                b[x][1] = movmatrix(take_pair<T>(pr[2], pr[3]));
-            }
-            const uint32_t va = smem_addr(vs) + ((lane & 7) + (lane >> 4) * 8) * C::kVStride + ((lane >> 3) & 1) * 16;
+            for (int x = 0; x < C::kTerms; x++)
+#pragma unroll
+                for (int h = 0; h < kSub; h++) {
+                    b[h][x][0] = movmatrix(take_pair<T>(pr[h][0], pr[h][1]));
+                    b[h][x][1] = movmatrix(take_pair<T>(pr[h][2], pr[h][3]));
+                }
+            // Key lane % 8 + 8 (lane / 16), 16-byte piece 2 (i % 4) + lane / 8 % 2.
+            const uint32_t va = smem_addr(vs) + ((lane & 7) + (lane >> 4) * 8) * 128,
+                           x0 = ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 #pragma unroll
             for (int i = 0; i < NT; i++) {
-                uint32_t a[4];
-                ldmatrix4<true>(va + i * 32, a);
                 float o[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int x = C::kTerms - 1; x >= 0; x--) mma_16<T>(o, a, b[x][0], b[x][1]);
+                for (int h = 0; h < kSub; h++) {
+                    uint32_t a[4];
+                    ldmatrix4<true>(va + (i / 4 * kWarpKeys + h * 16) * 128 + (x0 ^ (i % 4 * 32)), a);
+#pragma unroll
+                    for (int x = C::kTerms - 1; x >= 0; x--) mma_16<T>(o, a, b[h][x][0], b[h][x][1]);
+                }
                 acc[i][0] = fmaf(acc[i][0], f0, o[0]);
                 acc[i][1] = fmaf(acc[i][1], f1, o[1]);
                 acc[i][2] = fmaf(acc[i][2], f0, o[2]);
                 acc[i][3] = fmaf(acc[i][3], f1, o[3]);
             }
         } else {
-            // B fragments of the two 8-key steps: row g, keys t and t + 4.
+            // B fragments of the two 8-key steps: row g, keys 2t and 2t + 1.
             uint32_t bh[2][2], bl[2][2];
 #pragma unroll
             for (int k8 = 0; k8 < 2; k8++)
 #pragma unroll
                 for (int x = 0; x < 2; x++) {
-                    const int src = (t + 4 * x) * 4 + (g >> 1);
-                    const float a = __shfl_sync(0xffffffffu, pr[2 * k8], src);
-                    const float b = __shfl_sync(0xffffffffu, pr[2 * k8 + 1], src);
+                    const int src = (2 * t + x) * 4 + (g >> 1);
+                    const float a = __shfl_sync(0xffffffffu, pr[0][2 * k8], src);
+                    const float b = __shfl_sync(0xffffffffu, pr[0][2 * k8 + 1], src);
                     const float v = (g & 1) ? b : a;
                     bh[k8][x] = tf32_hi(v);
                     bl[k8][x] = tf32_lo(v, bh[k8][x]);
@@ -612,8 +680,9 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
 #pragma unroll
                 for (int k8 = 0; k8 < 2; k8++) {
                     float va[4], vb[4];
-                    Frag<T>::ld(vs + (8 * k8 + t) * C::kVStride + (j * 32 + 4 * g) * sizeof(T), va);
-                    Frag<T>::ld(vs + (8 * k8 + t + 4) * C::kVStride + (j * 32 + 4 * g) * sizeof(T), vb);
+                    const unsigned char *v0 = vs + (j * kWarpKeys + 8 * k8 + 2 * t) * 128;
+                    Frag<T>::ld(v0 + ((g ^ (2 * t)) << 4), va);
+                    Frag<T>::ld(v0 + 128 + ((g ^ (2 * t + 1)) << 4), vb);
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         const float f[4] = {va[2 * x], va[2 * x + 1], vb[2 * x], vb[2 * x + 1]};
@@ -643,12 +712,16 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             issue(stage, 1);
             issued++;
             if (issued < units) {
-                cursor_next(p, pc);
+                cursor_next(p, unit, pc);
                 look_up();
             }
+        } else if (unit == 1) {
+            cp_async_commit();
         }
-        cp_async_commit();
-        stage = stage + 1 == S ? 0 : stage + 1;
+        if (++stage == S) {
+            stage = 0;
+            phase ^= 1;
+        }
 
         if (!ends) {
             cc.tile++;
@@ -830,6 +903,14 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         fresh = true;
         cc = nc;
     }
+    // After a wait that gave up, copies may still be in flight: let them land
+    // before the CTA's shared memory is released.
+    if (unit > 1 && *abort && lane == 0)
+        for (int i = 0; i < 2 * S; i++) {
+            const uint64_t t0 = global_ns();
+            while (!mbar_try_wait(bar + i, phase ^ (i / 2 < stage)) && global_ns() - t0 < 100000000ull) {
+            }
+        }
 }
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
@@ -845,7 +926,10 @@ cudaError_t launch_pass(cudaStream_t s, const PagedPass &p) {
     static_assert(C::kStages >= 1 && C::kSmem <= 227 * 1024, "shared layout");
     static std::atomic<uint64_t> smem_set{0};
     set_smem_limit_once(paged_attention_kernel<T, DP>, C::kSmem, &smem_set);
-    launch_k(paged_attention_kernel<T, DP>, kSmCount, C::kThreads, C::kSmem, s, p);
+    PassArgs args{};
+    args.pass = p;
+    args.unit = paged_boxes(p.a, C::kWarpKeys, sizeof(T), std::is_same<T, __half>::value, true, &args.map);
+    launch_k(paged_attention_kernel<T, DP>, kSmCount, C::kThreads, C::kSmem, s, args);
     count_launch();
     return cudaGetLastError();
 }

@@ -27,8 +27,8 @@
 //          maximum would cost a quarter of the shared memory's bandwidth,
 //          which is what bounds an F32 cache).
 //   16     issues the MMAs: Q K^T of the next tile before P V of this one
-//   17     copies: one TMA box per page and 128-byte block into a ring of
-//          slots (pages that do not tile 128 rows in multiples of 8: 16-byte
+//   17     copies: TMA boxes of 8 to 128 keys of a page and 128 bytes into a
+//          ring of slots (pages that are not a multiple of 8 keys: 16-byte
 //          asynchronous copies, by warps 17..19)
 // The ring holds operands in the order K0 K1 V0 K2 V1 ..., so a slot is free
 // as soon as the MMAs kSlots back are done; three slots of pairs or six of
@@ -44,7 +44,6 @@
 #include "kernels.h"
 #include "paged.cuh"
 #include "tcgen05.cuh"
-#include "tensormap.h"
 #include "tma.cuh"
 
 namespace slc {
@@ -89,8 +88,8 @@ struct Cfg {
 
 struct RowsArgs {
     PagedPass pass;
-    CUtensorMap map;  // [pages][2][page][kv_heads][head_dim], box [128 bytes][1][unit][1][1]
-    int unit;         // keys per box; 1: no boxes
+    CUtensorMap map;
+    int unit;  // keys per box (paged_boxes); 1: no boxes
 };
 
 // A segment of the work line and a place in it. Key indexes run over
@@ -197,21 +196,7 @@ struct Tile {
     int b, kvh, i0;
     int sink, low, from, keys;
 };
-// Whether some row of the segment may see key index i.
-template <typename C>
-__device__ __forceinline__ bool live_key(const PagedPass &p, const C &c, int i) {
-    const int pos = i < c.sink ? i : i - c.sink + c.low;
-    return i < c.keys && (pos >= c.from || ((i < c.sink || c.sink == c.low) && pos < p.a.sinks));
-}
 
-__device__ __forceinline__ void tma_load_5d(void *dst, const void *map, int x, int y, int z, int u, int w,
-                                            uint64_t *bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes"
-        " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(smem_addr(dst)),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(u), "r"(w), "r"(smem_addr(bar))
-        : "memory");
-}
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
@@ -1061,24 +1046,9 @@ template <typename T, int DP>
 cudaError_t launch(cudaStream_t s, const PagedPass &p) {
     using C = Cfg<T, DP>;
     static_assert(C::kSmem <= 227 * 1024, "shared layout");
-    // Boxes of whole pages, or of 128 keys of a larger one, where they fill a
-    // tile without overlap and start on the swizzle's 8 rows.
     RowsArgs args{};
     args.pass = p;
-    args.unit = 1;
-    const PagedCache &c = p.a.cache;
-    if (c.page % 8 == 0 && (c.page % kKeys == 0 || kKeys % c.page == 0)) {
-        const int unit = c.page < kKeys ? c.page : kKeys;
-        const uint64_t dims[5] = {(uint64_t)p.a.head_dim, (uint64_t)p.a.kv_heads, (uint64_t)c.page, 2,
-                                  (uint64_t)c.pages};
-        const uint64_t strides[4] = {(uint64_t)p.a.head_dim * sizeof(T), (uint64_t)c.row_stride,
-                                     (uint64_t)c.parity_stride, (uint64_t)c.page_stride};
-        const uint32_t box[5] = {128 / (uint32_t)sizeof(T), 1, (uint32_t)unit, 1, 1};
-        const CUtensorMapDataType type = C::kPair  ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                         : C::kRaw ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
-                                                   : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-        if (encode_tensor_map_5d(&args.map, type, c.base, dims, strides, box, !C::kPair)) args.unit = unit;
-    }
+    args.unit = paged_boxes(p.a, kKeys, sizeof(T), C::kRaw, !C::kPair, &args.map);
     static std::atomic<uint64_t> smem_set{0};
     cudaError_t e = set_smem_limit_once(paged_rows_kernel<T, DP>, C::kSmem, &smem_set);
     if (e != cudaSuccess) return e;
