@@ -329,8 +329,6 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
     seq_load(p, unit, (int)found[0] * per, cc);
     cursor_at(p, unit, cc, u0 - found[1]);
     pc = cc;
-    pdl_wait();  // q and the cache come from earlier kernels; workspace use may overlap none
-
     // The producer's unit: lane b holds the table entry and the place in its
     // page of box b of the warp's keys, or, without boxes, lane r those of key
     // r (modulo the keys); read a tile before their use.
@@ -393,7 +391,8 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
     const int units = (int)(u1 - u0);
     int issued = 0;
     if (unit > 1 && threadIdx.x == 0) prefetch_tensormap(&args.map);
-    look_up();
+    look_up();   // lengths and tables come from uploads alone,
+    pdl_wait();  // q and the cache from earlier kernels; workspace use may overlap none
     for (; issued < S; issued++) {
         if (issued < units) {
             issue(issued, 0);
@@ -620,11 +619,13 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         if (!clear && unit > 1) {
             // Values of keys that no row sees may be anything, and meet zero
             // probabilities: they become zero.
-            for (int r = 0; r < kWarpKeys; r++)
-                if (!live_key(p, cc, w0i + r))
-                    for (int c = lane; c < C::kBlk * 8; c += 32)
-                        *reinterpret_cast<uint4 *>(vs + (c / 8 * kWarpKeys + r) * 128 + c % 8 * 16) =
-                            make_uint4(0, 0, 0, 0);
+            unsigned dead = __ballot_sync(0xffffffffu, lane < kWarpKeys && !live_key(p, cc, w0i + lane));
+            for (; dead; dead &= dead - 1) {
+                const int r = __ffs(dead) - 1;
+                for (int c = lane; c < C::kBlk * 8; c += 32)
+                    *reinterpret_cast<uint4 *>(vs + (c / 8 * kWarpKeys + r) * 128 + c % 8 * 16) =
+                        make_uint4(0, 0, 0, 0);
+            }
             fence_proxy_async_smem();
             __syncwarp();
         }

@@ -19,7 +19,7 @@
 //          S from TMEM, running maximum, P as f16 pairs back into the TMEM
 //          columns that S held
 //   4..7   output: one thread per row; O += P V of each tile in registers,
-//          the merge of a split segment, the result
+//          the result, or this CTA's piece of a split segment
 //   8..15  conversion in place: scale, f16 or f16 pair, zeros in rows that no
 //          query sees (they may hold anything). The scale is that of the
 //          operand before; a tile whose largest value does not suit it is
@@ -61,7 +61,7 @@ constexpr int kTop = 11;    // a tile's largest value around 2^11: from 2^9 to 2
 // conversion has two warpgroups.
 constexpr int kLaunchRegs = 96, kOutRegs = 184, kConvRegs = 64, kRestRegs = 72;
 static_assert(kLaunchRegs + kOutRegs + 2 * kConvRegs + kRestRegs <= 5 * kLaunchRegs, "register split");
-constexpr uint64_t kLimitNs = 4000000000ull;  // rows of values that are not finite take long
+constexpr uint64_t kLimitNs = 20000000000ull;  // rows of values that are not finite take long
 
 template <typename T, int DP>
 struct Cfg {
@@ -90,6 +90,7 @@ struct RowsArgs {
     PagedPass pass;
     CUtensorMap map;
     int unit;  // keys per box (paged_boxes); 1: no boxes
+    int join;  // split segments are merged by rows_join_kernel
 };
 
 // A segment of the work line and a place in it. Key indexes run over
@@ -145,20 +146,12 @@ __device__ __forceinline__ void row_tile_load(const PagedPass &p, int unit, Curs
     }
     c.tiles = (c.keys + kKeys - 1) / kKeys;
 }
-__device__ __forceinline__ long long seq_units(const PagedPass &p, int unit, Cursor &c) {
-    long long n = 0;
-    const int rts = row_tiles(p, c);
-    for (c.rt = 0; c.rt < rts; c.rt++) {
-        row_tile_load(p, unit, c);
-        n += c.tiles;
-    }
-    return n * p.a.kv_heads;
-}
-// Places the cursor on unit `at` of the line from sequence c.b on (c.rt 0).
+// Places the cursor on unit `at` of the line counted from row tile c.rt of
+// sequence c.b.
 __device__ __forceinline__ void cursor_at(const PagedPass &p, int unit, Cursor &c, long long at) {
     for (;;) {
         const int rts = row_tiles(p, c);
-        for (c.rt = 0; c.rt < rts; c.rt++) {
+        for (; c.rt < rts; c.rt++) {
             row_tile_load(p, unit, c);
             const long long n = (long long)c.tiles * p.a.kv_heads;
             if (at < n) {
@@ -170,6 +163,7 @@ __device__ __forceinline__ void cursor_at(const PagedPass &p, int unit, Cursor &
         }
         if (p.prefix_pass || c.b + 1 >= p.a.batch.seqs) return;
         seq_load(p, c.b + 1, c);
+        c.rt = 0;
     }
 }
 // The next unit; the line's end is the caller's to know.
@@ -184,7 +178,77 @@ __device__ __forceinline__ void cursor_next(const PagedPass &p, int unit, Cursor
     }
     if (p.prefix_pass || c.b + 1 >= p.a.batch.seqs) return;
     seq_load(p, c.b + 1, c);
+    c.rt = 0;
     cursor_at(p, unit, c, 0);
+}
+
+// The work line, added up by the first kM threads, each over a run of it: an
+// equal share of a sequence's row tiles, or several sequences. (A thread per
+// sequence took 14 us for two of 64 row tiles.)
+struct Line {
+    long long mine, upto;  // of this thread's run; up to its end
+    long long total;
+    int parts, per;  // runs per sequence, sequences per run
+};
+// The first row tile of a run and how many it has of that sequence (-1: the
+// run is whole sequences).
+__device__ __forceinline__ int run_start(const PagedPass &p, const Line &x, int run, Cursor &c) {
+    seq_load(p, run / x.parts * x.per, c);
+    c.rt = 0;
+    if (x.parts == 1) return -1;
+    const int rts = row_tiles(p, c), part = run % x.parts;
+    c.rt = (int)((long long)rts * part / x.parts);
+    return (int)((long long)rts * (part + 1) / x.parts) - c.rt;
+}
+// Every thread of the CTA calls it; sums: 6 words shared.
+__device__ __forceinline__ Line line_scan(const PagedPass &p, int unit, long long *sums) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, seqs = seq_count(p);
+    Line x;
+    x.mine = x.upto = x.total = 0;
+    x.parts = max(kM / seqs, 1);
+    x.per = (seqs + kM - 1) / kM;
+    if (warp < 4) {
+        const int first = (int)threadIdx.x / x.parts * x.per;
+        for (int b = first; b < min(first + x.per, seqs); b++) {
+            Cursor c;
+            int n = -1;
+            if (b == first)
+                n = run_start(p, x, threadIdx.x, c);
+            else
+                seq_load(p, b, c), c.rt = 0;
+            const int end = n < 0 ? row_tiles(p, c) : c.rt + n;
+            for (; c.rt < end; c.rt++) {
+                row_tile_load(p, unit, c);
+                x.mine += (long long)c.tiles * p.a.kv_heads;
+            }
+        }
+        x.upto = x.mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x.upto, o);
+            if (lane >= o) x.upto += y;
+        }
+        if (lane == 31) sums[warp] = x.upto;
+    }
+    __syncthreads();
+    for (int w = 0; w < 4; w++) {
+        if (w < warp) x.upto += sums[w];
+        x.total += sums[w];
+    }
+    return x;
+}
+// The thread whose run holds unit u leaves where that begins; after a barrier
+// line_place sets the cursor there.
+__device__ __forceinline__ void line_find(const Line &x, long long u, long long *sums) {
+    if (threadIdx.x < kM && x.upto - x.mine <= u && u < x.upto) {
+        sums[4] = threadIdx.x;
+        sums[5] = x.upto - x.mine;
+    }
+}
+__device__ __forceinline__ void line_place(const PagedPass &p, int unit, const Line &x, long long u,
+                                           const long long *sums, Cursor &c) {
+    run_start(p, x, (int)sums[4], c);
+    cursor_at(p, unit, c, u - sums[5]);
 }
 
 // Position of key index i.
@@ -264,6 +328,53 @@ __device__ __forceinline__ uint32_t operand_at(int row, int dim) {
     return (uint32_t)((dim >> 6) * kKeys * 128 + row * 128 + ((((dim & 63) >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2);
 }
 
+// Where a row's result goes: (o f + prefix o e) / l to the output, or for a
+// prefix pass o, m and l to where the next pass reads them.
+struct RowEnd {
+    float *dst;
+    const float *pre;
+    float l, f, e;
+    bool vec;  // dst is aligned for 16 bytes
+};
+__device__ __forceinline__ RowEnd row_end(const PagedPass &p, size_t qrow, float m, float l) {
+    const size_t at = qrow * p.a.head_dim;
+    if (p.prefix_pass) {
+        *reinterpret_cast<float2 *>(p.pre_ml + qrow * 2) = make_float2(m, l);
+        return {p.pre_o + at, nullptr, 1.f, 1.f, 0.f, true};
+    }
+    RowEnd x{p.a.out + at, nullptr, l, 1.f, 0.f, aligned16(p.a.out)};
+    if (p.pre_o) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.pre_ml) + qrow);
+        const float nm = fmaxf(m, ml.x), mu = nm == -INFINITY ? 0.f : nm;
+        x.pre = p.pre_o + at;
+        x.f = ex2(m - mu);
+        x.e = ex2(ml.x - mu);
+        x.l = fmaf(ml.y, x.e, l * x.f);
+    }
+    return x;
+}
+__device__ __forceinline__ void row_store(const RowEnd &x, int d, float4 o) {
+    if (x.pre) {
+        const float4 v = __ldcg(reinterpret_cast<const float4 *>(x.pre + d));
+        o.x = fmaf(v.x, x.e, o.x * x.f);
+        o.y = fmaf(v.y, x.e, o.y * x.f);
+        o.z = fmaf(v.z, x.e, o.z * x.f);
+        o.w = fmaf(v.w, x.e, o.w * x.f);
+    }
+    o.x = __fdiv_rn(o.x, x.l);
+    o.y = __fdiv_rn(o.y, x.l);
+    o.z = __fdiv_rn(o.z, x.l);
+    o.w = __fdiv_rn(o.w, x.l);
+    if (x.vec) {
+        *reinterpret_cast<float4 *>(x.dst + d) = o;
+    } else {
+        x.dst[d] = o.x;
+        x.dst[d + 1] = o.y;
+        x.dst[d + 2] = o.z;
+        x.dst[d + 3] = o.w;
+    }
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_constant__ RowsArgs args) {
     const PagedPass &p = args.pass;
@@ -323,33 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         for (int i = 0; i < 4; i++) most[i] = 0;
         for (int i = 0; i < 8; i++) poison[i] = 0;
     }
-    // The work line, as in paged_attention_kernel (the first kM threads).
-    const int seqs = seq_count(p);
-    const int per = (seqs + kM - 1) / kM;
-    long long mine = 0, upto = 0;
-    if (warp < 4) {
-        for (int i = 0; i < per; i++) {
-            const int b = threadIdx.x * per + i;
-            if (b < seqs) {
-                Cursor c;
-                seq_load(p, b, c);
-                mine += seq_units(p, unit, c);
-            }
-        }
-        upto = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
-        }
-        if (lane == 31) sums[warp] = upto;
-    }
-    __syncthreads();
-    long long U = 0;
-    for (int w = 0; w < 4; w++) {
-        if (w < warp) upto += sums[w];
-        U += sums[w];
-    }
+    const Line line = line_scan(p, unit, sums);
+    const long long U = line.total;
     const long long grid = min((long long)gridDim.x, U);
     if (blockIdx.x >= grid) {
         pdl_wait();
@@ -362,10 +448,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     const long long u0 = U * blockIdx.x / grid, u1 = U * (blockIdx.x + 1) / grid;
-    if (warp < 4 && upto - mine <= u0 && u0 < upto) {
-        sums[4] = threadIdx.x;
-        sums[5] = upto - mine;
-    }
+    line_find(line, u0, sums);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -373,8 +456,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     const uint32_t s_tm = tmem, o_tm = tmem + 256, q_tm = tmem + 384;  // S: two buffers
     const int N = (int)(u1 - u0);
     Cursor c;
-    seq_load(p, (int)sums[4] * per, c);
-    cursor_at(p, unit, c, u0 - sums[5]);
+    line_place(p, unit, line, u0, sums, c);
     pdl_wait();
 
     // Operand j of the ring: K of tile 0, then K of tile (j + 1) / 2 (odd j)
@@ -624,7 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 __syncwarp();
             }
             const long long a0 = u0 + n - c.tile, a1 = a0 + c.tiles;  // the segment's units
-            bool write = true;
+            bool write = live;
             if (a0 < u0 || a1 > u1) {
                 const int c_first = (int)(((a0 + 1) * grid - 1) / U), c_last = (int)((a1 * grid - 1) / U);
                 const size_t slot = 2 * blockIdx.x + (a0 >= u0 ? 1 : 0);
@@ -632,17 +714,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                 for (int d = 0; d < DP / 4; d++) po[d * kM] = four(d);
                 reinterpret_cast<float2 *>(p.part_ml)[slot * kM + r] = make_float2(m, l);
-                bar_sync(2, 128);
-                if (r == 0) {
-                    __threadfence();
-                    const unsigned ticket = atomicAdd(&p.a.tickets[c_first], 1u);
-                    *last_s = ticket == (unsigned)(c_last - c_first);
-                    if (*last_s) p.a.tickets[c_first] = 0u;
-                    __threadfence();
+                if (args.join) {
+                    write = false;
+                } else {
+                    bar_sync(2, 128);
+                    if (r == 0) {
+                        __threadfence();
+                        const unsigned ticket = atomicAdd(&p.a.tickets[c_first], 1u);
+                        *last_s = ticket == (unsigned)(c_last - c_first);
+                        if (*last_s) p.a.tickets[c_first] = 0u;
+                        __threadfence();
+                    }
+                    bar_sync(2, 128);
+                    write = live && *last_s;
+                    bar_sync(2, 128);
                 }
-                bar_sync(2, 128);
-                write = *last_s;
-                bar_sync(2, 128);
                 if (write) {
                     m = -INFINITY;
                     l = 0.f;
@@ -665,51 +751,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     }
                 }
             }
-            if (write && live) {
-                if (p.prefix_pass) {
-                    float *dst = p.pre_o + qrow * D;
+            if (write) {
+                const RowEnd end = row_end(p, qrow, m, l);
 #pragma unroll
-                    for (int d = 0; d < DP; d += 4)
-                        if (d < D)
-                            *reinterpret_cast<float4 *>(dst + d) = four(d / 4);
-                    *reinterpret_cast<float2 *>(p.pre_ml + qrow * 2) = make_float2(m, l);
-                } else {
-                    float f = 1.f, e = 0.f;
-                    const float *pre = p.pre_o ? p.pre_o + qrow * D : nullptr;
-                    if (pre) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p.pre_ml) + qrow);
-                        const float nm = fmaxf(m, ml.x), mu = nm == -INFINITY ? 0.f : nm;
-                        f = ex2(m - mu);
-                        e = ex2(ml.x - mu);
-                        l = fmaf(ml.y, e, l * f);
-                    }
-                    float *dst = p.a.out + qrow * D;
-                    const bool vec = aligned16(p.a.out);
-#pragma unroll
-                    for (int d = 0; d < DP; d += 4) {
-                        if (d >= D) continue;
-                        float4 o = four(d / 4);
-                        if (pre) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(pre + d));
-                            o.x = fmaf(v.x, e, o.x * f);
-                            o.y = fmaf(v.y, e, o.y * f);
-                            o.z = fmaf(v.z, e, o.z * f);
-                            o.w = fmaf(v.w, e, o.w * f);
-                        }
-                        o.x = __fdiv_rn(o.x, l);
-                        o.y = __fdiv_rn(o.y, l);
-                        o.z = __fdiv_rn(o.z, l);
-                        o.w = __fdiv_rn(o.w, l);
-                        if (vec) {
-                            *reinterpret_cast<float4 *>(dst + d) = o;
-                        } else {
-                            dst[d] = o.x;
-                            dst[d + 1] = o.y;
-                            dst[d + 2] = o.z;
-                            dst[d + 3] = o.w;
-                        }
-                    }
-                }
+                for (int d = 0; d < DP; d += 4)
+                    if (d < D) row_store(end, d, four(d / 4));
             }
 #pragma unroll
             for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
@@ -1040,6 +1086,81 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     }
 }
 
+// Merges the pieces of the segments that cuts of the work line split, a block
+// for every cut: a segment in k + 1 pieces has k of them, each for an equal
+// part of its rows. The pieces are added in ascending order, eight reads in
+// flight. Launched where segments are fewer than CTAs, and so in many pieces
+// each: for a prefix of 8192 keys in ten, the last CTA to finish one took 23 us
+// to merge it alone, this launch takes 6. With more segments than CTAs a
+// segment is in two pieces mostly, and a launch less was better by 17 us in 930
+// (two prompts of 2048 tokens).
+constexpr int kJoinThreads = 512;
+template <int DP>
+__global__ void __launch_bounds__(kJoinThreads) rows_join_kernel(const __grid_constant__ PagedPass p, int unit,
+                                                                 int ctas) {
+    __shared__ long long sums[6];
+    pdl_trigger();
+    const Line line = line_scan(p, unit, sums);
+    const long long U = line.total;
+    const long long grid = min((long long)ctas, U);
+    const int cut = 1 + blockIdx.x;  // before CTA `cut`
+    if (cut >= grid) {
+        pdl_wait();
+        return;
+    }
+    const long long u = U * cut / grid;
+    line_find(line, u, sums);
+    __syncthreads();
+    Cursor c;
+    line_place(p, unit, line, u, sums, c);
+    pdl_wait();
+    if (c.tile == 0) return;  // the cut lies between two segments
+    const long long a0 = u - c.tile, a1 = a0 + c.tiles;
+    const int first = (int)(((a0 + 1) * grid - 1) / U), last = (int)((a1 * grid - 1) / U);
+    const int shares = last - first, share = cut - first - 1;
+    const int lo = (int)((long long)c.rows * share / shares), n = (int)((long long)c.rows * (share + 1) / shares) - lo;
+    const int G = group_of(p), D = p.a.head_dim;
+    for (int i = threadIdx.x; i < n * (D / 4); i += kJoinThreads) {
+        const int d = i / n, r = lo + i % n, row = c.r0 + r, tok = row / G;
+        const size_t qrow = (size_t)(c.tok0 + tok) * p.a.heads + c.kvh * G + (row - tok * G);
+        float m = -INFINITY, l = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int x = first; x <= last; x += 8) {
+            float2 ml[8];
+            float4 v[8];
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                ml[y] = make_float2(-INFINITY, 0.f);
+                v[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (x + y > last) continue;
+                const size_t slot = 2 * (size_t)(x + y) + (x + y == first ? 1 : 0);
+                ml[y] = __ldcg(reinterpret_cast<const float2 *>(p.part_ml) + slot * kM + r);
+                v[y] = __ldcg(reinterpret_cast<const float4 *>(p.part_o) + (slot * (DP / 4) + d) * kM + r);
+            }
+            float nm = m;
+#pragma unroll
+            for (int y = 0; y < 8; y++) nm = fmaxf(nm, ml[y].x);
+            const float mu = nm == -INFINITY ? 0.f : nm, f = ex2(m - mu);
+            l *= f;
+            o.x *= f;
+            o.y *= f;
+            o.z *= f;
+            o.w *= f;
+#pragma unroll
+            for (int y = 0; y < 8; y++) {
+                const float e = ex2(ml[y].x - mu);
+                l = fmaf(ml[y].y, e, l);
+                o.x = fmaf(v[y].x, e, o.x);
+                o.y = fmaf(v[y].y, e, o.y);
+                o.z = fmaf(v[y].z, e, o.z);
+                o.w = fmaf(v[y].w, e, o.w);
+            }
+            m = nm;
+        }
+        row_store(row_end(p, qrow, m, l), 4 * d, o);
+    }
+}
+
 int padded_dim(int d) { return d <= 64 ? 64 : 128; }
 
 template <typename T, int DP>
@@ -1048,6 +1169,7 @@ cudaError_t launch(cudaStream_t s, const PagedPass &p) {
     static_assert(C::kSmem <= 227 * 1024, "shared layout");
     RowsArgs args{};
     args.pass = p;
+    args.join = ((size_t)p.a.tokens * (p.a.heads / p.a.kv_heads) + kM - 1) / kM * p.a.kv_heads < (size_t)kSmCount;
     args.unit = paged_boxes(p.a, kKeys, sizeof(T), C::kRaw, !C::kPair, &args.map);
     static std::atomic<uint64_t> smem_set{0};
     cudaError_t e = set_smem_limit_once(paged_rows_kernel<T, DP>, C::kSmem, &smem_set);
@@ -1060,6 +1182,11 @@ cudaError_t launch(cudaStream_t s, const PagedPass &p) {
     if (regs < kLaunchRegs) return cudaErrorInvalidConfiguration;
     launch_k(paged_rows_kernel<T, DP>, kSmCount, kThreads, C::kSmem, s, args);
     count_launch();
+    if ((e = cudaGetLastError()) != cudaSuccess) return e;
+    if (args.join) {
+        launch_k(rows_join_kernel<DP>, kSmCount - 1, kJoinThreads, 0, s, p, args.unit, kSmCount);
+        count_launch();
+    }
     return cudaGetLastError();
 }
 
