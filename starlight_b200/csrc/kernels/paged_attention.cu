@@ -760,6 +760,12 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         const int rows = min(kRows, cc.ntok * G - cc.rb * kRows);
         float4 o[kItems];
         float mm[kItems], ll[kItems];
+#pragma unroll
+        for (int i = 0; i < kItems; i++) {
+            o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+            mm[i] = -INFINITY;
+            ll[i] = 0.f;
+        }
         auto add = [&](int i, float m, float l, float4 v) {  // to an item's running sums
             const float nm = fmaxf(mm[i], m), mu = nm == -INFINITY ? 0.f : nm;
             const float f = ex2(mm[i] - mu), e = ex2(m - mu);
@@ -774,9 +780,6 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         for (int i = 0; i < kItems; i++) {
             int r, d;
             item(i, r, d);
-            o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-            mm[i] = -INFINITY;
-            ll[i] = 0.f;
             if (r >= rows || d >= D) continue;
             for (int w = 0; w < kWarps; w++) mm[i] = fmaxf(mm[i], mml[(w * kRows + r) * 2]);
             const float mu = mm[i] == -INFINITY ? 0.f : mm[i];
@@ -964,14 +967,30 @@ size_t part_floats(const PagedAttention &a) {
     return rows ? std::max(few, paged_rows_part_floats(a)) : few;
 }
 
+// A pass over the shared prefix saves the others' reads of it (from L2, mostly)
+// and costs launches and the merge, 7 to 25 us: it is taken where those reads
+// are kPrefixPass bytes or more. Measured, with the pass and without: 64
+// sequences of 8 kv heads of 128 bf16, prefix 256 (67 MB) 60 and 41 us, 512
+// 54 and 48, 1024 (268 MB) 56 and 65, 8192 78 and 301; 8 sequences, 2048
+// (67 MB) 23 and 22, 4096 28 and 31; 64 sequences of 4 kv heads of 64 f32,
+// 777 (102 MB) 38 and 41; 6 of them (10 MB) 16.4 and 15.3. Without it the rows
+// read the pages by their own table rows, which are the same.
+constexpr size_t kPrefixPass = (size_t)96 << 20;
+size_t prefix_bytes(const PagedAttention &a) {
+    const size_t row = (size_t)2 * a.kv_heads * a.head_dim * (a.cache.type == kPagedF32 ? 4 : 2);
+    return (size_t)a.batch.seqs * a.prefix * row;
+}
+
 }  // namespace
 
 size_t paged_attention_workspace_bytes(const PagedAttention &a) {
     return (part_floats(a) + prefix_floats(a)) * sizeof(float);
 }
 
-cudaError_t paged_attention(cudaStream_t s, const PagedAttention &a) {
+cudaError_t paged_attention(cudaStream_t s, const PagedAttention &call) {
+    PagedAttention a = call;
     if (a.tokens == 0 || a.batch.seqs == 0) return cudaSuccess;
+    if (prefix_bytes(a) < kPrefixPass) a.prefix = 0;
     if (paged_attention_workspace_bytes(a) > a.workspace_bytes) return cudaErrorMemoryAllocation;
     PagedPass p{};
     p.a = a;

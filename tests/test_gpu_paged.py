@@ -189,6 +189,32 @@ def test_long_sequences(dev, dtype, lens):
     check(attend(dev, b), b)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 1, 128), (8, 4, 64)])
+def test_few_rows_over_many_keys(dev, dtype, heads, kv_heads, dim):
+    # More rows than the kernel for few takes, in far fewer segments than CTAs.
+    b = Batch([(9000, 40), (10, 2)], heads=heads, kv_heads=kv_heads, dim=dim, page=16, layers=1, layer=0, dtype=dtype)
+    refs = upload(dev, b)
+    check(attend(dev, b, refs=refs), b)
+    check(attend(dev, b, window=3000, sinks=5, refs=refs), b, window=3000, sinks=5)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("page", [8, 24, 256])
+def test_page_sizes(dev, page, dtype):
+    b = Batch([(700, 1), (255, 2), (256, 70), (7, 1)], heads=8, kv_heads=2, dim=128, page=page, dtype=dtype)
+    refs = upload(dev, b)
+    check(attend(dev, b, refs=refs), b)
+    check(attend(dev, b, window=100, sinks=9, refs=refs), b, window=100, sinks=9)
+
+
+@pytest.mark.parametrize("window", [0, 50])
+@pytest.mark.parametrize("heads", [2, 40])
+def test_more_sequences_than_threads(dev, heads, window):
+    b = Batch([(i % 90, i % 3) for i in range(700)], heads=heads, kv_heads=2, dim=64, page=16, layers=1, layer=0)
+    check(attend(dev, b, window=window, sinks=2 if window else 0), b, window=window, sinks=2 if window else 0)
+
+
 def test_offsets_past_32_bits(dev):
     # A cache of more than 2^32 bytes; the sequence lives in its last pages.
     pages, page, hkv, d = 5000, 64, 8, 128
@@ -332,6 +358,54 @@ def test_prefix(dev, case, dtype):
     plain = attend(dev, b)  # the operator without a prefix gives the same
     check(plain, b)
     b.prefix = prefix
+
+
+# The prefix is read in a pass of its own from this many bytes of reads by all
+# sequences on; below, every sequence reads it by itself.
+PASS_BYTES = 96 << 20
+PASSES = [
+    # rows of one kv head: 16 (few), 64 (many), 160 (many, two row tiles), wide heads, odd pages
+    dict(lens=[(1700 + i, 1) for i in range(16)], prefix=1650, heads=8, kv_heads=8, dim=128, page=16),
+    dict(lens=[(800 + 3 * i, 1) for i in range(64)], prefix=799, heads=8, kv_heads=8, dim=128, page=64),
+    dict(lens=[(640 + i % 9, i % 3) for i in range(80)], prefix=640, heads=32, kv_heads=8, dim=64, page=16, pad=2),
+    dict(lens=[(1000 + i, 1) for i in range(16)], prefix=900, heads=16, kv_heads=8, dim=256, page=24),
+    dict(lens=[(1500 + i, i % 2) for i in range(31)], prefix=1500, heads=8, kv_heads=8, dim=72, page=5),
+    dict(lens=[(702, 0)] + [(702 + i, 1) for i in range(64)], prefix=701, heads=8, kv_heads=8, dim=72, page=7),
+]
+
+
+def pass_batch(case, dtype, **kw):
+    b = Batch(**case, layers=1, layer=0, dtype=dtype, **kw)
+    assert len(b.lens) * b.prefix * 2 * b.kv_heads * b.dim * (4 if dtype == F32 else 2) >= PASS_BYTES
+    return b
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("case", range(len(PASSES)))
+def test_prefix_in_a_pass_of_its_own(dev, case, dtype):
+    b = pass_batch(PASSES[case], dtype, seed=case)
+    refs = upload(dev, b)
+    first = attend(dev, b, offset=case % 2, refs=refs)
+    check(first, b)
+    for _ in range(3):
+        assert np.array_equal(first, attend(dev, b, offset=case % 2, refs=refs))
+
+
+@pytest.mark.parametrize("case", [0, 1, 4])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+def test_prefix_pass_with_values_that_are_not_finite(dev, value, case):
+    b = pass_batch(PASSES[case], F32, seed=case)
+    hurt = 3 if case != 4 else 5  # a sequence with a token of its own
+    put_values(b, [(hurt, b.lens[hurt][0], 1, value)])
+    got = attend(dev, b)
+    want, tol = b.attention(1 / math.sqrt(b.dim))
+    # Where the position lies in the prefix's last page, longer sequences see it too.
+    clean = np.all(np.isfinite(want), axis=1)
+    assert not clean[int(b.starts[hurt])] and np.any(clean)
+    assert np.all(np.abs(got[clean] - want[clean]) <= tol[clean])
+    assert not np.any(np.isfinite(got[~clean]))
+    put_values(b, [(hurt, 100, 0, np.nan)])  # shared: no row is left
+    assert not np.any(np.isfinite(attend(dev, b)))
 
 
 def test_prefix_of_zero(dev):
@@ -511,6 +585,50 @@ def test_decoding_captured_and_replayed(dtype, prefix):
     for a, b in zip(results[0][0], results[1][0]):
         assert all(np.array_equal(x, y) for x, y in zip(a, b))
     assert np.array_equal(results[0][1].view(np.uint32), results[1][1].view(np.uint32))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+@pytest.mark.parametrize("window", [0, 33])
+def test_prompts_captured_and_replayed(dtype, window):
+    # Chunks of prompts of changing lengths through one captured command, then
+    # a second graph on the same workspace.
+    batches = [Batch([(p, n), (20, 1), (m, 9)], heads=8, kv_heads=2, dim=64, page=16, dtype=dtype, width=40,
+                     extra_pages=40, pad=120 - n, seed=i)
+               for i, (p, n, m) in enumerate([(300, 90, 0), (0, 120, 7), (500, 1, 90), (17, 64, 400), (100, 33, 5),
+                                              (250, 100, 60)])]
+    pages = max(b.pages for b in batches)
+    shape = (pages, 2, 2, 16, 2, 64)
+    d = CudaDevice(0)
+    try:
+        d.set_capture(True)
+        cache = new_f32(d, state_words(shape, dtype))
+        table, past, starts = (put_u32(d, np.zeros(n)) for n in ((3, 40), 3, 4))
+        q, outs = new_f32(d, 130 * 512), [new_f32(d, 130 * 512) for _ in range(2)]
+        x = Value.f32((130, 512))
+        first = batches[0]
+        cmds = [d.command(first.op(OpCode.PagedAttention, scale=0.125), [q, table, past, starts, cache],
+                          [x, *first.described(), Value(dtype, shape, ValueRole.State)], [out], [x], [120, window, 1])
+                for out in outs]
+        for b in batches * 2:
+            assert b.tokens == 130
+            words = np.zeros(cache.len, np.float32)
+            words[:b.words.size] = b.words
+            d.upload_f32(cache.buffer, words)
+            d.upload_u32(table.buffer, b.table)
+            d.upload_u32(past.buffer, b.past)
+            d.upload_u32(starts.buffer, b.starts)
+            d.upload_f32(q.buffer, b.q)
+            for cmd in cmds:
+                cmd()
+            d.synchronize()
+            a, c = (get(d, out).reshape(130, -1) for out in outs)
+            live = int(b.starts[-1])
+            want, tol = b.attention(0.125, window, 1 if window else 0)
+            assert np.all(np.abs(a[:live] - want[:live]) <= tol[:live])
+            assert np.array_equal(a[:live], c[:live])
+        assert d.capture_stats()["replays"] >= 6
+    finally:
+        d.close()
 
 
 def test_decoding_matches_the_dense_cache(dev):
