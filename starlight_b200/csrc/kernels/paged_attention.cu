@@ -521,8 +521,11 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             qf1 = q_scale[2 * t + 1];
         }
         landed(stage, 0, phase);
+        const int w0i = cc.tile * kTileKeys + warp * kWarpKeys;
+        const bool more = issued < units, work = w0i < cc.keys;
         unsigned char *ks = ring + (warp * S + stage) * C::kStageBytes, *vs = ks + C::kHalfStage;
 
+        // A warp past the segment's keys has no work in its last tile.
         // S^T: keys g, g + 8 x rows 2t, 2t + 1; small products apart.
         float s[kSub][4][4];
 #pragma unroll
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
             for (int i = 0; i < 4; i++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) s[h][i][j] = 0.f;
-        {
+        if (work) {
             // 32 bytes of 16 keys a step: row lane % 16, 16-byte piece 2 (j % 4)
             // + lane / 16 of its 128-byte block, xored with the row.
             const uint32_t ka = smem_addr(ks) + (lane & 15) * 128, x0 = (((lane >> 4) ^ (lane & 7)) << 4);
@@ -569,142 +572,150 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
         }
         // The keys are read: their slot takes those of S tiles on.
         __syncwarp();
-        const bool more = issued < units;
         if (more)
             issue(stage, 0);
         else if (unit == 1)
             cp_async_commit();
 
-        const int w0i = cc.tile * kTileKeys + warp * kWarpKeys;
-        float pr[kSub][4];
-#pragma unroll
-        for (int h = 0; h < kSub; h++)
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                pr[h][j] =
-                    ((s[h][3][j] + s[h][2][j]) + (s[h][1][j] + s[h][0][j])) * ((j & 1) ? qf1 : qf0);
-        const bool clear = all_see(p, cc, w0i, w0i + kWarpKeys);
-        if (!clear)
+        float pr[kSub][4], f0, f1;
+        bool clear;
+        if (work) {
 #pragma unroll
             for (int h = 0; h < kSub; h++)
 #pragma unroll
                 for (int j = 0; j < 4; j++)
-                    if (!sees(p, cc, w0i + h * 16 + g + j / 2 * 8, (j & 1) ? at1 : at0)) pr[h][j] = -INFINITY;
-        float n0 = fmaxf(pr[0][0], pr[0][2]), n1 = fmaxf(pr[0][1], pr[0][3]);
-        if (kSub == 2) {
-            n0 = fmaxf(n0, fmaxf(pr[kSub - 1][0], pr[kSub - 1][2]));
-            n1 = fmaxf(n1, fmaxf(pr[kSub - 1][1], pr[kSub - 1][3]));
-        }
+                    pr[h][j] =
+                        ((s[h][3][j] + s[h][2][j]) + (s[h][1][j] + s[h][0][j])) * ((j & 1) ? qf1 : qf0);
+            clear = all_see(p, cc, w0i, w0i + kWarpKeys);
+            if (!clear)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
-            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
-        }
-        n0 = fmaxf(n0, m0);
-        n1 = fmaxf(n1, m1);
-        const float u_0 = n0 == -INFINITY ? 0.f : n0, u_1 = n1 == -INFINITY ? 0.f : n1;
-        const float f0 = ex2(m0 - u_0), f1 = ex2(m1 - u_1);
-        l0 *= f0;
-        l1 *= f1;
-        m0 = n0;
-        m1 = n1;
+                for (int h = 0; h < kSub; h++)
 #pragma unroll
-        for (int h = 0; h < kSub; h++) {
+                    for (int j = 0; j < 4; j++)
+                        if (!sees(p, cc, w0i + h * 16 + g + j / 2 * 8, (j & 1) ? at1 : at0)) pr[h][j] = -INFINITY;
+            float n0 = fmaxf(pr[0][0], pr[0][2]), n1 = fmaxf(pr[0][1], pr[0][3]);
+            if (kSub == 2) {
+                n0 = fmaxf(n0, fmaxf(pr[kSub - 1][0], pr[kSub - 1][2]));
+                n1 = fmaxf(n1, fmaxf(pr[kSub - 1][1], pr[kSub - 1][3]));
+            }
 #pragma unroll
-            for (int j = 0; j < 4; j++) pr[h][j] = ex2(pr[h][j] - (((j & 1) ? u_1 : u_0) - C::kShift));
-            l0 += pr[h][0] + pr[h][2];
-            l1 += pr[h][1] + pr[h][3];
+            for (int o = 4; o < 32; o <<= 1) {
+                n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, o));
+                n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, o));
+            }
+            n0 = fmaxf(n0, m0);
+            n1 = fmaxf(n1, m1);
+            const float u_0 = n0 == -INFINITY ? 0.f : n0, u_1 = n1 == -INFINITY ? 0.f : n1;
+            f0 = ex2(m0 - u_0);
+            f1 = ex2(m1 - u_1);
+            l0 *= f0;
+            l1 *= f1;
+            m0 = n0;
+            m1 = n1;
+#pragma unroll
+            for (int h = 0; h < kSub; h++) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) pr[h][j] = ex2(pr[h][j] - (((j & 1) ? u_1 : u_0) - C::kShift));
+                l0 += pr[h][0] + pr[h][2];
+                l1 += pr[h][1] + pr[h][3];
+            }
         }
         landed(stage, 1, phase);
-        if (!clear && unit > 1) {
-            // Values of keys that no row sees may be anything, and meet zero
-            // probabilities: they become zero.
-            unsigned dead = __ballot_sync(0xffffffffu, lane < kWarpKeys && !live_key(p, cc, w0i + lane));
-            for (; dead; dead &= dead - 1) {
-                const int r = __ffs(dead) - 1;
-                for (int c = lane; c < C::kBlk * 8; c += 32)
-                    *reinterpret_cast<uint4 *>(vs + (c / 8 * kWarpKeys + r) * 128 + c % 8 * 16) =
-                        make_uint4(0, 0, 0, 0);
+        if (work) {
+            if (!clear && unit > 1) {
+                // Values of keys that no row sees may be anything, and meet zero
+                // probabilities: they become zero.
+                const unsigned dead = __ballot_sync(0xffffffffu, lane < kWarpKeys && !live_key(p, cc, w0i + lane));
+                constexpr int kPieces = C::kBlk * 8, kStep = kPieces < 32 ? 32 / kPieces : 1;  // lanes: pieces, rows
+                const int c = lane % kPieces;
+#pragma unroll
+                for (int r0 = 0; r0 < kWarpKeys; r0 += kStep) {
+                    const int r = r0 + (kPieces < 32 ? lane / kPieces : 0);
+                    if ((dead >> r) & 1)
+                        for (int x = c; x < kPieces; x += 32)
+                            *reinterpret_cast<uint4 *>(vs + (x / 8 * kWarpKeys + r) * 128 + x % 8 * 16) =
+                                make_uint4(0, 0, 0, 0);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
             }
-            fence_proxy_async_smem();
-            __syncwarp();
-        }
 
-        // A tile's P V starts from zero and is added to the running output
-        // outside the tensor core, whose accumulation truncates: over
-        // thousands of keys that bias would grow past f32 rounding.
-        if constexpr (C::kHalf) {
-            // B fragments: row g, keys 2t, 2t + 1 and 8 + 2t, 9 + 2t.
-            uint32_t b[kSub][C::kTerms][2];
+            // A tile's P V starts from zero and is added to the running output
+            // outside the tensor core, whose accumulation truncates: over
+            // thousands of keys that bias would grow past f32 rounding.
+            if constexpr (C::kHalf) {
+                // B fragments: row g, keys 2t, 2t + 1 and 8 + 2t, 9 + 2t.
+                uint32_t b[kSub][C::kTerms][2];
 #pragma unroll
-            for (int x = 0; x < C::kTerms; x++)
+                for (int x = 0; x < C::kTerms; x++)
 #pragma unroll
-                for (int h = 0; h < kSub; h++) {
-                    b[h][x][0] = movmatrix(take_pair<T>(pr[h][0], pr[h][1]));
-                    b[h][x][1] = movmatrix(take_pair<T>(pr[h][2], pr[h][3]));
+                    for (int h = 0; h < kSub; h++) {
+                        b[h][x][0] = movmatrix(take_pair<T>(pr[h][0], pr[h][1]));
+                        b[h][x][1] = movmatrix(take_pair<T>(pr[h][2], pr[h][3]));
+                    }
+                // Key lane % 8 + 8 (lane / 16), 16-byte piece 2 (i % 4) + lane / 8 % 2.
+                const uint32_t va = smem_addr(vs) + ((lane & 7) + (lane >> 4) * 8) * 128,
+                               x0 = ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+#pragma unroll
+                for (int i = 0; i < NT; i++) {
+                    float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int h = 0; h < kSub; h++) {
+                        uint32_t a[4];
+                        ldmatrix4<true>(va + (i / 4 * kWarpKeys + h * 16) * 128 + (x0 ^ (i % 4 * 32)), a);
+#pragma unroll
+                        for (int x = C::kTerms - 1; x >= 0; x--) mma_16<T>(o, a, b[h][x][0], b[h][x][1]);
+                    }
+                    acc[i][0] = fmaf(acc[i][0], f0, o[0]);
+                    acc[i][1] = fmaf(acc[i][1], f1, o[1]);
+                    acc[i][2] = fmaf(acc[i][2], f0, o[2]);
+                    acc[i][3] = fmaf(acc[i][3], f1, o[3]);
                 }
-            // Key lane % 8 + 8 (lane / 16), 16-byte piece 2 (i % 4) + lane / 8 % 2.
-            const uint32_t va = smem_addr(vs) + ((lane & 7) + (lane >> 4) * 8) * 128,
-                           x0 = ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+            } else {
+                // B fragments of the two 8-key steps: row g, keys 2t and 2t + 1.
+                uint32_t bh[2][2], bl[2][2];
 #pragma unroll
-            for (int i = 0; i < NT; i++) {
-                float o[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int h = 0; h < kSub; h++) {
-                    uint32_t a[4];
-                    ldmatrix4<true>(va + (i / 4 * kWarpKeys + h * 16) * 128 + (x0 ^ (i % 4 * 32)), a);
-#pragma unroll
-                    for (int x = C::kTerms - 1; x >= 0; x--) mma_16<T>(o, a, b[h][x][0], b[h][x][1]);
-                }
-                acc[i][0] = fmaf(acc[i][0], f0, o[0]);
-                acc[i][1] = fmaf(acc[i][1], f1, o[1]);
-                acc[i][2] = fmaf(acc[i][2], f0, o[2]);
-                acc[i][3] = fmaf(acc[i][3], f1, o[3]);
-            }
-        } else {
-            // B fragments of the two 8-key steps: row g, keys 2t and 2t + 1.
-            uint32_t bh[2][2], bl[2][2];
-#pragma unroll
-            for (int k8 = 0; k8 < 2; k8++)
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int src = (2 * t + x) * 4 + (g >> 1);
-                    const float a = __shfl_sync(0xffffffffu, pr[0][2 * k8], src);
-                    const float b = __shfl_sync(0xffffffffu, pr[0][2 * k8 + 1], src);
-                    const float v = (g & 1) ? b : a;
-                    bh[k8][x] = tf32_hi(v);
-                    bl[k8][x] = tf32_lo(v, bh[k8][x]);
-                }
-#pragma unroll
-            for (int j = 0; j < DP / 32; j++) {
-                float o[2][4] = {};
-#pragma unroll
-                for (int k8 = 0; k8 < 2; k8++) {
-                    float va[4], vb[4];
-                    const unsigned char *v0 = vs + (j * kWarpKeys + 8 * k8 + 2 * t) * 128;
-                    Frag<T>::ld(v0 + ((g ^ (2 * t)) << 4), va);
-                    Frag<T>::ld(v0 + 128 + ((g ^ (2 * t + 1)) << 4), vb);
+                for (int k8 = 0; k8 < 2; k8++)
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const float f[4] = {va[2 * x], va[2 * x + 1], vb[2 * x], vb[2 * x + 1]};
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int z = 0; z < 4; z++) {
-                            hi[z] = tf32_hi(f[z]);
-                            lo[z] = tf32_lo(f[z], hi[z]);
-                        }
-                        mma_tf32(o[x], hi, bl[k8][0], bl[k8][1]);
-                        mma_tf32(o[x], lo, bh[k8][0], bh[k8][1]);
-                        mma_tf32(o[x], hi, bh[k8][0], bh[k8][1]);
+                        const int src = (2 * t + x) * 4 + (g >> 1);
+                        const float a = __shfl_sync(0xffffffffu, pr[0][2 * k8], src);
+                        const float b = __shfl_sync(0xffffffffu, pr[0][2 * k8 + 1], src);
+                        const float v = (g & 1) ? b : a;
+                        bh[k8][x] = tf32_hi(v);
+                        bl[k8][x] = tf32_lo(v, bh[k8][x]);
                     }
-                }
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    float(&a)[4] = acc[2 * j + x];
-                    a[0] = fmaf(a[0], f0, o[x][0]);
-                    a[1] = fmaf(a[1], f1, o[x][1]);
-                    a[2] = fmaf(a[2], f0, o[x][2]);
-                    a[3] = fmaf(a[3], f1, o[x][3]);
+                for (int j = 0; j < DP / 32; j++) {
+                    float o[2][4] = {};
+#pragma unroll
+                    for (int k8 = 0; k8 < 2; k8++) {
+                        float va[4], vb[4];
+                        const unsigned char *v0 = vs + (j * kWarpKeys + 8 * k8 + 2 * t) * 128;
+                        Frag<T>::ld(v0 + ((g ^ (2 * t)) << 4), va);
+                        Frag<T>::ld(v0 + 128 + ((g ^ (2 * t + 1)) << 4), vb);
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            const float f[4] = {va[2 * x], va[2 * x + 1], vb[2 * x], vb[2 * x + 1]};
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int z = 0; z < 4; z++) {
+                                hi[z] = tf32_hi(f[z]);
+                                lo[z] = tf32_lo(f[z], hi[z]);
+                            }
+                            mma_tf32(o[x], hi, bl[k8][0], bl[k8][1]);
+                            mma_tf32(o[x], lo, bh[k8][0], bh[k8][1]);
+                            mma_tf32(o[x], hi, bh[k8][0], bh[k8][1]);
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        float(&a)[4] = acc[2 * j + x];
+                        a[0] = fmaf(a[0], f0, o[x][0]);
+                        a[1] = fmaf(a[1], f1, o[x][1]);
+                        a[2] = fmaf(a[2], f0, o[x][2]);
+                        a[3] = fmaf(a[3], f1, o[x][3]);
+                    }
                 }
             }
         }
