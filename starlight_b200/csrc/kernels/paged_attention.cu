@@ -63,6 +63,14 @@ constexpr int kSmallRows = 32;  // query rows per kv head taken here; more go to
 template <typename T, int DP>
 struct Cfg {
     static constexpr bool kHalf = sizeof(T) == 2;
+    // CTAs per SM: the warps wait for latencies, not for a unit (3 in 4 issue
+    // slots are empty), so two are better where registers (128 a thread) and
+    // shared memory allow it. Heads of 64: 64 sequences of 8 kv heads in f32
+    // up to 8000 long 249 -> 182 us, up to 600 41 -> 35 us, f16 136 -> 126 us;
+    // one short sequence 7.9 -> 8.4 us. For 128, two of four warps each gain
+    // 1 % over long sequences in bf16 and lose 2 to 6 % over short ones, and
+    // with half the keys a tile the 16-bit types take 1.4 times as long.
+    static constexpr int kCtas = DP == 64 ? 2 : 1;
     static constexpr int kWarps = !kHalf && DP == 256 ? 4 : 8;
     static constexpr int kThreads = kWarps * 32;
     // 16 keys an MMA; two of them a tile give a warp independent work to
@@ -80,7 +88,7 @@ struct Cfg {
     static constexpr int kMergeStride = DP + 4;  // floats
     static constexpr int kQBytes = kRows * DP * (kHalf ? 2 * kTerms : 8);
     static constexpr int kFixed = kQBytes + kWarps * kRows * (kMergeStride + 2) * 4 + 1024 + 1024;
-    static constexpr int kFit = (224 * 1024 - kFixed) / (kWarps * kStageBytes);
+    static constexpr int kFit = ((kCtas == 1 ? 224 : 113) * 1024 - kFixed) / (kWarps * kStageBytes);
     static constexpr int kStages = kFit > 4 ? 4 : kFit;
     static constexpr int kSmem = kFixed + kStages * kWarps * kStageBytes;
 };
@@ -254,7 +262,7 @@ struct PassArgs {
 };
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
+__global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
     paged_attention_kernel(const __grid_constant__ PassArgs args) {
     const PagedPass &p = args.pass;
     const int unit = args.unit;
@@ -930,7 +938,8 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, 1)
 
 int padded_dim(int d) { return d <= 64 ? 64 : d <= 128 ? 128 : 256; }
 
-size_t partial_floats(int dp) { return (size_t)2 * kSmCount * kRows * (dp + 2); }
+constexpr size_t kPieces = 2 * 2 * kSmCount;  // two a CTA
+size_t partial_floats(int dp) { return kPieces * kRows * (dp + 2); }
 size_t prefix_floats(const PagedAttention &a) {
     return a.prefix ? (size_t)a.tokens * a.heads * (a.head_dim + 2) : 0;
 }
@@ -938,13 +947,13 @@ size_t prefix_floats(const PagedAttention &a) {
 template <typename T, int DP>
 cudaError_t launch_pass(cudaStream_t s, const PagedPass &p) {
     using C = Cfg<T, DP>;
-    static_assert(C::kStages >= 1 && C::kSmem <= 227 * 1024, "shared layout");
+    static_assert(C::kStages >= 1 && C::kCtas * (C::kSmem + 1024) <= 228 * 1024, "shared layout");
     static std::atomic<uint64_t> smem_set{0};
     set_smem_limit_once(paged_attention_kernel<T, DP>, C::kSmem, &smem_set);
     PassArgs args{};
     args.pass = p;
     args.unit = paged_boxes(p.a, C::kWarpKeys, sizeof(T), std::is_same<T, __half>::value, true, &args.map);
-    launch_k(paged_attention_kernel<T, DP>, kSmCount, C::kThreads, C::kSmem, s, args);
+    launch_k(paged_attention_kernel<T, DP>, kSmCount * C::kCtas, C::kThreads, C::kSmem, s, args);
     count_launch();
     return cudaGetLastError();
 }
@@ -1007,7 +1016,7 @@ cudaError_t paged_attention(cudaStream_t s, const PagedAttention &call) {
     p.a = a;
     p.scale_log2 = a.scale * kLog2e;
     p.part_o = static_cast<float *>(a.workspace);
-    p.part_ml = p.part_o + (size_t)2 * kSmCount * kRows * padded_dim(a.head_dim);
+    p.part_ml = p.part_o + kPieces * kRows * padded_dim(a.head_dim);
     p.small_rows = INT32_MAX;
     cudaError_t e = cudaSuccess;
     if (a.prefix) {
