@@ -17,10 +17,11 @@
 // One CTA per SM, 20 warps:
 //   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
 //          S from TMEM, running maximum, P as f16 pairs back into the TMEM
-//          columns that S held
+//          columns that S held (16-bit caches: with warps 8..11, two threads
+//          per row, each half of the keys)
 //   4..7   output: one thread per row; O += P V of each tile in registers,
 //          the result, or this CTA's piece of a split segment
-//   8..15  conversion in place: scale, f16 or f16 pair, zeros in rows that no
+//   8..15  (16-bit caches: 12..15) conversion in place: scale, f16 or f16 pair, zeros in rows that no
 //          query sees (they may hold anything). The scale is that of the
 //          operand before; a tile whose largest value does not suit it is
 //          read from the cache once more (a pass over each tile for its
@@ -52,17 +53,12 @@ namespace {
 
 constexpr int kM = 128;     // query rows per segment
 constexpr int kKeys = 128;  // keys per tile
-constexpr int kConv = 8;    // conversion warps
 constexpr int kCopy = 3;    // copying warps where TMA boxes do not fit the pages
 constexpr int kThreads = 20 * 32;
 constexpr int kShift = 14;  // a query row's largest value in [2^14, 2^15), probabilities up to 2^14
 constexpr int kTop = 11;    // a tile's largest value around 2^11: from 2^9 to 2^15
-// Registers a thread, by warpgroup: softmax keeps the 96 of the launch,
-// conversion has two warpgroups.
-constexpr int kLaunchRegs = 96, kOutRegs = 184, kConvRegs = 64, kRestRegs = 72;
-static_assert(kLaunchRegs + kOutRegs + 2 * kConvRegs + kRestRegs <= 5 * kLaunchRegs, "register split");
+constexpr int kLaunchRegs = 96;  // registers a thread at launch
 constexpr uint64_t kLimitNs = 20000000000ull;  // rows of values that are not finite take long
-
 template <typename T, int DP>
 struct Cfg {
     static constexpr bool kPair = sizeof(T) == 4;            // keys and values are f16 pairs
@@ -74,12 +70,22 @@ struct Cfg {
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
     static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (2 * 4 * kM + 4 * kM + 4 * 8 + 8 + 8 * 12 + 4 * DP + 16) + 8 * (3 * kKeys + 8 + 3 * kSlots + 8 + 20);
+    static constexpr int kSmall = 4 * (22 * kM + 4 * 8 + 8 + 8 * 12 + 4 * DP + 16) +
+                                  8 * (3 * kKeys + 8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
     static constexpr int kLpr = DP / kEpl;               // lanes per cache row
     static constexpr int kRpi = 32 / kLpr;               // rows per warp load
+    // An F32 cache keeps eight warps converting; 16-bit ones leave four of
+    // them to a second softmax warpgroup, each with half the keys of a tile.
+    static constexpr int kSoft = kPair ? 1 : 2;
+    static constexpr int kConv = kPair ? 8 : 4;
+    static constexpr int kConvWarp = 16 - kConv;
     static constexpr int kRows = kKeys / kConv / kRpi;   // 16-byte pieces per conversion lane
+    // Registers a thread, by warpgroup, out of those of the launch.
+    static constexpr int kSoftRegs = kPair ? 96 : 88, kOutRegs = 184, kConvRegs = kPair ? 64 : 56,
+                         kRestRegs = kPair ? 72 : 64;
+    static_assert(kSoft * kSoftRegs + kOutRegs + kConv / 4 * kConvRegs + kRestRegs <= 5 * kLaunchRegs, "registers");
     // f32 accumulators, f16 operands, K-major A; B K-major (S) or MN-major (O).
     static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
     static constexpr uint32_t kIdescO =
@@ -386,7 +392,9 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     unsigned char *ring = smem;                         // [S] operands: hi[, lo]
     float *row_ml = reinterpret_cast<float *>(smem + C::kRing);  // [4 tiles][kM][2]
     float *alpha = row_ml + 4 * kM * 2;                 // [4 tiles][kM]
-    float *k_scale = alpha + 4 * kM;                    // [8 tiles]
+    float *row_l2 = alpha + 4 * kM;                     // [4 tiles][kM] the second group's sums
+    float *half_max = row_l2 + 4 * kM;                  // [2 groups][3][kM] tiles in turn, Q
+    float *k_scale = half_max + 6 * kM;                 // [8 tiles]
     float *v_scale = k_scale + 8;                       // [8 tiles]
     uint32_t *most = reinterpret_cast<uint32_t *>(v_scale + 8);   // [4 operands, 4 unused]
     int *poison = reinterpret_cast<int *>(most + 8);    // [8 segments]
@@ -413,13 +421,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     if (threadIdx.x == 0) {
         for (int i = 0; i < S; i++) {
             mbar_init(&raw[i], unit > 1 ? 1 : kCopy);
-            mbar_init(&full[i], kConv);
+            mbar_init(&full[i], C::kConv);
             mbar_init(&empty[i], 1);
         }
-        mbar_init(q_full, 4);
+        mbar_init(q_full, 4 * C::kSoft);
         for (int i = 0; i < 2; i++) {
             mbar_init(&s_full[i], 1);
-            mbar_init(&p_full[i], 4);
+            mbar_init(&p_full[i], 4 * C::kSoft);
         }
         mbar_init(o_full, 1);
         mbar_init(o_empty, 4);
@@ -428,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             mbar_init(&k_sc[i], 1);
             mbar_init(&v_sc[i], 1);
         }
-        for (int i = 0; i < 4; i++) mbar_init(&a_full[i], 4);
+        for (int i = 0; i < 4; i++) mbar_init(&a_full[i], 4 * C::kSoft);
         fence_mbar_init();
         *abort = 0;
         for (int i = 0; i < 4; i++) most[i] = 0;
@@ -465,19 +473,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     auto is_v = [&](int j) { return j == total - 1 || (j > 0 && j % 2 == 0); };
     auto tile_of = [&](int j) { return j == total - 1 ? N - 1 : j == 0 ? 0 : j % 2 ? (j + 1) / 2 : j / 2 - 1; };
 
+    const bool soft = warp < 4 || (C::kSoft == 2 && warp >= 8 && warp < C::kConvWarp);
     // No wait below ends a loop: after one that gave up (the abort word is
     // set) every role runs through its remaining steps without waiting, so
     // that the barriers between its own threads stay matched.
-    if (warp >= 4 && warp < 8)
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kOutRegs));
-    else if (warp >= 8 && warp < 16)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvRegs));
-    else if (warp >= 16)
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRestRegs));
-    if (warp < 4) {
+    if (soft) {
         // ---- softmax ------------------------------------------------------
-        const int r = threadIdx.x;
-        const uint32_t lane_tm = (uint32_t)(warp * 32) << 16;
+        if (C::kSoftRegs < kLaunchRegs) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kSoftRegs));
+        const int r = threadIdx.x & (kM - 1), group = warp >> 3;
+        const uint32_t lane_tm = (uint32_t)((warp & 3) * 32) << 16;
+        // The larger of both groups' values for the row.
+        auto both = [&](float x, int buffer) {
+            if (C::kSoft == 1) return x;
+            half_max[(3 * group + buffer) * kM + r] = x;
+            bar_sync(4, 2 * kM);
+            return fmaxf(x, half_max[(3 * (1 - group) + buffer) * kM + r]);
+        };
         float m = -INFINITY, l = 0.f, qs = 1.f;
         int hi = 0, lo = 0;
         bool first = true;
@@ -493,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 const bool vec = aligned16(p.a.q);
                 float top = 0.f;
 #pragma unroll 1
-                for (int h = 0; h < DP; h += 32) {
+                for (int h = group * (DP / 2); h < (C::kSoft == 1 ? DP : (group + 1) * (DP / 2)); h += 32) {
                     float4 v[8];
 #pragma unroll
                     for (int y = 0; y < 8; y++) {
@@ -520,11 +531,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     }
                 }
                 tmem_wait_st();
+                top = both(top, 2);
                 const int ex = scale_exponent(__float_as_uint(top));
                 const float sc = pow2(kShift - ex);
                 qs = pow2(ex - kShift);
 #pragma unroll 1
-                for (int h = 0; h < DP; h += 32) {
+                for (int h = group * (DP / 2); h < (C::kSoft == 1 ? DP : (group + 1) * (DP / 2)); h += 32) {
                     uint32_t x[32], qh[16], ql[16];
                     tmem_ld32_async(q_tm + lane_tm + h, x);
                     tmem_wait_ld(x);
@@ -559,6 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             const bool masked = __any_sync(0xffffffffu, !whole);
             const float f = qs * k_scale[n & 7];
             const uint32_t st = s_tm + (n & 1) * 128 + lane_tm;
+            const int h_first = group * 2;
             // Both passes over the row, with the mask only where a row needs it.
             float nm, a;
             F2 sum2(0.f, 0.f);
@@ -567,7 +580,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 const int h0 = hi - i0, l0 = lo - i0, s0 = p.a.sinks - i0;
                 float mx = -INFINITY;
 #pragma unroll 1
-                for (int h = 0; h < 4; h++) {
+                for (int h = h_first; h < h_first + 4 / C::kSoft; h++) {
                     uint32_t x[32];
                     tmem_ld32_async(st + 32 * h, x);
                     tmem_wait_ld(x);
@@ -577,11 +590,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                         if (!kMask || (i < h0 && (i >= l0 || i < s0))) mx = fmaxf(mx, __uint_as_float(x[j]));
                     }
                 }
+                mx = both(mx, n & 1);
                 nm = fmaxf(m, mx == -INFINITY ? mx : mx * f);
                 const float mu = nm == -INFINITY ? 0.f : nm - (float)kShift;
                 a = m == -INFINITY ? 0.f : ex2(m - nm);
 #pragma unroll 1
-                for (int h = 0; h < 4; h++) {
+                for (int h = h_first; h < h_first + 4 / C::kSoft; h++) {
                     uint32_t x[32], ph[16], pl[16];
                     tmem_ld32_async(st + 32 * h, x);
                     tmem_wait_ld(x);
@@ -610,11 +624,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 row(std::false_type());
             m = nm;
             l = fmaf(l, a, sum2.get().x + sum2.get().y);
-            alpha[(n & 3) * kM + r] = a;
+            if (group == 0) alpha[(n & 3) * kM + r] = a;
             first = c.tile == c.tiles - 1;
             if (first || n == N - 1) {
-                row_ml[((n & 3) * kM + r) * 2] = m == -INFINITY ? m : m - (float)kShift;
-                row_ml[((n & 3) * kM + r) * 2 + 1] = l;
+                if (group == 0) {
+                    row_ml[((n & 3) * kM + r) * 2] = m == -INFINITY ? m : m - (float)kShift;
+                    row_ml[((n & 3) * kM + r) * 2 + 1] = l;
+                } else {
+                    row_l2[(n & 3) * kM + r] = l;
+                }
             }
             tmem_wait_st();
             tc_fence_before();
@@ -627,6 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         }
     } else if (warp < 8) {
         // ---- output -------------------------------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kOutRegs));
         const int r = threadIdx.x - 128, ow = warp - 4;
         const uint32_t lane_tm = (uint32_t)(ow * 32) << 16;
         F2 acc[DP / 2];
@@ -640,6 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             tc_fence_after();
             const float a = alpha[(n & 3) * kM + r], vs = v_scale[n & 7];
             float m = row_ml[((n & 3) * kM + r) * 2], l = row_ml[((n & 3) * kM + r) * 2 + 1];
+            if (C::kSoft == 2) l += row_l2[(n & 3) * kM + r];
             const uint32_t ot = o_tm + lane_tm;
 #pragma unroll
             for (int h = 0; h < DP / 16; h++) {
@@ -765,13 +785,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         }
     } else if (warp < 16) {
         // ---- conversion ---------------------------------------------------
-        const int pw = warp - 8;
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvRegs));
+        const int pw = warp - C::kConvWarp;
         // Piece i of a lane: row (i kConv + pw) kRpi + sub, 16 raw bytes from
         // dim `col` on. A piece on is a multiple of 8 rows on.
         const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
-        constexpr int kBatch = 4, kStep = kConv * C::kRpi * 128;
-        static_assert(C::kRows % kBatch == 0 && kConv % 8 == 0, "batches of pieces 8 rows apart");
-        auto row_of = [&](int i) { return (i * kConv + pw) * C::kRpi + sub; };
+        constexpr int kBatch = 4, kStep = C::kConv * C::kRpi * 128;
+        static_assert(C::kRows % kBatch == 0 && C::kConv * C::kRpi % 8 == 0, "batches of pieces 8 rows apart");
+        auto row_of = [&](int i) { return (i * C::kConv + pw) * C::kRpi + sub; };
         const uint32_t op0 = operand_at(row_of(0), col);
         const uint32_t raw0 = C::kPair ? (ch >> 3) * C::kBlockBytes + row_of(0) * 128 + (ch & 7) * 16 : op0;
         int e_k = 2, e_v = 2;  // exponents of the scales of the operands before
@@ -834,13 +855,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
                     const int place = (2 * j + again) & 3;
                     if (lane == 0) atomicMax(&most[place], mine);
-                    bar_sync(1, kConv * 32);
+                    bar_sync(1, C::kConv * 32);
                     const uint32_t all = *reinterpret_cast<volatile uint32_t *>(&most[place]);
-                    bar_sync(1, kConv * 32);
-                    if (threadIdx.x == 8 * 32) most[place] = 0;
+                    bar_sync(1, C::kConv * 32);
+                    if (threadIdx.x == C::kConvWarp * 32) most[place] = 0;
                     if (all == 0) break;
                     const int found = scale_exponent(all);
-                    if (threadIdx.x == 8 * 32 && all >= 0x7f800000u) poison[cu.seg & 7] = 1;
+                    if (threadIdx.x == C::kConvWarp * 32 && all >= 0x7f800000u) poison[cu.seg & 7] = 1;
                     (v ? e_v : e_k) = found;
                     if (again || (found <= ex + 3 && found >= ex - 2)) break;
                     // Once more, from the cache.
@@ -858,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     __syncwarp();
                 }
             }
-            if (threadIdx.x == 8 * 32) {
+            if (threadIdx.x == C::kConvWarp * 32) {
                 (v ? v_scale : k_scale)[n & 7] = C::kRaw ? 1.f : pow2(ex - kTop);
                 mbar_arrive(&(v ? v_sc : k_sc)[n & 7]);
             }
@@ -866,215 +887,220 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             __syncwarp();
             if (lane == 0) mbar_arrive(&full[j % S]);
         }
-    } else if (warp > 16) {
-        // ---- copies -------------------------------------------------------
-        int seg = 0;
-        // Before the copy of a tile's keys: the ring of eight is far behind.
-        auto tell = [&](int n, bool begins) {
-            Tile t;
-            t.begins = begins;
-            t.i0 = c.tile * kKeys;
-            t.whole = t.i0 + kKeys <= c.keys &&
-                      (key_pos(c, t.i0) >= c.from || key_pos(c, t.i0 + kKeys - 1) < p.a.sinks);
-            t.seg = seg;
-            t.b = c.b, t.kvh = c.kvh;
-            t.sink = c.sink, t.low = c.low, t.from = c.from, t.keys = c.keys;
-            tiles[n & 7] = t;
-        };
-        if (unit > 1) {
-            if (warp == 17) {
-                // Lane i copies box row i of the tile: `unit` keys of a page.
-                const int boxes = kKeys / unit;
-                constexpr int kBlk = DP * (int)sizeof(T) / 128;
-                uint32_t id = 0, id_v = 0;
-                int z = -1, z_v = -1, kvh_v = 0;  // key within the page; -1: no keys there
-                auto look_up = [&] {
-                    const int i = c.tile * kKeys + lane * unit;
-                    z = -1;
-                    if (lane < boxes && i < c.keys) {
-                        const int pos = key_pos(c, i), pg = page_of(p.a.cache, pos);
-                        z = pos - pg * p.a.cache.page;
-                        id = pg < p.a.batch.per_seq ? p.a.batch.table[(long long)c.b * p.a.batch.per_seq + pg] : ~0u;
-                    }
-                };
-                auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity, int n, bool begins) {
-                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
-                    if (__any_sync(0xffffffffu, *abort)) return;
-                    if (at >= 0 && page_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
-                        report_error(p.a.err, kErrGatherId);
-                        page_id = 0;
-                    }
-                    const int count = __popc(__ballot_sync(0xffffffffu, at >= 0));
-                    if (lane == 0) {
-                        if (!parity) tell(n, begins);
-                        mbar_arrive_expect_tx(&raw[j % S], count * unit * 128 * kBlk);
-                    }
-                    __syncwarp();
-                    unsigned char *slot = ring + (j % S) * C::kTileBytes + lane * unit * 128;
-                    if (at >= 0)
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRestRegs));
+        if (warp > 16) {
+            // ---- copies -------------------------------------------------------
+            int seg = 0;
+            // Before the copy of a tile's keys: the ring of eight is far behind.
+            auto tell = [&](int n, bool begins) {
+                Tile t;
+                t.begins = begins;
+                t.i0 = c.tile * kKeys;
+                t.whole = t.i0 + kKeys <= c.keys &&
+                          (key_pos(c, t.i0) >= c.from || key_pos(c, t.i0 + kKeys - 1) < p.a.sinks);
+                t.seg = seg;
+                t.b = c.b, t.kvh = c.kvh;
+                t.sink = c.sink, t.low = c.low, t.from = c.from, t.keys = c.keys;
+                tiles[n & 7] = t;
+            };
+            if (unit > 1) {
+                if (warp == 17) {
+                    // Lane i copies box row i of the tile: `unit` keys of a page.
+                    const int boxes = kKeys / unit;
+                    constexpr int kBlk = DP * (int)sizeof(T) / 128;
+                    uint32_t id = 0, id_v = 0;
+                    int z = -1, z_v = -1, kvh_v = 0;  // key within the page; -1: no keys there
+                    auto look_up = [&] {
+                        const int i = c.tile * kKeys + lane * unit;
+                        z = -1;
+                        if (lane < boxes && i < c.keys) {
+                            const int pos = key_pos(c, i), pg = page_of(p.a.cache, pos);
+                            z = pos - pg * p.a.cache.page;
+                            id = pg < p.a.batch.per_seq
+                                     ? p.a.batch.table[(long long)c.b * p.a.batch.per_seq + pg]
+                                     : ~0u;
+                        }
+                    };
+                    auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity, int n, bool begins) {
+                        if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+                        if (__any_sync(0xffffffffu, *abort)) return;
+                        if (at >= 0 && page_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
+                            report_error(p.a.err, kErrGatherId);
+                            page_id = 0;
+                        }
+                        const int count = __popc(__ballot_sync(0xffffffffu, at >= 0));
+                        if (lane == 0) {
+                            if (!parity) tell(n, begins);
+                            mbar_arrive_expect_tx(&raw[j % S], count * unit * 128 * kBlk);
+                        }
+                        __syncwarp();
+                        unsigned char *slot = ring + (j % S) * C::kTileBytes + lane * unit * 128;
+                        if (at >= 0)
 #pragma unroll
-                        for (int y = 0; y < kBlk; y++)
-                            tma_load_5d(slot + y * C::kBlockBytes, &args.map, y * (128 / (int)sizeof(T)), kvh, at, parity,
-                                        (int)page_id, &raw[j % S]);
-                };
-                if (lane == 0) prefetch_tensormap(&args.map);
-                look_up();
-                bool begins = true;
-                for (int n = 0; n < N; n++) {
-                    copy(n ? 2 * n - 1 : 0, id, z, c.kvh, 0, n, begins);
-                    if (n) copy(2 * n, id_v, z_v, kvh_v, 1, n, false);
-                    id_v = id;
-                    z_v = z;
-                    kvh_v = c.kvh;
-                    begins = c.tile == c.tiles - 1;
-                    seg += begins;
-                    if (n + 1 < N) {
-                        cursor_next(p, unit, c);
-                        look_up();
-                    }
-                }
-                copy(total - 1, id_v, z_v, kvh_v, 1, N, false);
-                // Copies still in flight must land before the CTA's shared
-                // memory is released (after a wait that gave up; else the
-                // MMAs have used them all).
-                if (*abort)
-                    for (int j = max(total - S, 0); j < total; j++) drain_wait(&raw[j % S], (j / S) & 1);
-            }
-        } else {
-            // Rows kRpi at a time, every kCopy-th of them a warp's, by 16-byte
-            // pieces; their places in the cache through a ring of three tiles.
-            const int w = warp - 17, sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
-            auto look_up = [&](int n) {
-                for (int r = threadIdx.x - 17 * 32; r < kKeys; r += kCopy * 32) {
-                    const int i = c.tile * kKeys + r;
-                    long long off = -1;
-                    if (i < c.keys)
-                        off = paged_row(p.a.cache, p.a.batch, c.b, key_pos(c, i), p.a.err) +
-                              c.kvh * D * (long long)sizeof(T);
-                    row_off[n % 3 * kKeys + r] = off;
-                }
-                bar_sync(3, kCopy * 32);
-            };
-            auto copy = [&](int j, int n, int parity) {
-                if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
-                unsigned char *slot = ring + (j % S) * C::kTileBytes;
-                const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
-#pragma unroll 4
-                for (int r = w * C::kRpi + sub; r < kKeys; r += kCopy * C::kRpi) {
-                    const long long off = row_off[n % 3 * kKeys + r];
-                    const bool live = off >= 0 && col < D;
-                    cp_async16_zfill(slot + (C::kPair ? (ch >> 3) * C::kBlockBytes + r * 128 + (ch & 7) * 16
-                                                      : operand_at(r, col)),
-                                     live ? base + off : p.a.cache.base, live ? 16 : 0);
-                }
-            };
-            int done_j = 0;
-            auto landed = [&](int j) {
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&raw[j % S]);
-            };
-            for (int j = 0; j < total; j++) {
-                const bool v = is_v(j);
-                const int n = tile_of(j);
-                if (!v) {
-                    bool begins = n == 0;
-                    if (n) {
+                            for (int y = 0; y < kBlk; y++)
+                                tma_load_5d(slot + y * C::kBlockBytes, &args.map, y * (128 / (int)sizeof(T)), kvh, at,
+                                            parity, (int)page_id, &raw[j % S]);
+                    };
+                    if (lane == 0) prefetch_tensormap(&args.map);
+                    look_up();
+                    bool begins = true;
+                    for (int n = 0; n < N; n++) {
+                        copy(n ? 2 * n - 1 : 0, id, z, c.kvh, 0, n, begins);
+                        if (n) copy(2 * n, id_v, z_v, kvh_v, 1, n, false);
+                        id_v = id;
+                        z_v = z;
+                        kvh_v = c.kvh;
                         begins = c.tile == c.tiles - 1;
                         seg += begins;
-                        cursor_next(p, unit, c);
+                        if (n + 1 < N) {
+                            cursor_next(p, unit, c);
+                            look_up();
+                        }
                     }
-                    look_up(n);
-                    if (w == 0 && lane == 0) tell(n, begins);
+                    copy(total - 1, id_v, z_v, kvh_v, 1, N, false);
+                    // Copies still in flight must land before the CTA's shared
+                    // memory is released (after a wait that gave up; else the
+                    // MMAs have used them all).
+                    if (*abort)
+                        for (int j = max(total - S, 0); j < total; j++) drain_wait(&raw[j % S], (j / S) & 1);
                 }
-                copy(j, n, v);
-                cp_async_commit();
-                if (j >= C::kAhead) {
-                    cp_async_wait<C::kAhead>();
-                    landed(done_j++);
-                }
-            }
-            cp_async_wait<0>();
-            while (done_j < total) landed(done_j++);
-        }
-    } else {
-        // ---- MMA issue ----------------------------------------------------
-        if (lane == 0) {
-        const uint32_t ra = smem_addr(ring);
-        int seg = 0;
-        auto slot_wait = [&](int j) {
-            mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
-            return ra + (j % S) * C::kTileBytes;
-        };
-        auto qk = [&](int n, bool begins, uint32_t kb) {
-            const int j = n ? 2 * n - 1 : 0;
-            if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
-            if (!*abort) {
-                tc_fence_after();
-                const uint32_t d = s_tm + (n & 1) * 128;
-                const uint64_t desc = sw128_desc(kb);
-#pragma unroll 1
-                for (int b = 0; b < C::kBlocks; b++) {
-                    // 64 dims: descriptors hold addresses in 16-byte units.
-                    const uint64_t kh = desc + b * (C::kBlockBytes / 16);
-                    const uint32_t qh = q_tm + b * 64;
-#pragma unroll
-                    for (int ks = 0; ks < 4; ks++) {
-                        const uint32_t at = qh + ks / 2 * 32 + ks % 2 * 8;
-                        mma_ts(d, at + 16, kh + ks * 2, C::kIdescS, b + ks);
-                        if (C::kPair) mma_ts(d, at, kh + ks * 2 + C::kHalfBytes / 16, C::kIdescS, 1u);
-                        mma_ts(d, at, kh + ks * 2, C::kIdescS, 1u);
-                    }
-                }
-                mma_commit(&empty[j % S]);
-                mma_commit(&s_full[n & 1]);
-            }
-        };
-        auto pv = [&](int n) {
-            mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-            const int j = n == N - 1 ? total - 1 : 2 * n + 2;
-            const uint32_t vb = slot_wait(j);
-            if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
-            if (!*abort) {
-                tc_fence_after();
-                const uint32_t pt = s_tm + (n & 1) * 128;
-                const uint64_t desc = sw128_desc_mn(vb, C::kBlockBytes);
-#pragma unroll 1
-                for (int b = 0; b < kKeys / 32; b++) {
-                    const uint64_t vh = desc + b * (2 * 2048 / 16);
-                    const uint32_t ph = pt + b * 32;
-#pragma unroll
-                    for (int ks = 0; ks < 2; ks++) {
-                        mma_ts(o_tm, ph + ks * 8 + 16, vh + ks * 128, C::kIdescO, b + ks);
-                        if (C::kPair)
-                            mma_ts(o_tm, ph + ks * 8, vh + ks * 128 + C::kHalfBytes / 16, C::kIdescO, 1u);
-                        mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
-                    }
-                }
-                mma_commit(&empty[j % S]);
-                mma_commit(o_full);
-            }
-        };
-        // Q K^T one tile ahead, but a segment's first waits for its Q, which
-        // the softmax warps write after the tile before: P V goes first there.
-        bool begins = true;
-        uint32_t kb = 0;
-        for (int nq = 0, np = 0, known = 0; np < N;) {
-            if (nq < N && nq <= np + 1 && known <= nq) {
-                kb = slot_wait(nq ? 2 * nq - 1 : 0);
-                begins = tiles[nq & 7].begins;
-                known = nq + 1;
-            }
-            if (nq < N && nq <= np + 1 && !(begins && np < nq)) {
-                qk(nq, begins, kb);
-                nq++;
             } else {
-                pv(np++);
+                // Rows kRpi at a time, every kCopy-th of them a warp's, by 16-byte
+                // pieces; their places in the cache through a ring of three tiles.
+                const int w = warp - 17, sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+                auto look_up = [&](int n) {
+                    for (int r = threadIdx.x - 17 * 32; r < kKeys; r += kCopy * 32) {
+                        const int i = c.tile * kKeys + r;
+                        long long off = -1;
+                        if (i < c.keys)
+                            off = paged_row(p.a.cache, p.a.batch, c.b, key_pos(c, i), p.a.err) +
+                                  c.kvh * D * (long long)sizeof(T);
+                        row_off[n % 3 * kKeys + r] = off;
+                    }
+                    bar_sync(3, kCopy * 32);
+                };
+                auto copy = [&](int j, int n, int parity) {
+                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+                    unsigned char *slot = ring + (j % S) * C::kTileBytes;
+                    const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
+#pragma unroll 4
+                    for (int r = w * C::kRpi + sub; r < kKeys; r += kCopy * C::kRpi) {
+                        const long long off = row_off[n % 3 * kKeys + r];
+                        const bool live = off >= 0 && col < D;
+                        cp_async16_zfill(slot + (C::kPair ? (ch >> 3) * C::kBlockBytes + r * 128 + (ch & 7) * 16
+                                                          : operand_at(r, col)),
+                                         live ? base + off : p.a.cache.base, live ? 16 : 0);
+                    }
+                };
+                int done_j = 0;
+                auto landed = [&](int j) {
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&raw[j % S]);
+                };
+                for (int j = 0; j < total; j++) {
+                    const bool v = is_v(j);
+                    const int n = tile_of(j);
+                    if (!v) {
+                        bool begins = n == 0;
+                        if (n) {
+                            begins = c.tile == c.tiles - 1;
+                            seg += begins;
+                            cursor_next(p, unit, c);
+                        }
+                        look_up(n);
+                        if (w == 0 && lane == 0) tell(n, begins);
+                    }
+                    copy(j, n, v);
+                    cp_async_commit();
+                    if (j >= C::kAhead) {
+                        cp_async_wait<C::kAhead>();
+                        landed(done_j++);
+                    }
+                }
+                cp_async_wait<0>();
+                while (done_j < total) landed(done_j++);
             }
-        }
-        // Every MMA issued must complete before TMEM is freed.
-        mma_commit(done);
-        drain_wait(done, 0);
+        } else {
+            // ---- MMA issue ----------------------------------------------------
+            if (lane == 0) {
+                const uint32_t ra = smem_addr(ring);
+                int seg = 0;
+                auto slot_wait = [&](int j) {
+                    mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
+                    return ra + (j % S) * C::kTileBytes;
+                };
+                auto qk = [&](int n, bool begins, uint32_t kb) {
+                    const int j = n ? 2 * n - 1 : 0;
+                    if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
+                    if (!*abort) {
+                        tc_fence_after();
+                        const uint32_t d = s_tm + (n & 1) * 128;
+                        const uint64_t desc = sw128_desc(kb);
+#pragma unroll 1
+                        for (int b = 0; b < C::kBlocks; b++) {
+                            // 64 dims: descriptors hold addresses in 16-byte units.
+                            const uint64_t kh = desc + b * (C::kBlockBytes / 16);
+                            const uint32_t qh = q_tm + b * 64;
+#pragma unroll
+                            for (int ks = 0; ks < 4; ks++) {
+                                const uint32_t at = qh + ks / 2 * 32 + ks % 2 * 8;
+                                mma_ts(d, at + 16, kh + ks * 2, C::kIdescS, b + ks);
+                                if (C::kPair) mma_ts(d, at, kh + ks * 2 + C::kHalfBytes / 16, C::kIdescS, 1u);
+                                mma_ts(d, at, kh + ks * 2, C::kIdescS, 1u);
+                            }
+                        }
+                        mma_commit(&empty[j % S]);
+                        mma_commit(&s_full[n & 1]);
+                    }
+                };
+                auto pv = [&](int n) {
+                    mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
+                    const int j = n == N - 1 ? total - 1 : 2 * n + 2;
+                    const uint32_t vb = slot_wait(j);
+                    if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
+                    if (!*abort) {
+                        tc_fence_after();
+                        const uint32_t pt = s_tm + (n & 1) * 128;
+                        const uint64_t desc = sw128_desc_mn(vb, C::kBlockBytes);
+#pragma unroll 1
+                        for (int b = 0; b < kKeys / 32; b++) {
+                            const uint64_t vh = desc + b * (2 * 2048 / 16);
+                            const uint32_t ph = pt + b * 32;
+#pragma unroll
+                            for (int ks = 0; ks < 2; ks++) {
+                                mma_ts(o_tm, ph + ks * 8 + 16, vh + ks * 128, C::kIdescO, b + ks);
+                                if (C::kPair)
+                                    mma_ts(o_tm, ph + ks * 8, vh + ks * 128 + C::kHalfBytes / 16, C::kIdescO, 1u);
+                                mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
+                            }
+                        }
+                        mma_commit(&empty[j % S]);
+                        mma_commit(o_full);
+                    }
+                };
+                // Q K^T one tile ahead, but a segment's first waits for its Q, which
+                // the softmax warps write after the tile before: P V goes first there.
+                bool begins = true;
+                uint32_t kb = 0;
+                for (int nq = 0, np = 0, known = 0; np < N;) {
+                    if (nq < N && nq <= np + 1 && known <= nq) {
+                        kb = slot_wait(nq ? 2 * nq - 1 : 0);
+                        begins = tiles[nq & 7].begins;
+                        known = nq + 1;
+                    }
+                    if (nq < N && nq <= np + 1 && !(begins && np < nq)) {
+                        qk(nq, begins, kb);
+                        nq++;
+                    } else {
+                        pv(np++);
+                    }
+                }
+                // Every MMA issued must complete before TMEM is freed.
+                mma_commit(done);
+                drain_wait(done, 0);
+            }
         }
     }
     tc_fence_before();
