@@ -267,14 +267,25 @@ struct Tile {
     int sink, low, from, keys;
 };
 
+// Called by a whole warp, issued by one lane (always the same).
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
         "{\n"
-        ".reg .pred p;\n"
+        ".reg .pred p, q;\n"
         "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "elect.sync _|q, 0xffffffff;\n"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
         "}\n" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void commit_one(uint64_t *bar) {
+    asm volatile(
+        "{\n"
+        ".reg .pred q;\n"
+        "elect.sync _|q, 0xffffffff;\n"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n"
+        "}\n" ::"r"(smem_addr(bar))
         : "memory");
 }
 __device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
@@ -1024,83 +1035,88 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             }
         } else {
             // ---- MMA issue ----------------------------------------------------
-            if (lane == 0) {
-                const uint32_t ra = smem_addr(ring);
-                int seg = 0;
-                auto slot_wait = [&](int j) {
-                    mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
-                    return ra + (j % S) * C::kTileBytes;
-                };
-                auto qk = [&](int n, bool begins, uint32_t kb) {
-                    const int j = n ? 2 * n - 1 : 0;
-                    if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
-                    if (!*abort) {
-                        tc_fence_after();
-                        const uint32_t d = s_tm + (n & 1) * 128;
-                        const uint64_t desc = sw128_desc(kb);
+            // The whole warp walks the loop and one elected lane issues. Inside
+            // one lane's branch 16 MMAs took 1600 cycles to issue, 1024 to run;
+            // uniform control flow takes two prompts of 2048 tokens from 619
+            // to 559 us over an f16 cache, from 896 to 868 us over f32. With
+            // all steps unrolled the code of the roles outgrows the
+            // instruction caches (676 and 1040 us); rolled up, f32 is at 849,
+            // bf16 at 693 instead of 724, f16 at 597.
+            const uint32_t ra = smem_addr(ring);
+            int seg = 0;
+            auto slot_wait = [&](int j) {
+                mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
+                return ra + (j % S) * C::kTileBytes;
+            };
+            auto qk = [&](int n, bool begins, uint32_t kb) {
+                const int j = n ? 2 * n - 1 : 0;
+                if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
+                if (!__any_sync(0xffffffffu, *abort)) {
+                    tc_fence_after();
+                    const uint32_t d = s_tm + (n & 1) * 128;
+                    const uint64_t desc = sw128_desc(kb);
 #pragma unroll 1
-                        for (int b = 0; b < C::kBlocks; b++) {
-                            // 64 dims: descriptors hold addresses in 16-byte units.
-                            const uint64_t kh = desc + b * (C::kBlockBytes / 16);
-                            const uint32_t qh = q_tm + b * 64;
-#pragma unroll
-                            for (int ks = 0; ks < 4; ks++) {
-                                const uint32_t at = qh + ks / 2 * 32 + ks % 2 * 8;
-                                mma_ts(d, at + 16, kh + ks * 2, C::kIdescS, b + ks);
-                                if (C::kPair) mma_ts(d, at, kh + ks * 2 + C::kHalfBytes / 16, C::kIdescS, 1u);
-                                mma_ts(d, at, kh + ks * 2, C::kIdescS, 1u);
-                            }
+                    for (int b = 0; b < C::kBlocks; b++) {
+                        // 64 dims: descriptors hold addresses in 16-byte units.
+                        const uint64_t kh = desc + b * (C::kBlockBytes / 16);
+                        const uint32_t qh = q_tm + b * 64;
+#pragma unroll(C::kRaw ? 4 : 1)
+                        for (int ks = 0; ks < 4; ks++) {
+                            const uint32_t at = qh + ks / 2 * 32 + ks % 2 * 8;
+                            mma_ts(d, at + 16, kh + ks * 2, C::kIdescS, b + ks);
+                            if (C::kPair) mma_ts(d, at, kh + ks * 2 + C::kHalfBytes / 16, C::kIdescS, 1u);
+                            mma_ts(d, at, kh + ks * 2, C::kIdescS, 1u);
                         }
-                        mma_commit(&empty[j % S]);
-                        mma_commit(&s_full[n & 1]);
                     }
-                };
-                auto pv = [&](int n) {
-                    mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-                    const int j = n == N - 1 ? total - 1 : 2 * n + 2;
-                    const uint32_t vb = slot_wait(j);
-                    if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
-                    if (!*abort) {
-                        tc_fence_after();
-                        const uint32_t pt = s_tm + (n & 1) * 128;
-                        const uint64_t desc = sw128_desc_mn(vb, C::kBlockBytes);
-#pragma unroll 1
-                        for (int b = 0; b < kKeys / 32; b++) {
-                            const uint64_t vh = desc + b * (2 * 2048 / 16);
-                            const uint32_t ph = pt + b * 32;
-#pragma unroll
-                            for (int ks = 0; ks < 2; ks++) {
-                                mma_ts(o_tm, ph + ks * 8 + 16, vh + ks * 128, C::kIdescO, b + ks);
-                                if (C::kPair)
-                                    mma_ts(o_tm, ph + ks * 8, vh + ks * 128 + C::kHalfBytes / 16, C::kIdescO, 1u);
-                                mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
-                            }
-                        }
-                        mma_commit(&empty[j % S]);
-                        mma_commit(o_full);
-                    }
-                };
-                // Q K^T one tile ahead, but a segment's first waits for its Q, which
-                // the softmax warps write after the tile before: P V goes first there.
-                bool begins = true;
-                uint32_t kb = 0;
-                for (int nq = 0, np = 0, known = 0; np < N;) {
-                    if (nq < N && nq <= np + 1 && known <= nq) {
-                        kb = slot_wait(nq ? 2 * nq - 1 : 0);
-                        begins = tiles[nq & 7].begins;
-                        known = nq + 1;
-                    }
-                    if (nq < N && nq <= np + 1 && !(begins && np < nq)) {
-                        qk(nq, begins, kb);
-                        nq++;
-                    } else {
-                        pv(np++);
-                    }
+                    commit_one(&empty[j % S]);
+                    commit_one(&s_full[n & 1]);
                 }
-                // Every MMA issued must complete before TMEM is freed.
-                mma_commit(done);
-                drain_wait(done, 0);
+            };
+            auto pv = [&](int n) {
+                mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
+                const int j = n == N - 1 ? total - 1 : 2 * n + 2;
+                const uint32_t vb = slot_wait(j);
+                if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
+                if (!__any_sync(0xffffffffu, *abort)) {
+                    tc_fence_after();
+                    const uint32_t pt = s_tm + (n & 1) * 128;
+                    const uint64_t desc = sw128_desc_mn(vb, C::kBlockBytes);
+#pragma unroll 1
+                    for (int b = 0; b < kKeys / 32; b++) {
+                        const uint64_t vh = desc + b * (2 * 2048 / 16);
+                        const uint32_t ph = pt + b * 32;
+#pragma unroll(C::kRaw ? 2 : 1)
+                        for (int ks = 0; ks < 2; ks++) {
+                            mma_ts(o_tm, ph + ks * 8 + 16, vh + ks * 128, C::kIdescO, b + ks);
+                            if (C::kPair)
+                                mma_ts(o_tm, ph + ks * 8, vh + ks * 128 + C::kHalfBytes / 16, C::kIdescO, 1u);
+                            mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
+                        }
+                    }
+                    commit_one(&empty[j % S]);
+                    commit_one(o_full);
+                }
+            };
+            // Q K^T one tile ahead, but a segment's first waits for its Q, which
+            // the softmax warps write after the tile before: P V goes first there.
+            bool begins = true;
+            uint32_t kb = 0;
+            for (int nq = 0, np = 0, known = 0; np < N;) {
+                if (nq < N && nq <= np + 1 && known <= nq) {
+                    kb = slot_wait(nq ? 2 * nq - 1 : 0);
+                    begins = tiles[nq & 7].begins;
+                    known = nq + 1;
+                }
+                if (nq < N && nq <= np + 1 && !(begins && np < nq)) {
+                    qk(nq, begins, kb);
+                    nq++;
+                } else {
+                    pv(np++);
+                }
             }
+            // Every MMA issued must complete before TMEM is freed.
+            commit_one(done);
+            drain_wait(done, 0);
         }
     }
     tc_fence_before();
