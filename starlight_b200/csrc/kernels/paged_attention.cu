@@ -9,17 +9,20 @@
 //
 // Work. A segment is (sequence, block of kRows query rows, kv head); its keys
 // are cut into tiles of kTileKeys. All tiles of all segments form one line
-// that the CTAs (one per SM) share out in equal contiguous ranges, so a batch
+// that the CTAs (one or two per SM) share out in equal contiguous ranges, so a batch
 // of any lengths keeps every SM busy to the end. The cuts are computed on the
 // device from the batch's lengths: a captured graph replays with new ones. A
 // segment that crosses a cut is merged by the last of its CTAs to finish
 // (ticket, no waiting), its pieces in ascending order: results do not depend
 // on the order of execution.
 //
-// A tile is 16 or 32 keys for each of the CTA's warps. A warp fetches its keys and
-// values into a ring of its own, kStages tiles ahead and across segment
+// A tile is 16 or 32 keys for each of the CTA's warps. A warp fetches its keys
+// and values into a ring of its own, kStages tiles ahead and across segment
 // borders, and shares nothing with the other warps until the segment's end,
-// where the warps' m, l and o merge in shared memory. It fetches them as TMA
+// where the warps' m, l and o merge in shared memory. (Independent warps, each
+// with a range of the line and a warp that copies for all, were slower: 430
+// instead of 363 us over 64 long sequences, 19 instead of 8 over a short one,
+// whose pieces are then eight times as many to merge.) It fetches them as TMA
 // boxes of 8 to 32 keys by 128 bytes, swizzled. (Pages that are not a
 // multiple of 8 keys go by 16-byte asynchronous copies: twice the
 // instructions in all, which is what bounds two warps per scheduler. Bulk
@@ -44,6 +47,14 @@
 // Rows that meet a NaN or an infinity are recomputed in plain f32 over the
 // keys that they see alone (the MMA multiplies masked values by zero, and the
 // split of an infinity is NaN).
+//
+// Bound by HBM over long sequences: 64 of 300 to 16000 keys in bf16 (1.97 GB)
+// 329 us, 6.0 TB/s; 8 of 1000 to 8000 in f32 (282 MB) 55 us, 5.1 TB/s; heads
+// of 64 f32, 64 sequences (1.09 GB), 182 us, 6.0 TB/s. Short segments are
+// bound by latency: with 8 warps an SM three of four issue slots are empty, a
+// segment's start and end (queries, merge, result) cost about 5000 cycles and
+// a tile of 256 keys 4500. One sequence of 512 keys takes 7.8 us, a launch
+// chain of dependent reads.
 #include <math.h>
 
 #include <algorithm>
@@ -58,7 +69,6 @@ namespace k {
 namespace {
 
 constexpr int kRows = 8;
-constexpr int kSmallRows = 32;  // query rows per kv head taken here; more go to paged_rows.cu
 
 template <typename T, int DP>
 struct Cfg {
@@ -975,10 +985,14 @@ cudaError_t launch_type(cudaStream_t s, const PagedPass &p) {
     }
 }
 
-// Whether rows * group query rows of one kv head are too many for
-// paged_attention_kernel, which reads the keys once per kRows of them.
+// Query rows of one kv head up to which a sequence is paged_attention_kernel's,
+// which reads the keys once per kRows of them; more are paged_rows.cu's.
+// Measured, 16 sequences of 1000 to 4000 keys, 8 kv heads of 128, with 16, 32
+// and 48 rows: f32 113, 174, 255 us here and 113, 122, 124 there; bf16 61, 92,
+// 130 and 92, 100, 101.
+int small_rows(const PagedAttention &a) { return a.cache.type == kPagedF32 ? 16 : 32; }
 bool many_rows(const PagedAttention &a, size_t rows) {
-    return paged_rows_supported(a) && rows * (size_t)(a.heads / a.kv_heads) > (size_t)kSmallRows;
+    return paged_rows_supported(a) && rows * (size_t)(a.heads / a.kv_heads) > (size_t)small_rows(a);
 }
 
 size_t part_floats(const PagedAttention &a) {
@@ -1030,7 +1044,7 @@ cudaError_t paged_attention(cudaStream_t s, const PagedAttention &call) {
     }
     // Sequences with many rows first, those with few after them.
     if (many_rows(a, a.max_new)) {
-        p.small_rows = kSmallRows;
+        p.small_rows = small_rows(a);
         e = paged_rows(s, p);
         if (e != cudaSuccess) return e;
     }
