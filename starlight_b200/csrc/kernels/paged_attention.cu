@@ -991,14 +991,30 @@ cudaError_t launch_type(cudaStream_t s, const PagedPass &p) {
 // and 48 rows: f32 113, 174, 255 us here and 113, 122, 124 there; bf16 61, 92,
 // 130 and 92, 100, 101.
 int small_rows(const PagedAttention &a) { return a.cache.type == kPagedF32 ? 16 : 32; }
-bool many_rows(const PagedAttention &a, size_t rows) {
-    return paged_rows_supported(a) && rows * (size_t)(a.heads / a.kv_heads) > (size_t)small_rows(a);
+// Where all keys that the call's shapes allow are few, tokens in all times keys
+// counted in blocks of kRows rows by a tile, it takes them whatever the rows:
+// paged_rows.cu has 20 us to start up and end. 1 sequence of 38 tokens over 160
+// keys (76 units) 7.5 us here and 33 there, of 128 new tokens in f32 (512)
+// 17.9 and 31, of 20 over 1000 (640) 21.9 and 25.7, of 64 over 1000 (2304) 41
+// and 28. Known from the shapes alone, so that a call gives the same results
+// captured and not.
+constexpr size_t kFewUnits = 1024;
+bool many_rows(const PagedAttention &a, size_t new_tokens, size_t runs, size_t keys) {
+    const size_t group = a.heads / a.kv_heads, tile = a.cache.type == kPagedF32 ? 128 : 256;
+    if (!paged_rows_supported(a) || new_tokens * group <= (size_t)small_rows(a)) return false;
+    const size_t blocks = (size_t)a.tokens * group / kRows + runs;
+    return blocks * a.kv_heads * ((keys + tile - 1) / tile) > kFewUnits;
 }
+bool many_rows(const PagedAttention &a) {
+    size_t keys = (size_t)a.batch.per_seq * a.cache.page;
+    if (a.window) keys = std::min(keys, (size_t)a.window + a.sinks + a.max_new);
+    return many_rows(a, a.max_new, a.batch.seqs, keys);
+}
+bool many_prefix_rows(const PagedAttention &a) { return a.prefix && many_rows(a, a.tokens, 1, a.prefix); }
 
 size_t part_floats(const PagedAttention &a) {
     const size_t few = partial_floats(padded_dim(a.head_dim));
-    const bool rows = many_rows(a, a.max_new) || (a.prefix && many_rows(a, a.tokens));
-    return rows ? std::max(few, paged_rows_part_floats(a)) : few;
+    return many_rows(a) || many_prefix_rows(a) ? std::max(few, paged_rows_part_floats(a)) : few;
 }
 
 // A pass over the shared prefix saves the others' reads of it (from L2, mostly)
@@ -1037,16 +1053,17 @@ cudaError_t paged_attention(cudaStream_t s, const PagedAttention &call) {
         p.pre_o = p.part_o + part_floats(a);
         p.pre_ml = p.pre_o + (size_t)a.tokens * a.heads * a.head_dim;
         p.prefix_pass = 1;
-        e = many_rows(a, a.tokens) ? paged_rows(s, p) : launch_type(s, p);
+        e = many_prefix_rows(a) ? paged_rows(s, p) : launch_type(s, p);
         if (e != cudaSuccess) return e;
         p.prefix_pass = 0;
         p.first = a.prefix;
     }
-    // Sequences with many rows first, those with few after them.
-    if (many_rows(a, a.max_new)) {
-        p.small_rows = small_rows(a);
+    // Sequences with many rows first, those with few after them (a sequence
+    // alone has its kernel: a launch for nothing takes 4 us).
+    if (many_rows(a)) {
+        p.small_rows = a.batch.seqs == 1 ? 0 : small_rows(a);
         e = paged_rows(s, p);
-        if (e != cudaSuccess) return e;
+        if (e != cudaSuccess || a.batch.seqs == 1) return e;
     }
     return launch_type(s, p);
 }

@@ -41,7 +41,7 @@ class Batch:
     pages is HOLE. `prefix` leading positions are shared pages."""
 
     def __init__(self, lens, heads=4, kv_heads=2, dim=64, page=16, layers=2, layer=1, dtype=DType.F32,
-                 prefix=0, pad=0, extra_pages=3, seed=0, width=None):
+                 prefix=0, pad=0, extra_pages=3, seed=0, width=None, narrow=False):
         self.lens, self.heads, self.kv_heads, self.dim = lens, heads, kv_heads, dim
         self.page, self.layers, self.layer, self.dtype, self.prefix = page, layers, layer, dtype, prefix
         r = self.rng = np.random.RandomState(seed)
@@ -49,7 +49,11 @@ class Batch:
         shared = -(-prefix // page)
         self.pages = shared + sum(max(k - shared, 0) for k in need) + extra_pages
         order = r.permutation(self.pages)
-        width = width or max(need + [1])
+        if width is None:
+            # Rows in numbers have their own kernel where the table leaves room
+            # for many keys; `narrow` tables have no more than they need.
+            many = max([n for _, n in lens] + [0]) * heads // kv_heads > 16
+            width = max(need + [1] + ([] if narrow or not many else [-(-(1 << 18) // page)]))
         self.table = np.full((len(lens), width), HOLE, np.uint32)
         used = shared
         for b, k in enumerate(need):

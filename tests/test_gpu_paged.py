@@ -199,6 +199,33 @@ def test_few_rows_over_many_keys(dev, dtype, heads, kv_heads, dim):
     check(attend(dev, b, window=3000, sinks=5, refs=refs), b, window=3000, sinks=5)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("window,sinks,page", [(1, 0, 16), (7, 2, 5), (64, 4, 32), (65, 63, 8), (200, 1000, 64)])
+def test_windows_of_many_rows(dev, window, sinks, page, dtype):
+    b = Batch([(300, 150), (0, 200), (62, 9), (390, 120), (5, 130)], heads=16, kv_heads=8, dim=64, page=page,
+              dtype=dtype, layers=1, layer=0)
+    check(attend(dev, b, window=window, sinks=sinks), b, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("page", [5, 16])
+def test_many_rows_over_few_keys(dev, page, dtype):
+    # A table with no room for more keys: the kernel for few rows takes them.
+    b = Batch([(40, 33), (3, 1), (0, 70), (100, 25)], heads=6, kv_heads=2, dim=72, page=page, dtype=dtype, pad=2,
+              narrow=True)
+    refs = upload(dev, b)
+    check(attend(dev, b, refs=refs), b)
+    check(attend(dev, b, window=20, sinks=3, refs=refs), b, window=20, sinks=3)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("past,new", [(0, 300), (1000, 1), (333, 40)])
+def test_one_sequence(dev, past, new, dtype):
+    # Alone in the batch, with max_new above what it has: one kernel does all.
+    b = Batch([(past, new)], heads=16, kv_heads=4, dim=128, page=16, dtype=dtype, width=4096)
+    check(attend(dev, b, max_new=500), b)
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("page", [8, 24, 256])
 def test_page_sizes(dev, page, dtype):
@@ -364,13 +391,14 @@ def test_prefix(dev, case, dtype):
 # sequences on; below, every sequence reads it by itself.
 PASS_BYTES = 96 << 20
 PASSES = [
-    # rows of one kv head: 16 (few), 64 (many), 160 (many, two row tiles), wide heads, odd pages
+    # rows of one kv head: 16, 64, 328, wide heads, odd pages; the last two over enough keys for the kernel for many
     dict(lens=[(1700 + i, 1) for i in range(16)], prefix=1650, heads=8, kv_heads=8, dim=128, page=16),
     dict(lens=[(800 + 3 * i, 1) for i in range(64)], prefix=799, heads=8, kv_heads=8, dim=128, page=64),
     dict(lens=[(640 + i % 9, i % 3) for i in range(80)], prefix=640, heads=32, kv_heads=8, dim=64, page=16, pad=2),
     dict(lens=[(1000 + i, 1) for i in range(16)], prefix=900, heads=16, kv_heads=8, dim=256, page=24),
     dict(lens=[(1500 + i, i % 2) for i in range(31)], prefix=1500, heads=8, kv_heads=8, dim=72, page=5),
-    dict(lens=[(702, 0)] + [(702 + i, 1) for i in range(64)], prefix=701, heads=8, kv_heads=8, dim=72, page=7),
+    dict(lens=[(702, 0)] + [(702 + i, 1) for i in range(64)], prefix=701, heads=64, kv_heads=8, dim=72, page=7),
+    dict(lens=[(1300 + i, 1) for i in range(48)], prefix=1290, heads=64, kv_heads=8, dim=128, page=16),
 ]
 
 
@@ -391,7 +419,7 @@ def test_prefix_in_a_pass_of_its_own(dev, case, dtype):
         assert np.array_equal(first, attend(dev, b, offset=case % 2, refs=refs))
 
 
-@pytest.mark.parametrize("case", [0, 1, 4])
+@pytest.mark.parametrize("case", [0, 1, 4, 6])
 @pytest.mark.parametrize("value", [np.nan, np.inf])
 def test_prefix_pass_with_values_that_are_not_finite(dev, value, case):
     b = pass_batch(PASSES[case], F32, seed=case)
@@ -592,7 +620,7 @@ def test_decoding_captured_and_replayed(dtype, prefix):
 def test_prompts_captured_and_replayed(dtype, window):
     # Chunks of prompts of changing lengths through one captured command, then
     # a second graph on the same workspace.
-    batches = [Batch([(p, n), (20, 1), (m, 9)], heads=8, kv_heads=2, dim=64, page=16, dtype=dtype, width=40,
+    batches = [Batch([(p, n), (20, 1), (m, 9)], heads=8, kv_heads=2, dim=64, page=16, dtype=dtype, width=400,
                      extra_pages=40, pad=120 - n, seed=i)
                for i, (p, n, m) in enumerate([(300, 90, 0), (0, 120, 7), (500, 1, 90), (17, 64, 400), (100, 33, 5),
                                               (250, 100, 60)])]
@@ -602,7 +630,7 @@ def test_prompts_captured_and_replayed(dtype, window):
     try:
         d.set_capture(True)
         cache = new_f32(d, state_words(shape, dtype))
-        table, past, starts = (put_u32(d, np.zeros(n)) for n in ((3, 40), 3, 4))
+        table, past, starts = (put_u32(d, np.zeros(n)) for n in ((3, 400), 3, 4))
         q, outs = new_f32(d, 130 * 512), [new_f32(d, 130 * 512) for _ in range(2)]
         x = Value.f32((130, 512))
         first = batches[0]
