@@ -184,7 +184,7 @@ typedef enum {
      *
      * PREFIX_ATTENTION: PAGED_ATTENTION without a window, for sequences whose
      * first `prefix` positions are the same pages of the cache; these are read
-     * once for all of them. Scalars max_new, prefix; prefix at most every
+     * once for all of them (by each, where that is quicker). Scalars max_new, prefix; prefix at most every
      * past, and the table's rows begin with the same ceil(prefix / page)
      * entries. */
     SLC_OP_EXT_PAGED_APPEND = 0x8003,
