@@ -8,7 +8,8 @@
 // computed in one pass over the keys with a running m, l and o.
 //
 // Work. A segment is (sequence, block of kRows query rows, kv head); its keys
-// are cut into tiles of kTileKeys. All tiles of all segments form one line
+// are cut into tiles of kTileKeys. All tiles of all segments, and one more unit
+// for a segment's end, which takes about a tile's time, form one line
 // that the CTAs (one or two per SM) share out in equal contiguous ranges, so a batch
 // of any lengths keeps every SM busy to the end. The cuts are computed on the
 // device from the batch's lengths: a captured graph replays with new ones. A
@@ -146,38 +147,47 @@ __device__ __forceinline__ void seq_load(const PagedPass &p, int unit, int b, Cu
 template <int kTile>
 __device__ __forceinline__ long long seq_units(const PagedPass &p, const Cursor<kTile> &c) {
     const long long rb = (c.ntok * (long long)(p.a.heads / p.a.kv_heads) + kRows - 1) / kRows;
-    return c.ntok > 0 ? rb * p.a.kv_heads * c.tiles : 0;
+    return c.ntok > 0 ? rb * p.a.kv_heads * (c.tiles + 1) : 0;
 }
 
-// Places the cursor on unit `at` counted from the start of sequence c.b.
+// Places the cursor on the tile at unit `at` counted from the start of sequence
+// c.b, or on the next one where that unit is a segment's end. Returns the units
+// passed over.
 template <int kTile>
-__device__ __forceinline__ void cursor_at(const PagedPass &p, int unit, Cursor<kTile> &c, long long at) {
+__device__ __forceinline__ int cursor_at(const PagedPass &p, int unit, Cursor<kTile> &c, long long at) {
     const int seqs = p.prefix_pass ? 1 : p.a.batch.seqs;
-    long long n = seq_units(p, c);
-    while (!p.prefix_pass && at >= n && c.b + 1 < seqs) {
-        at -= n;
-        seq_load(p, unit, c.b + 1, c);
-        n = seq_units(p, c);
+    long long n = seq_units(p, c), seg;
+    for (int passed = 0;; passed++, at++) {
+        while (!p.prefix_pass && at >= n && c.b + 1 < seqs) {
+            at -= n;
+            seq_load(p, unit, c.b + 1, c);
+            n = seq_units(p, c);
+        }
+        seg = at / (c.tiles + 1);
+        c.tile = (int)(at - seg * (c.tiles + 1));
+        if (c.tile < c.tiles || at >= n) {
+            c.left = n - at;
+            c.rb = (int)(seg / p.a.kv_heads);
+            c.kvh = (int)(seg - (long long)c.rb * p.a.kv_heads);
+            return passed;
+        }
     }
-    c.left = n - at;
-    const long long seg = at / max(c.tiles, 1);
-    c.tile = (int)(at - seg * c.tiles);
-    c.rb = (int)(seg / p.a.kv_heads);
-    c.kvh = (int)(seg - (long long)c.rb * p.a.kv_heads);
 }
 
+// To the next tile: a unit on, at a segment's end two.
 template <int kTile>
 __device__ __forceinline__ void cursor_next(const PagedPass &p, int unit, Cursor<kTile> &c) {
-    if (--c.left == 0) {
+    const bool ends = ++c.tile == c.tiles;
+    c.left -= ends ? 2 : 1;
+    if (!ends) return;
+    if (c.left == 0) {
         cursor_at(p, unit, c, seq_units(p, c));
         return;
     }
-    if (++c.tile == c.tiles) {
-        c.tile = 0;
-        if (++c.kvh == p.a.kv_heads) {
-            c.kvh = 0;
-            c.rb++;
-        }
+    c.tile = 0;
+    if (++c.kvh == p.a.kv_heads) {
+        c.kvh = 0;
+        c.rb++;
     }
 }
 
@@ -345,8 +355,12 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
     __syncthreads();
     Cur cc, pc;  // consumer and producer
     seq_load(p, unit, (int)found[0] * per, cc);
-    cursor_at(p, unit, cc, u0 - found[1]);
+    long long u = u0 + cursor_at(p, unit, cc, u0 - found[1]), pu = u;  // their units
     pc = cc;
+    if (u >= u1) {  // nothing but a segment's end
+        pdl_wait();
+        return;
+    }
     // The producer's unit: lane b holds the table entry and the place in its
     // page of box b of the warp's keys, or, without boxes, lane r those of key
     // r (modulo the keys); read a tile before their use.
@@ -406,19 +420,21 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
             cp_async_wait<2 * S - 1>();
         __syncwarp();
     };
-    const int units = (int)(u1 - u0);
-    int issued = 0;
     if (unit > 1 && threadIdx.x == 0) prefetch_tensormap(&args.map);
     look_up();   // lengths and tables come from uploads alone,
     pdl_wait();  // q and the cache from earlier kernels; workspace use may overlap none
-    for (; issued < S; issued++) {
-        if (issued < units) {
-            issue(issued, 0);
-            issue(issued, 1);
-            if (issued + 1 < units) {
-                cursor_next(p, unit, pc);
-                look_up();
-            }
+    auto advance = [&] {
+        pu += pc.tile + 1 == pc.tiles ? 2 : 1;
+        if (pu < u1) {
+            cursor_next(p, unit, pc);
+            look_up();
+        }
+    };
+    for (int i = 0; i < S; i++) {
+        if (pu < u1) {
+            issue(i, 0);
+            issue(i, 1);
+            advance();
         } else if (unit == 1) {  // one group a half, empty ones at the end
             cp_async_commit();
             cp_async_commit();
@@ -488,7 +504,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float qf0 = 0.f, qf1 = 0.f;  // S to log2 units, rows 2t and 2t + 1
     int at0 = 0, at1 = 0;        // their positions
-    long long seg_u0 = u0;       // this CTA's first unit of the current segment
+    long long seg_u0 = u;        // this CTA's first unit of the current segment
     bool fresh = true;
     int stage = 0, phase = 0;
     Cur nc = cc;                 // first unit of the segment after this one
@@ -505,10 +521,11 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
         const int row = cc.rb * kRows + r, tok = row / G;
         return (size_t)(cc.tok0 + tok) * H + cc.kvh * G + (row - tok * G);
     };
-    for (long long u = u0; u < u1; u++) {
+    while (u < u1) {
         const bool seg_end = cc.tile == cc.tiles - 1, ends = seg_end || u + 1 == u1;
+        const bool last = u + (seg_end ? 2 : 1) >= u1;  // of this CTA
         if (ends) {
-            if (u + 1 < u1) {
+            if (!last) {
                 nc = cc;
                 cursor_next(p, unit, nc);
                 load_q(nc);
@@ -540,7 +557,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
         }
         landed(stage, 0, phase);
         const int w0i = cc.tile * kTileKeys + warp * kWarpKeys;
-        const bool more = issued < units, work = w0i < cc.keys;
+        const bool more = pu < u1, work = w0i < cc.keys;
         unsigned char *ks = ring + (warp * S + stage) * C::kStageBytes, *vs = ks + C::kHalfStage;
 
         // A warp past the segment's keys has no work in its last tile.
@@ -740,11 +757,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
         __syncwarp();
         if (more) {
             issue(stage, 1);
-            issued++;
-            if (issued < units) {
-                cursor_next(p, unit, pc);
-                look_up();
-            }
+            advance();
         } else if (unit == 1) {
             cp_async_commit();
         }
@@ -756,6 +769,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
         if (!ends) {
             cc.tile++;
             cc.left--;
+            u++;
             continue;
         }
 
@@ -827,7 +841,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
             odd |= !finite(ll[i]) || !finite(o[i].x) || !finite(o[i].y) || !finite(o[i].z) || !finite(o[i].w);
             if (odd) atomicOr(bad_s, 1 << r);
         }
-        if (u + 1 < u1) stage_q();
+        if (!last) stage_q();
         __syncthreads();
         if (const int bad = *bad_s) {
             // Plain f32 over the visible keys of the piece, a warp per row.
@@ -862,7 +876,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
         }
 
         // ---- the segment's result, or a piece of it for the merge.
-        const long long a0 = u - cc.tile, a1 = a0 + cc.tiles;  // the segment's units
+        const long long a0 = u - cc.tile, a1 = a0 + cc.tiles;  // the segment's tiles
         bool write = true;
         if (a0 < u0 || a1 > u1) {
             const int c_first = (int)(((a0 + 1) * grid - 1) / U), c_last = (int)((a1 * grid - 1) / U);
@@ -935,6 +949,7 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
         }
         fresh = true;
         cc = nc;
+        u += seg_end ? 2 : 1;
     }
     // After a wait that gave up, copies may still be in flight: let them land
     // before the CTA's shared memory is released.
