@@ -121,7 +121,9 @@ template <int kTile>
 __device__ __forceinline__ void seq_load(const PagedPass &p, int unit, int b, Cursor<kTile> &c) {
     c.b = b;
     if (p.prefix_pass) {
-        c.b = paged_sequence_of(p.a.batch, 0);  // the first with tokens: its table row
+        // The first with tokens: its table row. Mostly sequence 0: one read
+        // instead of a chain of them.
+        c.b = p.a.batch.starts[1] ? 0 : paged_sequence_of(p.a.batch, 0);
         c.tok0 = 0;
         c.ntok = (int)p.a.batch.starts[p.a.batch.seqs];
         c.past = p.a.prefix;
@@ -142,7 +144,7 @@ __device__ __forceinline__ void seq_load(const PagedPass &p, int unit, int b, Cu
         }
         c.keys = c.sink + c.past + c.ntok - c.low;
     }
-    c.tiles = (c.keys + kTile - 1) / kTile;
+    c.tiles = c.ntok > 0 ? (c.keys + kTile - 1) / kTile : 0;
 }
 template <int kTile>
 __device__ __forceinline__ long long seq_units(const PagedPass &p, const Cursor<kTile> &c) {

@@ -120,7 +120,9 @@ __device__ __forceinline__ int seq_count(const PagedPass &p) { return p.prefix_p
 __device__ __forceinline__ void seq_load(const PagedPass &p, int b, Cursor &c) {
     c.b = b;
     if (p.prefix_pass) {
-        c.b = paged_sequence_of(p.a.batch, 0);  // the first with tokens: its table row
+        // The first with tokens: its table row. Mostly sequence 0: one read
+        // instead of a chain of them.
+        c.b = p.a.batch.starts[1] ? 0 : paged_sequence_of(p.a.batch, 0);
         c.tok0 = 0;
         c.ntok = (int)p.a.batch.starts[p.a.batch.seqs];
         c.past = p.a.prefix;
@@ -434,7 +436,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     const int D = p.a.head_dim, H = p.a.heads, G = group_of(p);
 
     pdl_trigger();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == kM) {  // its warp has no part in the scan below
         for (int i = 0; i < S; i++) {
             mbar_init(&raw[i], unit > 1 ? 1 : kCopy);
             mbar_init(&full[i], C::kConv);
