@@ -39,11 +39,11 @@
 //
 // Bound: 4 * pairs * D flops take 4 (16-bit cache) or 6 (F32) passes of half as
 // many MMA flops each, 2048 or 3072 cycles a tile. Two prompts of 2048 tokens,
-// 32 heads of 128, window 4096 (254 GFLOP): f32 849 us (7000 cycles a tile:
-// conversion and the MMAs share the shared memory), bf16 693 us, f16 553 us
-// (4500 cycles: the softmax warps' chain of TMEM reads, exponentials and
-// splits; the tensor pipe is busy for 45 % of it). 128 sequences of 64 heads
-// over 32768 shared keys in f16: 240 us of a call of 315.
+// 32 heads of 128, window 4096 (254 GFLOP): f32 886 us (7300 cycles a tile:
+// conversion and the MMAs share the shared memory), bf16 755 us, f16 590 us
+// (4800 cycles: the softmax warps' chain of TMEM reads, exponentials and
+// splits; the tensor pipe is busy for 40 % of it). 128 sequences of 64 heads
+// over 32768 shared keys in f16: 245 us of a call of 322.
 #include <math.h>
 
 #include "common.cuh"
@@ -1044,11 +1044,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             // ---- MMA issue ----------------------------------------------------
             // The whole warp walks the loop and one elected lane issues. Inside
             // one lane's branch 16 MMAs took 1600 cycles to issue, 1024 to run;
-            // uniform control flow takes two prompts of 2048 tokens from 619
+            // uniform control flow took two prompts of 2048 tokens from 619
             // to 559 us over an f16 cache, from 896 to 868 us over f32. With
-            // all steps unrolled the code of the roles outgrows the
-            // instruction caches (676 and 1040 us); rolled up, f32 is at 849,
-            // bf16 at 693 instead of 724, f16 at 597.
+            // all steps unrolled the code of the roles outgrew the
+            // instruction caches (676 and 1040 us); rolled up, f32 took 849,
+            // bf16 693 instead of 724, f16 597.
+            // The small products of a tile come before all large ones: the
+            // tensor core cuts its sums off at the size of what they hold, and
+            // the order halves the error (1.0e-6 to 4.6e-7 of the outputs'
+            // norm over 1100 f32 keys, 7.2e-7 to 4.5e-7 f16) for 3 % of time.
             const uint32_t ra = smem_addr(ring);
             int seg = 0;
             auto slot_wait = [&](int j) {
@@ -1072,8 +1076,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                             const uint32_t at = qh + ks / 2 * 32 + ks % 2 * 8;
                             mma_ts(d, at + 16, kh + ks * 2, C::kIdescS, b + ks);
                             if (C::kPair) mma_ts(d, at, kh + ks * 2 + C::kHalfBytes / 16, C::kIdescS, 1u);
-                            mma_ts(d, at, kh + ks * 2, C::kIdescS, 1u);
                         }
+                    }
+#pragma unroll 1
+                    for (int b = 0; b < C::kBlocks; b++) {
+                        const uint64_t kh = desc + b * (C::kBlockBytes / 16);
+                        const uint32_t qh = q_tm + b * 64;
+#pragma unroll(C::kRaw ? 4 : 1)
+                        for (int ks = 0; ks < 4; ks++)
+                            mma_ts(d, qh + ks / 2 * 32 + ks % 2 * 8, kh + ks * 2, C::kIdescS, 1u);
                     }
                     commit_one(&empty[j % S]);
                     commit_one(&s_full[n & 1]);
@@ -1097,8 +1108,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                             mma_ts(o_tm, ph + ks * 8 + 16, vh + ks * 128, C::kIdescO, b + ks);
                             if (C::kPair)
                                 mma_ts(o_tm, ph + ks * 8, vh + ks * 128 + C::kHalfBytes / 16, C::kIdescO, 1u);
-                            mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
                         }
+                    }
+#pragma unroll 1
+                    for (int b = 0; b < kKeys / 32; b++) {
+                        const uint64_t vh = desc + b * (2 * 2048 / 16);
+                        const uint32_t ph = pt + b * 32;
+#pragma unroll(C::kRaw ? 2 : 1)
+                        for (int ks = 0; ks < 2; ks++) mma_ts(o_tm, ph + ks * 8, vh + ks * 128, C::kIdescO, 1u);
                     }
                     commit_one(&empty[j % S]);
                     commit_one(o_full);
