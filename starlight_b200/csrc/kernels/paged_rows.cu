@@ -21,9 +21,9 @@
 //          per row, each half of the keys)
 //   4..7   output: one thread per row; O += P V of each tile in registers,
 //          the result, or this CTA's piece of a split segment
-//   8..15  (16-bit caches: 12..15) conversion in place: scale, f16 or f16 pair, zeros in rows that no
-//          query sees (they may hold anything). The scale is that of the
-//          operand before; a tile whose largest value does not suit it is
+//   8..15  (16-bit caches: 12..15) conversion in place: scale, f16 or f16
+//          pair, zeros in rows that no query sees (they may hold anything).
+//          The scale is that of the operand before; a tile whose largest value does not suit it is
 //          read from the cache once more (a pass over each tile for its
 //          maximum would cost a quarter of the shared memory's bandwidth,
 //          which is what bounds an F32 cache).
@@ -38,8 +38,8 @@
 // swizzle). TMEM: Q, two S / P buffers and O, 128 columns each.
 //
 // Bound: 4 * pairs * D flops take 4 (16-bit cache) or 6 (F32) passes of half as
-// many MMA flops each, 2048 or 3072 cycles a tile. Two prompts of 2048 tokens,
-// 32 heads of 128, window 4096 (254 GFLOP): f32 886 us (7300 cycles a tile:
+// many MMA flops each: 2048 cycles a tile, 3/2 of that for F32. Two prompts of
+// 2048 tokens, 32 heads of 128, window 4096 (254 GFLOP): f32 886 us (7300 cycles a tile:
 // conversion and the MMAs share the shared memory), bf16 755 us, f16 590 us
 // (4800 cycles: the softmax warps' chain of TMEM reads, exponentials and
 // splits; the tensor pipe is busy for 40 % of it). 128 sequences of 64 heads
