@@ -50,7 +50,7 @@
 // split of an infinity is NaN).
 //
 // Bound by HBM over long sequences: 64 of 300 to 16000 keys in bf16 (1.97 GB)
-// 329 us, 6.0 TB/s; 8 of 1000 to 8000 in f32 (282 MB) 55 us, 5.1 TB/s; heads
+// 347 us, 5.7 TB/s; 8 of 1000 to 8000 in f32 (282 MB) 57 us, 4.9 TB/s; heads
 // of 64 f32, 64 sequences (1.09 GB), 182 us, 6.0 TB/s. Short segments are
 // bound by latency: with 8 warps an SM three of four issue slots are empty, a
 // segment's start and end (queries, merge, result) cost about 5000 cycles and
@@ -1005,15 +1005,15 @@ cudaError_t launch_type(cudaStream_t s, const PagedPass &p) {
 // Query rows of one kv head up to which a sequence is paged_attention_kernel's,
 // which reads the keys once per kRows of them; more are paged_rows.cu's.
 // Measured, 16 sequences of 1000 to 4000 keys, 8 kv heads of 128, with 16, 32
-// and 48 rows: f32 113, 174, 255 us here and 113, 122, 124 there; bf16 61, 92,
-// 130 and 92, 100, 101.
+// and 48 rows: f32 109, 168, 244 us here and 117, 124, 126 there; bf16 60, 90,
+// 128 and 100, 105, 107.
 int small_rows(const PagedAttention &a) { return a.cache.type == kPagedF32 ? 16 : 32; }
 // Where all keys that the call's shapes allow are few, tokens in all times keys
 // counted in blocks of kRows rows by a tile, it takes them whatever the rows:
 // paged_rows.cu has 20 us to start up and end. 1 sequence of 38 tokens over 160
-// keys (76 units) 7.5 us here and 33 there, of 128 new tokens in f32 (512)
-// 17.9 and 31, of 20 over 1000 (640) 21.9 and 25.7, of 64 over 1000 (2304) 41
-// and 28. Known from the shapes alone, so that a call gives the same results
+// keys (76 units) 7.1 us here and 29 there, of 128 new tokens in f32 (512) 18
+// and 28, of 20 over 1000 (640) 21.5 and 21.0, of 64 over 1000 (2304) 41 and
+// 24. Known from the shapes alone, so that a call gives the same results
 // captured and not.
 constexpr size_t kFewUnits = 1024;
 bool many_rows(const PagedAttention &a, size_t new_tokens, size_t runs, size_t keys) {
@@ -1035,13 +1035,13 @@ size_t part_floats(const PagedAttention &a) {
 }
 
 // A pass over the shared prefix saves the others' reads of it (from L2, mostly)
-// and costs launches and the merge, 7 to 25 us: it is taken where those reads
+// and costs launches and the merge, 4 to 15 us: it is taken where those reads
 // are kPrefixPass bytes or more. Measured, with the pass and without: 64
-// sequences of 8 kv heads of 128 bf16, prefix 256 (67 MB) 60 and 41 us, 512
-// 54 and 48, 1024 (268 MB) 56 and 65, 8192 78 and 301; 8 sequences, 2048
-// (67 MB) 23 and 22, 4096 28 and 31; 64 sequences of 4 kv heads of 64 f32,
-// 777 (102 MB) 38 and 41; 6 of them (10 MB) 16.4 and 15.3. Without it the rows
-// read the pages by their own table rows, which are the same.
+// sequences of 8 kv heads of 128 bf16, prefix 256 (67 MB) 35 and 32 us, 512
+// (134 MB) 44 and 43, 1024 49 and 61, 8192 72 and 311; 8 sequences, 1024 (34
+// MB) 18 and 16, 2048 (67 MB) 19 and 21, 4096 24 and 28; 64 sequences of 4 kv
+// heads of 64 f32, 777 (102 MB) 28 and 33; 6 of them (10 MB) 18 and 10. Without
+// it the rows read the pages by their own table rows, which are the same.
 constexpr size_t kPrefixPass = (size_t)96 << 20;
 size_t prefix_bytes(const PagedAttention &a) {
     const size_t row = (size_t)2 * a.kv_heads * a.head_dim * (a.cache.type == kPagedF32 ? 4 : 2);
