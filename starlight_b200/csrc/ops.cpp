@@ -298,6 +298,8 @@ bool paged_ports(Checker &ck, uint64_t first, uint64_t tokens, Paged *o) {
         return false;
     }
     if (st[3] == 0) return no("paged state needs a nonzero page size");
+    // By itself: a table of no pages bounds no product with it.
+    if (st[3] > INT32_MAX) return no("paged state pages exceed 2^31 - 1 positions");
     char *base = ck.d->buffers[sr.buffer].ptr + sr.offset * 4;
     if (!k::paged_aligned(base)) {
         ck.fail(SLC_ERR_UNIMPLEMENTED, "paged state must start on a 16-byte boundary");

@@ -338,3 +338,14 @@ def test_sizes_past_32_bits_are_refused(dev):
     c.batch = [np.zeros((1, 70000), np.uint32), np.zeros(1, np.uint32), np.array([0, 1], np.uint32)]
     c.state = Value(DType.F32, (1, 2, 2, 65536, 2, 64), ValueRole.State)
     c.refused("exceeds 2\\^31")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [1 << 31, (1 << 31) + 1, (1 << 32) - 1])
+def test_page_sizes_past_31_bits_are_refused(dev, kind, page):
+    # A table without pages does not bound the page by their product.
+    c = Call(dev, kind, batch=Batch([(0, 0), (0, 0)], width=0))
+    c.state = Value(DType.F32, (0, 2, 2, page, 2, 64), ValueRole.State)
+    c.refused("exceed 2\\^31 - 1 positions")
+    c.state = Value(DType.F32, (0, 2, 2, (1 << 31) - 1, 2, 64), ValueRole.State)
+    c()
