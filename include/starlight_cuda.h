@@ -184,9 +184,10 @@ typedef enum {
      *
      * PREFIX_ATTENTION: PAGED_ATTENTION without a window, for sequences whose
      * first `prefix` positions are the same pages of the cache; these are read
-     * once for all of them (by each, where that is quicker). Scalars max_new, prefix; prefix at most every
-     * past, and the table's rows begin with the same ceil(prefix / page)
-     * entries. */
+     * once for all of them (by each, where that is quicker, or where the
+     * device's workspace does not hold a result of head_dim + 2 floats for
+     * every row and head). Scalars max_new, prefix; prefix at most every past,
+     * and the table's rows begin with the same ceil(prefix / page) entries. */
     SLC_OP_EXT_PAGED_APPEND = 0x8003,
     SLC_OP_EXT_PAGED_ATTENTION = 0x8004,
     SLC_OP_EXT_PREFIX_ATTENTION = 0x8005

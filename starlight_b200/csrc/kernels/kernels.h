@@ -149,7 +149,7 @@ struct PagedAttention {
     unsigned *tickets;  // zeroed, reset by the kernels
     uint32_t *err;
 };
-size_t paged_attention_workspace_bytes(const PagedAttention &a);
+size_t paged_attention_workspace_bytes(const PagedAttention &a);  // given a.workspace_bytes
 constexpr size_t kPagedTickets = 1024;  // tickets used at most
 cudaError_t paged_attention(cudaStream_t s, const PagedAttention &a);
 

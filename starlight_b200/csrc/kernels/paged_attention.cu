@@ -1047,17 +1047,27 @@ size_t prefix_bytes(const PagedAttention &a) {
     const size_t row = (size_t)2 * a.kv_heads * a.head_dim * (a.cache.type == kPagedF32 ? 4 : 2);
     return (size_t)a.batch.seqs * a.prefix * row;
 }
+// The call without its prefix where there is no pass over it: for the reads
+// that it saves, or because the workspace does not hold its results, one row
+// of head_dim + 2 floats for every query row (prompts, whose passes are bound
+// by the products in either case).
+PagedAttention as_run(const PagedAttention &call) {
+    PagedAttention a = call;
+    if (prefix_bytes(a) < kPrefixPass || (part_floats(a) + prefix_floats(a)) * sizeof(float) > a.workspace_bytes)
+        a.prefix = 0;
+    return a;
+}
 
 }  // namespace
 
-size_t paged_attention_workspace_bytes(const PagedAttention &a) {
+size_t paged_attention_workspace_bytes(const PagedAttention &call) {
+    const PagedAttention a = as_run(call);
     return (part_floats(a) + prefix_floats(a)) * sizeof(float);
 }
 
 cudaError_t paged_attention(cudaStream_t s, const PagedAttention &call) {
-    PagedAttention a = call;
-    if (a.tokens == 0 || a.batch.seqs == 0) return cudaSuccess;
-    if (prefix_bytes(a) < kPrefixPass) a.prefix = 0;
+    if (call.tokens == 0 || call.batch.seqs == 0) return cudaSuccess;
+    const PagedAttention a = as_run(call);
     if (paged_attention_workspace_bytes(a) > a.workspace_bytes) return cudaErrorMemoryAllocation;
     PagedPass p{};
     p.a = a;

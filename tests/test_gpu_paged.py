@@ -436,6 +436,54 @@ def test_prefix_pass_with_values_that_are_not_finite(dev, value, case):
     assert not np.any(np.isfinite(attend(dev, b)))
 
 
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_prefix_whose_pass_does_not_fit_the_workspace(dev, dtype):
+    b = pass_batch(PASSES[6], dtype, seed=6)
+    # Room for the pieces of split segments (19.7 MB) and 0.9 MB; the pass would leave 1.6 MB of results.
+    small = CudaDevice(0, workspace_bytes=2 * (2 * 148 * 128 * 130 * 4 + (9 << 17)))
+    try:
+        start = small.launch_count()
+        got = attend(small, b)
+        without = small.launch_count() - start
+        check(got, b)
+    finally:
+        small.close()
+    refs, start = upload(dev, b), dev.launch_count()
+    check(attend(dev, b, refs=refs), b)
+    assert dev.launch_count() - start > without
+    b.prefix = 0
+    assert np.array_equal(attend(dev, b, refs=refs), got)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_prompts_under_one_prefix(dev, dtype):
+    # Their results do not fit the workspace: the rows read the prefix themselves.
+    b = Batch([(512, 1)] * 4, prefix=512, heads=32, kv_heads=8, dim=128, page=16, layers=1, layer=0, dtype=dtype)
+    new, width = 2048, (512 + 2048) // 16
+    own = 32 + np.arange(4 * 128).reshape(4, 128)
+    b.table = np.concatenate([np.tile(np.arange(32), (4, 1)), own], 1).astype(np.uint32)
+    b.lens, b.tokens, b.pages = [(512, new)] * 4, 4 * new, 32 + 4 * 128
+    b.starts, b.shape = np.arange(5, dtype=np.uint32) * new, (b.pages, 1, 2, 16, 8, 128)
+    assert b.table.shape == (4, width)
+    r = np.random.RandomState(1)
+    b.stored, b.words = to_bits(r.standard_normal(b.shape).astype(np.float32), dtype)
+    b.q = r.standard_normal((b.tokens, 32 * 128)).astype(np.float32)
+    refs = upload(dev, b)
+    got = attend(dev, b, refs=refs)
+    b.prefix = 0
+    assert np.array_equal(got, attend(dev, b, refs=refs))
+    # A few rows against the definition.
+    k, v = b.keys(2)
+    for t in (0, 1000, 2047):
+        for h in (0, 31):
+            kk, vv = k[:513 + t, h // 4], v[:513 + t, h // 4]
+            s = kk @ b.q[2 * new + t, 128 * h:128 * h + 128].astype(np.float64) / math.sqrt(128)
+            w = np.exp(s - s.max())
+            ds = 9 * 2.0 ** -20 / math.sqrt(128) * (np.abs(kk) @ np.abs(b.q[2 * new + t, 128 * h:128 * h + 128])).max()
+            tol = (w / w.sum()) @ np.abs(vv) * (2 * ds + (8 + len(kk) / 64) * 2.0 ** -20)
+            assert np.all(np.abs(got[2 * new + t, 128 * h:128 * h + 128] - (w / w.sum()) @ vv) <= tol)
+
+
 def test_prefix_of_zero(dev):
     b = Batch([(20, 1), (3, 2)], heads=4, kv_heads=2, dim=64)
     refs = upload(dev, b)

@@ -349,3 +349,19 @@ def test_page_sizes_past_31_bits_are_refused(dev, kind, page):
     c.refused("exceed 2\\^31 - 1 positions")
     c.state = Value(DType.F32, (0, 2, 2, (1 << 31) - 1, 2, 64), ValueRole.State)
     c()
+
+
+@pytest.mark.parametrize("dtype", [DType.F32, DType.BF16])
+@pytest.mark.parametrize("heads", [32, 64])
+@pytest.mark.parametrize("seqs,new,prefix", [(4, 2048, 512), (8, 1024, 512), (7, 1000, 512), (8, 1024, 64),
+                                             (16, 4096, 20000), (1, 1, 16), (64, 1, 8192)])
+def test_prefix_takes_what_attention_takes(dev, seqs, new, prefix, heads, dtype):
+    # Prompts under one prefix: their rows' results do not all fit the workspace.
+    b = Batch([], heads=heads, kv_heads=8, dim=128, layers=1, layer=0, dtype=dtype)
+    b.lens = [(prefix, new)] * seqs
+    width = -(-(prefix + new) // b.page)
+    b.table = np.tile(np.arange(width, dtype=np.uint32), (seqs, 1))
+    b.past, b.starts = np.full(seqs, prefix, np.uint32), np.arange(seqs + 1, dtype=np.uint32) * new
+    b.tokens, b.pages, b.shape, b.prefix = seqs * new, width, (width, *b.shape[1:]), prefix
+    Call(dev, "attend", batch=b)()
+    Call(dev, "prefix", batch=b)()
