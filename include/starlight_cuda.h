@@ -155,7 +155,9 @@ typedef enum {
      * layout with a page of `page` positions in the place of a sequence; dtype
      * F32, F16 or BF16. It lives in an F32 buffer; a 16-bit state's BufferRef
      * counts 32-bit words (two elements each). Its offset is a multiple of 4
-     * words (16 bytes). head_dim is a multiple of 8, at most 256.
+     * words (16 bytes). head_dim is a multiple of 8, at most 256; heads and
+     * kv_heads at most 65536; a sequence's positions, the tokens and their query
+     * rows of one kv head at most 2^31 - 8192.
      *
      * Batch: three U32 inputs describe any number of sequences of any lengths.
      * table [sequences, n]: the pages of each sequence, in order (entry j holds

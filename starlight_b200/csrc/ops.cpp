@@ -269,6 +269,11 @@ struct Paged {
     const uint32_t *table = nullptr, *past = nullptr, *starts = nullptr;  // host copies
 };
 
+// Positions, tokens and query rows of a kv head end below it: the kernels count
+// them in 32 bits, in tiles of up to 256 and in steps of a grid (4736 tokens).
+constexpr uint64_t kPagedMost = (1ull << 31) - 8192;
+constexpr uint64_t kPagedMaxHeads = 1u << 16;
+
 bool paged_ports(Checker &ck, uint64_t first, uint64_t tokens, Paged *o) {
     const slc_op &op = *ck.c.op;
     auto no = [&](const char *msg) {
@@ -308,6 +313,11 @@ bool paged_ports(Checker &ck, uint64_t first, uint64_t tokens, Paged *o) {
     if (t[1] * st[3] > INT32_MAX || st[0] > INT32_MAX || t[0] > INT32_MAX || tokens > INT32_MAX ||
         t[1] > INT32_MAX)
         return no("paged batch exceeds 2^31 - 1 positions, pages, sequences or tokens");
+    if (tokens > kPagedMost) return no("paged batch exceeds 2^31 - 8192 tokens");
+    if (hkv > kPagedMaxHeads) {
+        ck.fail(SLC_ERR_UNIMPLEMENTED, "paged operators support 65536 heads");
+        return false;
+    }
     const long long size = sv.dtype == SLC_F32 ? 4 : 2;
     o->cache.type = sv.dtype == SLC_F32 ? k::kPagedF32 : sv.dtype == SLC_F16 ? k::kPagedF16 : k::kPagedBf16;
     o->cache.row_stride = (long long)(hkv * hd) * size;
@@ -352,6 +362,7 @@ bool paged_contents(Checker &ck, const Paged &g, uint64_t window, uint64_t sinks
         if (n == 0) continue;
         if (g.starts[b + 1] > g.tokens) return no("paged batch starts exceed the token rows");
         if (end > width * g.page) return no("past + new tokens exceed the table's pages");
+        if (end > kPagedMost) return no("paged batch exceeds 2^31 - 8192 positions");
         uint64_t low = 0, sink = 0;
         if (window) {
             low = past + 1 > window ? past + 1 - window : 0;
@@ -827,7 +838,9 @@ int run_op(slc_device *d, const Cmd &c, bool launch) {
         REQUIRE(paged_ports(ck, 1, tokens, &g));
         if (heads == 0) return ck.exec("heads must be nonzero");
         if (heads % kvh != 0) return ck.exec("heads must be a multiple of kv_heads");
-        if (heads > (1u << 16)) return ck.fail(SLC_ERR_UNIMPLEMENTED, "paged attention supports 65536 heads");
+        if (heads > kPagedMaxHeads) return ck.fail(SLC_ERR_UNIMPLEMENTED, "paged attention supports 65536 heads");
+        if (tokens * (heads / kvh) > kPagedMost)
+            return ck.exec("paged attention exceeds 2^31 - 8192 query rows of one kv head");
         REQUIRE(paged_contents(ck, g, window, sinks));
         const uint64_t width_pages = (uint64_t)g.batch.per_seq;
         const uint64_t shared_pages = (prefix + g.page - 1) / g.page;

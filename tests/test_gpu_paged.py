@@ -280,6 +280,19 @@ def test_offsets_past_32_bits(dev):
     dev.release(buf)
 
 
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new", [1, 40])
+def test_positions_near_31_bits(dev, new, dtype):
+    b = Batch([(4090, new)], heads=8, kv_heads=2, dim=64, page=4096, layers=1, layer=0, dtype=dtype)
+    want, tol = b.attention(0.125, 100)
+    pages = (1 << 19) - 4
+    table = np.full((1, pages + 2), HOLE, np.uint32)
+    table[0, pages:] = b.table[0, :2]
+    b.table, b.past = table, b.past + np.uint32(4096 * pages)
+    got = attend(dev, b, scale=0.125, window=100)
+    assert np.all(np.abs(got - want) <= tol)
+
+
 # ------------------------------------------------- values out of the ordinary
 
 def put_values(b, places):

@@ -365,3 +365,41 @@ def test_prefix_takes_what_attention_takes(dev, seqs, new, prefix, heads, dtype)
     b.tokens, b.pages, b.shape, b.prefix = seqs * new, width, (width, *b.shape[1:]), prefix
     Call(dev, "attend", batch=b)()
     Call(dev, "prefix", batch=b)()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_counts_near_31_bits_are_refused(dev, kind):
+    # The kernels round positions, tokens and rows up to tiles and steps in 32 bits.
+    most = (1 << 31) - 8192
+    width = (1 << 31) // 4096 - 1
+    b = Batch([], heads=1, kv_heads=1, dim=8, page=4096, layers=1, layer=0)
+    b.lens, b.tokens, b.pages, b.shape = [(most - 1, 1)], 1, width, (width, 1, 2, 4096, 1, 8)
+    b.table = np.arange(width, dtype=np.uint32)[None]
+    b.past, b.starts = np.array([most - 1], np.uint32), np.array([0, 1], np.uint32)
+    Call(dev, kind, batch=b)()
+    b.past[0] += 1
+    Call(dev, kind, batch=b).refused("exceeds 2\\^31 - 8192 positions")
+    b = Batch([(5, 1)], heads=1, kv_heads=1, dim=8)
+    c = Call(dev, kind, batch=b)
+    c.rows = most
+    c()
+    c.rows = most + 1
+    c.refused("exceeds 2\\^31 - 8192 tokens")
+
+
+@pytest.mark.parametrize("kind", ["attend", "prefix"])
+def test_query_rows_near_31_bits_are_refused(dev, kind):
+    b = Batch([(5, 1)], heads=8, kv_heads=1, dim=8)
+    c = Call(dev, kind, batch=b)
+    c.rows = ((1 << 31) - 8192) // 8
+    c()
+    c.rows += 1
+    c.refused("exceeds 2\\^31 - 8192 query rows")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_kv_heads_past_16_bits_are_refused(dev, kind):
+    b = Batch([], heads=1 << 16, kv_heads=1 << 16, dim=8, page=1, layers=1, layer=0, extra_pages=1)
+    Call(dev, kind, batch=b)()
+    b = Batch([], heads=(1 << 16) + 1, kv_heads=(1 << 16) + 1, dim=8, page=1, layers=1, layer=0, extra_pages=1)
+    Call(dev, kind, batch=b).refused("support 65536 heads", Status.Unimplemented)
