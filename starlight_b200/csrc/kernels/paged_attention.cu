@@ -976,7 +976,8 @@ cudaError_t launch_pass(cudaStream_t s, const PagedPass &p) {
     using C = Cfg<T, DP>;
     static_assert(C::kStages >= 1 && C::kCtas * (C::kSmem + 1024) <= 228 * 1024, "shared layout");
     static std::atomic<uint64_t> smem_set{0};
-    set_smem_limit_once(paged_attention_kernel<T, DP>, C::kSmem, &smem_set);
+    const cudaError_t e = set_smem_limit_once(paged_attention_kernel<T, DP>, C::kSmem, &smem_set);
+    if (e != cudaSuccess) return e;
     PassArgs args{};
     args.pass = p;
     args.unit = paged_boxes(p.a, C::kWarpKeys, sizeof(T), std::is_same<T, __half>::value, true, &args.map);
