@@ -160,32 +160,72 @@ struct Frag<__half> {
 // One query row against the keys i in [k0, k1) for which pos(i) is not
 // negative, in plain f32, by one warp: for rows whose tiles hold values that
 // are not finite. o[y]: dimension lane + 32 y, unnormalised; m in log2 units.
+// A lane takes a key's score, the warp 32 keys' values with two or four of them
+// in flight: 90 cycles a key where one key at a time took 800. A score that is NaN
+// or +infinity makes the whole row NaN and ends it.
 template <typename T, int DP, typename Pos>
 __device__ __noinline__ void plain_row(const PagedPass &p, const float *q, int b, int kvh, int k0, int k1, Pos pos,
                                        float &m, float &l, float (&o)[DP / 32]) {
+    constexpr int kEpl = 16 / (int)sizeof(T), kFly = DP > 128 ? 2 : 4;
     const int lane = threadIdx.x & 31, D = p.a.head_dim;
     m = -INFINITY;
     l = 0.f;
 #pragma unroll
     for (int y = 0; y < DP / 32; y++) o[y] = 0.f;
-    for (int i = k0; i < k1; i++) {
-        const int at = pos(i);
-        if (at < 0) continue;
-        const char *src = p.a.cache.base + paged_row(p.a.cache, p.a.batch, b, at, p.a.err) +
-                          (long long)kvh * D * (int)sizeof(T);
-        float dot = 0.f;
-        for (int d = lane; d < D; d += 32) dot = fmaf(q[d], Frag<T>::get(src + d * sizeof(T)), dot);
-        const float x = warp_sum(dot) * p.scale_log2;
-        const float nm = fmaxf(m, x), f = m == -INFINITY ? 0.f : ex2(m - nm);
-        const float e = x == -INFINITY ? 0.f : ex2(x - nm);
-        l = m == -INFINITY ? l + e : fmaf(l, f, e);
+    for (int i0 = k0; i0 < k1; i0 += 32) {
+        const int at = i0 + lane < k1 ? pos(i0 + lane) : -1;
+        long long off = 0;
+        float x = -INFINITY;
+        if (at >= 0) {
+            off = paged_row(p.a.cache, p.a.batch, b, at, p.a.err) + (long long)kvh * D * (int)sizeof(T);
+            const char *src = p.a.cache.base + off;
+            float part[kEpl];
 #pragma unroll
-        for (int y = 0; y < DP / 32; y++) {
-            const int d = lane + 32 * y;
-            const float v = d < D ? Frag<T>::get(src + p.a.cache.parity_stride + d * sizeof(T)) : 0.f;
-            o[y] = fmaf(e, v, m == -INFINITY ? o[y] : o[y] * f);
+            for (int e = 0; e < kEpl; e++) part[e] = 0.f;
+#pragma unroll 2
+            for (int d = 0; d < D; d += kEpl) {
+                float kv[kEpl];
+                Frag<T>::ld(src + d * (int)sizeof(T), kv);
+#pragma unroll
+                for (int e = 0; e < kEpl; e++) part[e] = fmaf(q[d + e], kv[e], part[e]);
+            }
+#pragma unroll
+            for (int w = kEpl / 2; w; w /= 2)
+#pragma unroll
+                for (int e = 0; e < w; e++) part[e] += part[e + w];
+            x = part[0] * p.scale_log2;
         }
+        if (__any_sync(0xffffffffu, !(x < INFINITY))) {
+            l = __int_as_float(0x7fffffff);
+#pragma unroll
+            for (int y = 0; y < DP / 32; y++) o[y] = l;
+            return;
+        }
+        const float nm = fmaxf(m, warp_max(x)), mu = nm == -INFINITY ? 0.f : nm;
+        const float f = ex2(m - mu), e = ex2(x - mu);
+        l = fmaf(l, f, warp_sum(e));
         m = nm;
+#pragma unroll
+        for (int y = 0; y < DP / 32; y++) o[y] *= f;
+        const unsigned seen = __ballot_sync(0xffffffffu, at >= 0);
+        for (int j0 = 0; j0 < 32; j0 += kFly) {
+            float ej[kFly], v[kFly][DP / 32];
+#pragma unroll
+            for (int j = 0; j < kFly; j++) {
+                const bool live = (seen >> (j0 + j)) & 1;
+                ej[j] = __shfl_sync(0xffffffffu, e, j0 + j);
+                const char *src = p.a.cache.base + p.a.cache.parity_stride + __shfl_sync(0xffffffffu, off, j0 + j);
+#pragma unroll
+                for (int y = 0; y < DP / 32; y++) {
+                    const int d = lane + 32 * y;
+                    v[j][y] = live && d < D ? Frag<T>::get(src + d * (int)sizeof(T)) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kFly; j++)
+#pragma unroll
+                for (int y = 0; y < DP / 32; y++) o[y] = fmaf(ej[j], v[j][y], o[y]);
+        }
     }
 }
 

@@ -20,6 +20,7 @@ whose smallest step is 2^-34 of a tile's largest key or value and 2^-39 of the
 query's largest element: as much again, rounded up to 2^-33, times the largest
 value, and times what multiplies it in a score."""
 import math
+import time
 
 import numpy as np
 import pytest
@@ -322,6 +323,40 @@ def test_keys_and_values_that_a_row_does_not_see(dev, value, dtype, heads, new):
     want, tol = b.attention(0.125, 44)
     assert np.all(np.abs(got[4:] - want[4:]) <= tol[4:])
     assert not np.any(np.isfinite(got[:4]))
+
+
+def seconds(dev, b, calls=3):
+    """The shortest of a few calls over the batch, with its upload left out."""
+    tables, cache = upload(dev, b)
+    x = Value.f32((b.tokens, b.heads * b.dim))
+    q, out = put_f32(dev, b.q), new_f32(dev, b.q.size)
+    cmd = dev.command(b.op(OpCode.PagedAttention, scale=b.dim ** -0.5), [q, *tables, cache],
+                      [x, *b.described(), b.state()], [out], [x], [b.max_new(), 0, 0])
+    took = []
+    for _ in range(calls):
+        dev.synchronize()
+        start = time.perf_counter()
+        cmd()
+        dev.synchronize()
+        took.append(time.perf_counter() - start)
+    got = get(dev, out).reshape(b.tokens, -1)
+    for ref in (*tables, cache, q, out):
+        dev.release(ref.buffer)
+    return min(took), got
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("parity,value,most", [(0, np.nan, 10), (0, np.inf, 10), (1, np.inf, 100)])
+def test_what_a_value_that_is_not_finite_costs_few_rows(dev, parity, value, most, dtype):
+    # One early position of every sequence. A NaN score ends its row (1.2 times
+    # the time of the clean call measured); a value's rows are done again in
+    # plain f32 (25 to 50 times).
+    b = Batch([(3000, 1)] * 32, heads=32, kv_heads=8, dim=128, page=16, layers=1, layer=0, dtype=dtype)
+    clean, _ = seconds(dev, b)
+    put_values(b, [(s, 5, parity, value) for s in range(32)])
+    hurt, got = seconds(dev, b)
+    assert not np.any(np.isfinite(got))
+    assert hurt < most * clean, (hurt, clean)
 
 
 @pytest.mark.parametrize("new", [1, 70])
