@@ -182,7 +182,12 @@ typedef enum {
      * sequence: it selects kernels), window, sinks. The token at position t
      * attends, through each head, to the positions p <= t, where window is not
      * 0 only to those with p > t - window or p < sinks. Its own key must have
-     * been appended. Output of q's shape.
+     * been appended. Output of q's shape. Where a kv head has more than
+     * some rows of a sequence (16 with an F32 state, 32 with a 16-bit one), an
+     * element of an F32 state counts to 2^-22 of itself, or a key's to 2^-28 of
+     * that key's largest element and a value's to 2^-26 of the largest of its
+     * dim among up to 128 neighbouring positions (BF16: exactly, or to the
+     * latter two); other states and rows have no such floor.
      *
      * PREFIX_ATTENTION: PAGED_ATTENTION without a window, for sequences whose
      * first `prefix` positions are the same pages of the cache; these are read

@@ -4,15 +4,19 @@
 // query rows, kv head), a tile 128 keys, and the products run on tcgen05.
 //
 // Arithmetic. kind::f16 with f32 accumulators on pairs of f16: x = hi + lo
-// keeps 22 bits, and f16's denormals keep what is below 2^-25, given scales
-// (powers of two, exact) that bring the largest value of a query row to
-// [2^14, 2^15) and of a key or value tile to [2^9, 2^15): the smallest step is
-// 2^-39 of a row's largest value, 2^-34 of a tile's. Probabilities are taken
-// 2^14 times as large for the same reason. An F32 cache needs three products
-// (lo hi, hi lo, hi hi) for S = Q K^T and for P V; F16 values are taken as
-// they are and BF16 values are one f16 each, two products. Every tile's P V
-// starts from zero and is added in f32 registers (TMEM accumulation over
-// thousands of keys would truncate thousands of times).
+// keeps 22 bits, down to a step of 2^-24 where f16 ends, given scales (powers
+// of two, exact): of a query row, whose largest value comes to [2^14, 2^15); of
+// a key, whose largest comes to [2^3, 2^15); of a value channel (a dim) in a
+// tile, whose largest comes to [2, 2^15). So an element is off by at most 2^-22
+// of itself or 2^-39 of the row's, 2^-28 of the key's, 2^-26 of the channel's
+// largest. Probabilities are taken 2^14 times as large for the same reason.
+// Keys share a scale within a tile and channels keep theirs from tile to tile
+// as long as those ranges hold, so most tiles are converted once, with scales
+// known beforehand, and the output is held in units of the channels' scales. An
+// F32 cache needs three products (lo hi, hi lo, hi hi) for S = Q K^T and for
+// P V; F16 values are taken as they are and BF16 values are one f16 each, two
+// products. Every tile's P V starts from zero and is added in f32 registers
+// (TMEM accumulation over thousands of keys would truncate thousands of times).
 //
 // One CTA per SM, 20 warps:
 //   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
@@ -23,10 +27,10 @@
 //          the result, or this CTA's piece of a split segment
 //   8..15  (16-bit caches: 12..15) conversion in place: scale, f16 or f16
 //          pair, zeros in rows that no query sees (they may hold anything).
-//          The scale is that of the operand before; a tile whose largest value does not suit it is
-//          read from the cache once more (a pass over each tile for its
-//          maximum would cost a quarter of the shared memory's bandwidth,
-//          which is what bounds an F32 cache).
+//          Keys or values that the scales at hand do not suit are read from the
+//          cache once more (a pass over each tile for its maxima would cost a
+//          quarter of the shared memory's bandwidth, which is what bounds an
+//          F32 cache).
 //   16     issues the MMAs: Q K^T of the next tile before P V of this one
 //   17     copies: TMA boxes of 8 to 128 keys of a page and 128 bytes into a
 //          ring of slots (pages that are not a multiple of 8 keys: 16-byte
@@ -61,7 +65,10 @@ constexpr int kKeys = 128;  // keys per tile
 constexpr int kCopy = 3;    // copying warps where TMA boxes do not fit the pages
 constexpr int kThreads = 20 * 32;
 constexpr int kShift = 14;  // a query row's largest value in [2^14, 2^15), probabilities up to 2^14
-constexpr int kTop = 11;    // a tile's largest value around 2^11: from 2^9 to 2^15
+constexpr int kTop = 11;    // a scale takes the largest value to 2^11 and serves from 2^1 to 2^15
+constexpr int kFirst = 2;   // exponent expected at first
+constexpr int kNear = 8;    // keys down to 2^-8 of the expected largest value share its scale
+constexpr int kDeep = 80;   // octaves that a channel's scale may fall within a segment
 constexpr int kLaunchRegs = 96;  // registers a thread at launch
 constexpr uint64_t kLimitNs = 20000000000ull;  // rows of values that are not finite take long
 template <typename T, int DP>
@@ -75,7 +82,7 @@ struct Cfg {
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
     static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (22 * kM + 4 * 8 + 8 + 8 * 12 + 4 * DP + 16) +
+    static constexpr int kSmall = 4 * (22 * kM + 8 * kKeys + 18 * DP + 80 + 8 * 12 + 4 * DP + 16) +
                                   8 * (3 * kKeys + 8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
@@ -301,6 +308,21 @@ __device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+// The same, and whether some thread passes true.
+__device__ __forceinline__ bool bar_or(int id, int threads, bool x) {
+    uint32_t any;
+    asm volatile(
+        "{\n"
+        ".reg .pred p, q;\n"
+        "setp.ne.u32 p, %3, 0;\n"
+        "barrier.red.or.pred q, %1, %2, p;\n"
+        "selp.u32 %0, 1, 0, q;\n"
+        "}\n"
+        : "=r"(any)
+        : "r"(id), "r"(threads), "r"((uint32_t)x)
+        : "memory");
+    return any != 0;
+}
 // (a, b) as an f16 pair, a low; and the value that it holds.
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
@@ -350,6 +372,155 @@ __device__ __forceinline__ void split2(F2 x, uint32_t &hi, uint32_t &lo) {
 // bytes, 16-byte chunks xored with the row.
 __device__ __forceinline__ uint32_t operand_at(int row, int dim) {
     return (uint32_t)((dim >> 6) * kKeys * 128 + row * 128 + ((((dim & 63) >> 3) ^ (row & 7)) << 4) + (dim & 7) * 2);
+}
+
+// Of a tile of keys: what takes its scale out of S; a byte for each conversion
+// warp, whether keys of its have scales of their own.
+struct KeyTile {
+    float scale;
+    uint32_t none;
+    unsigned char own[8];
+};
+// a / b of powers of two, from 2^-126 to 2^127.
+__device__ __forceinline__ float ratio2(float a, float b) {
+    return pow2(min(max((int)(__float_as_uint(a) >> 23) - (int)(__float_as_uint(b) >> 23), -126), 127));
+}
+
+// Cache values to operands: a conversion lane's 16 raw bytes at a time, of
+// row (i kConv + warp) kRpi + sub, from dim `col` on.
+template <typename T, int DP>
+struct Operand {
+    using C = Cfg<T, DP>;
+    static constexpr int kStep = C::kConv * C::kRpi * 128;
+    // To f16, or f16 pairs, with a scale for each element.
+    __device__ static __forceinline__ void convert(uint4 x, const F2 (&sc)[C::kEpl / 2], uint32_t dst) {
+        if constexpr (C::kPair) {
+            uint32_t h0, h1, l0, l1;
+            split2(mul2(F2(__uint_as_float(x.x), __uint_as_float(x.y)), sc[0]), h0, l0);
+            split2(mul2(F2(__uint_as_float(x.z), __uint_as_float(x.w)), sc[1]), h1, l1);
+            sts64(dst, h0, h1);
+            sts64(dst + C::kHalfBytes, l0, l1);
+        } else if constexpr (!C::kRaw) {
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            uint32_t h[4];
+#pragma unroll
+            for (int z = 0; z < 4; z++) {
+                const float2 f = mul2(F2(__uint_as_float(w[z] << 16), __uint_as_float(w[z] & 0xffff0000u)), sc[z]).get();
+                h[z] = pack_h2(f.x, f.y);
+            }
+            sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
+        }
+    }
+    // Magnitudes as bits, by word: one of f32 or two of 16 bits.
+    __device__ static __forceinline__ uint32_t size_of(uint32_t w) {
+        return w & (C::kPair ? 0x7fffffffu : 0x7fff7fffu);
+    }
+    __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+        return C::kPair ? max(a, b) : __vmaxu2(a, b);
+    }
+    // The largest magnitude of 16 bytes, as the bits of an f32.
+    __device__ static __forceinline__ uint32_t largest(uint4 x) {
+        const uint32_t t = larger(larger(size_of(x.x), size_of(x.y)), larger(size_of(x.z), size_of(x.w)));
+        return C::kPair ? t : max(t << 16, t & 0xffff0000u);
+    }
+    // The scale of an operand's channel, from what takes it out of the outputs.
+    __device__ static __forceinline__ float inverse(float x) { return ratio2(pow2(-kShift), x); }
+    // 16 bytes of the tile's keys or values from the cache; zeros where no row sees them.
+    __device__ static __forceinline__ uint4 fetch(const PagedPass &p, const Tile &cu, int row, int col, bool v) {
+        const int key = cu.i0 + row, pos = key < cu.sink ? key : key - cu.sink + cu.low, D = p.a.head_dim;
+        if (!live_key(p, cu, key) || col >= D) return make_uint4(0, 0, 0, 0);
+        return __ldcg(reinterpret_cast<const uint4 *>(
+            p.a.cache.base + paged_row(p.a.cache, p.a.batch, cu.b, pos, p.a.err) + (v ? p.a.cache.parity_stride : 0) +
+            (cu.kvh * D + col) * (long long)sizeof(T)));
+    }
+};
+
+// The rare ways of the conversion and of the softmax, behind branches marked as
+// unlikely: what is not executed costs as well, in instruction fetches.
+//
+// A conversion warp's keys from the cache again: those outside 2^-kNear to 2^3
+// of the expected largest value get a scale of their own, from their own.
+template <typename T, int DP>
+__device__ __forceinline__ void keys_again(const PagedPass &p, const Tile &cu, uint32_t to, int expect, float *rel,
+                                        int *poison) {
+    using C = Cfg<T, DP>;
+    using O = Operand<T, DP>;
+    const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) - C::kConvWarp;
+    const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+    for (int i = 0; i < C::kRows; i++) {
+        const int row = (i * C::kConv + pw) * C::kRpi + sub;
+        const uint4 x = O::fetch(p, cu, row, col, false);
+        uint32_t t = O::largest(x);
+        for (int o = 1; o < C::kLpr; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
+        if (t >= 0x7f800000u) *poison = 1;
+        int ex = t ? scale_exponent(t) : expect;
+        if (ex >= expect - kNear && ex <= expect + 3) ex = expect;
+        const float f = pow2(kTop - ex);
+        F2 sc[C::kEpl / 2];
+#pragma unroll
+        for (int e = 0; e < C::kEpl / 2; e++) sc[e] = F2(f, f);
+        O::convert(x, sc, to + i * O::kStep);
+        if (ch == 0) rel[row] = pow2(min(max(ex - expect, -126), 127));
+    }
+}
+// S's columns of keys with scales of their own.
+template <typename T, int DP>
+__device__ __forceinline__ void rescale_scores(uint32_t st, int first, const KeyTile *tile, const float *rel) {
+    using C = Cfg<T, DP>;
+    for (int i = first; i < first + kKeys / C::kSoft; i++)
+        if (tile->own[i / C::kRpi % C::kConv])
+            tmem_st1(st + i, __float_as_uint(__uint_as_float(tmem_ld1(st + i)) * rel[i]));
+    tmem_wait_st();
+}
+// All conversion warps' values of a tile from the cache again, with new scales
+// from the tile's own largest values. `now` takes them out of the outputs, as
+// `was` did. A scale falls by at most kDeep octaves within a segment, whose
+// outputs so far are held in units of it.
+template <typename T, int DP>
+__device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu, uint32_t to, uint32_t *most, int *high,
+                                          int *high_seg, const float *was, float *now, int *poison) {
+    using C = Cfg<T, DP>;
+    using O = Operand<T, DP>;
+    const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) - C::kConvWarp, ct = threadIdx.x - C::kConvWarp * 32;
+    const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+    uint32_t top[C::kEpl];
+#pragma unroll
+    for (int e = 0; e < C::kEpl; e++) top[e] = 0;
+    for (int i = 0; i < C::kRows; i++) {
+        const uint4 x = O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true);
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int e = 0; e < C::kEpl; e++) {
+            const uint32_t a = O::size_of(w[C::kPair ? e % 4 : e / 2 % 4]);
+            const uint32_t t = C::kPair ? a : e % 2 ? a & 0xffff0000u : a << 16;
+            if (t < 0x7f800000u)
+                top[e] = max(top[e], t);
+            else
+                *poison = 1;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < C::kEpl; e++) {
+        for (int o = C::kLpr; o < 32; o <<= 1) top[e] = max(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
+        if (sub == 0) most[pw * DP + col + e] = top[e];
+    }
+    bar_sync(1, C::kConv * 32);
+    if (ct < DP) {
+        uint32_t t = 0;
+        for (int w = 0; w < C::kConv; w++) t = max(t, most[w * DP + ct]);
+        const int before = (int)(__float_as_uint(was[ct]) >> 23) - 127 + kTop + kShift;
+        const int held = cu.begins ? -kDeep - 100 : *high_seg == cu.seg ? max(high[ct], before) : before;
+        const int ex = max(t ? scale_exponent(t) : before, held - kDeep);
+        now[ct] = pow2(ex - kTop - kShift);
+        high[ct] = max(ex, held);
+    }
+    bar_sync(1, C::kConv * 32);
+    if (ct == 0) *high_seg = cu.seg;
+    F2 sc[C::kEpl / 2];
+#pragma unroll
+    for (int e = 0; e < C::kEpl / 2; e++) sc[e] = F2(O::inverse(now[col + 2 * e]), O::inverse(now[col + 2 * e + 1]));
+    for (int i = 0; i < C::kRows; i++)
+        O::convert(O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true), sc, to + i * O::kStep);
 }
 
 // Where a row's result goes: (o f + prefix o e) / l to the output, or for a
@@ -412,10 +583,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     float *alpha = row_ml + 4 * kM * 2;                 // [4 tiles][kM]
     float *row_l2 = alpha + 4 * kM;                     // [4 tiles][kM] the second group's sums
     float *half_max = row_l2 + 4 * kM;                  // [2 groups][3][kM] tiles in turn, Q
-    float *k_scale = half_max + 6 * kM;                 // [8 tiles]
-    float *v_scale = k_scale + 8;                       // [8 tiles]
-    uint32_t *most = reinterpret_cast<uint32_t *>(v_scale + 8);   // [4 operands, 4 unused]
-    int *poison = reinterpret_cast<int *>(most + 8);    // [8 segments]
+    float *k_rel = half_max + 6 * kM;                   // [8 tiles][kKeys] keys' scales by their tile's
+    float *v_scale = k_rel + 8 * kKeys;                 // [8 changes][DP]
+    int *v_high = reinterpret_cast<int *>(v_scale + 8 * DP);      // [DP] largest exponents within the segment
+    uint32_t *v_most = reinterpret_cast<uint32_t *>(v_high + DP);  // [8 warps][DP] a tile's largest values
+    int *v_seg = reinterpret_cast<int *>(v_most + 8 * DP);  // the segment of v_high (4 words)
+    uint32_t *k_most = reinterpret_cast<uint32_t *>(v_seg + 4);  // [2][8 warps] keys' largest
+    int *v_change = reinterpret_cast<int *>(k_most + 16);  // [8 tiles] the channels' scales change here
+    KeyTile *key_tile = reinterpret_cast<KeyTile *>(v_change + 8);  // [8 tiles]
+    int *poison = reinterpret_cast<int *>(key_tile + 8);  // [8 segments]
     Tile *tiles = reinterpret_cast<Tile *>(poison + 8);           // [8 tiles]
     long long *row_off = reinterpret_cast<long long *>(tiles + 8);  // [3 tiles][kKeys]
     float *scratch = reinterpret_cast<float *>(row_off + 3 * kKeys);  // [4 warps][DP]
@@ -451,15 +627,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         mbar_init(o_empty, 4);
         mbar_init(done, 1);
         for (int i = 0; i < 8; i++) {
-            mbar_init(&k_sc[i], 1);
+            mbar_init(&k_sc[i], C::kConv);
             mbar_init(&v_sc[i], 1);
         }
         for (int i = 0; i < 4; i++) mbar_init(&a_full[i], 4 * C::kSoft);
         fence_mbar_init();
         *abort = 0;
-        for (int i = 0; i < 4; i++) most[i] = 0;
-        for (int i = 0; i < 8; i++) poison[i] = 0;
+        for (int i = 0; i < 8; i++) poison[i] = 0, key_tile[i] = KeyTile{};
+        *v_seg = -1;
     }
+    if (threadIdx.x >= kThreads - DP) v_scale[threadIdx.x - (kThreads - DP)] = pow2(kFirst - kTop - kShift);
     const Line line = line_scan(p, unit, sums);
     const long long U = line.total;
     const long long grid = min((long long)gridDim.x, U);
@@ -507,6 +684,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             bar_sync(4, 2 * kM);
             return fmaxf(x, half_max[(3 * (1 - group) + buffer) * kM + r]);
         };
+        // Queries are taken with the scale's sign; its size comes after the product.
+        const float sign = p.scale_log2 < 0.f ? -1.f : 1.f, size = fabsf(p.scale_log2);
         float m = -INFINITY, l = 0.f, qs = 1.f;
         int hi = 0, lo = 0;
         bool first = true;
@@ -538,10 +717,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                         for (int z = 0; z < 4; z++) {
                             const float4 f = v[4 * y + z];
-                            x[4 * z] = __float_as_uint(f.x * p.scale_log2);
-                            x[4 * z + 1] = __float_as_uint(f.y * p.scale_log2);
-                            x[4 * z + 2] = __float_as_uint(f.z * p.scale_log2);
-                            x[4 * z + 3] = __float_as_uint(f.w * p.scale_log2);
+                            x[4 * z] = __float_as_uint(f.x * sign);
+                            x[4 * z + 1] = __float_as_uint(f.y * sign);
+                            x[4 * z + 2] = __float_as_uint(f.z * sign);
+                            x[4 * z + 3] = __float_as_uint(f.w * sign);
                         }
 #pragma unroll
                         for (int z = 0; z < 16; z++) top = fmaxf(top, fabsf(__uint_as_float(x[z])));
@@ -581,15 +760,18 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 }
             }
             mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-            mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
+            if (!C::kRaw) mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
             tc_fence_after();
             const int i0 = c.tile * kKeys;
             // Rows past the tile's last hold zeros; they need no mask.
             const bool whole = i0 + kKeys <= hi && (i0 >= lo || i0 + kKeys <= p.a.sinks);
             const bool masked = __any_sync(0xffffffffu, !whole);
-            const float f = qs * k_scale[n & 7];
+            const uint4 kt = *reinterpret_cast<const uint4 *>(key_tile + (n & 7));
+            const float f = C::kRaw ? qs * size : qs * __uint_as_float(kt.x) * size;
             const uint32_t st = s_tm + (n & 1) * 128 + lane_tm;
             const int h_first = group * 2;
+            if (!C::kRaw && __builtin_expect((kt.z | kt.w) != 0, 0))
+                rescale_scores<T, DP>(st, 32 * h_first, key_tile + (n & 7), k_rel + (n & 7) * kKeys);
             // Both passes over the row, with the mask only where a row needs it.
             float nm, a;
             F2 sum2(0.f, 0.f);
@@ -646,10 +828,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             first = c.tile == c.tiles - 1;
             if (first || n == N - 1) {
                 if (group == 0) {
-                    row_ml[((n & 3) * kM + r) * 2] = m == -INFINITY ? m : m - (float)kShift;
-                    row_ml[((n & 3) * kM + r) * 2 + 1] = l;
+                    row_ml[((n & 3) * kM + r) * 2] = m;
+                    row_ml[((n & 3) * kM + r) * 2 + 1] = l * pow2(-kShift);
                 } else {
-                    row_l2[(n & 3) * kM + r] = l;
+                    row_l2[(n & 3) * kM + r] = l * pow2(-kShift);
                 }
             }
             tmem_wait_st();
@@ -666,8 +848,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::kOutRegs));
         const int r = threadIdx.x - 128, ow = warp - 4;
         const uint32_t lane_tm = (uint32_t)(ow * 32) << 16;
-        F2 acc[DP / 2];
-        int seg = 0, seg_n = 0;
+        F2 acc[DP / 2];  // in units of the channels' scales
+        int seg = 0, seg_n = 0, change = 0;
 #pragma unroll
         for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
         for (int n = 0; n < N; n++) {
@@ -675,7 +857,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
             mbar_wait(o_full, n & 1, p.a.err, abort, kLimitNs);
             tc_fence_after();
-            const float a = alpha[(n & 3) * kM + r], vs = v_scale[n & 7];
+            const float a = alpha[(n & 3) * kM + r];
+            if (!C::kRaw && __builtin_expect(v_change[n & 7], 0)) {
+                const float *was = v_scale + (change++ & 7) * DP, *now = v_scale + (change & 7) * DP;
+#pragma unroll
+                for (int d = 0; d < DP / 2; d++) {
+                    const float2 x = *reinterpret_cast<const float2 *>(was + 2 * d),
+                                 y = *reinterpret_cast<const float2 *>(now + 2 * d);
+                    acc[d] = mul2(acc[d], F2(ratio2(x.x, y.x), ratio2(x.y, y.y)));
+                }
+            }
             float m = row_ml[((n & 3) * kM + r) * 2], l = row_ml[((n & 3) * kM + r) * 2 + 1];
             if (C::kSoft == 2) l += row_l2[(n & 3) * kM + r];
             const uint32_t ot = o_tm + lane_tm;
@@ -686,7 +877,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     F2 &d = acc[8 * h + j];
-                    d = fma2(d, F2(a, a), mul2(F2(x[2 * j], x[2 * j + 1]), F2(vs, vs)));
+                    d = fma2(d, F2(a, a), F2(x[2 * j], x[2 * j + 1]));
                 }
             }
             tc_fence_before();
@@ -702,6 +893,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 const float2 x = acc[2 * d].get(), y = acc[2 * d + 1].get();
                 return make_float4(x.x, x.y, y.x, y.y);
             };
+            const float *vs = v_scale + (change & 7) * DP;
+#pragma unroll
+            for (int d = 0; d < DP / 2; d++) {
+                const float2 x = C::kRaw ? make_float2(pow2(-kShift), pow2(-kShift))
+                                         : *reinterpret_cast<const float2 *>(vs + 2 * d);
+                acc[d] = mul2(acc[d], F2(x.x, x.y));
+            }
             const bool bad_tiles = poison[seg & 7] != 0;
             bar_sync(2, 128);
             if (r == 0) poison[seg & 7] = 0;
@@ -804,16 +1002,21 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     } else if (warp < 16) {
         // ---- conversion ---------------------------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kConvRegs));
+        using O = Operand<T, DP>;
         const int pw = warp - C::kConvWarp;
         // Piece i of a lane: row (i kConv + pw) kRpi + sub, 16 raw bytes from
         // dim `col` on. A piece on is a multiple of 8 rows on.
         const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
-        constexpr int kBatch = 4, kStep = C::kConv * C::kRpi * 128;
+        constexpr int kBatch = C::kPair ? 4 : 2, kStep = C::kConv * C::kRpi * 128;
         static_assert(C::kRows % kBatch == 0 && C::kConv * C::kRpi % 8 == 0, "batches of pieces 8 rows apart");
         auto row_of = [&](int i) { return (i * C::kConv + pw) * C::kRpi + sub; };
         const uint32_t op0 = operand_at(row_of(0), col);
         const uint32_t raw0 = C::kPair ? (ch >> 3) * C::kBlockBytes + row_of(0) * 128 + (ch & 7) * 16 : op0;
-        int e_k = 2, e_v = 2;  // exponents of the scales of the operands before
+        int e_k = kFirst;    // exponent of the largest value expected of a tile's keys
+        F2 vs[C::kEpl / 2];  // this lane's channels' scales
+        int change = 0;      // of them
+#pragma unroll
+        for (int e = 0; e < C::kEpl / 2; e++) vs[e] = F2(pow2(kTop - kFirst), pow2(kTop - kFirst));
         for (int j = 0; j < total; j++) {
             const bool v = is_v(j);
             const int n = tile_of(j);
@@ -827,83 +1030,93 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 for (int i = 0; i < C::kRows; i++)
                     if (!live_key(p, cu, cu.i0 + row_of(i)))
                         *reinterpret_cast<uint4 *>(slot + raw0 + i * kStep) = make_uint4(0, 0, 0, 0);
-            int ex = kTop;  // the scale is 2^(kTop - ex)
-            if (!C::kRaw) {
-                const uint32_t at = smem_addr(slot);
-                ex = v ? e_v : e_k;
-                for (int again = 0; again < 2; again++) {
-                    const F2 sc(pow2(kTop - ex), pow2(kTop - ex));
-                    float top = 0.f;
+            const uint32_t to = smem_addr(slot) + op0;
+            if (!C::kRaw && !v) {
+                const float f = pow2(kTop - e_k);
+                F2 sc[C::kEpl / 2];
+#pragma unroll
+                for (int e = 0; e < C::kEpl / 2; e++) sc[e] = F2(f, f);
+                uint32_t top = 0, low = 0xffffffffu;  // low: less 1, so that zeros do not count
 #pragma unroll 1
-                    for (int ib = 0; ib < C::kRows; ib += kBatch) {
-                        const unsigned char *from = slot + raw0 + ib * kStep;
-                        const uint32_t to = at + op0 + ib * kStep;
-                        uint4 x[kBatch];
+                for (int ib = 0; ib < C::kRows; ib += kBatch) {
+                    uint4 x[kBatch];
 #pragma unroll
-                        for (int y = 0; y < kBatch; y++) x[y] = *reinterpret_cast<const uint4 *>(from + y * kStep);
-                        __syncwarp();  // a row of pairs is read whole before it is written
+                    for (int y = 0; y < kBatch; y++)
+                        x[y] = *reinterpret_cast<const uint4 *>(slot + raw0 + (ib + y) * kStep);
+                    __syncwarp();  // a row of pairs is read whole before it is written
 #pragma unroll
-                        for (int y = 0; y < kBatch; y++) {
-                            const uint32_t dst = to + y * kStep;
-                            const uint32_t w[4] = {x[y].x, x[y].y, x[y].z, x[y].w};
-                            if (C::kPair) {
-#pragma unroll
-                                for (int z = 0; z < 4; z++) top = fmaxf(top, fabsf(__uint_as_float(w[z])));
-                                uint32_t h0, h1, l0, l1;
-                                split2(mul2(F2(__uint_as_float(w[0]), __uint_as_float(w[1])), sc), h0, l0);
-                                split2(mul2(F2(__uint_as_float(w[2]), __uint_as_float(w[3])), sc), h1, l1);
-                                sts64(dst, h0, h1);
-                                sts64(dst + C::kHalfBytes, l0, l1);
-                            } else {
-                                uint32_t h[4];
-#pragma unroll
-                                for (int z = 0; z < 4; z++) {
-                                    const float a = __uint_as_float(w[z] << 16),
-                                                b = __uint_as_float(w[z] & 0xffff0000u);
-                                    top = fmaxf(top, fmaxf(fabsf(a), fabsf(b)));
-                                    const float2 f = mul2(F2(a, b), sc).get();
-                                    h[z] = pack_h2(f.x, f.y);
-                                }
-                                sts128(dst, make_uint4(h[0], h[1], h[2], h[3]));
-                            }
-                        }
+                    for (int y = 0; y < kBatch; y++) {
+                        const uint32_t t = O::largest(x[y]);
+                        top = max(top, t);
+                        low = min(low, t - 1);
+                        O::convert(x[y], sc, to + (ib + y) * kStep);
                     }
-                    // The tile's largest magnitude, over the conversion warps
-                    // (a NaN is not counted: it shows in the results).
-                    const uint32_t mine = __reduce_max_sync(0xffffffffu, __float_as_uint(top));
-                    const int place = (2 * j + again) & 3;
-                    if (lane == 0) atomicMax(&most[place], mine);
-                    bar_sync(1, C::kConv * 32);
-                    const uint32_t all = *reinterpret_cast<volatile uint32_t *>(&most[place]);
-                    bar_sync(1, C::kConv * 32);
-                    if (threadIdx.x == C::kConvWarp * 32) most[place] = 0;
-                    if (all == 0) break;
-                    const int found = scale_exponent(all);
-                    if (threadIdx.x == C::kConvWarp * 32 && all >= 0x7f800000u) poison[cu.seg & 7] = 1;
-                    (v ? e_v : e_k) = found;
-                    if (again || (found <= ex + 3 && found >= ex - 2)) break;
-                    // Once more, from the cache.
-                    ex = found;
-#pragma unroll 1
-                    for (int i = 0; i < C::kRows; i++) {
-                        const int key = cu.i0 + row_of(i), pos = key < cu.sink ? key : key - cu.sink + cu.low;
-                        uint4 x = make_uint4(0, 0, 0, 0);
-                        if (live_key(p, cu, key) && col < D)
-                            x = __ldcg(reinterpret_cast<const uint4 *>(
-                                p.a.cache.base + paged_row(p.a.cache, p.a.batch, cu.b, pos, p.a.err) +
-                                (v ? p.a.cache.parity_stride : 0) + (cu.kvh * D + col) * (long long)sizeof(T)));
-                        *reinterpret_cast<uint4 *>(slot + raw0 + i * kStep) = x;
-                    }
-                    __syncwarp();
                 }
-            }
-            if (threadIdx.x == C::kConvWarp * 32) {
-                (v ? v_scale : k_scale)[n & 7] = C::kRaw ? 1.f : pow2(ex - kTop);
-                mbar_arrive(&(v ? v_sc : k_sc)[n & 7]);
+                top = __reduce_max_sync(0xffffffffu, top);
+                // A warp with 16 bytes (a key, perhaps) that the scale does not
+                // suit takes its keys from the cache once more.
+                const bool off = __any_sync(0xffffffffu, (top && scale_exponent(top) > e_k + 3) ||
+                                                             (int)(low >> 23) - 127 < e_k - kNear);
+                if (__builtin_expect(off, 0))
+                    keys_again<T, DP>(p, cu, to, e_k, k_rel + (n & 7) * kKeys, &poison[cu.seg & 7]);
+                if (lane == 0) {
+                    k_most[8 * (n & 1) + pw] = top;
+                    key_tile[n & 7].own[pw] = off;
+                    if (pw == 0) key_tile[n & 7].scale = pow2(e_k - kTop);
+                }
+            } else if (!C::kRaw) {
+                uint32_t top[4] = {0, 0, 0, 0};
+#pragma unroll 1
+                for (int ib = 0; ib < C::kRows; ib += kBatch) {
+                    uint4 x[kBatch];
+#pragma unroll
+                    for (int y = 0; y < kBatch; y++)
+                        x[y] = *reinterpret_cast<const uint4 *>(slot + raw0 + (ib + y) * kStep);
+                    __syncwarp();  // a row of pairs is read whole before it is written
+#pragma unroll
+                    for (int y = 0; y < kBatch; y++) {
+                        top[0] = O::larger(top[0], O::size_of(x[y].x));
+                        top[1] = O::larger(top[1], O::size_of(x[y].y));
+                        top[2] = O::larger(top[2], O::size_of(x[y].z));
+                        top[3] = O::larger(top[3], O::size_of(x[y].w));
+                        O::convert(x[y], vs, to + (ib + y) * kStep);
+                    }
+                }
+                // Channels keep their scales while the largest value of this
+                // lane's keys, scaled, is from 2^1 to 2^15.
+                bool off = false;
+#pragma unroll
+                for (int e = 0; e < C::kEpl; e++) {
+                    const uint32_t t =
+                        C::kPair ? top[e % 4] : e % 2 ? top[e / 2 % 4] & 0xffff0000u : top[e / 2 % 4] << 16;
+                    const float2 f = vs[e / 2].get();
+                    const float at = __uint_as_float(t) * (e % 2 ? f.y : f.x);
+                    off |= t && !(at >= 2.f && at < 32768.f);
+                }
+                off = bar_or(1, C::kConv * 32, off);
+                if (__builtin_expect(off, 0)) {
+                    const float *was = v_scale + (change++ & 7) * DP;
+                    float *now = v_scale + (change & 7) * DP;
+                    values_again<T, DP>(p, cu, to, v_most, v_high, v_seg, was, now, &poison[cu.seg & 7]);
+#pragma unroll
+                    for (int e = 0; e < C::kEpl / 2; e++)
+                        vs[e] = F2(O::inverse(now[col + 2 * e]), O::inverse(now[col + 2 * e + 1]));
+                }
+                // The keys' largest values that the barrier has brought together.
+                const uint32_t t = __reduce_max_sync(
+                    0xffffffffu, lane < C::kConv ? k_most[8 * (min(n + 1, N - 1) & 1) + lane] : 0u);
+                if (t && t < 0x7f800000u) e_k = scale_exponent(t);
+                if (lane == 0 && pw == 0) v_change[n & 7] = off;
             }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&full[j % S]);
+            if (lane == 0) {
+                if (!v)
+                    mbar_arrive(&k_sc[n & 7]);
+                else if (pw == 0)
+                    mbar_arrive(&v_sc[n & 7]);
+                mbar_arrive(&full[j % S]);
+            }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::kRestRegs));

@@ -405,6 +405,52 @@ def test_values_of_very_different_sizes(dev, dtype, new):
     assert np.all(np.abs(got - want) <= tol)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("page", [5, 16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_value_channels_of_very_different_sizes(dev, dim, page, dtype):
+    # Each channel is held as finely as if it were alone: to 2^-22 of a value
+    # or 2^-26 of the channel's largest among a tile's keys, 2^-25 with those
+    # of the probabilities. Sizes change along the keys too, so that the scales
+    # of a tile do not suit the next.
+    b = Batch([(150, 40), (300, 90)], heads=8, kv_heads=2, dim=dim, page=page, layers=1, layer=0, dtype=dtype)
+    b.stored[..., 1, :, :, :] *= 2.0 ** (-10.0 * (np.arange(dim) % 4))
+    put = [(1, pos, 2.0 ** (9 * (pos // 100 % 3))) for pos in range(390)]
+    for seq, pos, size in put:
+        b.stored[int(b.table[seq, pos // page]), 0, 1, pos % page] *= size
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    scale = dim ** -0.5
+    got = attend(dev, b).reshape(b.tokens, 8, dim)
+    want = b.attention(scale)[0].reshape(b.tokens, 8, dim)
+    for i, (p, n) in enumerate(b.lens):
+        k, v = b.keys(i)
+        for t in range(n):
+            for h in range(8):
+                kk, vv = k[:p + t + 1, h // 4], v[:p + t + 1, h // 4]
+                tile = v[:min(p + n, 128 * ((p + t) // 128 + 1)), h // 4]
+                q = b.q[b.starts[i] + t].reshape(8, dim)[h].astype(np.float64)
+                s = kk @ q * scale
+                w = np.exp(s - s.max())
+                ds = 9 * 2.0 ** -20 * scale * (np.abs(kk) @ np.abs(q)).max()
+                tol = (w / w.sum()) @ np.abs(vv) * (2 * ds + (8 + len(kk) / 64) * 2.0 ** -20)
+                tol += 2.0 ** -25 * np.abs(tile).max(0)
+                row = b.starts[i] + t
+                assert np.all(np.abs(got[row, h] - want[row, h]) <= tol), (row, h)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads", [2, 8])
+def test_large_keys_that_a_row_does_not_see(dev, heads, dtype):
+    # From position 40 on keys are 2^13 or 2^24 times as large: the rows before
+    # keep their precision, which the bound takes from what they see.
+    b = Batch([(0, 100), (30, 60)], heads=heads, kv_heads=2, dim=64, page=16, layers=1, layer=0, dtype=dtype)
+    for seq in range(2):
+        for pos in range(40, sum(b.lens[seq])):
+            b.stored[int(b.table[seq, pos // 16]), 0, 0, pos % 16] *= 2.0 ** (13 if dtype == F16 else 24)
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    check(attend(dev, b), b)
+
+
 def test_extreme_scores(dev):
     # Scores of +-20000: only differences count.
     b = Batch([(200, 1), (90, 40)], heads=4, kv_heads=2, dim=64, page=16)
