@@ -652,7 +652,11 @@ __global__ void __launch_bounds__(Cfg<T, DP>::kThreads, Cfg<T, DP>::kCtas)
 #pragma unroll
             for (int h = 0; h < kSub; h++) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) pr[h][j] = ex2(pr[h][j] - (((j & 1) ? u_1 : u_0) - C::kShift));
+                for (int j = 0; j < 4; j++) {
+                    // The distance first: of scores past 2^24 it is exact, u less kShift is not.
+                    const float d = pr[h][j] - ((j & 1) ? u_1 : u_0);
+                    pr[h][j] = ex2(C::kShift ? d + C::kShift : d);
+                }
                 l0 += pr[h][0] + pr[h][2];
                 l1 += pr[h][1] + pr[h][3];
             }

@@ -18,6 +18,13 @@
 // products. Every tile's P V starts from zero and is added in f32 registers
 // (TMEM accumulation over thousands of keys would truncate thousands of times).
 //
+// Infinities and NaN. A key's reach S by themselves; a score that they make NaN
+// is taken once more from the cache, for it may be -infinity, and its row goes
+// on without it. A value's are taken out of the operand, where they would reach
+// the rows that do not see them, and put into the results at the segment's end.
+// What is done twice is the conversion of their tiles, one product for every
+// such score, and a look through the values of their segments.
+//
 // One CTA per SM, 20 warps:
 //   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
 //          S from TMEM, running maximum, P as f16 pairs back into the TMEM
@@ -48,6 +55,7 @@
 // (4800 cycles: the softmax warps' chain of TMEM reads, exponentials and
 // splits; the tensor pipe is busy for 40 % of it). 128 sequences of 64 heads
 // over 32768 shared keys in f16: 245 us of a call of 322.
+#include <float.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -68,9 +76,9 @@ constexpr int kShift = 14;  // a query row's largest value in [2^14, 2^15), prob
 constexpr int kTop = 11;    // a scale takes the largest value to 2^11 and serves from 2^1 to 2^15
 constexpr int kFirst = 2;   // exponent expected at first
 constexpr int kNear = 8;    // keys down to 2^-8 of the expected largest value share its scale
+constexpr float kLarge = 4194304.f;  // 2^22
 constexpr int kDeep = 80;   // octaves that a channel's scale may fall within a segment
 constexpr int kLaunchRegs = 96;  // registers a thread at launch
-constexpr uint64_t kLimitNs = 20000000000ull;  // rows of values that are not finite take long
 template <typename T, int DP>
 struct Cfg {
     static constexpr bool kPair = sizeof(T) == 4;            // keys and values are f16 pairs
@@ -82,7 +90,7 @@ struct Cfg {
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
     static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (22 * kM + 8 * kKeys + 18 * DP + 80 + 8 * 12 + 4 * DP + 16) +
+    static constexpr int kSmall = 4 * (22 * kM + 8 * kKeys + 18 * DP + 88 + 8 * 12 + 16 + 2 * DP / 32 * kM) +
                                   8 * (3 * kKeys + 8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
@@ -95,8 +103,8 @@ struct Cfg {
     static constexpr int kConvWarp = 16 - kConv;
     static constexpr int kRows = kKeys / kConv / kRpi;   // 16-byte pieces per conversion lane
     // Registers a thread, by warpgroup, out of those of the launch.
-    static constexpr int kSoftRegs = kPair ? 96 : 88, kOutRegs = 184, kConvRegs = kPair ? 64 : 56,
-                         kRestRegs = kPair ? 72 : 64;
+    static constexpr int kSoftRegs = kPair ? 96 : 88, kOutRegs = kPair ? 184 : 192, kConvRegs = kPair ? 64 : 56,
+                         kRestRegs = kPair ? 72 : 56;
     static_assert(kSoft * kSoftRegs + kOutRegs + kConv / 4 * kConvRegs + kRestRegs <= 5 * kLaunchRegs, "registers");
     // f32 accumulators, f16 operands, K-major A; B K-major (S) or MN-major (O).
     static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
@@ -308,6 +316,11 @@ __device__ __forceinline__ void sts64(uint32_t addr, uint32_t a, uint32_t b) {
 __device__ __forceinline__ void bar_sync(int id, int threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
 // The same, and whether some thread passes true.
 __device__ __forceinline__ bool bar_or(int id, int threads, bool x) {
     uint32_t any;
@@ -418,6 +431,23 @@ struct Operand {
     __device__ static __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
         return C::kPair ? max(a, b) : __vmaxu2(a, b);
     }
+    // Takes what is not finite out of 16 bytes; whether there was any.
+    __device__ static __forceinline__ bool clean(uint4 &x) {
+        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+        bool any = false;
+#pragma unroll
+        for (int z = 0; z < 4; z++) {
+            if constexpr (C::kPair) {
+                if (size_of(w[z]) >= 0x7f800000u) any = true, w[z] = 0;
+            } else {
+                constexpr uint32_t kInf = C::kRaw ? 0x7c00u : 0x7f80u;
+                if ((size_of(w[z]) & 0xffffu) >= kInf) any = true, w[z] &= 0xffff0000u;
+                if (size_of(w[z]) >> 16 >= kInf) any = true, w[z] &= 0xffffu;
+            }
+        }
+        x = make_uint4(w[0], w[1], w[2], w[3]);
+        return any;
+    }
     // The largest magnitude of 16 bytes, as the bits of an f32.
     __device__ static __forceinline__ uint32_t largest(uint4 x) {
         const uint32_t t = larger(larger(size_of(x.x), size_of(x.y)), larger(size_of(x.z), size_of(x.w)));
@@ -436,13 +466,14 @@ struct Operand {
 };
 
 // The rare ways of the conversion and of the softmax, behind branches marked as
-// unlikely: what is not executed costs as well, in instruction fetches.
+// unlikely: what is not executed costs as well, in instruction fetches. They
+// are part of their roles' code, not calls, so that each keeps to the registers
+// that its role has given itself.
 //
 // A conversion warp's keys from the cache again: those outside 2^-kNear to 2^3
 // of the expected largest value get a scale of their own, from their own.
 template <typename T, int DP>
-__device__ __forceinline__ void keys_again(const PagedPass &p, const Tile &cu, uint32_t to, int expect, float *rel,
-                                        int *poison) {
+__device__ __forceinline__ void keys_again(const PagedPass &p, const Tile &cu, uint32_t to, int expect, float *rel) {
     using C = Cfg<T, DP>;
     using O = Operand<T, DP>;
     const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) - C::kConvWarp;
@@ -452,7 +483,6 @@ __device__ __forceinline__ void keys_again(const PagedPass &p, const Tile &cu, u
         const uint4 x = O::fetch(p, cu, row, col, false);
         uint32_t t = O::largest(x);
         for (int o = 1; o < C::kLpr; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
-        if (t >= 0x7f800000u) *poison = 1;
         int ex = t ? scale_exponent(t) : expect;
         if (ex >= expect - kNear && ex <= expect + 3) ex = expect;
         const float f = pow2(kTop - ex);
@@ -472,13 +502,20 @@ __device__ __forceinline__ void rescale_scores(uint32_t st, int first, const Key
             tmem_st1(st + i, __float_as_uint(__uint_as_float(tmem_ld1(st + i)) * rel[i]));
     tmem_wait_st();
 }
+// S less a number of the row.
+template <typename T, int DP>
+__device__ __forceinline__ void shift_scores(uint32_t st, int first, float by) {
+    for (int i = first; i < first + kKeys / Cfg<T, DP>::kSoft; i++)
+        tmem_st1(st + i, __float_as_uint(__uint_as_float(tmem_ld1(st + i)) - by));
+    tmem_wait_st();
+}
 // All conversion warps' values of a tile from the cache again, with new scales
 // from the tile's own largest values. `now` takes them out of the outputs, as
 // `was` did. A scale falls by at most kDeep octaves within a segment, whose
 // outputs so far are held in units of it.
 template <typename T, int DP>
 __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu, uint32_t to, uint32_t *most, int *high,
-                                          int *high_seg, const float *was, float *now, int *poison) {
+                                          int *high_seg, const float *was, float *now, int *odd) {
     using C = Cfg<T, DP>;
     using O = Operand<T, DP>;
     const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) - C::kConvWarp, ct = threadIdx.x - C::kConvWarp * 32;
@@ -493,10 +530,7 @@ __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu,
         for (int e = 0; e < C::kEpl; e++) {
             const uint32_t a = O::size_of(w[C::kPair ? e % 4 : e / 2 % 4]);
             const uint32_t t = C::kPair ? a : e % 2 ? a & 0xffff0000u : a << 16;
-            if (t < 0x7f800000u)
-                top[e] = max(top[e], t);
-            else
-                *poison = 1;
+            if (t < 0x7f800000u) top[e] = max(top[e], t);
         }
     }
 #pragma unroll
@@ -519,8 +553,135 @@ __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu,
     F2 sc[C::kEpl / 2];
 #pragma unroll
     for (int e = 0; e < C::kEpl / 2; e++) sc[e] = F2(O::inverse(now[col + 2 * e]), O::inverse(now[col + 2 * e + 1]));
-    for (int i = 0; i < C::kRows; i++)
-        O::convert(O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true), sc, to + i * O::kStep);
+    for (int i = 0; i < C::kRows; i++) {
+        uint4 x = O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true);
+        if (O::clean(x)) *odd = 1;
+        O::convert(x, sc, to + i * O::kStep);
+    }
+}
+// A conversion lane's part of a tile of F16 values, which is otherwise taken
+// as it is, cleaned.
+template <typename T, int DP>
+__device__ __forceinline__ void clean_values(unsigned char *at, int *odd) {
+    for (int i = 0; i < Cfg<T, DP>::kRows; i++) {
+        uint4 x = *reinterpret_cast<const uint4 *>(at + i * Operand<T, DP>::kStep);
+        if (!Operand<T, DP>::clean(x)) continue;
+        *reinterpret_cast<uint4 *>(at + i * Operand<T, DP>::kStep) = x;
+        *odd = 1;
+    }
+}
+// The values that are not finite, zero in the operand, into the results of a
+// piece of a segment: four warps look through its keys [k0, k1) once more and
+// note for every dim which rows see a +infinity and which a -infinity (a NaN is
+// both); then thread r puts them into row r's result, dim d at
+// dst[d / 4 * step + d % 4]. bits: zero, and left so.
+template <typename T, int DP>
+__device__ __noinline__ void odd_values(const PagedPass &p, Cursor c, int k0, int k1, float *dst, int step, bool live,
+                                        uint32_t *bits) {
+    using C = Cfg<T, DP>;
+    constexpr int kFly = 4, kWords = kM / 32;
+    const int r = threadIdx.x & (kM - 1), warp = r >> 5, lane = r & 31, D = p.a.head_dim, G = group_of(p);
+    const int col = lane % C::kLpr * C::kEpl;
+    const char *base = p.a.cache.base + p.a.cache.parity_stride + (c.kvh * D + col) * (long long)sizeof(T);
+    for (int i0 = k0 + warp * C::kRpi + lane / C::kLpr; __any_sync(0xffffffffu, i0 < k1); i0 += 4 * C::kRpi * kFly) {
+        uint4 x[kFly];
+#pragma unroll
+        for (int y = 0; y < kFly; y++) {
+            const int i = i0 + y * 4 * C::kRpi, pos = i < c.sink ? i : i - c.sink + c.low;
+            x[y] = make_uint4(0, 0, 0, 0);
+            if (i < k1 && col < D)
+                x[y] = __ldcg(
+                    reinterpret_cast<const uint4 *>(base + paged_row(p.a.cache, p.a.batch, c.b, pos, p.a.err)));
+        }
+#pragma unroll 1
+        for (int y = 0; y < kFly; y++) {
+            uint4 kept = x[y];
+            if (!Operand<T, DP>::clean(kept)) continue;
+            const int i = i0 + y * 4 * C::kRpi, pos = i < c.sink ? i : i - c.sink + c.low;
+            // Rows [from, to) see the key.
+            long long from = 0, to = c.rows;
+            if (!p.prefix_pass) {
+                if (pos < p.first || (pos < c.from && pos >= p.a.sinks)) continue;
+                from = max((long long)(pos - c.past) * G - c.r0, 0ll);
+                if (p.a.window && pos >= p.a.sinks)
+                    to = min((((long long)pos + p.a.window) - c.past) * G - c.r0, to);
+            }
+            float v[C::kEpl];
+            Frag<T>::ld(&x[y], v);
+#pragma unroll 1
+            for (int w = 0; w < kWords; w++) {
+                const int lo = (int)max(from - 32 * w, 0ll), hi = (int)min(to - 32 * w, 32ll);
+                if (lo >= hi) continue;
+                const uint32_t rows = (0xffffffffu >> (32 - hi)) & (0xffffffffu << lo);
+#pragma unroll
+                for (int e = 0; e < C::kEpl; e++) {
+                    if (finite(v[e])) continue;
+                    uint32_t *word = bits + (col + e) * kWords + w;
+                    if (!(v[e] < 0.f) && (*word & rows) != rows) atomicOr(word, rows);
+                    if (!(v[e] > 0.f) && (word[DP * kWords] & rows) != rows) atomicOr(word + DP * kWords, rows);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    bar_sync(2, kM);
+    for (int d = 0; d < D; d++) {
+        const uint32_t plus = bits[d * kWords + warp] >> lane & 1, minus = bits[(DP + d) * kWords + warp] >> lane & 1;
+        if (!live || !(plus | minus)) continue;
+        float &o = dst[(size_t)(d / 4) * step + d % 4];
+        o = (plus ? INFINITY : 0.f) - (minus ? INFINITY : 0.f) + o;
+    }
+    bar_sync(2, kM);
+    for (int i = r; i < 2 * DP * kWords; i += kM) bits[i] = 0;
+    bar_sync(2, kM);
+}
+// S's columns that the row does not see, all but i < hi with i >= lo or
+// i < sinks, to -infinity.
+template <typename T, int DP>
+__device__ __forceinline__ void mask_scores(uint32_t st, int first, int hi, int lo, int sinks) {
+#pragma unroll 1
+    for (int i = first; i < first + kKeys / Cfg<T, DP>::kSoft; i += 16) {
+        float s[16];
+        uint32_t x[16];
+        tmem_ld16(st + i, s);
+#pragma unroll
+        for (int j = 0; j < 16; j++)
+            x[j] = __float_as_uint(i + j < hi && (i + j >= lo || i + j < sinks) ? s[j] : -INFINITY);
+        tmem_st16(st + i, x);
+    }
+    tmem_wait_st();
+}
+// The scores of row q against the tile's keys that came out NaN though the row
+// holds none and is not NaN yet (alive): a key with an infinity has a score of
+// +-infinity, or NaN after all. Takes those from the cache, in f32. Columns
+// first .. first + kKeys / kSoft of S. Returns the row's largest.
+template <typename T, int DP>
+__device__ __forceinline__ float repair_scores(const PagedPass &p, uint32_t st, int first, const float *q, int b, int kvh,
+                                               int i0, int sink, int low, bool alive) {
+    using C = Cfg<T, DP>;
+    const int D = p.a.head_dim;
+    const float sign = p.scale_log2 < 0.f ? -1.f : 1.f;
+    float mx = -INFINITY;
+    for (int i = first; i < first + kKeys / C::kSoft; i++) {
+        float x = __uint_as_float(tmem_ld1(st + i));
+        const bool wrong = alive && x != x;
+        if (__any_sync(0xffffffffu, wrong)) {
+            if (wrong) {
+                const int key = i0 + i, pos = key < sink ? key : key - sink + low;
+                const char *src = p.a.cache.base + paged_row(p.a.cache, p.a.batch, b, pos, p.a.err) +
+                                  (long long)kvh * D * (int)sizeof(T);
+                x = 0.f;
+#pragma unroll 4
+                for (int d = 0; d < D; d++) x = fmaf(q[d] * sign, Frag<T>::get(src + d * (int)sizeof(T)), x);
+                alive = x == x;
+            }
+            __syncwarp();
+            tmem_st1(st + i, __float_as_uint(x));
+        }
+        mx = fmaxf(mx, x);
+    }
+    tmem_wait_st();
+    return mx;
 }
 
 // Where a row's result goes: (o f + prefix o e) / l to the output, or for a
@@ -591,11 +752,11 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     uint32_t *k_most = reinterpret_cast<uint32_t *>(v_seg + 4);  // [2][8 warps] keys' largest
     int *v_change = reinterpret_cast<int *>(k_most + 16);  // [8 tiles] the channels' scales change here
     KeyTile *key_tile = reinterpret_cast<KeyTile *>(v_change + 8);  // [8 tiles]
-    int *poison = reinterpret_cast<int *>(key_tile + 8);  // [8 segments]
-    Tile *tiles = reinterpret_cast<Tile *>(poison + 8);           // [8 tiles]
+    int *seg_odd = reinterpret_cast<int *>(key_tile + 8);         // [8 segments] some values are not finite
+    uint32_t *odd_bits = reinterpret_cast<uint32_t *>(seg_odd + 8);  // [+, -][DP][kM / 32] outputs that see such
+    Tile *tiles = reinterpret_cast<Tile *>(odd_bits + 2 * DP / 32 * kM);  // [8 tiles]
     long long *row_off = reinterpret_cast<long long *>(tiles + 8);  // [3 tiles][kKeys]
-    float *scratch = reinterpret_cast<float *>(row_off + 3 * kKeys);  // [4 warps][DP]
-    int *flags = reinterpret_cast<int *>(scratch + 4 * DP);
+    int *flags = reinterpret_cast<int *>(row_off + 3 * kKeys);
     volatile int *abort = flags;
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(flags + 1);
     int *last_s = flags + 2;
@@ -628,14 +789,16 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         mbar_init(done, 1);
         for (int i = 0; i < 8; i++) {
             mbar_init(&k_sc[i], C::kConv);
-            mbar_init(&v_sc[i], 1);
+            mbar_init(&v_sc[i], C::kConv);
         }
         for (int i = 0; i < 4; i++) mbar_init(&a_full[i], 4 * C::kSoft);
         fence_mbar_init();
         *abort = 0;
-        for (int i = 0; i < 8; i++) poison[i] = 0, key_tile[i] = KeyTile{};
+        for (int i = 0; i < 8; i++) key_tile[i] = KeyTile{};
+        for (int i = 0; i < 8; i++) seg_odd[i] = 0;
         *v_seg = -1;
     }
+    for (int i = threadIdx.x; i < 2 * DP / 32 * kM; i += kThreads) odd_bits[i] = 0;
     if (threadIdx.x >= kThreads - DP) v_scale[threadIdx.x - (kThreads - DP)] = pow2(kFirst - kTop - kShift);
     const Line line = line_scan(p, unit, sums);
     const long long U = line.total;
@@ -682,13 +845,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             if (C::kSoft == 1) return x;
             half_max[(3 * group + buffer) * kM + r] = x;
             bar_sync(4, 2 * kM);
-            return fmaxf(x, half_max[(3 * (1 - group) + buffer) * kM + r]);
+            return max_nan(x, half_max[(3 * (1 - group) + buffer) * kM + r]);
         };
         // Queries are taken with the scale's sign; its size comes after the product.
         const float sign = p.scale_log2 < 0.f ? -1.f : 1.f, size = fabsf(p.scale_log2);
         float m = -INFINITY, l = 0.f, qs = 1.f;
         int hi = 0, lo = 0;
-        bool first = true;
+        bool first = true, sound = true;  // sound: a row with a finite query
         for (int n = 0; n < N; n++) {
             if (first) {
                 // The row to TMEM: first as it is, 128 columns, while its largest
@@ -723,13 +886,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                             x[4 * z + 3] = __float_as_uint(f.w * sign);
                         }
 #pragma unroll
-                        for (int z = 0; z < 16; z++) top = fmaxf(top, fabsf(__uint_as_float(x[z])));
+                        for (int z = 0; z < 16; z++) top = max_nan(top, fabsf(__uint_as_float(x[z])));
                         tmem_st16(q_tm + lane_tm + h + 16 * y, x);
                     }
                 }
                 tmem_wait_st();
                 top = both(top, 2);
                 const int ex = scale_exponent(__float_as_uint(top));
+                sound = live && top < INFINITY;
                 const float sc = pow2(kShift - ex);
                 qs = pow2(ex - kShift);
 #pragma unroll 1
@@ -759,69 +923,82 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     if (p.a.window) lo = max(at - p.a.window + 1 - c.low, 0) + c.sink;
                 }
             }
-            mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
-            if (!C::kRaw) mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
+            mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort);
+            if (!C::kRaw) mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort);
             tc_fence_after();
             const int i0 = c.tile * kKeys;
             // Rows past the tile's last hold zeros; they need no mask.
             const bool whole = i0 + kKeys <= hi && (i0 >= lo || i0 + kKeys <= p.a.sinks);
             const bool masked = __any_sync(0xffffffffu, !whole);
             const uint4 kt = *reinterpret_cast<const uint4 *>(key_tile + (n & 7));
-            const float f = C::kRaw ? qs * size : qs * __uint_as_float(kt.x) * size;
+            // Not 0, which would make NaN of -infinity.
+            const float f = max_nan(C::kRaw ? qs * size : qs * __uint_as_float(kt.x) * size, FLT_MIN);
             const uint32_t st = s_tm + (n & 1) * 128 + lane_tm;
             const int h_first = group * 2;
             if (!C::kRaw && __builtin_expect((kt.z | kt.w) != 0, 0))
                 rescale_scores<T, DP>(st, 32 * h_first, key_tile + (n & 7), k_rel + (n & 7) * kKeys);
-            // Both passes over the row, with the mask only where a row needs it.
-            float nm, a;
+            // Where some row's mask hides keys of the tile, S there becomes
+            // -infinity first: two forms of the passes below would be twice the
+            // code, whose fetches cost the other roles more.
+            if (masked) mask_scores<T, DP>(st, 32 * h_first, hi - i0, lo - i0, p.a.sinks - i0);
+            float mx = -INFINITY;
+#pragma unroll 1
+            for (int h = h_first; h < h_first + 4 / C::kSoft; h++) {
+                uint32_t x[32];
+                tmem_ld32_async(st + 32 * h, x);
+                tmem_wait_ld(x);
+#pragma unroll
+                for (int j = 0; j < 32; j++) mx = max_nan(mx, __uint_as_float(x[j]));
+            }
+            float other = -INFINITY;
+            float *mine = half_max + (3 * group + (n & 1)) * kM + r, *theirs = mine + (1 - 2 * group) * 3 * kM;
+            if (C::kSoft == 2) {
+                *mine = mx;
+                bar_sync(4, 2 * kM);
+                other = *theirs;
+            }
+            // NaN among a finite query's scores: a key holds what is not finite.
+            // The two warps of a row see the same and meet once more.
+            if (__builtin_expect(__any_sync(0xffffffffu, sound && (mx != mx || other != other)), 0)) {
+                const int tok = (c.r0 + r) / G;
+                const float *q = p.a.q + ((size_t)(c.tok0 + tok) * H + c.kvh * G + (c.r0 + r - tok * G)) * D;
+                mx = repair_scores<T, DP>(p, st, 32 * h_first, q, c.b, c.kvh, i0, c.sink, c.low, sound && l == l);
+                if (C::kSoft == 2) {
+                    bar_sync(5 + (warp & 3), 64);
+                    *mine = mx;
+                    bar_sync(5 + (warp & 3), 64);
+                    other = *theirs;
+                }
+            }
+            mx = fmaxf(mx, other);
+            const float own = mx == -INFINITY ? mx : mx * f, nm = fmaxf(m, own);
+            float mu = nm == -INFINITY ? 0.f : nm - (float)kShift;
+            // Scores past 2^22, whose rounding is not small against 1: their
+            // distance from the largest is taken first, or that one's
+            // probability would not be near 1.
+            const bool large = fabsf(nm) >= kLarge && fabsf(nm) < INFINITY;
+            if (__builtin_expect(__any_sync(0xffffffffu, large), 0)) {
+                shift_scores<T, DP>(st, 32 * h_first, large ? own >= m ? mx : m / f : 0.f);
+                mu = large ? -(float)kShift : mu;
+            }
+            const float a = m == -INFINITY ? 0.f : ex2(m - nm);
             F2 sum2(0.f, 0.f);
-            auto row = [&](auto mask) {
-                constexpr bool kMask = decltype(mask)::value;
-                const int h0 = hi - i0, l0 = lo - i0, s0 = p.a.sinks - i0;
-                float mx = -INFINITY;
 #pragma unroll 1
-                for (int h = h_first; h < h_first + 4 / C::kSoft; h++) {
-                    uint32_t x[32];
-                    tmem_ld32_async(st + 32 * h, x);
-                    tmem_wait_ld(x);
+            for (int h = h_first; h < h_first + 4 / C::kSoft; h++) {
+                uint32_t x[32], ph[16], pl[16];
+                tmem_ld32_async(st + 32 * h, x);
+                tmem_wait_ld(x);
 #pragma unroll
-                    for (int j = 0; j < 32; j++) {
-                        const int i = 32 * h + j;
-                        if (!kMask || (i < h0 && (i >= l0 || i < s0))) mx = fmaxf(mx, __uint_as_float(x[j]));
-                    }
+                for (int j = 0; j < 16; j++) {
+                    const float2 z =
+                        fma2(F2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), F2(f, f), F2(-mu, -mu)).get();
+                    const F2 e(ex2(z.x), ex2(z.y));
+                    sum2 = add2(sum2, e);
+                    split2(e, ph[j], pl[j]);
                 }
-                mx = both(mx, n & 1);
-                nm = fmaxf(m, mx == -INFINITY ? mx : mx * f);
-                const float mu = nm == -INFINITY ? 0.f : nm - (float)kShift;
-                a = m == -INFINITY ? 0.f : ex2(m - nm);
-#pragma unroll 1
-                for (int h = h_first; h < h_first + 4 / C::kSoft; h++) {
-                    uint32_t x[32], ph[16], pl[16];
-                    tmem_ld32_async(st + 32 * h, x);
-                    tmem_wait_ld(x);
-#pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const float2 z =
-                            fma2(F2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1])), F2(f, f), F2(-mu, -mu))
-                                .get();
-                        float e0 = ex2(z.x), e1 = ex2(z.y);
-                        if (kMask) {
-                            const int i = 32 * h + 2 * j;
-                            if (!(i < h0 && (i >= l0 || i < s0))) e0 = 0.f;
-                            if (!(i + 1 < h0 && (i + 1 >= l0 || i + 1 < s0))) e1 = 0.f;
-                        }
-                        const F2 e(e0, e1);
-                        sum2 = add2(sum2, e);
-                        split2(e, ph[j], pl[j]);
-                    }
-                    tmem_st16(st + 32 * h, ph);
-                    tmem_st16(st + 32 * h + 16, pl);
-                }
-            };
-            if (masked)
-                row(std::true_type());
-            else
-                row(std::false_type());
+                tmem_st16(st + 32 * h, ph);
+                tmem_st16(st + 32 * h + 16, pl);
+            }
             m = nm;
             l = fmaf(l, a, sum2.get().x + sum2.get().y);
             if (group == 0) alpha[(n & 3) * kM + r] = a;
@@ -849,13 +1026,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         const int r = threadIdx.x - 128, ow = warp - 4;
         const uint32_t lane_tm = (uint32_t)(ow * 32) << 16;
         F2 acc[DP / 2];  // in units of the channels' scales
-        int seg = 0, seg_n = 0, change = 0;
+        int change = 0, seg = 0, seg_n = 0;
 #pragma unroll
         for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
         for (int n = 0; n < N; n++) {
-            mbar_wait(&a_full[n & 3], (n >> 2) & 1, p.a.err, abort, kLimitNs);
-            mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort, kLimitNs);
-            mbar_wait(o_full, n & 1, p.a.err, abort, kLimitNs);
+            mbar_wait(&a_full[n & 3], (n >> 2) & 1, p.a.err, abort);
+            mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort);
+            mbar_wait(o_full, n & 1, p.a.err, abort);
             tc_fence_after();
             const float a = alpha[(n & 3) * kM + r];
             if (!C::kRaw && __builtin_expect(v_change[n & 7], 0)) {
@@ -900,47 +1077,17 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                                          : *reinterpret_cast<const float2 *>(vs + 2 * d);
                 acc[d] = mul2(acc[d], F2(x.x, x.y));
             }
-            const bool bad_tiles = poison[seg & 7] != 0;
-            bar_sync(2, 128);
-            if (r == 0) poison[seg & 7] = 0;
+            const bool has_odd = bar_or(2, 128, seg_odd[seg & 7] != 0);  // one answer for all, whatever was waited for
+            if (r == 0) seg_odd[seg & 7] = 0;
             __syncwarp();
             if (lane == 0) mbar_arrive(o_empty);
             const bool live = r < c.rows;
-            const int row = c.r0 + r, tok = row / G, at = c.past + tok;
+            auto add_odd = [&](float *dst, int step, bool mine) {
+                odd_values<T, DP>(p, c, (c.tile - (n - seg_n)) * kKeys, min(c.keys, (c.tile + 1) * kKeys), dst, step,
+                                  mine, odd_bits);
+            };
+            const int row = c.r0 + r, tok = row / G;
             const size_t qrow = (size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G);
-            bool bad = bad_tiles || !finite(l) || !(m < INFINITY);
-#pragma unroll
-            for (int d = 0; d < DP / 2; d++) bad |= !finite(acc[d].get().x) || !finite(acc[d].get().y);
-            unsigned todo = __ballot_sync(0xffffffffu, bad && live);
-            while (todo) {
-                const int src = __ffs(todo) - 1;
-                todo &= todo - 1;
-                const size_t qr = __shfl_sync(0xffffffffu, (unsigned long long)qrow, src);
-                const int rat = __shfl_sync(0xffffffffu, at, src);
-                const int k0 = (c.tile - (n - seg_n)) * kKeys, k1 = min(c.keys, (c.tile + 1) * kKeys);
-                float rm, rl, ro[DP / 32];
-                plain_row<T, DP>(
-                    p, p.a.q + qr * D, c.b, c.kvh, k0, k1,
-                    [&](int i) {
-                        const int pos = i < c.sink ? i : i - c.sink + c.low;
-                        if (p.prefix_pass) return pos;
-                        const bool sees =
-                            pos <= rat && pos >= p.first && (!p.a.window || pos > rat - p.a.window || pos < p.a.sinks);
-                        return sees ? pos : -1;
-                    },
-                    rm, rl, ro);
-#pragma unroll
-                for (int y = 0; y < DP / 32; y++) scratch[ow * DP + lane + 32 * y] = ro[y];
-                __syncwarp();
-                if (lane == src) {
-                    m = rm;
-                    l = rl;
-#pragma unroll
-                    for (int d = 0; d < DP / 2; d++)
-                        acc[d] = F2(scratch[ow * DP + 2 * d], scratch[ow * DP + 2 * d + 1]);
-                }
-                __syncwarp();
-            }
             const long long a0 = u0 + n - c.tile, a1 = a0 + c.tiles;  // the segment's units
             bool write = live;
             if (a0 < u0 || a1 > u1) {
@@ -950,6 +1097,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
                 for (int d = 0; d < DP / 4; d++) po[d * kM] = four(d);
                 reinterpret_cast<float2 *>(p.part_ml)[slot * kM + r] = make_float2(m, l);
+                if (__builtin_expect(has_odd, 0)) add_odd(reinterpret_cast<float *>(po), 4 * kM, true);
                 if (args.join) {
                     write = false;
                 } else {
@@ -993,6 +1141,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 for (int d = 0; d < DP; d += 4)
                     if (d < D) row_store(end, d, four(d / 4));
             }
+            if (__builtin_expect(has_odd && a0 >= u0 && a1 <= u1, 0))
+                add_odd((p.prefix_pass ? p.pre_o : p.a.out) + (live ? qrow * D : 0), 4, live);
 #pragma unroll
             for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
             seg++;
@@ -1020,7 +1170,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         for (int j = 0; j < total; j++) {
             const bool v = is_v(j);
             const int n = tile_of(j);
-            mbar_wait(&raw[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
+            mbar_wait(&raw[j % S], (j / S) & 1, p.a.err, abort);
             unsigned char *slot = ring + (j % S) * C::kTileBytes;
             const Tile &cu = tiles[n & 7];
             const bool whole = cu.whole;
@@ -1058,7 +1208,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 const bool off = __any_sync(0xffffffffu, (top && scale_exponent(top) > e_k + 3) ||
                                                              (int)(low >> 23) - 127 < e_k - kNear);
                 if (__builtin_expect(off, 0))
-                    keys_again<T, DP>(p, cu, to, e_k, k_rel + (n & 7) * kKeys, &poison[cu.seg & 7]);
+                    keys_again<T, DP>(p, cu, to, e_k, k_rel + (n & 7) * kKeys);
                 if (lane == 0) {
                     k_most[8 * (n & 1) + pw] = top;
                     key_tile[n & 7].own[pw] = off;
@@ -1097,7 +1247,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 if (__builtin_expect(off, 0)) {
                     const float *was = v_scale + (change++ & 7) * DP;
                     float *now = v_scale + (change & 7) * DP;
-                    values_again<T, DP>(p, cu, to, v_most, v_high, v_seg, was, now, &poison[cu.seg & 7]);
+                    values_again<T, DP>(p, cu, to, v_most, v_high, v_seg, was, now, &seg_odd[cu.seg & 7]);
 #pragma unroll
                     for (int e = 0; e < C::kEpl / 2; e++)
                         vs[e] = F2(O::inverse(now[col + 2 * e]), O::inverse(now[col + 2 * e + 1]));
@@ -1108,12 +1258,22 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 if (t && t < 0x7f800000u) e_k = scale_exponent(t);
                 if (lane == 0 && pw == 0) v_change[n & 7] = off;
             }
+            if (C::kRaw && v) {
+                uint32_t odd = 0;  // bit 15 of each half: its magnitude is 0x7c00 or more
+#pragma unroll 4
+                for (int i = 0; i < C::kRows; i++) {
+                    const uint4 x = *reinterpret_cast<const uint4 *>(slot + raw0 + i * kStep);
+                    odd |= (O::size_of(x.x) + 0x04000400u) | (O::size_of(x.y) + 0x04000400u) |
+                           (O::size_of(x.z) + 0x04000400u) | (O::size_of(x.w) + 0x04000400u);
+                }
+                if (__builtin_expect((odd & 0x80008000u) != 0, 0)) clean_values<T, DP>(slot + raw0, &seg_odd[cu.seg & 7]);
+            }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) {
                 if (!v)
                     mbar_arrive(&k_sc[n & 7]);
-                else if (pw == 0)
+                else
                     mbar_arrive(&v_sc[n & 7]);
                 mbar_arrive(&full[j % S]);
             }
@@ -1154,7 +1314,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                         }
                     };
                     auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity, int n, bool begins) {
-                        if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+                        if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort);
                         if (__any_sync(0xffffffffu, *abort)) return;
                         if (at >= 0 && page_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
                             report_error(p.a.err, kErrGatherId);
@@ -1212,7 +1372,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     bar_sync(3, kCopy * 32);
                 };
                 auto copy = [&](int j, int n, int parity) {
-                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, kLimitNs);
+                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort);
                     unsigned char *slot = ring + (j % S) * C::kTileBytes;
                     const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
 #pragma unroll 4
@@ -1269,12 +1429,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             const uint32_t ra = smem_addr(ring);
             int seg = 0;
             auto slot_wait = [&](int j) {
-                mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, kLimitNs);
+                mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort);
                 return ra + (j % S) * C::kTileBytes;
             };
             auto qk = [&](int n, bool begins, uint32_t kb) {
                 const int j = n ? 2 * n - 1 : 0;
-                if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, kLimitNs);
+                if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort);
                 if (!__any_sync(0xffffffffu, *abort)) {
                     tc_fence_after();
                     const uint32_t d = s_tm + (n & 1) * 128;
@@ -1304,10 +1464,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 }
             };
             auto pv = [&](int n) {
-                mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, kLimitNs);
+                mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort);
                 const int j = n == N - 1 ? total - 1 : 2 * n + 2;
                 const uint32_t vb = slot_wait(j);
-                if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, kLimitNs);
+                if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort);
                 if (!__any_sync(0xffffffffu, *abort)) {
                     tc_fence_after();
                     const uint32_t pt = s_tm + (n & 1) * 128;

@@ -379,6 +379,104 @@ def test_scores_of_minus_infinity_leave_the_others(dev, new):
             assert np.all(np.abs(got[t, 8 * h:8 * h + 8] - want) <= 1e-3)
 
 
+def outputs(b, window=0, sinks=0):
+    """The definition in 64 bits, infinities and NaN with it: a value counts by
+    its sign where its key's score is not -infinity."""
+    scale, G = b.dim ** -0.5, b.heads // b.kv_heads
+    out = np.full((b.tokens, b.heads, b.dim), np.nan)
+    with np.errstate(invalid="ignore"):
+        for i, (p, n) in enumerate(b.lens):
+            k, v = b.keys(i)
+            for t in range(n):
+                pos = np.arange(p + t + 1)
+                if window:
+                    pos = pos[(pos > p + t - window) | (pos < sinks)]
+                for h in range(b.heads):
+                    row = int(b.starts[i]) + t
+                    s = k[pos, h // G] @ b.q[row, h * b.dim:(h + 1) * b.dim].astype(np.float64) * scale
+                    if np.all(s < np.inf):
+                        w = np.exp(s - s.max())
+                        seen = s > -np.inf
+                        out[row, h] = ((w / w.sum())[seen, None] * v[pos[seen], h // G]).sum(0)
+    return out.reshape(b.tokens, -1)
+
+
+def check_odd(got, b, window=0, sinks=0):
+    """Infinities and NaN where the definition has them, and the rest within
+    the bound that the same batch has with small numbers in their places."""
+    want = outputs(b, window, sinks)
+    places = ~np.isfinite(b.stored)
+    keep = b.stored.copy()
+    b.stored[places] = 0
+    tol = b.attention(b.dim ** -0.5, window, sinks)[1] * 2
+    b.stored = keep
+    live = int(b.starts[-1])
+    got, want, tol = got[:live], want[:live], tol[:live]
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    for sign in (np.inf, -np.inf):
+        assert np.array_equal(got == sign, want == sign)
+    ok = np.isfinite(want)
+    assert np.any(ok) and np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("heads,new,page", [(2, 5, 16), (4, 150, 16), (16, 40, 5)])
+def test_channels_that_are_not_finite(dev, dtype, window, heads, new, page):
+    # Single values: their channels alone are lost, in the rows that see them.
+    b = Batch([(100, new), (0, new), (33, 1)], heads=heads, kv_heads=2, dim=64, page=page, layers=1, layer=0, dtype=dtype)
+    for seq, pos, head, d, value in [(0, 3, 0, 1, np.inf), (0, 90, 1, 63, -np.inf), (0, 103, 0, 2, np.nan),
+                                     (0, 102, 0, 1, -np.inf), (1, 2, 1, 8, np.inf), (1, new - 1, 0, 31, np.inf)]:
+        b.stored[int(b.table[seq, pos // page]), 0, 1, pos % page, head, d] = value
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    check_odd(attend(dev, b, window=window, sinks=2 if window else 0), b, window, 2 if window else 0)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,new", [(2, 5), (4, 150), (16, 70)])
+def test_scores_that_are_infinite(dev, dtype, heads, new):
+    # Keys with one infinity: scores of +infinity end a row, -infinity leaves
+    # it without that key.
+    b = Batch([(100, new), (0, new)], heads=heads, kv_heads=2, dim=64, page=16, layers=1, layer=0, dtype=dtype)
+    b.q.reshape(b.tokens, heads, 64)[:, :, 7] = np.where(np.arange(b.tokens) % 3, 0.5, -0.5)[:, None]
+    for seq, pos, value in [(0, 20, -np.inf), (0, 21, -np.inf), (0, 104, -np.inf), (1, 1, -np.inf), (1, 3, -np.inf)]:
+        b.stored[int(b.table[seq, pos // 16]), 0, 0, pos % 16, :, 7] = value
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    check_odd(attend(dev, b), b)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,new", [(2, 5), (4, 150)])
+@pytest.mark.parametrize("value", [np.inf, np.nan])
+def test_queries_that_are_not_finite(dev, value, dtype, heads, new):
+    b = Batch([(100, new), (9, 1)], heads=heads, kv_heads=2, dim=64, page=16, layers=1, layer=0, dtype=dtype)
+    q = b.q.reshape(b.tokens, heads, 64)
+    q[1, 0, 5] = q[new, heads - 1, 63] = value
+    got = attend(dev, b).reshape(q.shape)
+    assert np.all(np.isnan(got[1, 0])) and np.all(np.isnan(got[new, heads - 1]))
+    q[1, 0, 5] = q[new, heads - 1, 63] = 0
+    want, tol = (x.reshape(q.shape) for x in b.attention(0.125))
+    rest = np.ones((b.tokens, heads), bool)
+    rest[1, 0] = rest[new, heads - 1] = False
+    assert np.all(np.abs(got - want)[rest] <= tol[rest])
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("parity,value", [(0, np.nan), (0, -np.inf), (1, np.inf)])
+def test_what_a_value_that_is_not_finite_costs_many_rows(dev, parity, value, dtype):
+    # One early position, or one in eight, in a prompt whose rows nearly all see it.
+    b = Batch([(0, 2048)], heads=8, kv_heads=2, dim=128, page=16, layers=1, layer=0, dtype=dtype)
+    clean, _ = seconds(dev, b)
+    put_values(b, [(0, 5, parity, value)])
+    hurt, got = seconds(dev, b)
+    assert np.all(np.isfinite(got[:5])) and not np.any(np.isfinite(got[5:]))
+    assert hurt < 10 * clean, (hurt, clean)
+    put_values(b, [(0, pos, parity, value) for pos in range(5, 2048, 8)])
+    hurt, got = seconds(dev, b)
+    assert np.all(np.isfinite(got[:5])) and not np.any(np.isfinite(got[5:]))
+    assert hurt < 100 * clean, (hurt, clean)
+
+
 @pytest.mark.parametrize("new", [1, 40])
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("size", [2.0 ** -100, 2.0 ** -12, 2.0 ** 12, 2.0 ** 60])
@@ -457,6 +555,32 @@ def test_extreme_scores(dev):
     check(attend(dev, b, scale=300.0), b, scale=300.0)
     check(attend(dev, b, scale=0.0), b, scale=0.0)
     check(attend(dev, b, scale=-0.125), b, scale=-0.125)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("new", [1, 40])
+def test_scores_past_24_bits(dev, new, dtype):
+    # Scores of 10^8 and more, whose steps in f32 are larger than 1: nothing
+    # overflows, and a row whose largest score leads by more than the steps of
+    # all has that key's value (to 2^-16: a probability of at most e^-40 beside
+    # one, and what its pair and the value's keep).
+    b = Batch([(200, new), (30, new)], heads=4, kv_heads=2, dim=64, page=16, dtype=dtype)
+    for scale in (1e7, -1e8):
+        got = attend(dev, b, scale=scale)
+        want, _ = b.attention(scale)
+        assert np.all(np.isfinite(got))
+        for i, (p, n) in enumerate(b.lens):
+            k, v = b.keys(i)
+            for t in range(n):
+                for h in range(4):
+                    row = int(b.starts[i]) + t
+                    q = b.q[row, 64 * h:64 * h + 64].astype(np.float64)
+                    s = k[:p + t + 1, h // 2] @ q * scale
+                    ds = 16 * 2.0 ** -20 * abs(scale) * (np.abs(k[:p + t + 1, h // 2]) @ np.abs(q)).max()
+                    top = np.sort(s)[::-1]
+                    if len(top) == 1 or top[0] - top[1] > 2 * ds + 40:
+                        x, w = got[row, 64 * h:64 * h + 64], want[row, 64 * h:64 * h + 64]
+                        assert np.all(np.abs(x - w) <= 2.0 ** -16 * np.abs(v).max())
 
 
 # ---------------------------------------------------------------- prefix ----
