@@ -428,7 +428,17 @@ class CudaDevice:
     def dispatch(self, op: Op, inputs: Sequence[BufferRef], input_values: Sequence[Value],
                  outputs: Sequence[BufferRef], output_values: Sequence[Value],
                  scalars: Sequence[int] = ()) -> None:
-        Command(self, op, inputs, input_values, outputs, output_values, scalars)()
+        # The same as a Command called once, without one's cost (0.5 us of 6).
+        ni, no, ns = len(inputs), len(outputs), len(scalars)
+        if ni != len(input_values) or no != len(output_values):
+            raise DeviceError(Status.Execution, "inputs and input_values have different lengths")
+        ir = (_BufferRef * max(ni, 1))(*[_BufferRef(r.buffer, 0, r.offset, r.len) for r in inputs])
+        iv = (_Value * max(ni, 1))(*[v._c() for v in input_values])
+        orf = (_BufferRef * max(no, 1))(*[_BufferRef(r.buffer, 0, r.offset, r.len) for r in outputs])
+        ov = (_Value * max(no, 1))(*[v._c() for v in output_values])
+        sc = (C.c_uint32 * max(ns, 1))(*[int(s) for s in scalars])
+        o = op._c()
+        self._check(self._lib.slc_dispatch(self._d, C.byref(o), ir, iv, ni, orf, ov, no, sc, ns))
 
     def command(self, op: Op, inputs: Sequence[BufferRef], input_values: Sequence[Value],
                 outputs: Sequence[BufferRef], output_values: Sequence[Value],

@@ -403,3 +403,20 @@ def test_kv_heads_past_16_bits_are_refused(dev, kind):
     Call(dev, kind, batch=b)()
     b = Batch([], heads=(1 << 16) + 1, kv_heads=(1 << 16) + 1, dim=8, page=1, layers=1, layer=0, extra_pages=1)
     Call(dev, kind, batch=b).refused("support 65536 heads", Status.Unimplemented)
+
+
+def test_dispatch_prepares_no_command(dev, monkeypatch):
+    # A dispatch made once does not pay for one that is repeated.
+    def refuse(*args):
+        raise AssertionError("a Command was made")
+    b = Batch(LENS)
+    n = b.tokens * b.heads * b.dim
+    x, state = Value.f32((b.tokens, b.heads * b.dim)), dev.f32(D.state_words(b.shape, b.dtype))
+    ports = [dev.f32(n), *[dev.u32(a) for a in (b.table, b.past, b.starts)], state]
+    out = dev.f32(n)
+    monkeypatch.setattr(D, "Command", refuse)
+    before = dev._lib.host_recorded()
+    dev.dispatch(b.op(OpCode.PagedAttention, scale=1.0), ports, [x, *b.described(), b.state()], [out], [x], [3, 0, 0])
+    assert dev._lib.host_recorded() == before + 1
+    with pytest.raises(DeviceError, match="different lengths"):
+        dev.dispatch(b.op(OpCode.PagedAttention), ports, [x], [out], [x], [3, 0, 0])
