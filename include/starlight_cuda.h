@@ -186,8 +186,11 @@ typedef enum {
      * some rows of a sequence (16 with an F32 state, 32 with a 16-bit one), an
      * element of an F32 state counts to 2^-22 of itself, or a key's to 2^-28 of
      * that key's largest element and a value's to 2^-26 of the largest of its
-     * dim among up to 128 neighbouring positions (BF16: exactly, or to the
-     * latter two); other states and rows have no such floor.
+     * dim among up to 128 neighbouring positions and 2^-90 of the largest of
+     * its dim (BF16: exactly, or to the latter); other states and rows have no
+     * such floor. A row that sees a NaN or an infinity among the values is NaN
+     * or infinite in that dim, one with a score of NaN or +infinity is NaN; what
+     * a row does not see never reaches it.
      *
      * PREFIX_ATTENTION: PAGED_ATTENTION without a window, for sequences whose
      * first `prefix` positions are the same pages of the cache; these are read

@@ -77,7 +77,7 @@ constexpr int kTop = 11;    // a scale takes the largest value to 2^11 and serve
 constexpr int kFirst = 2;   // exponent expected at first
 constexpr int kNear = 8;    // keys down to 2^-8 of the expected largest value share its scale
 constexpr float kLarge = 4194304.f;  // 2^22
-constexpr int kDeep = 80;   // octaves that a channel's scale may fall within a segment
+constexpr int kDeep = 60;   // octaves that a channel's scale may fall within a segment
 constexpr int kLaunchRegs = 96;  // registers a thread at launch
 template <typename T, int DP>
 struct Cfg {

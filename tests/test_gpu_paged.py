@@ -536,6 +536,37 @@ def test_value_channels_of_very_different_sizes(dev, dim, page, dtype):
                 assert np.all(np.abs(got[row, h] - want[row, h]) <= tol), (row, h)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("window", [0, 100])
+@pytest.mark.parametrize("sizes", [[0, 25, -25, 20, -10], [0, 90, -100, 80, 3]])
+def test_values_that_rise_and_fall(dev, sizes, window, dtype):
+    # Blocks of 400 positions of one size: the channels' scales follow, up and
+    # down, and what the rows hold so far with them. A value counts to 2^-26 of
+    # the largest of its dim among 128 neighbours, and to 2^-90 of the largest
+    # of all.
+    b = Batch([(0, 2000), (1900, 100)], heads=4, kv_heads=2, dim=64, page=16, layers=1, layer=0, dtype=dtype)
+    for seq in range(2):
+        for pos in range(2000):
+            b.stored[int(b.table[seq, pos // 16]), 0, 1, pos % 16] *= 2.0 ** sizes[pos // 400]
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    got = attend(dev, b, window=window).reshape(b.tokens, 4, 64)
+    for i, rows in (0, range(0, 2000, 37)), (1, range(0, 100, 9)):
+        k, v = b.keys(i)
+        for t in rows:
+            at, row = b.lens[i][0] + t, int(b.starts[i]) + t
+            low = max(at + 1 - window, 0) if window else 0
+            for h in range(4):
+                kk, vv, q = k[low:at + 1, h // 2], v[low:at + 1, h // 2], b.q[row, 64 * h:64 * h + 64].astype(np.float64)
+                s = kk @ q / 8
+                w = np.exp(s - s.max())
+                w /= w.sum()
+                ds = 9 * 2.0 ** -20 / 8 * (np.abs(kk) @ np.abs(q)).max()
+                near = np.abs(v[max(low - 127, 0):at + 128, h // 2]).max(0)
+                tol = w @ np.abs(vv) * (2 * ds + (8 + len(kk) / 64) * 2.0 ** -20) + 2.0 ** -25 * near
+                tol += 2.0 ** -89 * np.abs(v[:, h // 2]).max(0)
+                assert np.all(np.abs(got[row, h] - w @ vv) <= tol), (row, h)
+
+
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("heads", [2, 8])
 def test_large_keys_that_a_row_does_not_see(dev, heads, dtype):
