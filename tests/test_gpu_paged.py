@@ -20,6 +20,7 @@ whose smallest step is 2^-34 of a tile's largest key or value and 2^-39 of the
 query's largest element: as much again, rounded up to 2^-33, times the largest
 value, and times what multiplies it in a score."""
 import math
+import random
 import time
 
 import numpy as np
@@ -612,6 +613,38 @@ def test_scores_past_24_bits(dev, new, dtype):
                     if len(top) == 1 or top[0] - top[1] > 2 * ds + 40:
                         x, w = got[row, 64 * h:64 * h + 64], want[row, 64 * h:64 * h + 64]
                         assert np.all(np.abs(x - w) <= 2.0 ** -16 * np.abs(v).max())
+
+
+def random_batch(r, seed):
+    """A batch and (window, sinks) of any sizes that a test can afford."""
+    while True:
+        kv, G = r.choice([1, 1, 2, 3, 4, 8]), r.choice([1, 1, 2, 4, 7, 8, 16])
+        seqs = r.choice([1, 1, 2, 3, 5, 9, 30, 150])
+        hi = r.choice([3, 40, 300, 1500]) // (8 if seqs > 20 else 1) + 1
+        most = r.choice([1, 1, 2, 5, 40, 200]) // (10 if seqs > 20 else 1) + 1
+        lens = [(r.randrange(hi), r.randrange(most + 1)) for _ in range(seqs)]
+        if sum(n for _, n in lens) and sum(n for _, n in lens) * kv * G * (hi + most) < 1.5e6:
+            break
+    prefix = window = sinks = 0
+    kind = r.random()
+    if kind < 0.25:
+        prefix = r.randrange(1, hi + 1)
+        lens = [(p + prefix, n) for p, n in lens]
+    elif kind < 0.6:
+        window, sinks = r.choice([1, 2, 15, 16, 17, 33, 100, 1000]), r.choice([0, 0, 1, 4, 16, 33, 200])
+    layers = r.choice([1, 2])
+    b = Batch(lens, heads=kv * G, kv_heads=kv, dim=8 * r.choice([1, 4, 8, 8, 9, 12, 16, 16, 16, 25, 32]),
+              page=r.choice([3, 5, 8, 16, 16, 24, 32, 64, 100, 128]), layers=layers, layer=r.randrange(layers),
+              dtype=r.choice([F32, F16, BF16]), prefix=prefix, pad=r.randrange(3), seed=seed, narrow=r.random() < 0.4)
+    return b, window, sinks
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_batches(dev, seed):
+    r = random.Random(seed)
+    b, window, sinks = random_batch(r, seed)
+    got = attend(dev, b, window=window, sinks=sinks, offset=seed % 2, max_new=b.max_new() + r.choice([0, 0, 50]))
+    check(got, b, window=window, sinks=sinks)
 
 
 # ---------------------------------------------------------------- prefix ----
