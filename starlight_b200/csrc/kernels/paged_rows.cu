@@ -103,8 +103,8 @@ struct Cfg {
     static constexpr int kConvWarp = 16 - kConv;
     static constexpr int kRows = kKeys / kConv / kRpi;   // 16-byte pieces per conversion lane
     // Registers a thread, by warpgroup, out of those of the launch.
-    static constexpr int kSoftRegs = kPair ? 96 : 88, kOutRegs = kPair ? 184 : 192, kConvRegs = kPair ? 64 : 56,
-                         kRestRegs = kPair ? 72 : 56;
+    static constexpr int kSoftRegs = kPair ? 96 : 88, kOutRegs = kPair ? 200 : 192, kConvRegs = kPair ? 64 : 56,
+                         kRestRegs = 56;
     static_assert(kSoft * kSoftRegs + kOutRegs + kConv / 4 * kConvRegs + kRestRegs <= 5 * kLaunchRegs, "registers");
     // f32 accumulators, f16 operands, K-major A; B K-major (S) or MN-major (O).
     static constexpr uint32_t kIdescS = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kM >> 4) << 24);
@@ -478,10 +478,12 @@ __device__ __forceinline__ void keys_again(const PagedPass &p, const Tile &cu, u
     using O = Operand<T, DP>;
     const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) - C::kConvWarp;
     const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
+#pragma unroll 1
     for (int i = 0; i < C::kRows; i++) {
         const int row = (i * C::kConv + pw) * C::kRpi + sub;
         const uint4 x = O::fetch(p, cu, row, col, false);
         uint32_t t = O::largest(x);
+#pragma unroll 1
         for (int o = 1; o < C::kLpr; o <<= 1) t = max(t, __shfl_xor_sync(0xffffffffu, t, o));
         int ex = t ? scale_exponent(t) : expect;
         if (ex >= expect - kNear && ex <= expect + 3) ex = expect;
@@ -497,6 +499,7 @@ __device__ __forceinline__ void keys_again(const PagedPass &p, const Tile &cu, u
 template <typename T, int DP>
 __device__ __forceinline__ void rescale_scores(uint32_t st, int first, const KeyTile *tile, const float *rel) {
     using C = Cfg<T, DP>;
+#pragma unroll 1
     for (int i = first; i < first + kKeys / C::kSoft; i++)
         if (tile->own[i / C::kRpi % C::kConv])
             tmem_st1(st + i, __float_as_uint(__uint_as_float(tmem_ld1(st + i)) * rel[i]));
@@ -523,6 +526,7 @@ __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu,
     uint32_t top[C::kEpl];
 #pragma unroll
     for (int e = 0; e < C::kEpl; e++) top[e] = 0;
+#pragma unroll 1
     for (int i = 0; i < C::kRows; i++) {
         const uint4 x = O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true);
         const uint32_t w[4] = {x.x, x.y, x.z, x.w};
@@ -535,12 +539,14 @@ __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu,
     }
 #pragma unroll
     for (int e = 0; e < C::kEpl; e++) {
+#pragma unroll 1
         for (int o = C::kLpr; o < 32; o <<= 1) top[e] = max(top[e], __shfl_xor_sync(0xffffffffu, top[e], o));
         if (sub == 0) most[pw * DP + col + e] = top[e];
     }
     bar_sync(1, C::kConv * 32);
     if (ct < DP) {
         uint32_t t = 0;
+#pragma unroll 1
         for (int w = 0; w < C::kConv; w++) t = max(t, most[w * DP + ct]);
         const int before = (int)(__float_as_uint(was[ct]) >> 23) - 127 + kTop + kShift;
         const int held = cu.begins ? -kDeep - 100 : *high_seg == cu.seg ? max(high[ct], before) : before;
@@ -553,6 +559,7 @@ __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu,
     F2 sc[C::kEpl / 2];
 #pragma unroll
     for (int e = 0; e < C::kEpl / 2; e++) sc[e] = F2(O::inverse(now[col + 2 * e]), O::inverse(now[col + 2 * e + 1]));
+#pragma unroll 1
     for (int i = 0; i < C::kRows; i++) {
         uint4 x = O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true);
         if (O::clean(x)) *odd = 1;
@@ -1157,7 +1164,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         // Piece i of a lane: row (i kConv + pw) kRpi + sub, 16 raw bytes from
         // dim `col` on. A piece on is a multiple of 8 rows on.
         const int sub = lane / C::kLpr, ch = lane % C::kLpr, col = ch * C::kEpl;
-        constexpr int kBatch = C::kPair ? 4 : 2, kStep = C::kConv * C::kRpi * 128;
+        constexpr int kBatch = 2, kStep = C::kConv * C::kRpi * 128;
         static_assert(C::kRows % kBatch == 0 && C::kConv * C::kRpi % 8 == 0, "batches of pieces 8 rows apart");
         auto row_of = [&](int i) { return (i * C::kConv + pw) * C::kRpi + sub; };
         const uint32_t op0 = operand_at(row_of(0), col);
