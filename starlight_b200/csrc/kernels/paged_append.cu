@@ -16,7 +16,7 @@
 // kTokens tokens at a time: its threads first evaluate the tokens' sines and
 // cosines (each once for all heads), then move 4 pairs of keys and 8 values
 // per item with 128-bit accesses. Measured: prompts of 11598 tokens, 8 kv heads
-// of 128 in f32 (190 MB) 33.5 us, 5.7 TB/s; one token 2.4 us in a graph, 5.4 us
+// of 128 in f32 (190 MB) 33.5 us, 5.7 TB/s; one token 2.4 us in a graph, 5.3 us
 // as a call (the host's part).
 #include <math.h>
 

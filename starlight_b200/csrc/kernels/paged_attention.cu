@@ -47,14 +47,16 @@
 //
 // Rows that meet a NaN or an infinity are recomputed in plain f32 over the
 // keys that they see alone (the MMA multiplies masked values by zero, and the
-// split of an infinity is NaN).
+// split of an infinity is NaN), until a score of NaN or +infinity ends them. One
+// infinite value in each of 64 sequences of 3000 keys makes 0.25 ms 8.9 ms, one
+// NaN among the keys 0.29 ms.
 //
 // Bound by HBM over long sequences: 64 of 300 to 16000 keys in bf16 (1.97 GB)
-// 347 us, 5.7 TB/s; 8 of 1000 to 8000 in f32 (282 MB) 57 us, 4.9 TB/s; heads
+// 334 us, 5.9 TB/s; 8 of 1000 to 8000 in f32 (282 MB) 55 us, 5.1 TB/s; heads
 // of 64 f32, 64 sequences (1.09 GB), 182 us, 6.0 TB/s. Short segments are
 // bound by latency: with 8 warps an SM three of four issue slots are empty, a
 // segment's start and end (queries, merge, result) cost about 5000 cycles and
-// a tile of 256 keys 4500. One sequence of 512 keys takes 7.8 us, a launch
+// a tile of 256 keys 4500. One sequence of 512 keys takes 8.0 us, a launch
 // chain of dependent reads.
 #include <math.h>
 
@@ -1010,15 +1012,16 @@ cudaError_t launch_type(cudaStream_t s, const PagedPass &p) {
 // Query rows of one kv head up to which a sequence is paged_attention_kernel's,
 // which reads the keys once per kRows of them; more are paged_rows.cu's.
 // Measured, 16 sequences of 1000 to 4000 keys, 8 kv heads of 128, with 16, 32
-// and 48 rows: f32 109, 168, 244 us here and 117, 124, 126 there; bf16 60, 90,
-// 128 and 100, 105, 107.
+// and 48 rows: f32 109, 169, 245 us here and 121, 139, 141 there; bf16 60, 90,
+// 129 and 103, 107, 108. (paged_rows.cu takes heads up to 128: wider ones come
+// here with any rows, 2048 tokens of 16 heads of 256 in bf16 580 us.)
 int small_rows(const PagedAttention &a) { return a.cache.type == kPagedF32 ? 16 : 32; }
 // Where all keys that the call's shapes allow are few, tokens in all times keys
 // counted in blocks of kRows rows by a tile, it takes them whatever the rows:
 // paged_rows.cu has 20 us to start up and end. 1 sequence of 38 tokens over 160
-// keys (76 units) 7.1 us here and 29 there, of 128 new tokens in f32 (512) 18
-// and 28, of 20 over 1000 (640) 21.5 and 21.0, of 64 over 1000 (2304) 41 and
-// 24. Known from the shapes alone, so that a call gives the same results
+// keys (76 units) 7.2 us here and 28 there, of 128 new tokens in f32 (512) 18
+// and 28, of 20 over 1000 (640) 21.6 and 20.9, of 64 over 1000 (2304) 41 and
+// 30. Known from the shapes alone, so that a call gives the same results
 // captured and not.
 constexpr size_t kFewUnits = 1024;
 bool many_rows(const PagedAttention &a, size_t new_tokens, size_t runs, size_t keys) {
@@ -1043,10 +1046,12 @@ size_t part_floats(const PagedAttention &a) {
 // and costs launches and the merge, 4 to 15 us: it is taken where those reads
 // are kPrefixPass bytes or more. Measured, with the pass and without: 64
 // sequences of 8 kv heads of 128 bf16, prefix 256 (67 MB) 35 and 32 us, 512
-// (134 MB) 44 and 43, 1024 49 and 61, 8192 72 and 311; 8 sequences, 1024 (34
-// MB) 18 and 16, 2048 (67 MB) 19 and 21, 4096 24 and 28; 64 sequences of 4 kv
-// heads of 64 f32, 777 (102 MB) 28 and 33; 6 of them (10 MB) 18 and 10. Without
-// it the rows read the pages by their own table rows, which are the same.
+// (134 MB) 44 and 43, 1024 49 and 61, 8192 72 and 313; 8 sequences, 1024 (34
+// MB) 18 and 16, 2048 (67 MB) 19 and 21, 4096 24 and 29; 64 sequences of 4 kv
+// heads of 64 f32, 777 (102 MB) 28 and 33; 6 of them (10 MB) 18 and 11. The
+// border is a compromise: few sequences gain from 60 MB on, many from 150 MB,
+// and between those the two differ by 2 us. Without it the rows read the pages by
+// their own table rows, which are the same.
 constexpr size_t kPrefixPass = (size_t)96 << 20;
 size_t prefix_bytes(const PagedAttention &a) {
     const size_t row = (size_t)2 * a.kv_heads * a.head_dim * (a.cache.type == kPagedF32 ? 4 : 2);

@@ -50,11 +50,13 @@
 //
 // Bound: 4 * pairs * D flops take 4 (16-bit cache) or 6 (F32) passes of half as
 // many MMA flops each: 2048 cycles a tile, 3/2 of that for F32. Two prompts of
-// 2048 tokens, 32 heads of 128, window 4096 (254 GFLOP): f32 886 us (7300 cycles a tile:
-// conversion and the MMAs share the shared memory), bf16 755 us, f16 590 us
-// (4800 cycles: the softmax warps' chain of TMEM reads, exponentials and
-// splits; the tensor pipe is busy for 40 % of it). 128 sequences of 64 heads
-// over 32768 shared keys in f16: 245 us of a call of 322.
+// 2048 tokens, 32 heads of 128, window 4096 (254 GFLOP), three sets of inputs in
+// turn: f32 943 us, some 8300 cycles a tile (conversion and the MMAs share the
+// shared memory; the tensor pipe is active for 37 %), bf16 817 us (29 %: four
+// warps convert), f16 552 us, some 4900 (43 %: the softmax warps' chain of TMEM
+// reads, exponentials and splits). The roles' code is more than the instruction
+// caches hold: each of the rare ways below costs 1 to 3 % of an f32 prompt's time
+// where it is never taken.
 #include <float.h>
 #include <math.h>
 
@@ -1424,15 +1426,15 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             // ---- MMA issue ----------------------------------------------------
             // The whole warp walks the loop and one elected lane issues. Inside
             // one lane's branch 16 MMAs took 1600 cycles to issue, 1024 to run;
-            // uniform control flow took two prompts of 2048 tokens from 619
-            // to 559 us over an f16 cache, from 896 to 868 us over f32. With
-            // all steps unrolled the code of the roles outgrew the
-            // instruction caches (676 and 1040 us); rolled up, f32 took 849,
-            // bf16 693 instead of 724, f16 597.
+            // uniform control flow took 10 % off two prompts of 2048 tokens over
+            // an f16 cache, 3 % over f32. With all steps unrolled the code of the
+            // roles outgrew the instruction caches (1.2 times as long in either);
+            // rolled up, f32 and bf16 took 2 to 4 % less than half unrolled, f16
+            // 7 % more.
             // The small products of a tile come before all large ones: the
             // tensor core cuts its sums off at the size of what they hold, and
             // the order halves the error (1.0e-6 to 4.6e-7 of the outputs'
-            // norm over 1100 f32 keys, 7.2e-7 to 4.5e-7 f16) for 3 % of time.
+            // norm over 1100 f32 keys, 7.2e-7 to 4.5e-7 f16) for 3 to 4 % of time.
             const uint32_t ra = smem_addr(ring);
             int seg = 0;
             auto slot_wait = [&](int j) {
