@@ -23,7 +23,8 @@
 // on without it. A value's are taken out of the operand, where they would reach
 // the rows that do not see them, and put into the results at the segment's end.
 // What is done twice is the conversion of their tiles, one product for every
-// such score, and a look through the values of their segments.
+// such score, and a look through the values between a segment's first such tile
+// and its last.
 //
 // One CTA per SM, 20 warps:
 //   0..3   softmax: one thread per row; Q of a segment to TMEM as f16 pairs;
@@ -58,6 +59,7 @@
 // caches hold: each of the rare ways below costs 1 to 3 % of an f32 prompt's time
 // where it is never taken.
 #include <float.h>
+#include <limits.h>
 #include <math.h>
 
 #include "common.cuh"
@@ -92,7 +94,7 @@ struct Cfg {
     static constexpr int kSlots = kPair && DP == 128 ? 3 : 6;
     static constexpr int kAhead = kSlots / 2;                // asynchronous copies: operands in flight
     static constexpr int kRing = kSlots * kTileBytes;
-    static constexpr int kSmall = 4 * (22 * kM + 8 * kKeys + 18 * DP + 88 + 8 * 12 + 16 + 2 * DP / 32 * kM) +
+    static constexpr int kSmall = 4 * (22 * kM + 8 * kKeys + 18 * DP + 96 + 8 * 12 + 16 + 2 * DP / 32 * kM) +
                                   8 * (3 * kKeys + 8 + 3 * kSlots + 8 + 20);
     static constexpr int kSmem = 1024 + kRing + kSmall;
     static constexpr int kEpl = 16 / (int)sizeof(T);    // elements of a 16-byte load
@@ -119,6 +121,14 @@ struct RowsArgs {
     CUtensorMap map;
     int unit;  // keys per box (paged_boxes); 1: no boxes
     int join;  // split segments are merged by rows_join_kernel
+    uint64_t limit;  // of a wait, ns: the output warps may look through a segment's values (odd_values)
+};
+constexpr uint64_t kLimitNs = 1000000000ull, kLimitKeyNs = 500;  // a key took them 150 ns
+
+// Where a segment has values that are not finite: key indexes [from, to) of
+// whole tiles.
+struct OddKeys {
+    int from, to;
 };
 
 // A segment of the work line and a place in it. Key indexes run over
@@ -514,13 +524,17 @@ __device__ __forceinline__ void shift_scores(uint32_t st, int first, float by) {
         tmem_st1(st + i, __float_as_uint(__uint_as_float(tmem_ld1(st + i)) - by));
     tmem_wait_st();
 }
+__device__ __forceinline__ void note_odd(OddKeys *odd, int i0) {
+    atomicMin(&odd->from, i0);
+    atomicMax(&odd->to, i0 + kKeys);
+}
 // All conversion warps' values of a tile from the cache again, with new scales
 // from the tile's own largest values. `now` takes them out of the outputs, as
 // `was` did. A scale falls by at most kDeep octaves within a segment, whose
 // outputs so far are held in units of it.
 template <typename T, int DP>
 __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu, uint32_t to, uint32_t *most, int *high,
-                                          int *high_seg, const float *was, float *now, int *odd) {
+                                          int *high_seg, const float *was, float *now, OddKeys *odd) {
     using C = Cfg<T, DP>;
     using O = Operand<T, DP>;
     const int lane = threadIdx.x & 31, pw = (threadIdx.x >> 5) - C::kConvWarp, ct = threadIdx.x - C::kConvWarp * 32;
@@ -564,23 +578,23 @@ __device__ __forceinline__ void values_again(const PagedPass &p, const Tile &cu,
 #pragma unroll 1
     for (int i = 0; i < C::kRows; i++) {
         uint4 x = O::fetch(p, cu, (i * C::kConv + pw) * C::kRpi + sub, col, true);
-        if (O::clean(x)) *odd = 1;
+        if (O::clean(x)) note_odd(odd, cu.i0);
         O::convert(x, sc, to + i * O::kStep);
     }
 }
 // A conversion lane's part of a tile of F16 values, which is otherwise taken
 // as it is, cleaned.
 template <typename T, int DP>
-__device__ __forceinline__ void clean_values(unsigned char *at, int *odd) {
+__device__ __forceinline__ void clean_values(unsigned char *at, int i0, OddKeys *odd) {
     for (int i = 0; i < Cfg<T, DP>::kRows; i++) {
         uint4 x = *reinterpret_cast<const uint4 *>(at + i * Operand<T, DP>::kStep);
         if (!Operand<T, DP>::clean(x)) continue;
         *reinterpret_cast<uint4 *>(at + i * Operand<T, DP>::kStep) = x;
-        *odd = 1;
+        note_odd(odd, i0);
     }
 }
 // The values that are not finite, zero in the operand, into the results of a
-// piece of a segment: four warps look through its keys [k0, k1) once more and
+// piece of a segment: four warps look through the keys [k0, k1) once more and
 // note for every dim which rows see a +infinity and which a -infinity (a NaN is
 // both); then thread r puts them into row r's result, dim d at
 // dst[d / 4 * step + d % 4]. bits: zero, and left so.
@@ -761,7 +775,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
     uint32_t *k_most = reinterpret_cast<uint32_t *>(v_seg + 4);  // [2][8 warps] keys' largest
     int *v_change = reinterpret_cast<int *>(k_most + 16);  // [8 tiles] the channels' scales change here
     KeyTile *key_tile = reinterpret_cast<KeyTile *>(v_change + 8);  // [8 tiles]
-    int *seg_odd = reinterpret_cast<int *>(key_tile + 8);         // [8 segments] some values are not finite
+    OddKeys *seg_odd = reinterpret_cast<OddKeys *>(key_tile + 8);  // [8 segments]
     uint32_t *odd_bits = reinterpret_cast<uint32_t *>(seg_odd + 8);  // [+, -][DP][kM / 32] outputs that see such
     Tile *tiles = reinterpret_cast<Tile *>(odd_bits + 2 * DP / 32 * kM);  // [8 tiles]
     long long *row_off = reinterpret_cast<long long *>(tiles + 8);  // [3 tiles][kKeys]
@@ -804,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         fence_mbar_init();
         *abort = 0;
         for (int i = 0; i < 8; i++) key_tile[i] = KeyTile{};
-        for (int i = 0; i < 8; i++) seg_odd[i] = 0;
+        for (int i = 0; i < 8; i++) seg_odd[i] = {INT_MAX, 0};
         *v_seg = -1;
     }
     for (int i = threadIdx.x; i < 2 * DP / 32 * kM; i += kThreads) odd_bits[i] = 0;
@@ -932,8 +946,8 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     if (p.a.window) lo = max(at - p.a.window + 1 - c.low, 0) + c.sink;
                 }
             }
-            mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort);
-            if (!C::kRaw) mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort);
+            mbar_wait(&s_full[n & 1], (n >> 1) & 1, p.a.err, abort, args.limit);
+            if (!C::kRaw) mbar_wait(&k_sc[n & 7], (n >> 3) & 1, p.a.err, abort, args.limit);
             tc_fence_after();
             const int i0 = c.tile * kKeys;
             // Rows past the tile's last hold zeros; they need no mask.
@@ -1035,13 +1049,13 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         const int r = threadIdx.x - 128, ow = warp - 4;
         const uint32_t lane_tm = (uint32_t)(ow * 32) << 16;
         F2 acc[DP / 2];  // in units of the channels' scales
-        int change = 0, seg = 0, seg_n = 0;
+        int change = 0, seg = 0;
 #pragma unroll
         for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
         for (int n = 0; n < N; n++) {
-            mbar_wait(&a_full[n & 3], (n >> 2) & 1, p.a.err, abort);
-            mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort);
-            mbar_wait(o_full, n & 1, p.a.err, abort);
+            mbar_wait(&a_full[n & 3], (n >> 2) & 1, p.a.err, abort, args.limit);
+            mbar_wait(&v_sc[n & 7], (n >> 3) & 1, p.a.err, abort, args.limit);
+            mbar_wait(o_full, n & 1, p.a.err, abort, args.limit);
             tc_fence_after();
             const float a = alpha[(n & 3) * kM + r];
             if (!C::kRaw && __builtin_expect(v_change[n & 7], 0)) {
@@ -1086,14 +1100,14 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                                          : *reinterpret_cast<const float2 *>(vs + 2 * d);
                 acc[d] = mul2(acc[d], F2(x.x, x.y));
             }
-            const bool has_odd = bar_or(2, 128, seg_odd[seg & 7] != 0);  // one answer for all, whatever was waited for
-            if (r == 0) seg_odd[seg & 7] = 0;
+            const OddKeys odd = seg_odd[seg & 7];
+            const bool has_odd = bar_or(2, 128, odd.to != 0);  // one answer for all, whatever was waited for
+            if (r == 0) seg_odd[seg & 7] = {INT_MAX, 0};
             __syncwarp();
             if (lane == 0) mbar_arrive(o_empty);
             const bool live = r < c.rows;
             auto add_odd = [&](float *dst, int step, bool mine) {
-                odd_values<T, DP>(p, c, (c.tile - (n - seg_n)) * kKeys, min(c.keys, (c.tile + 1) * kKeys), dst, step,
-                                  mine, odd_bits);
+                odd_values<T, DP>(p, c, odd.from, min(c.keys, odd.to), dst, step, mine, odd_bits);
             };
             const int row = c.r0 + r, tok = row / G;
             const size_t qrow = (size_t)(c.tok0 + tok) * H + c.kvh * G + (row - tok * G);
@@ -1155,7 +1169,6 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
 #pragma unroll
             for (int d = 0; d < DP / 2; d++) acc[d] = F2(0.f, 0.f);
             seg++;
-            seg_n = n + 1;
             if (n + 1 < N) cursor_next(p, unit, c);
         }
     } else if (warp < 16) {
@@ -1179,7 +1192,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
         for (int j = 0; j < total; j++) {
             const bool v = is_v(j);
             const int n = tile_of(j);
-            mbar_wait(&raw[j % S], (j / S) & 1, p.a.err, abort);
+            mbar_wait(&raw[j % S], (j / S) & 1, p.a.err, abort, args.limit);
             unsigned char *slot = ring + (j % S) * C::kTileBytes;
             const Tile &cu = tiles[n & 7];
             const bool whole = cu.whole;
@@ -1275,7 +1288,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     odd |= (O::size_of(x.x) + 0x04000400u) | (O::size_of(x.y) + 0x04000400u) |
                            (O::size_of(x.z) + 0x04000400u) | (O::size_of(x.w) + 0x04000400u);
                 }
-                if (__builtin_expect((odd & 0x80008000u) != 0, 0)) clean_values<T, DP>(slot + raw0, &seg_odd[cu.seg & 7]);
+                if (__builtin_expect((odd & 0x80008000u) != 0, 0)) clean_values<T, DP>(slot + raw0, cu.i0, &seg_odd[cu.seg & 7]);
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -1323,7 +1336,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                         }
                     };
                     auto copy = [&](int j, uint32_t page_id, int at, int kvh, int parity, int n, bool begins) {
-                        if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort);
+                        if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, args.limit);
                         if (__any_sync(0xffffffffu, *abort)) return;
                         if (at >= 0 && page_id >= (uint32_t)p.a.cache.pages) {  // checked on the host; see paged_row
                             report_error(p.a.err, kErrGatherId);
@@ -1381,7 +1394,7 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                     bar_sync(3, kCopy * 32);
                 };
                 auto copy = [&](int j, int n, int parity) {
-                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort);
+                    if (j >= S) mbar_wait(&empty[j % S], (j / S - 1) & 1, p.a.err, abort, args.limit);
                     unsigned char *slot = ring + (j % S) * C::kTileBytes;
                     const char *base = p.a.cache.base + (parity ? p.a.cache.parity_stride : 0) + col * (int)sizeof(T);
 #pragma unroll 4
@@ -1438,12 +1451,12 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
             const uint32_t ra = smem_addr(ring);
             int seg = 0;
             auto slot_wait = [&](int j) {
-                mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort);
+                mbar_wait(&full[j % S], (j / S) & 1, p.a.err, abort, args.limit);
                 return ra + (j % S) * C::kTileBytes;
             };
             auto qk = [&](int n, bool begins, uint32_t kb) {
                 const int j = n ? 2 * n - 1 : 0;
-                if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort);
+                if (begins) mbar_wait(q_full, seg++ & 1, p.a.err, abort, args.limit);
                 if (!__any_sync(0xffffffffu, *abort)) {
                     tc_fence_after();
                     const uint32_t d = s_tm + (n & 1) * 128;
@@ -1473,10 +1486,10 @@ __global__ void __launch_bounds__(kThreads, 1) paged_rows_kernel(const __grid_co
                 }
             };
             auto pv = [&](int n) {
-                mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort);
+                mbar_wait(&p_full[n & 1], (n >> 1) & 1, p.a.err, abort, args.limit);
                 const int j = n == N - 1 ? total - 1 : 2 * n + 2;
                 const uint32_t vb = slot_wait(j);
-                if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort);
+                if (n >= 1) mbar_wait(o_empty, (n - 1) & 1, p.a.err, abort, args.limit);
                 if (!__any_sync(0xffffffffu, *abort)) {
                     tc_fence_after();
                     const uint32_t pt = s_tm + (n & 1) * 128;
@@ -1617,6 +1630,7 @@ cudaError_t launch(cudaStream_t s, const PagedPass &p) {
     static_assert(C::kSmem <= 227 * 1024, "shared layout");
     RowsArgs args{};
     args.pass = p;
+    args.limit = kLimitNs + kLimitKeyNs * (uint64_t)p.a.batch.per_seq * (uint64_t)p.a.cache.page;
     args.join = ((size_t)p.a.tokens * (p.a.heads / p.a.kv_heads) + kM - 1) / kM * p.a.kv_heads < (size_t)kSmCount;
     args.unit = paged_boxes(p.a, kKeys, sizeof(T), C::kRaw, !C::kPair, &args.map);
     static std::atomic<uint64_t> smem_set{0};

@@ -434,6 +434,19 @@ def test_channels_that_are_not_finite(dev, dtype, window, heads, new, page):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("lens", [[(2500, 40), (2000, 3), (30, 50)], [(3000 - 20 * i, 30 + i) for i in range(12)]])
+def test_channels_that_are_not_finite_far_apart(dev, lens, dtype):
+    # In the first, a middle and the last tile of segments, split ones too.
+    b = Batch(lens, heads=8, kv_heads=2, dim=64, page=16, layers=1, layer=0, dtype=dtype)
+    for seq in range(0, len(lens), 2):
+        end = sum(lens[seq])
+        for pos, head, d, value in [(1, 0, 3, np.inf), (end // 2, 1, 40, -np.inf), (end - 4, 0, 9, np.nan)]:
+            b.stored[int(b.table[seq, pos // 16]), 0, 1, pos % 16, head, d] = value
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    check_odd(attend(dev, b), b)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
 @pytest.mark.parametrize("heads,new", [(2, 5), (4, 150), (16, 70)])
 def test_scores_that_are_infinite(dev, dtype, heads, new):
     # Keys with one infinity: scores of +infinity end a row, -infinity leaves
