@@ -395,16 +395,17 @@ def outputs(b, window=0, sinks=0):
                 for h in range(b.heads):
                     row = int(b.starts[i]) + t
                     s = k[pos, h // G] @ b.q[row, h * b.dim:(h + 1) * b.dim].astype(np.float64) * scale
-                    if np.all(s < np.inf):
+                    if np.all(s < np.inf) and np.any(s > -np.inf):
                         w = np.exp(s - s.max())
                         seen = s > -np.inf
                         out[row, h] = ((w / w.sum())[seen, None] * v[pos[seen], h // G]).sum(0)
     return out.reshape(b.tokens, -1)
 
 
-def check_odd(got, b, window=0, sinks=0):
-    """Infinities and NaN where the definition has them, and the rest within
-    the bound that the same batch has with small numbers in their places."""
+def check_odd(got, b, window=0, sinks=0, some=True):
+    """Infinities and NaN where the definition has them, and the rest (some,
+    where the batch is made for it) within the bound that the same batch has
+    with small numbers in their places."""
     want = outputs(b, window, sinks)
     places = ~np.isfinite(b.stored)
     keep = b.stored.copy()
@@ -417,7 +418,8 @@ def check_odd(got, b, window=0, sinks=0):
     for sign in (np.inf, -np.inf):
         assert np.array_equal(got == sign, want == sign)
     ok = np.isfinite(want)
-    assert np.any(ok) and np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
+    assert np.any(ok) or not some
+    assert np.all(np.abs(got[ok] - want[ok]) <= tol[ok])
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -457,6 +459,20 @@ def test_scores_that_are_infinite(dev, dtype, heads, new):
         b.stored[int(b.table[seq, pos // 16]), 0, 0, pos % 16, :, 7] = value
     b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
     check_odd(attend(dev, b), b)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("heads,new", [(2, 3), (8, 60)])
+def test_rows_whose_scores_are_all_minus_infinity(dev, dtype, heads, new):
+    # The first row sees one key, of score -infinity: it is NaN, the others
+    # leave that key out.
+    b = Batch([(0, new), (20, 1)], heads=heads, kv_heads=2, dim=64, page=16, layers=1, layer=0, dtype=dtype)
+    b.q.reshape(b.tokens, heads, 64)[:, :, 7] = 0.5
+    b.stored[int(b.table[0, 0]), 0, 0, 0, :, 7] = -np.inf
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), dtype)
+    got = attend(dev, b)
+    assert np.all(np.isnan(got[0]))
+    check_odd(got, b)
 
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
@@ -658,6 +674,25 @@ def test_random_batches(dev, seed):
     b, window, sinks = random_batch(r, seed)
     got = attend(dev, b, window=window, sinks=sinks, offset=seed % 2, max_new=b.max_new() + r.choice([0, 0, 50]))
     check(got, b, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_random_batches_with_values_that_are_not_finite(dev, seed):
+    r = random.Random(1000 + seed)
+    b, window, sinks = random_batch(r, seed)
+    used = set()
+    seen = [(i, pos) for i, (p, n) in enumerate(b.lens) if n for pos in range(p + n)]
+    for _ in range(r.choice([1, 3, 20])):
+        i, pos = r.choice(seen)
+        slot = (int(b.table[i, pos // b.page]), pos % b.page)
+        if slot in used:  # a key and its value at once: 0 times infinity
+            continue
+        used.add(slot)
+        parity = int(r.random() < 0.7)
+        value = r.choice([np.inf, -np.inf, np.nan]) if parity else r.choice([np.inf, -np.inf, -np.inf, np.nan])
+        b.stored[slot[0], b.layer, parity, slot[1], r.randrange(b.kv_heads), r.randrange(b.dim)] = value
+    b.stored, b.words = to_bits(b.stored.astype(np.float32), b.dtype)
+    check_odd(attend(dev, b, window=window, sinks=sinks, offset=seed % 2), b, window, sinks, some=False)
 
 
 # ---------------------------------------------------------------- prefix ----
